@@ -12,6 +12,13 @@ from .flash_attn_interface import (  # noqa: F401
     kv_store,
     varlen_prefill_with_kvcache,
 )
+from .kv4 import (  # noqa: F401
+    alloc_kv4_cache,
+    decode_paged_kv4,
+    flash_attn_with_kv4cache,
+    kv4_load,
+    kv4_store,
+)
 from .paged import BlockAllocator, SlotCacheManager  # noqa: F401
 
 __version__ = "0.1.0"

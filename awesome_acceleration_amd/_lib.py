@@ -91,6 +91,21 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, [_p, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _p, _i32, _i32, _p, _i32, _p]),
     "aac_kv_import_paged": (
         _c_int, [_p, _p, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _p, _i32, _i32, _i32, _p]),
+    "aac_kv4_store": (
+        _c_int, [_p, _p, _i64, _i64, _p, _i64, _i32, _p, _i64, _i32, _i32, _i32, _p]),
+    "aac_kv4_append": (
+        _c_int, [_p, _p, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _i32, _i32, _i32, _i32, _p]),
+    "aac_kv4_load": (_c_int, [_p, _i64, _i32, _p, _i64, _i32, _i32, _p, _p, _i32, _p]),
+    "aac_kv4_decode_workspace_bytes": (_size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "aac_kv4_decode": (
+        _c_int,
+        [_p, _i64, _p, _i64, _i32, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p,
+         _i64, _p, _size, _i32, _i32, _p]),
+    "aac_step_maps": (
+        _c_int, [_p, _p, _p, _i32, _i32, _i32, _p, _i32, _i64, _p, _p, _p, _p, _p, _p]),
+    "aac_logprobs_workspace_bytes": (_size, [_i64, _i64, _i32]),
+    "aac_token_logprobs": (
+        _c_int, [_p, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _p, _p, _size, _i32, _p]),
 }
 
 ABI_VERSION = 2
@@ -133,3 +148,23 @@ def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().aac_strerror(rc).decode()
         raise RuntimeError(f"{what} failed: {msg} (code {rc})")
+
+
+# The current stream's handle by device index, without the Stream object that
+# torch.cuda.current_stream builds (0.1 us against 1.4).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(name: str, device_index: int, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of that
+    device; a device that is not the current one is made so for the call (a
+    null stream is the current device's).  Raises as ``check``."""
+    fn = getattr(lib(), name)
+    if device_index == torch.cuda.current_device():
+        rc = fn(*args, raw_stream(device_index))
+    else:
+        with torch.cuda.device(device_index):
+            rc = fn(*args, raw_stream(device_index))
+    if rc != 0:
+        check(rc, name)

@@ -58,6 +58,7 @@
 #include <climits>
 #include <mutex>
 
+#include "decode_reduce.h"
 #include "qk_head.h"
 
 
@@ -228,15 +229,6 @@ __device__ __forceinline__ int seq_of_rank(const DecodeArgs& a, int rank, int ti
   }
   __syncthreads();
   return s_pick;
-}
-
-template <Dt DT>
-__device__ __forceinline__ void store_out2(void* out, int64_t idx, float x0, float x1) {
-  if constexpr (DT == Dt::FP32) {
-    *reinterpret_cast<float2*>(reinterpret_cast<float*>(out) + idx) = make_float2(x0, x1);
-  } else {
-    *reinterpret_cast<u32*>(reinterpret_cast<u16*>(out) + idx) = Elem<DT>::pack2(x0, x1);
-  }
 }
 
 // A (sequence, KV head)'s partial rows and log-sum-exps in the workspace
@@ -796,59 +788,14 @@ __global__ __launch_bounds__(256, G <= 2 ? 4 : 2) void decode_paged_kernel(Decod
   }
 }
 
-// Combine the partitions of every (sequence, query head) whose context was
-// split: out = sum_p 2^(lse_p - LSE) o_p with LSE = log2 sum_p 2^lse_p.
-// Four wavefronts per (sequence, query head): each finds the largest lse (one
-// load per 64 partitions), then wave w sums partitions w, w + 4, ... with four
-// in flight, and the four sums meet in LDS.  The chain of loads is what it
-// costs: one wave walking the partitions one by one took 5.2 us at 11 partitions
-// of 24 sequences.
+// Partitions combined in a launch of their own (decode_reduce.h).
 template <Dt DT>
 __global__ __launch_bounds__(256) void decode_reduce_kernel(DecodeArgs a) {
   const int hq = blockIdx.x, b = blockIdx.y;
   const int np = parts_of(a, context_len(a, b));
   if (np <= 1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t slot0 = ((int64_t)b * a.hq + hq) * a.n_parts;
-  float mx = -INFINITY;
-  for (int p = lane; p < np; p += 64) mx = fmaxf(mx, a.ws_lse[slot0 + p]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  float W = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int p = wave; p < np; p += 16) {
-    float lse[4];
-    float2 o[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t slot = slot0 + min(p + 4 * u, np - 1);
-      lse[u] = a.ws_lse[slot];
-      o[u] = *reinterpret_cast<const float2*>(a.ws_o + slot * kHeadDim + 2 * lane);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      // past the end: nothing, not 0 x the last partition's (infinite?) result
-      const bool in = p + 4 * u < np;
-      const float w = fast_exp2(lse[u] - mx);
-      W += in ? w : 0.f;
-      o0 = in ? fmaf(w, o[u].x, o0) : o0;
-      o1 = in ? fmaf(w, o[u].y, o1) : o1;
-    }
-  }
-  __shared__ float sw[4];
-  __shared__ float2 so[4][64];
-  so[wave][lane] = make_float2(o0, o1);
-  if (lane == 0) sw[wave] = W;
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    W += sw[w];
-    o0 += so[w][lane].x;
-    o1 += so[w][lane].y;
-  }
-  const float inv = 1.f / W;
-  store_out2<DT>(a.out, (int64_t)b * a.out_seq_stride + (int64_t)hq * kHeadDim + 2 * lane, o0 * inv,
-                 o1 * inv);
+  combine_partitions<DT>(a.ws_o, a.ws_lse, ((int64_t)b * a.hq + hq) * a.n_parts, np, a.out,
+                         (int64_t)b * a.out_seq_stride + (int64_t)hq * kHeadDim);
 }
 
 // ------------------------------------------------------------------ planning

@@ -1,0 +1,428 @@
+// Decode attention over the 4-bit paged KV cache (gfx950).  Format: kv4.h.
+//
+//   out[b, hq] = sum_t softmax_t(scale q[b, hq] . k_t) v_t,   t < context of b
+//
+// A workgroup takes one KV head's group of G <= 16 query heads over one partition of
+// a sequence's tokens; its four waves take steps of 32 tokens in turn and keep an
+// online softmax each (log2 domain), merged at the end; partitions are combined by
+// a second launch.
+//
+// Both products run on v_mfma_f32_16x16x32_bf16.  A cached value is a 2-bit significand
+// times a power of two, so its bfloat16 is exact (v_cvt_scalef32_pk_bf16_fp4: two
+// values an instruction, the scale included).  What is rounded is the other operand:
+//   bf16 queries are exact; probabilities are rounded to bf16, and the row sum adds
+//   the rounded ones (the choice of the 16-bit decode kernel);
+//   fp16 and fp32 queries and probabilities are split in 2 and 3 bfloat16 terms whose
+//   sum is exact to 16 and 24 bits, one product for each.
+// Sums, the running maximum and the partial results are float.
+//
+// Scores are computed transposed, S^T = K Q^T: lane (t = lane % 16, j = lane / 16)
+// reads 16 bytes of token t's codes, dims 32 j .. 32 j + 31, which is one scale and
+// (in four instructions of 8 dims) the K operand.  The result has query lane % 16
+// and tokens 4 j .. 4 j + 3 in each lane, which is, for two tiles of 16 tokens, the P
+// operand of O^T += V^T P^T with tokens in the order (tile, 4 j + i).  V^T needs four
+// tokens of one dim a lane: V is converted in token order like K, written to the
+// wave's own 8 KiB of LDS as bf16 and read back with the transposing load
+// ds_read_b64_tr_b16.  Chunks of 32 bytes sit at c ^ (t & 7), which spreads the
+// four rows a quarter-wave reads, and the eight a b128 write covers, over the banks.
+#include <algorithm>
+#include <climits>
+
+#include "decode_reduce.h"
+#include "kv4.h"
+
+namespace aac {
+namespace kv4 {
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+constexpr float kRescale = 8.f;  // probabilities up to 2^8 before the reference moves
+
+struct DecArgs {
+  const void* q;
+  int64_t q_stride;  // elements
+  Cache c;
+  const int32_t* block_tables;
+  int32_t max_blocks;
+  const int32_t* lens;
+  int32_t lens_add;
+  int32_t n_seqs, hq, g;
+  float scale_log2;
+  void* out;
+  int64_t out_stride;
+  int32_t n_parts, part_tokens;
+  float* ws_o;    // [n_seqs, hq, n_parts, 128]
+  float* ws_lse;  // [n_seqs, hq, n_parts]
+  // tile number -> block: (tile * magic) >> shift
+  uint64_t magic;
+  int32_t shift;
+};
+
+__device__ __forceinline__ int context_len(const DecArgs& a, int b) {
+  const int64_t ctx = (int64_t)a.lens[b] + a.lens_add, cap = (int64_t)a.max_blocks * a.c.block_size;
+  return (int)(ctx < 0 ? 0 : ctx > cap ? cap : ctx);
+}
+__device__ __forceinline__ int parts_of(const DecArgs& a, int ctx) {
+  return min(a.n_parts, (int)(((u32)ctx + (u32)a.part_tokens - 1) / (u32)a.part_tokens));
+}
+
+// The high halves of two floats as a bf16 pair, and what is left of each
+__device__ __forceinline__ u32 take_bf16(float& x, float& y) {
+  const u32 w = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), kSelHi);
+  x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+  return w;
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                 c, 0, 0, 0);
+}
+
+// eight codes (a dword) times 2^(byte - 127), as bf16
+__device__ __forceinline__ u32x4 values8(u32 w, float scale) {
+  return u32x4{__builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+               __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+               __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+               __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+
+// one step's codes and scale bytes of a lane, K and V of two tiles
+struct Raw {
+  u32x4 k[2], v[2];
+  u32 ks[2], vs[2];
+};
+
+template <Dt DT>
+__global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel(DecArgs a) {
+  constexpr int NT = DT == Dt::BF16 ? 1 : DT == Dt::FP16 ? 2 : 3;
+  constexpr int kWaveLds = 32 * 256;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kWaveLds];
+  __shared__ float sm_m[4][16], sm_l[4][16];
+  const int h = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ctx = context_len(a, b);
+  const int np = parts_of(a, ctx);
+  if (part >= np) {  // workgroup-uniform
+    if (part == 0) {  // an empty context
+      for (int i = tid; i < a.g * (kDim / 2); i += 256)
+        store_out2<DT>(a.out, (int64_t)b * a.out_stride + (int64_t)h * a.g * kDim + 2 * i, 0.f, 0.f);
+    }
+    return;
+  }
+  const int beg = part * a.part_tokens, end = min(ctx, beg + a.part_tokens);
+
+  // Q operand: query n's dims 32 j + 8 i .. + 7 for product i, in NT terms
+  const bool flip = a.scale_log2 < 0.f;  // -q and -scale: the largest product has the largest score
+  const float cs = fabsf(a.scale_log2);
+  u32x4 qf[NT][4];
+  {
+    const bool row = n < a.g;
+    const int64_t at = (int64_t)b * a.q_stride + (int64_t)(h * a.g + (row ? n : 0)) * kDim + 32 * j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == Dt::BF16) {
+        u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const u16*>(a.q) + at + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[0][i][e] = row ? (flip ? w[e] ^ 0x80008000u : w[e]) : 0u;
+      } else {
+        float x[8];
+        if constexpr (DT == Dt::FP16) {
+          Elem<DT>::unpack8(*reinterpret_cast<const u32x4*>(reinterpret_cast<const u16*>(a.q) + at + 8 * i), x);
+        } else {
+          const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.q) + at + 8 * i);
+          const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = lo[e];
+            x[4 + e] = hi[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row ? (flip ? -x[e] : x[e]) : 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[t][i][e] = take_bf16(x[2 * e], x[2 * e + 1]);
+      }
+    }
+  }
+
+  const int32_t* table = a.block_tables + (int64_t)b * a.max_blocks;
+  const int64_t pb = a.c.page_bytes();
+  const int tpb = a.c.block_size / kTile;
+  const int last_tile = (end - 1) / kTile;
+  auto load = [&](int t0, Raw& r) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int tile = min(t0 / kTile + s, last_tile);
+      const int bi = (int)((tile * a.magic) >> a.shift);
+      int blk = table[bi];
+      blk = blk < 0 || blk >= a.c.num_blocks ? 0 : blk;
+      const unsigned char* page = a.c.page(blk, h);
+      const int row = (tile - bi * tpb) * kTile + n;
+      const unsigned char* p = page + row * kRowBytes + 16 * j;
+      const unsigned char* ps = page + a.c.block_size * kRowBytes + row * kScaleBytes + j;
+      r.k[s] = *reinterpret_cast<const u32x4*>(p);
+      r.v[s] = *reinterpret_cast<const u32x4*>(p + pb);
+      r.ks[s] = *ps;
+      r.vs[s] = ps[pb];
+    }
+  };
+
+  lds_u8* vb = (lds_u8*)lds + wave * kWaveLds;
+  // writes: token n's dims 32 j + 8 i at chunk 2 j + i / 2; reads: this quarter's
+  // tokens 4 j + (n >> 2), dims 16 d + 4 (n & 3)
+  const int rt = 4 * j + (n >> 2);
+  f32x4 o[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // reference of the exponents (the running maximum, 0 while that is -inf), lane-partial sum
+  float m = -INFINITY, ref = 0.f, l = 0.f;
+
+  for (int t0 = beg + 32 * wave; t0 < end; t0 += 128) {
+    Raw r;
+    load(t0, r);
+    float s[8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      const float sc = __uint_as_float(r.ks[k] << 23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 kf = values8(r.k[k][i], sc);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc = mfma(kf, qf[t][i], acc);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[4 * k + i] = acc[i] * cs;
+        if (t0 + 16 * k + 4 * j + i >= end) s[4 * k + i] = -INFINITY;
+      }
+    }
+    // V to LDS: rows past the end stand for nothing (their bytes may stand for NaN)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bool in = t0 + 16 * k + n < end;
+      const float sc = in ? __uint_as_float(r.vs[k] << 23) : 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 w = values8(in ? r.v[k][i] : 0u, sc);
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(
+            vb + (16 * k + n) * 256 + ((2 * j + (i >> 1)) ^ (n & 7)) * 32 + (i & 1) * 16) = w;
+      }
+    }
+    float mx = vmax3(s[0], s[1], s[2]);
+    mx = vmax3(mx, s[3], s[4]);
+    mx = vmax3(mx, s[5], s[6]);
+    mx = vmax(mx, s[7]);
+    if (__ballot(mx > m + kRescale)) {
+      mx = vmax(mx, __shfl_xor(mx, 16));
+      mx = vmax(mx, __shfl_xor(mx, 32));
+      const float mn = vmax(m, mx), alpha = fast_exp2(m - mn);
+      // (m = -inf: nothing is summed yet)
+      const float f = m == -INFINITY ? 0.f : alpha;
+      m = mn;
+      ref = mn == -INFINITY ? 0.f : mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= f;
+    }
+    u32x4 pf[NT];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float x = fast_exp2(s[2 * w] - ref), y = fast_exp2(s[2 * w + 1] - ref);
+      if constexpr (NT == 1) {
+        pf[0][w] = Elem<Dt::BF16>::pack2_hw(x, y);
+        l = Elem<Dt::BF16>::dot2(pf[0][w], Elem<Dt::BF16>::kOnes, l);
+      } else {
+        l += x + y;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) pf[t][w] = take_bf16(x, y);
+      }
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const int at = rt * 256 + ((d ^ (rt & 7)) * 32) + 8 * (n & 3);
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + at));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + at + 16 * 256));
+      const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
+      const u32x4 vf = {a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[d] = mfma(vf, pf[t], o[d]);
+    }
+    asm volatile("" ::: "memory");
+  }
+
+  // merge the waves
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(lds);  // [wave][query][128]
+  if (n < a.g) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      *reinterpret_cast<f32x4*>(so + (wave * 16 + n) * kDim + 16 * d + 4 * j) = o[d];
+    if (j == 0) {
+      sm_m[wave][n] = m;
+      sm_l[wave][n] = l;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < a.g * (kDim / 2); i += 256) {
+    const int g = i >> 6, d = (i & 63) * 2;
+    float mx = sm_m[0][g];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mx = vmax(mx, sm_m[w][g]);
+    float L = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      // a wave without a token has -inf, and nothing summed
+      const float f = sm_m[w][g] == -INFINITY ? 0.f : fast_exp2(sm_m[w][g] - mx);
+      L = fmaf(sm_l[w][g], f, L);
+      const float* p = so + (w * 16 + g) * kDim + d;
+      o0 = fmaf(p[0], f, o0);
+      o1 = fmaf(p[1], f, o1);
+    }
+    const float inv = 1.f / L;
+    const int hq = h * a.g + g;
+    if (np == 1) {
+      store_out2<DT>(a.out, (int64_t)b * a.out_stride + (int64_t)hq * kDim + d, o0 * inv, o1 * inv);
+    } else {
+      const int64_t slot = ((int64_t)b * a.hq + hq) * a.n_parts + part;
+      *reinterpret_cast<float2*>(a.ws_o + slot * kDim + d) = make_float2(o0 * inv, o1 * inv);
+      if (d == 0) a.ws_lse[slot] = mx + __log2f(L);
+    }
+  }
+}
+
+template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArgs a) {
+  const int hq = blockIdx.x, b = blockIdx.y;
+  const int np = parts_of(a, context_len(a, b));
+  if (np <= 1) return;
+  combine_partitions<DT>(a.ws_o, a.ws_lse, ((int64_t)b * a.hq + hq) * a.n_parts, np, a.out,
+                         (int64_t)b * a.out_stride + (int64_t)hq * kDim);
+}
+
+struct Plan {
+  int32_t part_tokens, n_parts;
+  size_t ws_bytes;
+};
+
+static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, int32_t max_blocks,
+                 int32_t max_context_len, int32_t part_tokens) {
+  constexpr int kIter = 128;  // tokens of one turn of the workgroup's waves
+  Plan p;
+  int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, INT32_MAX - kIter);
+  if (max_context_len > 0 && max_context_len < cap) cap = max_context_len;
+  if (cap < 1) cap = 1;
+  int64_t part = part_tokens > 0 ? cdiv(part_tokens, kIter) * kIter : 0;
+  if (part == 0) {
+    const int64_t items = (int64_t)n_seqs * hkv;
+    part = cap;
+    if (!((items >= 512 && cap <= 4096) || cap <= 2 * kIter)) {
+      for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        part = k * kIter;
+        if (items * cdiv(cap, part) <= 3072 && cdiv(cap, part) <= 64) break;
+      }
+    }
+  }
+  part = cdiv(std::min(part, cap), kIter) * kIter;
+  p.part_tokens = (int32_t)part;
+  p.n_parts = (int32_t)cdiv(cap, part);
+  p.ws_bytes = p.n_parts > 1 ? (size_t)n_seqs * hq * p.n_parts * (kDim + 1) * sizeof(float) : 0;
+  return p;
+}
+
+template <Dt DT> static void launch(const DecArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((kv4_decode_kernel<DT>), dim3(a.c.hkv, a.n_parts, a.n_seqs), dim3(256), 0, s, a);
+  if (a.n_parts > 1)
+    hipLaunchKernelGGL((kv4_reduce_kernel<DT>), dim3(a.hq, a.n_seqs), dim3(256), 0, s, a);
+}
+
+}  // namespace kv4
+}  // namespace aac
+
+using namespace aac;
+
+extern "C" size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim, int32_t block_size,
+                                                 int32_t max_blocks_per_seq, int32_t max_context_len,
+                                                 int32_t partition_tokens) {
+  (void)head_dim;
+  if (n_seqs <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
+    return 0;
+  return kv4::plan(n_seqs, n_q_heads, n_kv_heads, block_size, max_blocks_per_seq, max_context_len,
+                   partition_tokens).ws_bytes;
+}
+
+extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* cache, int64_t num_blocks,
+                              int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                              const int32_t* context_lens, int32_t lens_add, int32_t n_seqs,
+                              int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads,
+                              int32_t head_dim, float scale, void* out, int64_t out_seq_stride,
+                              void* workspace, size_t workspace_bytes, int32_t partition_tokens,
+                              int32_t dtype, void* stream) {
+  if (n_seqs < 0 || n_q_heads <= 0 || max_blocks_per_seq <= 0 || q_seq_stride < 0 || out_seq_stride < 0)
+    return AAC_ERR_INVALID_ARGUMENT;
+  if (dtype != AAC_DTYPE_BF16 && dtype != AAC_DTYPE_FP16 && dtype != AAC_DTYPE_FP32)
+    return AAC_ERR_UNSUPPORTED;
+  if (n_seqs == 0) return AAC_OK;
+  const int rc = kv4::check_cache(cache, num_blocks, block_size, n_kv_heads, head_dim);
+  if (rc != AAC_OK) return rc;
+  if (n_q_heads % n_kv_heads) return AAC_ERR_SHAPE;
+  if (n_q_heads / n_kv_heads > 16 || num_blocks > INT32_MAX || n_seqs > 65535) return AAC_ERR_UNSUPPORTED;
+  if (!q || !block_tables || !context_lens || !out) return AAC_ERR_INVALID_ARGUMENT;
+  const int64_t width = (int64_t)n_q_heads * head_dim;
+  if (q_seq_stride < width || out_seq_stride < width) return AAC_ERR_SHAPE;
+  const int es = dtype == AAC_DTYPE_FP32 ? 4 : 2;
+  if ((uintptr_t)q % 16 || (q_seq_stride * es) % 16 || (uintptr_t)out % 8 || (out_seq_stride * es) % 8)
+    return AAC_ERR_MISALIGNED;
+  const kv4::Plan p = kv4::plan(n_seqs, n_q_heads, n_kv_heads, block_size, max_blocks_per_seq,
+                                max_context_len, partition_tokens);
+  if (p.n_parts > 65535) return AAC_ERR_UNSUPPORTED;
+  if (p.ws_bytes) {
+    if (!workspace || workspace_bytes < p.ws_bytes) return AAC_ERR_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return AAC_ERR_MISALIGNED;
+  }
+  kv4::DecArgs a = {};
+  a.q = q;
+  a.q_stride = q_seq_stride;
+  a.c = {(unsigned char*)const_cast<void*>(cache), num_blocks, block_size, n_kv_heads};
+  a.block_tables = block_tables;
+  a.max_blocks = max_blocks_per_seq;
+  a.lens = context_lens;
+  a.lens_add = lens_add;
+  a.n_seqs = n_seqs;
+  a.hq = n_q_heads;
+  a.g = n_q_heads / n_kv_heads;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out;
+  a.out_stride = out_seq_stride;
+  a.n_parts = p.n_parts;
+  a.part_tokens = p.part_tokens;
+  // Granlund and Montgomery 1994, Theorem 4.2, for tile numbers below 2^27 (a
+  // context is below 2^31 tokens): magic = floor(2^(27 + l) / d) + 1, l = ceil(log2 d)
+  const u32 d = (u32)(block_size / kv4::kTile);
+  const int l = d == 1 ? 0 : 32 - __builtin_clz(d - 1);
+  a.magic = (uint64_t(1) << (27 + l)) / d + 1;
+  a.shift = 27 + l;
+  if (p.ws_bytes) {
+    a.ws_o = reinterpret_cast<float*>(workspace);
+    a.ws_lse = a.ws_o + (size_t)n_seqs * n_q_heads * p.n_parts * kv4::kDim;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case AAC_DTYPE_BF16: kv4::launch<Dt::BF16>(a, s); break;
+    case AAC_DTYPE_FP16: kv4::launch<Dt::FP16>(a, s); break;
+    default: kv4::launch<Dt::FP32>(a, s); break;
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? AAC_OK : (int)e;
+}

@@ -47,10 +47,7 @@ __all__ = [
 _CHECK = os.environ.get("AAC_CHECK", "0") not in ("", "0")
 
 
-# The current stream's handle by device index, without the Stream object that
-# torch.cuda.current_stream builds (0.1 us against 1.4).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_raw_stream = _lib.raw_stream
 
 
 def _stream(t: torch.Tensor) -> int:

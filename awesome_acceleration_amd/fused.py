@@ -3,15 +3,16 @@ RMSNorm + RoPE + KV store, SiLU * up).  Device tensors only; every op runs on
 the current stream and fails loudly without the HIP library."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .flash_attn_interface import _stream
+from .flash_attn_interface import _on_gpu, _stream, check_mode
 
 __all__ = ["rmsnorm", "qk_norm_rope_store", "qkv_norm_rope_store", "silu_mul", "linear",
-           "linear_supported", "rmsnorm_supported", "rmsnorm_linear", "argmax"]
+           "linear_supported", "rmsnorm_supported", "rmsnorm_linear", "argmax",
+           "token_logprobs", "TokenLogprobs"]
 
 
 def _req(cond: bool, msg: str):
@@ -227,4 +228,53 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
                                     logits.shape[1], out.data_ptr(), _lib.AAC_DTYPE[logits.dtype],
                                     _stream(logits))
     _lib.check(rc, "aac_argmax_rows")
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # fp32 [rows]: log softmax at each row's token
+    entropy: torch.Tensor       # fp32 [rows], in nats
+    top_logprobs: torch.Tensor  # fp32 [rows, top_k], largest first
+    top_ids: torch.Tensor       # int64 [rows, top_k]
+
+
+MAX_TOP_LOGPROBS = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int64 ``[rows]``) under ``softmax(logits)``
+    (``[rows, cols]``, any row stride), the entropy of each row, and its ``top_k``
+    (up to 32) most likely tokens: ``torch.log_softmax(logits.float(), -1)`` gathered,
+    in one read of the logits.
+
+    Among equal logits the first index comes first and a NaN counts as the largest, as
+    in ``argmax``.  A negative token is padding and gets 0; one past the row gets NaN
+    (with ``AAC_CHECK=1`` an ``IndexError``, at one device sync).  A row with a NaN
+    or +inf, or masked to -inf throughout, gets NaN, as ``log_softmax`` gives."""
+    _on_gpu(logits, tokens)
+    _req(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+         "logits must be [rows, cols] with contiguous rows")
+    _req(logits.dtype in _lib.AAC_DTYPE, f"unsupported dtype {logits.dtype}")
+    rows, cols = logits.shape
+    _req(tokens.dtype == torch.int64 and tokens.shape == (rows,) and tokens.is_contiguous(),
+         "tokens must be contiguous int64 [rows]")
+    _req(cols > 0, "logits must have a column")
+    _req(0 <= top_k <= min(MAX_TOP_LOGPROBS, cols),
+         f"top_k must be within [0, {min(MAX_TOP_LOGPROBS, cols)}]")
+    if check_mode() and rows and int(tokens.max()) >= cols:
+        raise IndexError(f"index {int(tokens.max())} is out of bounds for dimension 1 with size {cols}")
+    dev = logits.device
+    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    out = TokenLogprobs(both[0], both[1], top, ids)
+    if rows == 0:
+        return out
+    nbytes = _lib.lib().aac_logprobs_workspace_bytes(rows, cols, top_k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    stride = logits.stride(0) if rows > 1 else cols
+    _req(stride >= cols, "rows of logits must not overlap")
+    _lib.launch("aac_token_logprobs", logits.get_device(), logits.data_ptr(), stride, rows, cols,
+                tokens.data_ptr(), top_k, both.data_ptr(), both.data_ptr() + 4 * rows,
+                top.data_ptr(), ids.data_ptr(), ws.data_ptr(), nbytes, _lib.AAC_DTYPE[logits.dtype])
     return out

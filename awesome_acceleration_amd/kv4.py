@@ -1,0 +1,203 @@
+"""The paged KV cache in four bits: store, append, load and decode attention.
+
+A cached element is an E2M1 code times a power of two shared by 32 dims (OCP
+microscaling FP4), 136 bytes a token and KV head for K and V against 512 in bf16.
+The cache is one uint8 tensor ``[num_blocks, Hkv, 2, block_size * 68]``: for each block
+and KV head the K page, then the V page; a page holds ``block_size`` rows of 64 bytes
+(dim ``2 i`` in the low nibble of byte ``i``) and then ``block_size`` rows of 4 scale
+bytes (``2^(byte - 127)``; 255: NaN).  Blocks, block tables and slot mappings are those
+of the 16-bit paged cache; ``block_size`` is a multiple of 16 and ``head_dim`` 128.
+
+``kv4_store`` and ``kv4_load`` stand beside ``kv_store`` and the KV export,
+``decode_paged_kv4`` and ``flash_attn_with_kv4cache`` beside ``decode_paged`` and
+``flash_attn_with_kvcache``, with their conventions: ``RuntimeError`` for a rejected
+argument, the current stream, no synchronisation, new outputs, caches updated in place.
+"""
+from __future__ import annotations
+
+import functools
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .flash_attn_interface import (_check_slots, _dtype_code, _on_gpu, _require, _scale,
+                                   _token_rows)
+
+__all__ = ["alloc_kv4_cache", "kv4_store", "kv4_load", "decode_paged_kv4",
+           "flash_attn_with_kv4cache", "BYTES_PER_TOKEN"]
+
+HEAD_DIM = 128
+PAGE_BYTES = 68        # of a token's K or V row of one head: 64 of codes, 4 of scales
+BYTES_PER_TOKEN = 136  # K and V of one token and KV head
+TILE = 16              # block sizes are multiples of it
+
+
+def alloc_kv4_cache(num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int = HEAD_DIM, *,
+                    device, n_layers: Optional[int] = None) -> torch.Tensor:
+    """A zero-filled cache (every value 0), ``[num_blocks, Hkv, 2, block_size * 68]``,
+    with ``n_layers`` in front where given."""
+    _require(head_dim == HEAD_DIM, f"the 4-bit cache is built for head_dim {HEAD_DIM}")
+    _require(block_size > 0 and block_size % TILE == 0, f"block_size must be a multiple of {TILE}")
+    shape = (num_blocks, n_kv_heads, 2, block_size * PAGE_BYTES)
+    return torch.zeros(shape if n_layers is None else (n_layers, *shape), dtype=torch.uint8,
+                       device=device)
+
+
+def _cache(kv_cache: torch.Tensor) -> tuple[int, int, int]:
+    """(num_blocks, block_size, Hkv) of a cache, checked."""
+    shape = kv_cache.shape
+    if (kv_cache.dtype is not torch.uint8 or len(shape) != 4 or shape[2] != 2
+            or not kv_cache.is_contiguous()):
+        raise RuntimeError("kv_cache must be contiguous uint8 [num_blocks, Hkv, 2, block_size * 68]")
+    bs = shape[3] // PAGE_BYTES
+    if shape[3] != bs * PAGE_BYTES or bs == 0 or bs % TILE:
+        raise RuntimeError(f"kv_cache pages must be block_size * {PAGE_BYTES} bytes, block_size a "
+                           f"multiple of {TILE}")
+    return shape[0], bs, shape[1]
+
+
+def _slots(slot_mapping: torch.Tensor, n: Optional[int]) -> None:
+    _require(slot_mapping.dtype == torch.int64 and slot_mapping.dim() == 1
+             and slot_mapping.is_contiguous() and (n is None or slot_mapping.shape[0] == n),
+             "slot_mapping must be contiguous int64 [N]")
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
+              slot_mapping: torch.Tensor) -> None:
+    """Quantise ``k``/``v`` (``[N, Hkv, 128]``, any token stride; bf16, fp16 or fp32) into
+    the cache rows ``slot_mapping`` (int64 ``[N]``), as ``kv_store`` stores them: negative
+    and out-of-range slots are skipped, ``IndexError`` for them with ``AAC_CHECK=1``.
+    Slots are distinct (a row named twice holds parts of both tokens)."""
+    _on_gpu(k, v, kv_cache, slot_mapping)
+    nb, bs, hkv = _cache(kv_cache)
+    ks, vs = _token_rows(k, "k"), _token_rows(v, "v")
+    _require(k.shape == v.shape and k.dtype == v.dtype, "k and v must have one shape and dtype")
+    _require(tuple(k.shape[1:]) == (hkv, HEAD_DIM), "row shape != [Hkv, 128]")
+    _slots(slot_mapping, k.shape[0])
+    _check_slots(slot_mapping, nb * bs)
+    _lib.launch("aac_kv4_store", k.get_device(), k.data_ptr(), v.data_ptr(), ks, vs,
+                kv_cache.data_ptr(), nb, bs, slot_mapping.data_ptr(), k.shape[0], hkv, HEAD_DIM,
+                _dtype_code(k))
+
+
+def kv4_load(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The K and V rows ``[N, Hkv, 128]`` that the cache holds at ``slot_mapping`` (int64
+    ``[N]``), in ``dtype``; zeros for a slot outside the cache."""
+    _on_gpu(kv_cache, slot_mapping)
+    nb, bs, hkv = _cache(kv_cache)
+    _slots(slot_mapping, None)
+    n = slot_mapping.shape[0]
+    _require(dtype in _lib.AAC_DTYPE, f"unsupported dtype {dtype}")
+    k = torch.empty((n, hkv, HEAD_DIM), dtype=dtype, device=kv_cache.device)
+    v = torch.empty_like(k)
+    _lib.launch("aac_kv4_load", kv_cache.get_device(), kv_cache.data_ptr(), nb, bs,
+                slot_mapping.data_ptr(), n, hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(),
+                _lib.AAC_DTYPE[dtype])
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(*args: int) -> int:
+    """aac_kv4_decode_workspace_bytes: host arithmetic on its integer arguments."""
+    return _lib.lib().aac_kv4_decode_workspace_bytes(*args)
+
+
+def _decode(q, q_stride, n, hq, kv_cache, cache, tables, lens, lens_add, scale, mcl, part, out):
+    nb, bs, hkv = cache
+    mb = tables.shape[1]
+    nbytes = _ws_bytes(n, hq, hkv, HEAD_DIM, bs, mb, mcl, part)
+    # from the allocator, in stream order: a captured call's belongs to its graph
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.launch("aac_kv4_decode", q.get_device(), q.data_ptr(), q_stride, kv_cache.data_ptr(), nb, bs,
+                tables.data_ptr(), mb, lens.data_ptr(), lens_add, n, mcl, hq, hkv, HEAD_DIM, scale,
+                out.data_ptr(), out.stride(0) if n > 1 else hq * HEAD_DIM,
+                None if ws is None else ws.data_ptr(), nbytes, part, _dtype_code(q))
+
+
+def _heads(hq: int, hkv: int, d: int) -> None:
+    if d != HEAD_DIM:
+        raise RuntimeError(f"head_dim must be {HEAD_DIM}")
+    if hq % hkv or hq // hkv > 16:
+        raise RuntimeError("query heads must be 1 to 16 times the KV heads")
+
+
+def _table(block_tables, n: int) -> None:
+    if (block_tables.dtype is not torch.int32 or block_tables.dim() != 2
+            or block_tables.shape[0] != n or block_tables.shape[1] == 0
+            or not block_tables.is_contiguous()):
+        raise RuntimeError("block_tables must be contiguous int32 [B, max_blocks]")
+
+
+def decode_paged_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, softmax_scale: Optional[float] = None,
+                     max_context_len: Optional[int] = None, partition_tokens: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``decode_paged`` over the 4-bit cache: ``q [B, Hq, 128]`` (bf16, fp16 or fp32)
+    against the first ``context_lens[b]`` tokens of each sequence, in the values that
+    the cache stands for; a sequence of none gets zeros.  1 to 16 query heads a KV head."""
+    _on_gpu(q, kv_cache, block_tables, context_lens, out)
+    cache = _cache(kv_cache)
+    _require(q.dim() == 3, "q must be [B, Hq, 128]")
+    n, hq, d = q.shape
+    _heads(hq, cache[2], d)
+    _require(q.stride(2) == 1 and q.stride(1) == d, "q heads/head_dim must be contiguous")
+    _table(block_tables, n)
+    _require(context_lens.dtype == torch.int32 and context_lens.shape == (n,)
+             and context_lens.is_contiguous(), "context_lens must be contiguous int32 [B]")
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    else:
+        _require(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+                 and out.stride(1) == d, "out must be [B, Hq, 128] like q")
+    _decode(q, q.stride(0) if n > 1 else hq * d, n, hq, kv_cache, cache, block_tables, context_lens, 0,
+            _scale(softmax_scale, d), int(max_context_len or 0), int(partition_tokens), out)
+    return out
+
+
+def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
+                             k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None, *,
+                             cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                             softmax_scale: Optional[float] = None,
+                             max_context_len: Optional[int] = None) -> torch.Tensor:
+    """``flash_attn_with_kvcache`` over the 4-bit cache: ``q [B, 1, Hq, 128]``; ``k``/``v``
+    (``[B, 1, Hkv, 128]``), where given, are quantised into the cache at position
+    ``cache_seqlens[b]`` and the call attends over ``cache_seqlens[b] + 1`` tokens,
+    otherwise over ``cache_seqlens[b]``.  The new token is attended to as the cache holds
+    it.  All rows are written before any is read; ``cache_seqlens`` is not modified."""
+    if q.dim() != 4:
+        raise RuntimeError("q must be [B, S, Hq, 128]")
+    n, s, hq, d = q.shape
+    if s != 1:
+        raise NotImplementedError("only one query token per sequence (decode) is supported")
+    if (k is None) != (v is None):
+        raise RuntimeError("k and v must be given together")
+    _on_gpu(q, kv_cache, k, v, cache_seqlens, block_table)
+    cache = _cache(kv_cache)
+    nb, bs, hkv = cache
+    _heads(hq, hkv, d)
+    _table(block_table, n)
+    if (cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (n,)
+            or not cache_seqlens.is_contiguous()):
+        raise RuntimeError("cache_seqlens must be contiguous int32 [B]")
+    if q.stride(3) != 1 or q.stride(2) != d:
+        q = q.contiguous()
+    out = torch.empty((n, 1, hq, d), dtype=q.dtype, device=q.device)
+    if k is not None:
+        if k.shape != v.shape or k.shape != (n, 1, hkv, d):
+            raise RuntimeError("k/v must be [B, 1, Hkv, 128]")
+        if k.dtype is not q.dtype or v.dtype is not q.dtype:
+            raise RuntimeError("k/v dtype mismatch")
+        if k.stride(3) != 1 or k.stride(2) != d:
+            k = k.contiguous()
+        if v.stride(3) != 1 or v.stride(2) != d:
+            v = v.contiguous()
+        row = hkv * d
+        _lib.launch("aac_kv4_append", q.get_device(), k.data_ptr(), v.data_ptr(),
+                    k.stride(0) if n > 1 else row, v.stride(0) if n > 1 else row,
+                    kv_cache.data_ptr(), nb, bs, block_table.data_ptr(), block_table.shape[1],
+                    cache_seqlens.data_ptr(), n, hkv, d, _dtype_code(q))
+    _decode(q, q.stride(0) if n > 1 else hq * d, n, hq, kv_cache, cache, block_table, cache_seqlens,
+            0 if k is None else 1, _scale(softmax_scale, d), int(max_context_len or 0), 0, out)
+    return out

@@ -11,16 +11,18 @@ unchanged.
 Metadata produced here mirrors llm.py:127-140 (``cu_seqlens``, positions and
 the flat scatter index, called ``slot_mapping``), generalised to block
 tables, and is shipped to the device with a single host-to-device copy per
-tensor.
+tensor; ``build_step_maps`` builds the same on the GPU from the request lengths.
 """
 from __future__ import annotations
 
 import bisect
 import math
-from typing import Iterable, Sequence
+from typing import Iterable, NamedTuple, Sequence
 
 import numpy as np
 import torch
+
+from . import _lib
 
 __all__ = [
     "SlotCacheManager",
@@ -30,6 +32,8 @@ __all__ = [
     "prefill_slot_mapping",
     "decode_slot_mapping",
     "build_prefill_metadata",
+    "build_step_maps",
+    "StepMaps",
     "pad_block_tables",
     "check_slots",
     "padded_prefill_slot_mapping",
@@ -256,3 +260,67 @@ def build_prefill_metadata(seq_lens: Sequence[int], block_tables: np.ndarray, bl
     slots = prefill_slot_mapping(block_tables, lens, block_size, num_cache_rows=num_cache_rows)
     to = lambda a: torch.from_numpy(a).to(device, non_blocking=False)  # noqa: E731
     return to(cu), to(positions), to(slots)
+
+
+class StepMaps(NamedTuple):
+    cu_seqlens: torch.Tensor    # int32 [n + 1]
+    positions: torch.Tensor     # int64 [n_tokens]
+    slot_mapping: torch.Tensor  # int64 [n_tokens]
+    context_lens: torch.Tensor  # int32 [n]: cached + new
+    blocks_taken: torch.Tensor  # int32 [1]: blocks asked of free_blocks
+
+
+MAX_MAP_SEQS = 8192
+
+
+def build_step_maps(new_lens: torch.Tensor, cached_lens: torch.Tensor | None,
+                    block_tables: torch.Tensor, block_size: int, n_tokens: int, *,
+                    free_blocks: torch.Tensor | None = None) -> StepMaps:
+    """A step's maps built on the GPU from its request lengths, in one launch.
+
+    Sequence ``b`` holds ``cached_lens[b]`` tokens (``None``: none yet) and gets
+    ``new_lens[b]`` more; ``n_tokens`` rows of maps are written, at least the sum of
+    ``new_lens`` (rows behind the last sequence: slot -1, position 0, so that a
+    captured step may be padded).  The values are ``build_prefill_metadata``'s:
+    ``cu_seqlens``, each token's position and its cache row through ``block_tables``
+    (int32 ``[n, width]``), -1 where it has no block.
+
+    With ``free_blocks`` (int32, the pool's free list) the blocks a sequence needs
+    beyond the ``ceil(cached / block_size)`` it holds are taken from the list in order,
+    sequence by sequence, and written into ``block_tables``; ``blocks_taken`` tells how
+    many were asked for (more than the list holds: the missing ones are -1).  The
+    lengths and the list are not modified.  Nothing synchronises."""
+    req = lambda c, m: None if c else _raise(m)  # noqa: E731
+    ints = dict(new_lens=new_lens, cached_lens=cached_lens, free_blocks=free_blocks)
+    dev = new_lens.get_device()
+    for name, t in ints.items():
+        if t is not None:
+            req(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(),
+                f"{name} must be contiguous int32, one-dimensional")
+            req(t.get_device() == dev and dev >= 0, "all tensors must be on the same GPU")
+    n = new_lens.shape[0]
+    req(n <= MAX_MAP_SEQS, f"at most {MAX_MAP_SEQS} sequences")
+    req(cached_lens is None or cached_lens.shape[0] == n, "one cached length per sequence")
+    req(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == n
+        and block_tables.shape[1] > 0 and block_tables.is_contiguous()
+        and block_tables.get_device() == dev, "block_tables must be contiguous int32 [n, width] "
+        "on the lengths' GPU")
+    req(block_size > 0, "block_size must be positive")
+    req(0 <= n_tokens < 1 << 31, "n_tokens must be within [0, 2^31)")
+    # one allocation: positions and slots, then the 32-bit results
+    both = torch.empty((2, n_tokens), dtype=torch.int64, device=new_lens.device)
+    small = torch.empty(2 * n + 2, dtype=torch.int32, device=new_lens.device)
+    p, at = both.data_ptr(), small.data_ptr()
+    out = StepMaps(small[:n + 1], both[0], both[1], small[n + 2:], small[n + 1:n + 2])
+    n_free = 0 if free_blocks is None else free_blocks.shape[0]
+    # an empty list is a list: every block asked of it is missing
+    free = 0 if free_blocks is None else free_blocks.data_ptr() or at
+    _lib.launch("aac_step_maps", dev, new_lens.data_ptr(),
+                None if cached_lens is None else cached_lens.data_ptr(), block_tables.data_ptr(), n,
+                block_tables.shape[1], block_size, free or None, n_free, n_tokens, at, p,
+                p + 8 * n_tokens, at + 4 * (n + 2), at + 4 * (n + 1))
+    return out
+
+
+def _raise(message: str):
+    raise RuntimeError(message)

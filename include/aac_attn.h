@@ -438,6 +438,99 @@ int aac_kv_import_paged(const void* src, void* kv_cache, int64_t layer_stride, i
                         int32_t n_kv_heads, int32_t head_dim, const int32_t* block_table,
                         int32_t max_blocks, int32_t length, int32_t dtype, void* stream);
 
+/*
+ * The paged KV cache in four bits.  cache: uint8 [num_blocks][n_kv_heads][K, V]
+ * [block_size * 68], 64-byte aligned, block_size a multiple of 16, head_dim 128.  A
+ * page holds block_size rows of 64 bytes (E2M1 codes, dim 2 i in the low nibble of
+ * byte i), then block_size rows of 4 scale bytes (E8M0, one for 32 dims): an element
+ * is code * 2^(byte - 127), NaN where the byte is 255.  With a = max |x| of 32 dims, the
+ * store sets byte - 127 = (exponent of a rounded to two significant bits) - 2, within
+ * [-125, 125], and rounds x / 2^(byte - 127) to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6,
+ * halves to the even code; 32 dims with an infinity or a NaN are stored as NaN.
+ *
+ * aac_kv4_store: row slot_mapping[t] of the cache (block slot / block_size, row slot
+ * mod block_size) gets k[t] and v[t]; slots outside the cache (negative: padding) are
+ * skipped.  Slots are distinct: a row named twice holds parts of both.
+ * aac_kv4_append: the same for one token a sequence at position cache_seqlens[b], as
+ * aac_kv_append_paged.
+ * aac_kv4_load: k_out[t], v_out[t] ([n_tokens, n_kv_heads, 128], 16-byte aligned) =
+ * the values of row slot_mapping[t], rounded to dtype; zeros for a slot outside.
+ * dtype BF16, FP16 or FP32; k and v have any token stride and alignment.
+ */
+int aac_kv4_store(const void* k, const void* v, int64_t k_tok_stride, int64_t v_tok_stride,
+                  void* cache, int64_t num_blocks, int32_t block_size, const int64_t* slot_mapping,
+                  int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                  void* stream);
+int aac_kv4_append(const void* k, const void* v, int64_t k_seq_stride, int64_t v_seq_stride,
+                   void* cache, int64_t num_blocks, int32_t block_size, const int32_t* block_tables,
+                   int32_t max_blocks_per_seq, const int32_t* cache_seqlens, int32_t n_seqs,
+                   int32_t n_kv_heads, int32_t head_dim, int32_t dtype, void* stream);
+int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block_size,
+                 const int64_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim,
+                 void* k_out, void* v_out, int32_t dtype, void* stream);
+
+/*
+ * Attend-only decode over the 4-bit cache: out[b] = softmax(scale q[b] K^T) V over the
+ * first context_lens[b] + lens_add tokens of sequence b (at most the table's capacity;
+ * none: zeros), read through block_tables as aac_decode_paged reads them.
+ * q, out [n_seqs, n_q_heads, 128] BF16, FP16 or FP32; n_q_heads / n_kv_heads from 1 to 16.
+ * max_context_len: 0, or a bound on every context (a longer one is cut).  Contexts
+ * split over workgroups need aac_kv4_decode_workspace_bytes(...) bytes of workspace,
+ * 16-byte aligned, any contents, not shared with a call that may overlap.
+ * partition_tokens: 0, or the tokens of a partition (rounded up to 128).
+ */
+size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
+                                      int32_t head_dim, int32_t block_size,
+                                      int32_t max_blocks_per_seq, int32_t max_context_len,
+                                      int32_t partition_tokens);
+int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* cache, int64_t num_blocks,
+                   int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                   const int32_t* context_lens, int32_t lens_add, int32_t n_seqs,
+                   int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                   float scale, void* out, int64_t out_seq_stride, void* workspace,
+                   size_t workspace_bytes, int32_t partition_tokens, int32_t dtype, void* stream);
+
+/*
+ * A step's maps from its request lengths.  Sequence b holds cached_lens[b] tokens (null:
+ * none) and gets new_lens[b] more (negative lengths count as 0; the new ones sum to less
+ * than 2^31):
+ *   cu_seqlens [n_seqs + 1]  prefix sums of new_lens
+ *   positions, slot_mapping [n_tokens]  of token i of sequence b, at cu_seqlens[b] + i:
+ *       cached_lens[b] + i, and its cache row through the block table; a slot is -1
+ *       without a block or past the table, and behind the last sequence (position 0)
+ *   context_lens [n_seqs]  cached + new
+ * With free_blocks (n_free of them) the blocks a sequence needs beyond the
+ * ceil(cached / block_size) it holds are taken from it in order, sequence by sequence,
+ * and written to block_tables; past its end they are -1.  blocks_taken[0] = the blocks
+ * asked for: more than n_free means that some are missing.  Null: the tables are
+ * complete and only read.  n_seqs up to AAC_STEP_MAPS_MAX_SEQS.
+ * Replaces the host's metadata construction (llm.py:127-140).
+ */
+#define AAC_STEP_MAPS_MAX_SEQS 8192
+int aac_step_maps(const int32_t* new_lens, const int32_t* cached_lens, int32_t* block_tables,
+                  int32_t n_seqs, int32_t max_blocks_per_seq, int32_t block_size,
+                  const int32_t* free_blocks, int32_t n_free, int64_t n_tokens,
+                  int32_t* cu_seqlens, int64_t* positions, int64_t* slot_mapping,
+                  int32_t* context_lens, int32_t* blocks_taken, void* stream);
+
+/*
+ * For each row of logits [n_rows, n_cols] (row stride row_stride elements, any
+ * alignment; BF16, FP16 or FP32): logprobs[r] = log softmax(row)[tokens[r]] (0 for a
+ * negative token, NaN for one past the row), entropy[r] of the softmax, and the top_k
+ * (0 to AAC_LOGPROBS_MAX_TOP, at most n_cols) largest: top_logprobs, top_ids [n_rows,
+ * top_k], the first index first among equal logits, a NaN counting as the largest.  A
+ * row with a NaN or +inf, or of -inf alone, gets NaN, as torch.log_softmax.
+ * n_cols up to AAC_LOGPROBS_MAX_COLS.  workspace: aac_logprobs_workspace_bytes(...) bytes,
+ * 16-byte aligned, any contents, not shared with a call that may overlap.
+ */
+#define AAC_LOGPROBS_MAX_TOP 32
+#define AAC_LOGPROBS_MAX_COLS (1 << 20)
+size_t aac_logprobs_workspace_bytes(int64_t n_rows, int64_t n_cols, int32_t top_k);
+int aac_token_logprobs(const void* logits, int64_t row_stride, int64_t n_rows, int64_t n_cols,
+                       const int64_t* tokens, int32_t top_k, float* logprobs, float* entropy,
+                       float* top_logprobs, int64_t* top_ids, void* workspace,
+                       size_t workspace_bytes, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,406 @@
+"""The 4-bit KV cache on the GPU against the float64 oracle (oracle/kv4.py): store, append
+and load byte for byte, decode attention within a bound on its roundings."""
+import numpy as np
+import pytest
+import torch
+
+from awesome_acceleration_amd import kv4
+from oracle import kv4 as oracle4
+from gpu_util import f64
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+SCALE = 128 ** -0.5
+
+
+def _say(*a):
+    print("case:", *a, flush=True)
+
+
+def _rand(rs, *shape, dtype, size=1.0):
+    return torch.from_numpy((rs.standard_normal(shape) * size).astype(np.float32)).to(dtype)
+
+
+def _cache_np(c):
+    return c.cpu().numpy()
+
+
+# ---------------------------------------------------------------- store, load
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, hkv, bs", [(1, 1, 16), (5, 8, 16), (33, 3, 48), (200, 4, 256)])
+def test_store_and_load_are_exact(gpu, dtype, n, hkv, bs):
+    _say("store", dtype, n, hkv, bs)
+    rs = np.random.RandomState(n)
+    dt = DTYPES[dtype]
+    k, v = (_rand(rs, n, hkv, 128, dtype=dt, size=np.exp(rs.uniform(-4, 4, (n, hkv, 1)))) for _ in "kv")
+    nb = n // bs + 2
+    slots = rs.permutation(nb * bs)[:n]
+    slots[::7] = -1
+    if n > 2:
+        slots[2] = nb * bs  # just past the cache
+    start = rs.randint(0, 256, (nb, hkv, 2, bs * 68)).astype(np.uint8)
+    want = start.copy()
+    oracle4.store(want, bs, f64(k), f64(v), slots)
+    cache = torch.from_numpy(start).to(gpu)
+    sm = torch.from_numpy(slots).to(gpu)
+    kv4.kv4_store(k.to(gpu), v.to(gpu), cache, sm)
+    assert np.array_equal(_cache_np(cache), want)  # every byte, also of the rows not named
+    kl, vl = kv4.kv4_load(cache, sm, dtype=dt)
+    for got, ref in zip((kl, vl), oracle4.load(want, bs, slots)):
+        ref = torch.from_numpy(ref).to(torch.float32).to(dt)  # exact in float32 here
+        assert torch.equal(got.cpu(), ref)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_store_of_special_values(gpu, dtype):
+    _say("special values", dtype)
+    dt = DTYPES[dtype]
+    big = 2.0 ** 127 * 1.9
+    x = torch.zeros(12, 1, 128, dtype=torch.float32)
+    x[1] = -0.0
+    x[2, 0, ::3] = torch.inf
+    x[3, 0, 31] = -torch.inf
+    x[4, 0, 32] = torch.nan
+    x[5, 0, :5] = torch.tensor([4.0, 0.25, 0.75, -2.5, 3.5])
+    x[6, 0, 0], x[6, 0, 32], x[6, 0, 64] = 6.96875, 7.0, 1.75   # bf16 values about the rounding of the scale
+    x[7] = big
+    x[8] = 2.0 ** -130                                           # subnormal
+    x[9, 0, 0], x[9, 0, 1] = 2.0 ** -125, 2.0 ** -126
+    x[10] = torch.arange(128) - 64.0
+    x[11, 0, 5] = 1e-30
+    x = x.to(dt)
+    y = x.flip(0).contiguous()
+    want = np.zeros((1, 1, 2, 16 * 68), np.uint8)
+    oracle4.store(want, 16, f64(x), f64(y), range(12))
+    cache = torch.zeros_like(torch.from_numpy(want), device=gpu)
+    slots = torch.arange(12, device=gpu)
+    kv4.kv4_store(x.to(gpu), y.to(gpu), cache, slots)
+    got = _cache_np(cache)
+    # an empty block's sign bits apart (-0), the bytes are the oracle's
+    assert np.array_equal(got, want)
+    kl, _ = kv4.kv4_load(cache, slots, dtype=torch.float32)
+    ref, _ = oracle4.load(want, 16, range(12))
+    assert np.array_equal(f64(kl), ref, equal_nan=True)
+
+
+def test_load_reads_byte_255_as_nan_whatever_the_codes(gpu):
+    cache = torch.zeros((1, 1, 2, 16 * 68), dtype=torch.uint8, device=gpu)
+    cache[..., 16 * 64:] = 255
+    for dt in DTYPES.values():
+        for x in kv4.kv4_load(cache, torch.tensor([3, 99], device=gpu), dtype=dt):
+            assert x[0].isnan().all() and (x[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_store_of_strided_and_misaligned_rows(gpu, dtype):
+    rs = np.random.RandomState(3)
+    dt = DTYPES[dtype]
+    n, hkv = 37, 2
+    k = _rand(rs, n, 3 * hkv * 128 + 1, dtype=dt).to(gpu)[:, 1:1 + hkv * 128].view(n, hkv, 128)
+    v = _rand(rs, n, 4, hkv, 128, dtype=dt).to(gpu)[:, 2]
+    cache = kv4.alloc_kv4_cache(3, 16, hkv, device=gpu)
+    slots = torch.from_numpy(rs.permutation(48)[:n]).to(gpu)
+    kv4.kv4_store(k, v, cache, slots)
+    want = np.zeros(cache.shape, np.uint8)
+    oracle4.store(want, 16, f64(k), f64(v), slots.tolist())
+    assert np.array_equal(_cache_np(cache), want)
+
+
+def test_store_and_load_past_4_gib(gpu):
+    hkv, bs = 8, 256
+    nb = (4 << 30) // (hkv * 2 * bs * 68) + 3
+    cache = torch.empty((nb, hkv, 2, bs * 68), dtype=torch.uint8, device=gpu)
+    rs = np.random.RandomState(4)
+    k, v = (_rand(rs, 5, hkv, 128, dtype=torch.bfloat16).to(gpu) for _ in "kv")
+    slots = torch.tensor([nb * bs - 1, nb * bs - 300, 0, nb * bs, 7], device=gpu)
+    kv4.kv4_store(k, v, cache, slots)
+    got, _ = kv4.kv4_load(cache, slots, dtype=torch.float32)
+    want = oracle4.values(*oracle4.quantise(f64(k)))
+    want[3] = 0
+    assert np.array_equal(f64(got), want)
+    # and attention over rows there
+    q = _rand(rs, 1, 16, 128, dtype=torch.bfloat16).to(gpu)
+    cache[nb - 1].random_(0, 120)
+    last = _cache_np(cache[nb - 1:])
+    out = kv4.decode_paged_kv4(q, cache, torch.tensor([[nb - 1]], dtype=torch.int32, device=gpu),
+                               torch.tensor([bs], dtype=torch.int32, device=gpu))
+    _check(out, q, last, bs, np.zeros((1, 1), np.int32), [bs], SCALE)
+
+
+# ---------------------------------------------------------------- attention
+def _check(out, q, cache, bs, tables, lens, scale, what=""):
+    """Within the roundings of the output and of the arithmetic.  With A = sum p |v| and
+    z = max sum |q||k| scale (nats):
+      bf16: probabilities to bf16 (2^-8) above and below the fraction line: 2 * 2^-8 A;
+      fp16, fp32: 2 and 3 truncated bfloat16 terms leave 2^-14 and 2^-21 of each;
+      float scores: 128 products of a dot at 2^-24 z each, the exponent's argument, and
+      the float sums, at most 2^-16 of A for these lengths: (2^-16 z + 2^-16) A;
+      fp16's subnormals are 2^-24 apart, so half a step of a small value is 2^-25."""
+    dt = out.dtype
+    ref, absv, z = oracle4.decode(f64(q), cache, bs, np.asarray(tables), lens, scale)
+    half = torch.finfo(dt).eps / 2
+    p = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -14, torch.float32: 2.0 ** -21}[dt]
+    lim = half * np.abs(ref) + (p + 2.0 ** -16 * (1 + z)) * absv * (1 + half) + 2.0 ** -25
+    err = np.abs(f64(out).reshape(ref.shape) - ref)
+    assert np.isfinite(err).all(), what
+    assert (err <= lim).all(), f"{what}: worst {float((err - lim).max()):.3e} beyond the bound"
+
+
+def _case(gpu, lens, hq, hkv, bs, dtype, seed, junk=True, spare=2):
+    """Random 4-bit pages; what lies behind each context is NaN."""
+    rs = np.random.RandomState(seed)
+    need = [max(1, -(-x // bs)) for x in lens]
+    nb = sum(need) + spare
+    ids = rs.permutation(nb)
+    tables = np.zeros((len(lens), max(need) + 1), np.int32)
+    at = 0
+    for b, m in enumerate(need):
+        tables[b, :m] = ids[at:at + m]
+        at += m
+    cache = np.full((nb, hkv, 2, bs * 68), 255, np.uint8)
+    if not junk:
+        cache[:] = 0
+    for b, L in enumerate(lens):
+        if L:
+            p = np.arange(L)
+            k = rs.standard_normal((L, hkv, 128)) * np.exp(rs.uniform(-1, 1, (1, hkv, 128)))
+            oracle4.store(cache, bs, k, rs.standard_normal((L, hkv, 128)), tables[b, p // bs] * bs + p % bs)
+    q = _rand(rs, len(lens), hq, 128, dtype=DTYPES[dtype]).to(gpu)
+    return dict(q=q, cache=cache, gcache=torch.from_numpy(cache).to(gpu), tables=tables,
+                gtables=torch.from_numpy(tables).to(gpu), lens=lens, bs=bs,
+                ctx=torch.tensor(lens, dtype=torch.int32, device=gpu))
+
+
+def _attend(c, **o):
+    return kv4.decode_paged_kv4(c["q"], c["gcache"], c["gtables"], c["ctx"], **o)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 2), (6, 3), (16, 8), (7, 1), (16, 2), (24, 2), (16, 1)])
+def test_attention_lengths_and_groups(gpu, dtype, hq, hkv):
+    _say("attend", dtype, hq, hkv)
+    c = _case(gpu, [0, 1, 2, 15, 16, 17, 31, 32, 33, 100, 127, 128, 129, 300], hq, hkv, 16, dtype, hq)
+    _check(_attend(c), c["q"], c["cache"], 16, c["tables"], c["lens"], SCALE)
+
+
+@pytest.mark.parametrize("bs", [16, 48, 64, 80, 256])
+@pytest.mark.parametrize("part", [0, 128, 200])
+def test_attention_block_sizes_and_partitions(gpu, bs, part):
+    _say("attend blocks", bs, part)
+    c = _case(gpu, [1, 130, 0, 513, 700], 8, 2, bs, "bf16", bs)
+    _check(_attend(c, partition_tokens=part), c["q"], c["cache"], bs, c["tables"], c["lens"], SCALE)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_long_contexts(gpu, dtype):
+    c = _case(gpu, [5000, 1, 3333], 8, 1, 64, dtype, 9)
+    _check(_attend(c), c["q"], c["cache"], 64, c["tables"], c["lens"], SCALE)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0, 1e-3])
+def test_attention_scales(gpu, scale):
+    for dtype in DTYPES:
+        c = _case(gpu, [40, 333], 4, 2, 16, dtype, 5)
+        _check(_attend(c, softmax_scale=scale), c["q"], c["cache"], 16, c["tables"], c["lens"], scale)
+
+
+def test_attention_large_scores_move_the_reference(gpu):
+    """Scores that rise along the context by far more than one rescaling step."""
+    c = _case(gpu, [400], 4, 1, 16, "fp32", 6)
+    q = c["q"] * 30
+    out = kv4.decode_paged_kv4(q, c["gcache"], c["gtables"], c["ctx"])
+    _check(out, q, c["cache"], 16, c["tables"], c["lens"], SCALE)
+
+
+def test_attention_strided_q_and_out(gpu):
+    c = _case(gpu, [40, 7, 200], 8, 2, 16, "bf16", 7)
+    wide = torch.zeros((3, 3, 8, 128), dtype=torch.bfloat16, device=gpu)
+    wide[:, 1] = c["q"]
+    out = torch.full((3, 2, 8, 128), 7.0, dtype=torch.bfloat16, device=gpu)
+    got = kv4.decode_paged_kv4(wide[:, 1], c["gcache"], c["gtables"], c["ctx"], out=out[:, 1])
+    assert got.data_ptr() == out[:, 1].data_ptr()
+    assert torch.equal(got, _attend(c)) and (out[:, 0] == 7.0).all()
+
+
+def test_attention_with_bad_blocks_reads_block_0(gpu):
+    c = _case(gpu, [60, 33], 4, 2, 16, "bf16", 8, junk=False)
+    t = c["tables"].copy()
+    t[0, 1], t[0, 2], t[1, 0] = -5, len(c["cache"]), 2 ** 31 - 1
+    out = kv4.decode_paged_kv4(c["q"], c["gcache"], torch.from_numpy(t).to(gpu), c["ctx"])
+    _check(out, c["q"], c["cache"], 16, t, c["lens"], SCALE)
+
+
+def test_attention_clips_lengths_to_the_table(gpu):
+    c = _case(gpu, [48, 48], 4, 2, 16, "bf16", 10, junk=False)
+    ctx = torch.tensor([10000, -3], dtype=torch.int32, device=gpu)
+    out = kv4.decode_paged_kv4(c["q"], c["gcache"], c["gtables"], ctx)
+    _check(out, c["q"], c["cache"], 16, c["tables"], [10000, -3], SCALE)
+
+
+def test_attention_nan_in_the_context_stays_with_its_head(gpu):
+    c = _case(gpu, [50, 50], 4, 2, 16, "bf16", 11)
+    blk, row = int(c["tables"][0, 1]), 3
+    c["gcache"][blk, 1, 0, 16 * 64 + row * 4] = 255     # K of head 1, sequence 0
+    blk = int(c["tables"][1, 2])
+    c["gcache"][blk, 0, 1, 16 * 64 + 1 * 4 + 2] = 255   # V dims 64..95 of head 0, sequence 1
+    out = _attend(c)
+    assert out[0, 2:].isnan().all() and out[0, :2].isfinite().all()
+    assert out[1, :2, 64:96].isnan().all() and out[1, :2, :64].isfinite().all()
+    assert out[1, :2, 96:].isfinite().all() and out[1, 2:].isfinite().all()
+
+
+def test_attention_is_the_same_on_every_run_and_stream(gpu):
+    c = _case(gpu, [900, 3, 2000], 16, 4, 64, "bf16", 12)
+    first = _attend(c, partition_tokens=128)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        others = [_attend(c, partition_tokens=128) for _ in range(3)]
+    mine = [_attend(c, partition_tokens=128) for _ in range(3)]
+    torch.cuda.synchronize()
+    for o in others + mine:
+        assert torch.equal(o, first)
+
+
+def test_attention_of_no_sequence(gpu):
+    c = _case(gpu, [5], 4, 2, 16, "bf16", 13)
+    out = kv4.decode_paged_kv4(c["q"][:0], c["gcache"], c["gtables"][:0], c["ctx"][:0])
+    assert out.shape == (0, 4, 128)
+
+
+# ---------------------------------------------------------------- append
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_then_attend(gpu, dtype):
+    rs = np.random.RandomState(20)
+    cached = [0, 1, 15, 16, 63, 200, 47]
+    c = _case(gpu, [x + 1 for x in cached], 8, 2, 16, dtype, 20)
+    n = len(cached)
+    k, v = (_rand(rs, n, 1, 2, 128, dtype=DTYPES[dtype]) for _ in "kv")
+    lens = torch.tensor(cached, dtype=torch.int32, device=gpu)
+    slots = [int(c["tables"][b, p // 16]) * 16 + p % 16 for b, p in enumerate(cached)]
+    want = c["cache"].copy()
+    oracle4.store(want, 16, f64(k)[:, 0], f64(v)[:, 0], slots)
+    out = kv4.flash_attn_with_kv4cache(c["q"][:, None], c["gcache"], k=k.to(gpu), v=v.to(gpu),
+                                       cache_seqlens=lens, block_table=c["gtables"])
+    assert np.array_equal(_cache_np(c["gcache"]), want)
+    assert lens.tolist() == cached and out.shape == (n, 1, 8, 128)
+    _check(out, c["q"], want, 16, c["tables"], c["lens"], SCALE)
+    again = kv4.flash_attn_with_kv4cache(c["q"][:, None], c["gcache"], cache_seqlens=lens + 1,
+                                         block_table=c["gtables"])
+    assert torch.equal(again, out)
+
+
+def test_append_rows_of_one_sequence_see_each_other(gpu):
+    """One sequence given as three rows at positions 30, 31, 32: all are written before
+    any is read."""
+    rs = np.random.RandomState(21)
+    c = _case(gpu, [33], 8, 2, 16, "bf16", 21)
+    q = _rand(rs, 3, 1, 8, 128, dtype=torch.bfloat16).to(gpu)
+    k, v = (_rand(rs, 3, 1, 2, 128, dtype=torch.bfloat16).to(gpu) for _ in "kv")
+    tables = np.repeat(c["tables"], 3, 0)
+    want = c["cache"].copy()
+    oracle4.store(want, 16, f64(k)[:, 0], f64(v)[:, 0],
+                  [int(tables[0, p // 16]) * 16 + p % 16 for p in (30, 31, 32)])
+    out = kv4.flash_attn_with_kv4cache(q, c["gcache"], k=k, v=v, block_table=torch.from_numpy(tables).to(gpu),
+                                       cache_seqlens=torch.tensor([30, 31, 32], dtype=torch.int32, device=gpu))
+    _check(out, q[:, 0], want, 16, tables, [31, 32, 33], SCALE)
+
+
+def test_append_past_the_table_writes_nothing(gpu):
+    c = _case(gpu, [40], 4, 2, 16, "bf16", 22)
+    before = c["gcache"].clone()
+    k = torch.ones((1, 1, 2, 128), dtype=torch.bfloat16, device=gpu)
+    for pos in (c["tables"].shape[1] * 16, -1):
+        kv4.flash_attn_with_kv4cache(c["q"][:, None], c["gcache"], k=k, v=k, block_table=c["gtables"],
+                                     cache_seqlens=torch.tensor([pos], dtype=torch.int32, device=gpu))
+        assert torch.equal(c["gcache"], before)
+
+
+def test_append_of_strided_rows(gpu):
+    rs = np.random.RandomState(23)
+    c = _case(gpu, [18, 33], 8, 2, 16, "fp16", 23)
+    qkv = _rand(rs, 2, 1, 12 * 128 + 8, dtype=torch.float16).to(gpu)
+    q, k, v = (qkv[..., a * 128:b * 128].unflatten(-1, (-1, 128)) for a, b in ((0, 8), (8, 10), (10, 12)))
+    args = dict(cache_seqlens=c["ctx"] - 1, block_table=c["gtables"])
+    other = c["gcache"].clone()
+    out = kv4.flash_attn_with_kv4cache(q, c["gcache"], k=k, v=v, **args)
+    ref = kv4.flash_attn_with_kv4cache(q.contiguous(), other, k=k.contiguous(), v=v.contiguous(), **args)
+    assert torch.equal(out, ref) and torch.equal(c["gcache"], other)
+
+
+def test_captured_steps_replay(gpu):
+    """Two captured steps (append + attend over split contexts) replayed in turn with eager
+    calls between: each equals the eager result every time."""
+    rs = np.random.RandomState(24)
+    cs = [_case(gpu, lens, 8, 2, 16, "bf16", 24 + i, junk=False)
+          for i, lens in enumerate(([700, 40, 1000], [300, 900]))]
+    news = [[_rand(rs, len(c["lens"]), 1, 2, 128, dtype=torch.bfloat16).to(gpu) for _ in "kv"] for c in cs]
+
+    def step(i):
+        c = cs[i]
+        return kv4.flash_attn_with_kv4cache(c["q"][:, None], c["gcache"], k=news[i][0], v=news[i][1],
+                                            cache_seqlens=lens[i], block_table=c["gtables"])
+
+    lens = [c["ctx"] - 1 for c in cs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(2):
+            step(i)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    other = torch.cuda.Stream()
+    for turn in range(3):
+        for x in news:
+            for t in x:
+                t.normal_()
+        refs = [step(i).clone() for i in range(2)]
+        other.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(other):  # the two at once
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for o, r in zip(outs, refs):
+            assert torch.equal(o, r), turn
+
+
+# ---------------------------------------------------------------- refusals
+def test_python_surface_refuses(gpu):
+    c = _case(gpu, [5, 6], 4, 2, 16, "bf16", 30)
+    q, cache, t, ctx = c["q"], c["gcache"], c["gtables"], c["ctx"]
+    k = torch.zeros((2, 2, 128), dtype=torch.bfloat16, device=gpu)
+    s = torch.zeros(2, dtype=torch.int64, device=gpu)
+
+    def no(match, f, *a, err=RuntimeError, **o):
+        with pytest.raises(err, match=match):
+            f(*a, **o)
+
+    no("uint8", kv4.kv4_store, k, k, cache.to(torch.int8), s)
+    no("pages", kv4.kv4_store, k, k, torch.zeros((2, 2, 2, 24 * 68), dtype=torch.uint8, device=gpu), s)
+    no("one shape", kv4.kv4_store, k, k.float(), cache, s)
+    no("row shape", kv4.kv4_store, k[:, :1].contiguous(), k[:, :1].contiguous(), cache, s)
+    no("slot_mapping", kv4.kv4_store, k, k, cache, s.int())
+    no("slot_mapping", kv4.kv4_store, k, k, cache, s[:1])
+    no("dtype", kv4.kv4_store, k.double(), k.double(), cache, s)
+    no("dtype", kv4.kv4_load, cache, s, torch.float64)
+    no("1 to 16", kv4.decode_paged_kv4, q[:, :3], cache, t, ctx)
+    no("1 to 16", kv4.decode_paged_kv4, q.repeat(1, 9, 1), cache, t, ctx)
+    no("head_dim", kv4.decode_paged_kv4, q[..., :64], cache, t, ctx)
+    no("block_tables", kv4.decode_paged_kv4, q, cache, t.long(), ctx)
+    no("block_tables", kv4.decode_paged_kv4, q, cache, t[:1], ctx)
+    no("context_lens", kv4.decode_paged_kv4, q, cache, t, ctx.long())
+    no("out", kv4.decode_paged_kv4, q, cache, t, ctx, out=q[:1])
+    no("dtype", kv4.decode_paged_kv4, q.double(), cache, t, ctx)
+    a = dict(cache_seqlens=ctx, block_table=t)
+    no("one query", kv4.flash_attn_with_kv4cache, q[:1].view(1, 1, 4, 128).repeat(1, 2, 1, 1), cache,
+       err=NotImplementedError, **a)
+    no("together", kv4.flash_attn_with_kv4cache, q[:, None], cache, k=k[:, None], **a)
+    no("mismatch", kv4.flash_attn_with_kv4cache, q[:, None], cache, k=k[:, None].half(), v=k[:, None].half(), **a)
+    no("k/v must", kv4.flash_attn_with_kv4cache, q[:, None], cache, k=k[:, None, :1], v=k[:, None, :1], **a)
+    no("cache_seqlens", kv4.flash_attn_with_kv4cache, q[:, None], cache, cache_seqlens=ctx.long(), block_table=t)

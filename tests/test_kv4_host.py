@@ -1,0 +1,168 @@
+"""The 4-bit cache, the step maps and the token log probabilities without a GPU: the
+oracle's format against a search over the grid, and the refusals of every entry
+point, which come before any launch."""
+import numpy as np
+import pytest
+import torch
+
+from awesome_acceleration_amd import _lib, fused, kv4, paged
+from oracle import kv4 as oracle4
+
+P = 1 << 20  # a placeholder address, never read
+
+
+def test_quantise_takes_the_nearest_value_and_the_stated_scale():
+    rs = np.random.RandomState(0)
+    x = rs.standard_normal((50, 128)) * np.exp(rs.uniform(-60, 60, (50, 1)))
+    x[0] = 0.0
+    codes, scales = oracle4.quantise(x)
+    got = oracle4.values(codes, scales)
+    for r in range(50):
+        for b in range(4):
+            blk = x[r, 32 * b:32 * b + 32]
+            a = np.abs(blk).max()
+            e = int(scales[r, b]) - 127
+            if a:
+                n = int(np.floor(np.log2(a)))
+                assert e == n - 2 + (a >= 1.75 * 2.0 ** n)
+            grid = np.concatenate((oracle4.GRID, -oracle4.GRID)) * 2.0 ** e
+            d = np.abs(blk[:, None] - grid).min(-1)
+            assert np.array_equal(np.abs(got[r, 32 * b:32 * b + 32] - blk), d)
+
+
+def test_quantise_ties_bounds_and_bad_blocks():
+    x = np.zeros((6, 128))
+    x[0, :9] = [4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, -0.25, -2.5]  # scale 1: ties to the even code
+    x[1, 0], x[1, 40] = 6.99, 7.0                                   # stays at 6, becomes 4 x 2
+    x[2, 0] = 2.0 ** 127.9                                          # past the largest scale
+    x[3, 0] = 2.0 ** -140                                           # below the smallest
+    x[4, 0], x[5, 127] = np.inf, np.nan
+    codes, scales = oracle4.quantise(x)
+    v = oracle4.values(codes, scales)
+    assert v[0, :9].tolist() == [4.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 0.0, -2.0]
+    assert v[1, 0] == 6.0 and v[1, 40] == 8.0
+    assert scales[2, 0] == 252 and v[2, 0] == 6.0 * 2.0 ** 125
+    assert scales[3, 0] == 2 and v[3, 0] == 0.0
+    assert scales[4].tolist()[0] == 255 and np.isnan(v[4, :32]).all() and (v[4, 32:] == 0).all()
+    assert scales[5, 3] == 255 and np.isnan(v[5, 96:]).all()
+
+
+def test_pack_and_rows_round_trip():
+    rs = np.random.RandomState(1)
+    cache = np.zeros((3, 2, 2, 16 * 68), np.uint8)
+    k, v = rs.standard_normal((5, 2, 128)), rs.standard_normal((5, 2, 128))
+    slots = [7, -1, 47, 48, 0]
+    oracle4.store(cache, 16, k, v, slots)
+    kl, vl = oracle4.load(cache, 16, slots)
+    want = oracle4.values(*oracle4.quantise(k))
+    for t in (0, 2, 4):
+        assert np.array_equal(kl[t], want[t])
+    assert (kl[[1, 3]] == 0).all() and (vl[[1, 3]] == 0).all()
+
+
+def _store(**o):
+    a = dict(k=P, v=P, ks=1024, vs=1024, c=P, nb=4, bs=16, s=P, n=4, h=8, d=128, dt=0)
+    a.update(o)
+    return _lib.lib().aac_kv4_store(*a.values(), None)
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(k=None), -1), (dict(v=None), -1), (dict(c=None), -1), (dict(s=None), -1), (dict(n=-1), -1),
+    (dict(nb=0), -1), (dict(bs=0), -1), (dict(h=0), -1), (dict(dt=9), -2), (dict(d=64), -2),
+    (dict(bs=24), -5), (dict(ks=1000), -5), (dict(vs=1000), -5), (dict(c=P + 16), -3),
+    (dict(k=P + 1), -3), (dict(n=0, k=None), 0)])
+def test_store_refusals(change, code):
+    assert _store(**change) == code
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(k=None), -1), (dict(t=None), -1), (dict(l=None), -1), (dict(w=0), -1), (dict(n=-1), -1),
+    (dict(bs=8), -5), (dict(ks=1000), -5), (dict(dt=3), -2), (dict(c=P + 32), -3), (dict(n=0), 0)])
+def test_append_refusals(change, code):
+    a = dict(k=P, v=P, ks=1024, vs=1024, c=P, nb=4, bs=16, t=P, w=3, l=P, n=4, h=8, d=128, dt=0)
+    a.update(change)
+    assert _lib.lib().aac_kv4_append(*a.values(), None) == code
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(c=None), -1), (dict(s=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(n=-1), -1),
+    (dict(k=P + 8), -3), (dict(bs=20), -5), (dict(d=64), -2), (dict(dt=-1), -2), (dict(n=0), 0)])
+def test_load_refusals(change, code):
+    a = dict(c=P, nb=4, bs=16, s=P, n=4, h=8, d=128, k=P, v=P, dt=0)
+    a.update(change)
+    assert _lib.lib().aac_kv4_load(*a.values(), None) == code
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(q=None), -1), (dict(c=None), -1), (dict(t=None), -1), (dict(l=None), -1), (dict(o=None), -1),
+    (dict(n=-1), -1), (dict(w=0), -1), (dict(hq=0), -1), (dict(hq=12), -5), (dict(hq=136, qs=17408, os=17408), -2),
+    (dict(d=64), -2), (dict(dt=3), -2), (dict(n=70000), -2), (dict(qs=1000), -5), (dict(os=1000), -5),
+    (dict(q=P + 8), -3), (dict(qs=2052), -3), (dict(o=P + 4), -3), (dict(bs=17), -5), (dict(c=P + 8), -3),
+    (dict(part=128, w=64), -4), (dict(part=128, w=64, ws=P, wsb=1 << 10), -4),
+    (dict(part=128, w=64, ws=P + 8, wsb=1 << 30), -3), (dict(n=0), 0)])
+def test_decode_refusals(change, code):
+    a = dict(q=P, qs=2048, c=P, nb=4, bs=16, t=P, w=3, l=P, add=0, n=4, mcl=0, hq=16, h=8, d=128,
+             scale=1.0, o=P, os=2048, ws=None, wsb=0, part=0, dt=0)
+    a.update(change)
+    assert _lib.lib().aac_kv4_decode(*a.values(), None) == code
+
+
+def test_decode_workspace_is_what_the_plan_writes():
+    f = _lib.lib().aac_kv4_decode_workspace_bytes
+    assert f(4, 16, 8, 128, 16, 3, 0, 0) == 0
+    # 64 blocks of 16 in 256-token partitions: 4 partitions x (128 + 1) floats
+    assert f(3, 16, 8, 128, 16, 64, 0, 256) == 3 * 16 * 4 * 129 * 4
+    assert f(3, 16, 8, 128, 16, 64, 256, 256) == 0
+    assert f(0, 16, 8, 128, 16, 64, 0, 256) == 0
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(new=None), -1), (dict(t=None), -1), (dict(ctx=None), -1), (dict(cu=None), -1),
+    (dict(taken=None), -1), (dict(pos=None), -1), (dict(slots=None), -1), (dict(n=-1), -1),
+    (dict(w=0), -1), (dict(bs=0), -1), (dict(f=None), -1), (dict(nf=-1), -1), (dict(tok=-1), -1),
+    (dict(n=8193), -2), (dict(tok=1 << 31), -2)])
+def test_step_maps_refusals(change, code):
+    a = dict(new=P, cached=None, t=P, n=4, w=3, bs=16, f=P, nf=5, tok=10, cu=P, pos=P, slots=P, ctx=P,
+             taken=P)
+    a.update(change)
+    assert _lib.lib().aac_step_maps(*a.values(), None) == code
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(x=None), -1), (dict(t=None), -1), (dict(lp=None), -1), (dict(h=None), -1), (dict(tl=None), -1),
+    (dict(ti=None), -1), (dict(rows=-1), -1), (dict(cols=0), -1), (dict(stride=99), -1), (dict(k=-1), -1),
+    (dict(k=33), -2), (dict(cols=(1 << 20) + 1, stride=1 << 21), -2), (dict(dt=3), -2),
+    (dict(cols=3, k=4), -5), (dict(x=P + 1), -3), (dict(ws=None), -4), (dict(wsb=8), -4),
+    (dict(ws=P + 8), -3), (dict(rows=0), 0)])
+def test_token_logprobs_refusals(change, code):
+    a = dict(x=P, stride=100, rows=4, cols=100, t=P, k=5, lp=P, h=P, tl=P, ti=P, ws=P, wsb=1 << 20, dt=0)
+    a.update(change)
+    assert _lib.lib().aac_token_logprobs(*a.values(), None) == code
+
+
+def test_alloc_refuses_shapes_the_kernels_are_not_built_for():
+    c = kv4.alloc_kv4_cache(3, 32, 2, device="cpu", n_layers=2)
+    assert c.shape == (2, 3, 2, 2, 32 * 68) and c.dtype == torch.uint8 and not c.any()
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        kv4.alloc_kv4_cache(3, 24, 2, device="cpu")
+    with pytest.raises(RuntimeError, match="head_dim"):
+        kv4.alloc_kv4_cache(3, 32, 2, 64, device="cpu")
+
+
+def test_every_surface_refuses_host_tensors():
+    c = kv4.alloc_kv4_cache(3, 32, 2, device="cpu")
+    k = torch.zeros(4, 2, 128)
+    i64, i32 = torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)
+    t = torch.zeros(4, 2, dtype=torch.int32)
+    for f in (lambda: kv4.kv4_store(k, k, c, i64), lambda: kv4.kv4_load(c, i64),
+              lambda: kv4.decode_paged_kv4(k, c, t, i32),
+              lambda: kv4.flash_attn_with_kv4cache(k[:, None], c, cache_seqlens=i32, block_table=t),
+              lambda: paged.build_step_maps(i32, i32, t, 16, 4),
+              lambda: fused.token_logprobs(torch.zeros(4, 9), i64)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            f()
+
+
+def test_top_orders_ties_nan_and_signed_zeros():
+    x = np.array([[1.0, np.nan, 1.0, -0.0, 0.0, -np.inf]])
+    assert oracle4.top(x, 6).tolist() == [[1, 0, 2, 3, 4, 5]]
