@@ -13,12 +13,15 @@
 // its registers, forms the maximum, then S and T about it, and writes them for each
 // wave, and the maximum of each group of 128 neighbouring values (fp32: 64), which
 // the 16 lanes of a DPP row hold.  The second, a workgroup a row, joins the sums and
-// finds the top k from the group maxima: with groups ordered by (maximum, lowest
-// index), a value outside the first k groups has k better ones, so only those k
-// groups, k x 256 bytes, are read again.  (Collecting candidates in the first
-// launch instead, from a bound of each segment, had every wave go through nearly all
-// of its values a second time: 197 us against the 17 of the read at 256 x 151,936.)
-// Bound by the read of the logits.
+// finds the top k from the group maxima: a value above a bound that k groups reach
+// lies in a group that reaches it, so only some k groups of 256 bytes are read again.
+// Bound by the read of the logits (bf16, us): 256 x 151,936 17 of the first launch and
+// 3 (no alternatives) to 10 (20) of the second, whose chain of small steps is its
+// cost; 1500 rows 76, 6.0 TB/s (fp32 6.5).  Tried instead: candidates collected in the
+// first launch, where every wave goes through nearly all of its values again (197
+// against 17); one launch with a workgroup of 16 waves a row, maxima in LDS (as fast at
+// 256 rows, 30% slower at 300, 512 and 3900, where rows do not fill the GPU evenly
+// or the search for the top k leaves the memory idle).
 #include <algorithm>
 #include <climits>
 
@@ -27,10 +30,13 @@
 namespace aac {
 namespace lp {
 
+typedef unsigned long long u64;
+
 constexpr int kThreads = 256;
 constexpr int kChunks = 8;     // 16-byte chunks a thread of the first launch
 constexpr int kGroup = 16;     // chunks of a group
 constexpr int kMaxTop = 32;
+constexpr int kSegChunks = kThreads * kChunks;
 
 struct Args {
   const char* x;
@@ -42,7 +48,7 @@ struct Args {
   float* entropy;
   float* top_logp;
   int64_t* top_ids;
-  float* ws_sum;  // [n_rows, n_seg * 4 waves, 4]: m, S, T (base 2: sum of 2^d and d 2^d)
+  float* ws_sum;  // [n_rows, n_seg * 4 waves, 4]: m, S, T (base 2: sum of 2^d and d 2^d), d of x = m
   float* ws_max;  // [n_rows, n_seg * 128]: group maxima
 };
 
@@ -95,11 +101,11 @@ __device__ __forceinline__ u32 order_key(float x) {
   if (b == 0x80000000u) b = 0;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// candidate order: larger value first, then lower index
-__device__ __forceinline__ bool before(u32 ka, u32 ia, u32 kb, u32 ib) {
-  return ka > kb || (ka == kb && ia < ib);
+// the float of a key whose low `shift` bits were dropped (they are those of the type)
+__device__ __forceinline__ float key_float(u32 key, int shift) {
+  const u32 b = key << shift;
+  return __uint_as_float((b & 0x80000000u ? b ^ 0x80000000u : ~b) >> shift << shift);
 }
-
 __device__ __forceinline__ float wave_sum(float x) {
   x = row16_sum(x);
   x += __shfl_xor(x, 16);
@@ -113,68 +119,133 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // S and T of one chunk about m, base 2.  The exponent d = x log2 e - m log2 e is one
 // fma; the rounding of nm = -m log2 e moves all of them alike and is taken out where the
-// sums are joined (`residue`).  Where m log2 e may overflow (and for -inf) x - m comes
-// first.
+// sums are joined (`residue`).  An x of -inf has to add 0 to T, so values far below any
+// m of this form are raised to a finite one first, two in an instruction in the 16-bit
+// types (as unsigned numbers the negative bfloat16 go up with their size); it adds 2^d
+// = 0 as before.  Where m is near those values or m log2 e may overflow (FAR), x - m
+// comes first.
+template <Dt DT> __device__ __forceinline__ bool is_far(float m) {
+  return !(m <= 1e36f) || m < (DT == Dt::FP16 ? -6e4f : -1e36f);
+}
 template <Dt DT, bool FAR>
-__device__ __forceinline__ void add_chunk(const u32x4& w, float m, float nm, float& S, float& T) {
+__device__ __forceinline__ void add_chunk(u32x4 w, float m, float nm, float& S, float& T) {
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  if constexpr (!FAR) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32 x = w[i];  // (a bit cast of a vector's element itself reads its first)
+      if constexpr (DT == Dt::BF16)  // at least -9.97e36
+        w[i] = __builtin_bit_cast(u32, __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), (u16x2){0xfcf0, 0xfcf0}));
+      else if constexpr (DT == Dt::FP16)  // at least -65504
+        w[i] = __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(f16x2, x),
+                                                                 (f16x2){(_Float16)-65504.f, (_Float16)-65504.f}));
+    }
+  }
   float v[Row<DT>::kE];
   Row<DT>::unpack(w, v);
 #pragma unroll
   for (int e = 0; e < Row<DT>::kE; ++e) {
-    const float d = FAR ? (v[e] - m) * kLog2e : fmaf(v[e], kLog2e, nm);
+    float d;
+    if constexpr (FAR) d = (v[e] - m) * kLog2e;
+    else d = fmaf(DT == Dt::FP32 ? fmaxf(v[e], -1e37f) : v[e], kLog2e, nm);
     const float p = fast_exp2(d);
     S += p;
-    T = fmaf(p, fmaxf(d, -1e30f), T);  // (d = -inf: adds 0; a NaN stays in S)
+    T = fmaf(p, FAR ? fmaxf(d, -1e30f) : d, T);
   }
 }
-__device__ __forceinline__ bool is_far(float m) { return !(fabsf(m) <= 1e38f); }
 // what d of x = m is, in place of 0
-__device__ __forceinline__ float residue(float m) {
-  return is_far(m) ? 0.f : fmaf(m, kLog2e, -(m * kLog2e));
+template <Dt DT> __device__ __forceinline__ float residue(float m) {
+  return is_far<DT>(m) ? 0.f : fmaf(m, kLog2e, -(m * kLog2e));
+}
+
+// Chunks c0, c0 + step, ... of a row, NC of them.  All loads first, from chunks that lie
+// within the row (another one's place for those that do not), then the few chunks at
+// the row's ends (only where `ends`, the same for the whole wave).
+template <Dt DT, int NC>
+__device__ __forceinline__ void load_chunks(const char* p, int mis, int cols, int64_t c0, int step, bool ends,
+                                            u32x4* w) {
+  typedef Row<DT> R;
+  const int64_t c_lo = mis ? 1 : 0, c_hi = (cols + mis) / R::kE - 1;  // whole chunks
+  if (c_lo <= c_hi) {
+#pragma unroll
+    for (int u = 0; u < NC; ++u)
+      w[u] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4*>(p + (min(max(c0 + step * u, c_lo), c_hi) * R::kE - mis) * R::kEs));
+  }
+  if (ends) {
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+      const int64_t c = c0 + step * u;
+      if (c < c_lo || c > c_hi) w[u] = R::chunk(p, mis, cols, c);
+    }
+  }
+}
+// whether any of the n chunks from c on is not whole
+template <Dt DT> __device__ __forceinline__ bool has_ends(int mis, int cols, int64_t c, int n) {
+  return c < (mis ? 1 : 0) || c + n - 1 > (cols + mis) / Row<DT>::kE - 1;
+}
+
+// The maximum over a wave of its chunks (NaN if one is), returned, and those of the
+// groups: lane l gets chunk (l >> kOwn) & (NC - 1)'s of its 16 lanes.
+// In each step a lane hands half of its values to its partner (lane ^ 15, ^ 7, then ^ 2,
+// ^ 1) and keeps the other half, until one is left.
+template <int NC> constexpr int kOwn = NC == 8 ? 1 : 2;  // log2 of the lanes that end with one chunk
+template <Dt DT, int NC> __device__ __forceinline__ float chunk_maxima(const u32x4* w, int lane, float* group) {
+  static_assert(NC == 4 || NC == 8, "two or three halvings");
+  constexpr int E = Row<DT>::kE;
+  float cm[NC];
+#pragma unroll
+  for (int u = 0; u < NC; ++u) {
+    float v[E];
+    Row<DT>::unpack(w[u], v);
+    cm[u] = vmax3(v[0], v[1], v[2]);
+#pragma unroll
+    for (int e = 3; e + 1 < E; e += 2) cm[u] = vmax3(cm[u], v[e], v[e + 1]);
+    cm[u] = vmax(cm[u], v[E - 1]);
+  }
+  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
+  constexpr int H = NC / 2, Q = NC / 4;
+  float h[H], q[Q], g;
+#pragma unroll
+  for (int i = 0; i < H; ++i) h[i] = vmax(b3 ? cm[i + H] : cm[i], dpp_f<kDppRowMirror>(b3 ? cm[i] : cm[i + H]));
+#pragma unroll
+  for (int i = 0; i < Q; ++i) q[i] = vmax(b2 ? h[i + Q] : h[i], dpp_f<kDppRowHalfMirror>(b2 ? h[i] : h[i + Q]));
+  if constexpr (NC == 8) g = vmax(b1 ? q[1] : q[0], dpp_f<kDppQuadXor2>(b1 ? q[0] : q[1]));
+  else g = vmax(q[0], dpp_f<kDppQuadXor2>(q[0]));
+  g = vmax(g, dpp_f<kDppQuadXor1>(g));
+  *group = g;
+  float m = vmax(g, dpp_f<kDppQuadXor2>(g));
+  m = vmax(m, dpp_f<kDppRowHalfMirror>(m));
+  m = vmax(m, dpp_f<kDppRowMirror>(m));
+  m = vmax(m, __shfl_xor(m, 16));
+  return vmax(m, __shfl_xor(m, 32));
 }
 
 template <Dt DT>
-__global__ __launch_bounds__(kThreads) void logprobs_segment_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, 6) void logprobs_segment_kernel(Args a) {
   typedef Row<DT> R;
-  constexpr int E = R::kE;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x / a.n_seg;
   const int seg = (int)(blockIdx.x % a.n_seg);
   const char* p = a.x + row * a.stride;
   const int mis = (int)((uintptr_t)p & 15) / R::kEs;
-  const int64_t c0 = (int64_t)seg * (kThreads * kChunks) + tid;  // chunk c0 + 256 u
-
+  const int64_t s0 = (int64_t)seg * kSegChunks;
   u32x4 w[kChunks];
+  load_chunks<DT, kChunks>(p, mis, a.cols, s0 + tid, kThreads, has_ends<DT>(mis, a.cols, s0, kSegChunks), w);
+  float group;
+  const float m = chunk_maxima<DT, kChunks>(w, lane, &group);
+  if (a.top > 0 && (lane & ((1 << kOwn<kChunks>) - 1)) == 0)
+    a.ws_max[(row * a.n_seg + seg) * (kSegChunks / kGroup) +
+             ((lane >> kOwn<kChunks>) & (kChunks - 1)) * (kThreads / kGroup) + wave * 4 + (lane >> 4)] = group;
+  // The values are unpacked again from here: kept from the maxima they take 64 registers
+  // and half of the waves (1500 rows of bf16: 83 against 79 us).
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) w[u] = R::chunk(p, mis, a.cols, c0 + kThreads * u);
-
-  float gm[kChunks], m = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    float v[E];
-    R::unpack(w[u], v);
-    gm[u] = v[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) gm[u] = fmaxf(gm[u], v[e]);
-    gm[u] = row16_max(gm[u]);
-    m = fmaxf(m, gm[u]);
-  }
-  m = fmaxf(m, __shfl_xor(m, 16));
-  m = fmaxf(m, __shfl_xor(m, 32));
-  if (a.top > 0) {  // lane u of each 16 writes the maximum of chunk u's group
-    float g = gm[0];
-#pragma unroll
-    for (int u = 1; u < kChunks; ++u) g = (lane & 15) == u ? gm[u] : g;
-    if ((lane & 15) < kChunks)
-      a.ws_max[(row * a.n_seg + seg) * (kThreads / kGroup * kChunks) + (lane & 15) * (kThreads / kGroup) +
-               wave * 4 + (lane >> 4)] = g;
-  }
-
+  for (int u = 0; u < kChunks; ++u) asm volatile("" : "+v"(w[u]));
   float S = 0.f, T = 0.f;
-  if (is_far(m)) {
+  if (is_far<DT>(m)) {  // (a NaN or +inf is here, and makes S a NaN; -inf alone adds nothing)
     const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
+#pragma unroll
     for (int u = 0; u < kChunks; ++u) add_chunk<DT, true>(w[u], ref, 0.f, S, T);
   } else {
     const float nm = -(m * kLog2e);
@@ -184,148 +255,252 @@ __global__ __launch_bounds__(kThreads) void logprobs_segment_kernel(Args a) {
   S = wave_sum(S);
   T = wave_sum(T);
   if (lane == 0)
-    *reinterpret_cast<f32x4*>(a.ws_sum + ((row * a.n_seg + seg) * 4 + wave) * 4) = f32x4{m, S, T, 0.f};
+    *reinterpret_cast<f32x4*>(a.ws_sum + ((row * a.n_seg + seg) * 4 + wave) * 4) =
+        f32x4{m, S, T, residue<DT>(m)};
 }
 
-// The wave's k-th largest of 64 keys (0 if it has fewer above 0), bit by bit.
-__device__ __forceinline__ u32 kth_of_wave(u32 key, int k, int bits) {
-  u32 tau = 0;
+// The wave's k-th and j-th largest of 64 keys (0 where it has fewer above 0), bit by bit.
+__device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, int bits, int drop) {
+  u32 tk = 0, tj = 0;
 #pragma unroll 1
-  for (u32 bit = 1u << (bits - 1); bit; bit >>= 1)
-    if ((int)__popcll(__ballot(key >= (tau | bit))) >= k) tau |= bit;
-  return tau;
+  for (u32 bit = 1u << (bits - 1); bit >> drop; bit >>= 1) {
+    if ((int)__popcll(__ballot(key >= (tk | bit))) >= k) tk |= bit;
+    if ((int)__popcll(__ballot(key >= (tj | bit))) >= j) tj |= bit;
+  }
+  return make_uint2(tk, tj);
 }
 
-// rank[i] of the list's n entries, handed to put(rank, entry) for the first k
-template <typename F>
-__device__ __forceinline__ void ranked(const uint2* list, int n, int k, F put) {
+__device__ __forceinline__ u32 lanes_below(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi((u32)(mask >> 32), __builtin_amdgcn_mbcnt_lo((u32)mask, 0u));
+}
+
+// A candidate as one number: larger for the larger value, then for the lower index.
+__device__ __forceinline__ u64 entry(u32 key, u32 index) { return (u64)key << 32 | (u32)~index; }
+__device__ __forceinline__ u32 index_of(u64 e) { return ~(u32)e; }
+
+// Hands each of the list's n entries that is among the k largest to put(rank, entry).
+// The list is read eight entries at a time, so that the reads overlap: entries n to the
+// next multiple of eight are set to 0 first, which is below every entry.
+template <typename F> __device__ __forceinline__ void ranked(u64* list, int n, int k, F put) {
+  if ((int)threadIdx.x < 8) list[n + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint2 c = list[i];
+    const u64 c = list[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += before(list[j].x, list[j].y, c.x, c.y);
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+      for (int z = 0; z < 8; ++z) rank += list[j + z] > c;
+    }
     if (rank < k) put(rank, c);
   }
 }
 
-// Entries (key, index) a list has to hold: in each of the four waves fewer than k lanes
-// have a key above the bound, `per` entries each, and k entries equal to it are kept.
-__host__ __device__ inline int list_cap(int k, int per) { return 4 * ((k - 1) * per + k); }
+// Entries a list has to hold in the ordered search: in each of the four waves fewer than k
+// lanes have a key above the bound, `per` entries each, and k entries equal to it are kept.
+__host__ __device__ inline int list_cap(int k, int per) { return 4 * ((k - 1) * per + k) + 8; }
+constexpr int kFast = 512;      // entries the list holds in the plain search
+constexpr int kFastGroups = 64;
 
+// (m, S, T) of one part of a row, joined with others' about the row's m.  r: d of x = m.
+struct Sums {
+  float m = -INFINITY, S = 0.f, T = 0.f;
+};
+__device__ __forceinline__ void join(Sums& row, const f32x4& part) {
+  // (a part of -inf alone has S = T = 0)
+  const float d = fmaxf((part[0] - row.m) * kLog2e, -1e30f) - part[3], f = fast_exp2(d);
+  row.S = fmaf(part[1], f, row.S);
+  row.T += f * fmaf(d, part[1], part[2]);
+}
+
+// The log of a row's sum, NaN where there is no distribution; writes the entropy and the
+// token's log probability (one thread).
 template <Dt DT>
-__global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
+__device__ __forceinline__ float finish_sums(const Args& a, int64_t row, const Sums& s, int64_t token, float xt) {
+  const bool fine = fabsf(s.m) < INFINITY && s.S == s.S;
+  const float log_s = fine ? logf(s.S) : __uint_as_float(0x7fc00000u);
+  if (threadIdx.x == 0) {
+    a.entropy[row] = log_s - s.T / s.S * 0.6931471805599453f;
+    a.logp[row] = token < 0 ? 0.f : token < a.cols ? xt - s.m - log_s : __uint_as_float(0x7fc00000u);
+  }
+  return log_s;
+}
+
+// The top k of a row from its group maxima, by a workgroup of four waves.
+template <Dt DT>
+__device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums& sums, float log_s,
+                                          const float* gmax, int n_groups, u64* list) {
   typedef Row<DT> R;
   constexpr int E = R::kE, kShift = R::kKeyShift, kBits = 32 - kShift;
-  extern __shared__ uint2 list[];
-  __shared__ u32 s_tau[4], s_n[2];
+  __shared__ uint2 s_tau[4];
+  __shared__ u32 s_n[4];
   __shared__ u32 s_group[kMaxTop], s_sorted[kMaxTop];
-  __shared__ uint2 s_best[4];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ u64 s_best[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const char* x = a.x + row * a.stride;
-  const int n_groups = a.n_seg * (kThreads / kGroup * kChunks);
-  const float* gmax = a.ws_max + row * n_groups;
-  const int64_t token = a.tokens[row];
-  const bool real = token >= 0 && token < a.cols;
-  const float xt = R::one(x + (real ? token : 0) * R::kEs);
-  if (tid < 2) s_n[tid] = 0;
+  const int k = a.top;
+  float* top_logp = a.top_logp + row * k;
+  int64_t* top_ids = a.top_ids + row * k;
+  auto key_of = [](float v) { return order_key(v) >> kShift; };
+  auto put = [&](int r, u64 c) {
+    top_logp[r] = key_float((u32)(c >> 32), kShift) - sums.m - log_s;
+    top_ids[r] = index_of(c);
+  };
 
-  // every wave joins the sums for itself
-  const f32x4* sums = reinterpret_cast<const f32x4*>(a.ws_sum) + row * a.n_seg * 4;
-  float m = -INFINITY, S = 0.f, T = 0.f;
-  for (int s = lane; s < a.n_seg * 4; s += 64) m = fmaxf(m, sums[s][0]);
-  m = wave_max(m);
-  for (int s = lane; s < a.n_seg * 4; s += 64) {
-    const f32x4 v = sums[s];
-    const float r = residue(v[0]);
-    // (a wave of -inf alone has S = T = 0)
-    const float d = fmaxf((v[0] - m) * kLog2e, -1e30f), f = fast_exp2(d - r);
-    S = fmaf(v[1], f, S);
-    T += f * fmaf(d - r, v[1], v[2]);
-  }
-  S = wave_sum(S);
-  T = wave_sum(T);
-  const bool fine = fabsf(m) < INFINITY && S == S;
-  const float log_s = fine ? logf(S) : __uint_as_float(0x7fc00000u);
-  if (tid == 0) {
-    a.entropy[row] = log_s - T / S * 0.6931471805599453f;
-    a.logp[row] = real ? xt - m - log_s : token < 0 ? 0.f : __uint_as_float(0x7fc00000u);
-  }
-  if (a.top == 0) return;
-  float* top_logp = a.top_logp + row * a.top;
-  int64_t* top_ids = a.top_ids + row * a.top;
-
-  if (!fine && !(m == -INFINITY && S == S)) {
+  if (!(sums.S == sums.S) || sums.m == INFINITY) {
     // a NaN or +inf somewhere: k selections over the row, by value and index
-    u32 lk = 0xffffffffu, li = 0;
-    for (int r = 0; r < a.top; ++r) {
-      u32 bk = 0, bi = 0xffffffffu;
+    u64 last = ~(u64)0;
+    for (int r = 0; r < k; ++r) {
+      u64 best = 0;
       for (int i = tid; i < a.cols; i += kThreads) {
-        const u32 key = order_key(R::one(x + (int64_t)i * R::kEs));
-        if ((r == 0 || before(lk, li, key, (u32)i)) && before(key, (u32)i, bk, bi)) {
-          bk = key;
-          bi = (u32)i;
-        }
+        const u64 e = entry(order_key(R::one(x + (int64_t)i * R::kEs)), (u32)i);
+        if ((r == 0 || e < last) && e > best) best = e;
       }
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) {
-        const u32 ok = __shfl_xor(bk, o), oi = __shfl_xor(bi, o);
-        if (before(ok, oi, bk, bi)) {
-          bk = ok;
-          bi = oi;
-        }
+        const u64 other = (u64)__shfl_xor((u32)(best >> 32), o) << 32 | (u32)__shfl_xor((u32)best, o);
+        best = max(best, other);
       }
-      if (lane == 0) s_best[wave] = make_uint2(bk, bi);
+      if (lane == 0) s_best[wave] = best;
       __syncthreads();
-      uint2 best = s_best[0];
-      for (int q = 1; q < 4; ++q)
-        if (before(s_best[q].x, s_best[q].y, best.x, best.y)) best = s_best[q];
-      lk = best.x;
-      li = best.y;
+      for (int q = 0; q < 4; ++q) best = max(best, s_best[q]);
+      last = best;
       if (tid == 0) {
         top_logp[r] = __uint_as_float(0x7fc00000u);
-        top_ids[r] = li;
+        top_ids[r] = index_of(best);
       }
       __syncthreads();
     }
     return;
   }
 
-  // In a wave, the k-th largest of the lanes' best keys has k entries at or above it; the
-  // largest such bound of the four waves bounds the row's k-th.
-  const int k = a.top;
-  auto bound = [&](u32 best) {
-    const u32 t = kth_of_wave(best, k, kBits);
+  if (tid < 4) s_n[tid] = 0;
+  constexpr int kHeld = 6;  // group maxima a thread keeps
+  u32 held[kHeld], best = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int g = tid + i * kThreads;
+    held[i] = g < n_groups ? key_of(gmax[g]) : 0;
+    best = max(best, held[i]);
+  }
+  for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) best = max(best, key_of(gmax[g]));
+
+  // A bound of the row's k-th largest from the lanes' best keys: in a wave the k-th
+  // largest has k entries at or above it, so the largest of the waves' holds; and so does
+  // the smallest of the (k / n)-th largest of n waves, which lies higher for values in no
+  // order (top 20 of four waves: some 30 of 256 lanes are above it, not 80).  The first
+  // keeps the lists short whatever the order.  `drop` low bits of the keys are left at 0.
+  auto bound = [&](u32 key, int n, int drop) {
+    const uint2 t = kth_of_wave(key, k, (k + n - 1) / n, kBits, drop);
     if (lane == 0) s_tau[wave] = t;
     __syncthreads();
-    return max(max(s_tau[0], s_tau[1]), max(s_tau[2], s_tau[3]));
+    u32 hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      hi = max(hi, s_tau[q].x);
+      if (q < n) lo = min(lo, s_tau[q].y);
+    }
+    return max(hi, lo);
   };
-  u32 best = 0;
-  for (int g = tid; g < n_groups; g += kThreads) best = max(best, order_key(gmax[g]) >> kShift);
-  u32 tau = bound(best);
-  u32 ties = 0;  // of this wave, in index order
-  for (int g0 = wave * 64; g0 < n_groups; g0 += kThreads) {
-    const int g = g0 + lane;
-    const u32 key = g < n_groups ? order_key(gmax[g]) >> kShift : 0;
-    if (g < n_groups && key > tau) list[atomicAdd(&s_n[0], 1u)] = make_uint2(key, g);
-    const unsigned long long eq = __ballot(g < n_groups && key == tau);
-    const u32 at = ties + __builtin_amdgcn_mbcnt_hi((u32)(eq >> 32), __builtin_amdgcn_mbcnt_lo((u32)eq, 0u));
-    if (g < n_groups && key == tau && at < (u32)k) list[atomicAdd(&s_n[0], 1u)] = make_uint2(key, g);
-    ties += (u32)__popcll(eq);
-  }
+
+  // Plain search: a bound to 16 bits, every group that reaches it, every value of those
+  // that reaches it, their ranks.  Some 1.5 k groups and 2 k values of a row in no order.
+  u32 tau = bound(best, min(4, n_groups / 64), kBits - 16);
+  auto list_group = [&](u32 key, u32 g) {
+    if (key >= tau) {
+      const u32 at = atomicAdd(&s_n[0], 1u);
+      if (at < (u32)kFastGroups) list[at] = g;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (__ballot(held[i] >= tau)) list_group(held[i], tid + i * kThreads);
+  for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) list_group(key_of(gmax[g]), g);
   __syncthreads();
+  const int mis = (int)((uintptr_t)x & 15) / R::kEs;
+  const u32 n_listed = s_n[0];
+  if (n_listed <= (u32)kFastGroups) {
+    constexpr int kFastPer = kFastGroups * kGroup / kThreads;
+    u32x4 w[kFastPer];
+    int64_t i0[kFastPer];
+#pragma unroll
+    for (int q = 0; q < kFastPer; ++q) {
+      const u32 c = tid + q * kThreads;
+      i0[q] = INT_MAX;
+      if (c / kGroup < n_listed) {
+        const int64_t ch = (int64_t)list[c / kGroup] * kGroup + c % kGroup;
+        i0[q] = ch * E - mis;
+        w[q] = R::chunk(x, mis, a.cols, ch);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kFastPer; ++q) {
+      if (q * (kThreads / kGroup) >= (int)n_listed) break;  // workgroup-uniform
+      float v[E];
+      R::unpack(w[q], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const u32 key = key_of(v[e]);
+        if (key >= tau && i0[q] + e >= 0 && i0[q] + e < a.cols) {
+          const u32 at = atomicAdd(&s_n[1], 1u);
+          if (at < (u32)kFast) list[at] = entry(key, (u32)(i0[q] + e));
+        }
+      }
+    }
+    __syncthreads();
+    const int n = (int)s_n[1];
+    if (n <= kFast) {
+      ranked(list, n, k, put);
+      return;
+    }
+  }
+
+  // Ordered search, for rows with many equal values (a mask of -inf) or values in order:
+  // exact bounds, and of the entries equal to a bound only the first k of each wave.
+  __syncthreads();
+  tau = bound(best, min(4, n_groups / 64), 0);
+  // This wave's entries above the bound go to the list in any order, of those equal to it
+  // the first k in index order (group g0 + lane, g0 rising).
+  auto each_group = [&](auto f) {
+    for (int g0 = wave * 64, i = 0; g0 < n_groups; g0 += kThreads, ++i) {
+      const int g = g0 + lane;
+      u32 key = 0;
+#pragma unroll
+      for (int z = 0; z < kHeld; ++z) key = i == z ? held[z] : key;
+      if (i >= kHeld && g < n_groups) key = key_of(gmax[g]);
+      f(key, (u32)g);
+    }
+  };
+  u32 above = 0, ties = 0;
+  each_group([&](u32 key, u32) {
+    above += (u32)__popcll(__ballot(key > tau));
+    ties += (u32)__popcll(__ballot(key == tau));
+  });
+  u32 at = 0;
+  if (lane == 0) at = atomicAdd(&s_n[2], above + min(ties, (u32)k));
+  at = __builtin_amdgcn_readfirstlane(at);
+  u32 tie_at = at + above;
+  const u32 tie_end = tie_at + min(ties, (u32)k);
+  each_group([&](u32 key, u32 g) {
+    const unsigned long long gt = __ballot(key > tau), eq = __ballot(key == tau);
+    const u32 pos = key > tau ? at + lanes_below(gt) : tie_at + lanes_below(eq);
+    if (key > tau || (key == tau && pos < tie_end)) list[pos] = entry(key, g);
+    at += (u32)__popcll(gt);
+    tie_at += (u32)__popcll(eq);
+  });
   if (tid < kMaxTop) s_group[tid] = 0xffffffffu;
   __syncthreads();
-  ranked(list, (int)s_n[0], k, [&](int r, uint2 c) { s_group[r] = c.y; });
+  ranked(list, (int)s_n[2], k, [&](int r, u64 c) { s_group[r] = index_of(c); });
   __syncthreads();
   // the k groups in index order, so that their values' lanes are in index order too
   if (tid < k) {
     int r = 0;
-    for (int j = 0; j < k; ++j) r += s_group[j] < s_group[tid] || (s_group[j] == s_group[tid] && j < tid);
+#pragma unroll
+    for (int j = 0; j < kMaxTop; ++j) r += s_group[j] < s_group[tid];
     s_sorted[r] = s_group[tid];
   }
   __syncthreads();
 
-  const int mis = (int)((uintptr_t)x & 15) / R::kEs;
   constexpr int kPer = kMaxTop * kGroup / kThreads;  // chunks a thread
   u32x4 w[kPer];
   int64_t i0[kPer];
@@ -334,7 +509,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
   for (int q = 0; q < kPer; ++q) {
     const int c = tid + q * kThreads;  // a wave's chunks: groups in order
     i0[q] = INT_MAX;
-    if (c < k * kGroup && s_sorted[c / kGroup] != 0xffffffffu) {
+    if (c < k * kGroup) {
       const int64_t ch = (int64_t)s_sorted[c / kGroup] * kGroup + c % kGroup;
       w[q] = R::chunk(x, mis, a.cols, ch);
       i0[q] = ch * E - mis;
@@ -342,57 +517,89 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
       R::unpack(w[q], v);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (i0[q] + e >= 0 && i0[q] + e < a.cols) best = max(best, order_key(v[e]) >> kShift);
+        if (i0[q] + e >= 0 && i0[q] + e < a.cols) best = max(best, key_of(v[e]));
     }
   }
-  tau = bound(best);
-  ties = 0;
+  tau = bound(best, min(4, (k * kGroup + 63) / 64), 0);
+  // Per lane: values above the bound (11 bits), ties in each of the two chunks (10 bits
+  // each, of at most 8 x 64); one scan over the wave gives every lane its places.
+  static_assert(kPer <= 2, "two counts of ties");
+  u32 key[kPer][E], count = 0;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
-    if (__ballot(i0[q] < a.cols) == 0) continue;
-    u32 key[E], mine = 0;
     float v[E];
     R::unpack(w[q], v);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const bool in = i0[q] + e >= 0 && i0[q] + e < a.cols;
-      key[e] = in ? order_key(v[e]) >> kShift : 0;
-      if (in && key[e] > tau) list[atomicAdd(&s_n[1], 1u)] = make_uint2(key[e], (u32)(i0[q] + e));
-      mine += in && key[e] == tau;
+      key[q][e] = in ? key_of(v[e]) : 0;
+      count += key[q][e] > tau ? 1u : 0u;
+      count += in && key[q][e] == tau ? 1u << (11 + 10 * q) : 0u;
     }
-    u32 incl = mine;
+  }
+  u32 incl = count;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u32 t = __shfl_up(incl, o);
-      if (lane >= o) incl += t;
-    }
-    u32 at = ties + incl - mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const u32 t = __shfl_up(incl, o);
+    if (lane >= o) incl += t;
+  }
+  const u32 all = __builtin_amdgcn_readlane(incl, 63), mine = incl - count;
+  above = all & 0x7ffu;
+  ties = min((all >> 11 & 0x3ffu) + (all >> 21), (u32)k);
+  at = 0;
+  if (lane == 0) at = atomicAdd(&s_n[3], above + ties);
+  at = __builtin_amdgcn_readfirstlane(at);
+  u32 pos = at + (mine & 0x7ffu);
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    u32 tie = q == 0 ? mine >> 11 & 0x3ffu : (all >> 11 & 0x3ffu) + (mine >> 21);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const bool in = i0[q] + e >= 0 && i0[q] + e < a.cols;
-      if (in && key[e] == tau && at++ < (u32)k) list[atomicAdd(&s_n[1], 1u)] = make_uint2(key[e], (u32)(i0[q] + e));
+      if (key[q][e] > tau) list[pos++] = entry(key[q][e], (u32)(i0[q] + e));
+      if (in && key[q][e] == tau) {
+        if (tie < ties) list[at + above + tie] = entry(key[q][e], (u32)(i0[q] + e));
+        ++tie;
+      }
     }
-    ties += __shfl(incl, 63);
   }
   __syncthreads();
-  ranked(list, (int)s_n[1], k, [&](int r, uint2 c) {
-    top_logp[r] = R::one(x + (int64_t)c.y * R::kEs) - m - log_s;
-    top_ids[r] = c.y;
-  });
+  ranked(list, (int)s_n[3], k, put);
+}
+
+template <Dt DT>
+__global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
+  typedef Row<DT> R;
+  extern __shared__ u64 list[];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int n_groups = a.n_seg * (kSegChunks / kGroup);
+  const int64_t token = a.tokens[row];
+  const float xt = R::one(a.x + row * a.stride + (token >= 0 && token < a.cols ? token : 0) * R::kEs);
+  // every wave joins the sums for itself
+  const f32x4* parts = reinterpret_cast<const f32x4*>(a.ws_sum) + row * a.n_seg * 4;
+  Sums s;
+  for (int i = lane; i < a.n_seg * 4; i += 64) s.m = fmaxf(s.m, parts[i][0]);
+  s.m = wave_max(s.m);
+  for (int i = lane; i < a.n_seg * 4; i += 64) join(s, parts[i]);
+  s.S = wave_sum(s.S);
+  s.T = wave_sum(s.T);
+  const float log_s = finish_sums<DT>(a, row, s, token, xt);
+  if (a.top > 0) write_top<DT>(a, row, s, log_s, a.ws_max + row * n_groups, n_groups, list);
 }
 
 static int seg_of(int64_t cols, int es) {
   const int e = 16 / es;
   // the row may start anywhere within its first chunk
-  return (int)cdiv(cols + 2 * (e - 1), (int64_t)e * kThreads * kChunks);
+  return (int)cdiv(cols + 2 * (e - 1), (int64_t)e * kSegChunks);
 }
 
 template <Dt DT> static void launch(const Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((logprobs_segment_kernel<DT>), dim3((unsigned)(a.n_rows * a.n_seg)), dim3(kThreads), 0, s, a);
-  // group maxima a lane of the second launch, or chunks' elements
-  const int per = std::max(a.n_seg * (kThreads / kGroup * kChunks) / kThreads + 1,
+  // group maxima a lane of the second launch goes through, or its chunks' elements
+  const int per = std::max(a.n_seg * (kSegChunks / kGroup) / kThreads + 1,
                            kMaxTop * kGroup / kThreads * Row<DT>::kE);
-  const size_t lds = a.top ? (size_t)list_cap(a.top, per) * sizeof(uint2) : 0;
+  const size_t lds = a.top ? (size_t)std::max(list_cap(a.top, per), kFast + 8) * sizeof(u64) : 0;
+  hipLaunchKernelGGL((logprobs_segment_kernel<DT>), dim3((unsigned)(a.n_rows * a.n_seg)), dim3(kThreads), 0, s, a);
   hipLaunchKernelGGL((logprobs_merge_kernel<DT>), dim3((unsigned)a.n_rows), dim3(kThreads), lds, s, a);
 }
 
