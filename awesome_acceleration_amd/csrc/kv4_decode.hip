@@ -37,6 +37,7 @@ namespace kv4 {
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
+typedef unsigned long long u64;
 
 constexpr float kRescale = 8.f;  // probabilities up to 2^8 before the reference moves
 
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
 
   // Q operand: query n's dims 32 j + 8 i .. + 7 for product i, in NT terms
   const bool flip = a.scale_log2 < 0.f;  // -q and -scale: the largest product has the largest score
-  const float cs = fabsf(a.scale_log2);
+  const float cs = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: equal scores)
   u32x4 qf[NT][4];
   {
     const bool row = n < a.g;
@@ -151,82 +152,108 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     }
   }
 
-  const int32_t* table = a.block_tables + (int64_t)b * a.max_blocks;
-  const int64_t pb = a.c.page_bytes();
+  // Addresses are a scalar base for each tile, from the block number, and offsets that
+  // each lane keeps.
+  typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
+  const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
+  const u32 pb = (u32)a.c.page_bytes();
   const int tpb = a.c.block_size / kTile;
   const int last_tile = (end - 1) / kTile;
-  auto load = [&](int t0, Raw& r) {
+  const u32 voff = n * kRowBytes + 16 * j, soff = n * kScaleBytes + j;
+  struct Where {
+    int block[2], row[2];  // of two tiles: table entry, first row in the block
+  };
+  auto look = [&](int t0) {
+    Where w;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int tile = min(t0 / kTile + s, last_tile);
-      const int bi = (int)((tile * a.magic) >> a.shift);
-      int blk = table[bi];
-      blk = blk < 0 || blk >= a.c.num_blocks ? 0 : blk;
+      const int tile = min(t0 / kTile + s, last_tile);  // past the end: the last again
+      const int bi = (int)(((u64)(u32)tile * a.magic) >> a.shift);
+      w.block[s] = table[bi];
+      w.row[s] = (tile - bi * tpb) * kTile;
+    }
+    return w;
+  };
+  auto load = [&](const Where& w, Raw& r) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32 blk = (u32)w.block[s] < (u32)a.c.num_blocks ? (u32)w.block[s] : 0u;
       const unsigned char* page = a.c.page(blk, h);
-      const int row = (tile - bi * tpb) * kTile + n;
-      const unsigned char* p = page + row * kRowBytes + 16 * j;
-      const unsigned char* ps = page + a.c.block_size * kRowBytes + row * kScaleBytes + j;
-      r.k[s] = *reinterpret_cast<const u32x4*>(p);
-      r.v[s] = *reinterpret_cast<const u32x4*>(p + pb);
-      r.ks[s] = *ps;
-      r.vs[s] = ps[pb];
+      const unsigned char* p = page + (u32)w.row[s] * kRowBytes;
+      const unsigned char* ps = page + (u32)(a.c.block_size * kRowBytes + w.row[s] * kScaleBytes);
+      r.k[s] = *reinterpret_cast<const u32x4*>(p + voff);
+      r.v[s] = *reinterpret_cast<const u32x4*>(p + pb + voff);
+      r.ks[s] = ps[soff];
+      r.vs[s] = (ps + pb)[soff];
     }
   };
 
   lds_u8* vb = (lds_u8*)lds + wave * kWaveLds;
   // writes: token n's dims 32 j + 8 i at chunk 2 j + i / 2; reads: this quarter's
   // tokens 4 j + (n >> 2), dims 16 d + 4 (n & 3)
-  const int rt = 4 * j + (n >> 2);
+  const int wt = n * 256 + ((2 * j ^ (n & 7)) << 5);
+  const int rt = 4 * j + (n >> 2), rd = rt * 256 + ((rt & 7) << 5) + 8 * (n & 3);
   f32x4 o[8];
 #pragma unroll
   for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // reference of the exponents (the running maximum, 0 while that is -inf), lane-partial sum
+  // running maximum of q . k, the exponents' reference (cs times it; 0 while it is -inf),
+  // lane-partial sum
   float m = -INFINITY, ref = 0.f, l = 0.f;
+  const float margin = kRescale / cs;
 
-  for (int t0 = beg + 32 * wave; t0 < end; t0 += 128) {
-    Raw r;
-    load(t0, r);
-    float s[8];
+  Raw r;
+  int t0 = beg + 32 * wave;
+  Where ahead = look(t0);  // (past the end: a tile of the partition all the same)
+  load(ahead, r);
+  ahead = look(t0 + 128);
+  for (; t0 < end; t0 += 128) {
+    Raw next;
+    load(ahead, next);
+    ahead = look(t0 + 256);
+    f32x4 s[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      s[k] = f32x4{0.f, 0.f, 0.f, 0.f};
       const float sc = __uint_as_float(r.ks[k] << 23);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const u32x4 kf = values8(r.k[k][i], sc);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc = mfma(kf, qf[t][i], acc);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[4 * k + i] = acc[i] * cs;
-        if (t0 + 16 * k + 4 * j + i >= end) s[4 * k + i] = -INFINITY;
+        for (int t = 0; t < NT; ++t) s[k] = mfma(kf, qf[t][i], s[k]);
       }
     }
-    // V to LDS: rows past the end stand for nothing (their bytes may stand for NaN)
+    if (t0 + 32 > end) {  // the last step: rows past the end stand for nothing
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t0 + 16 * k + 4 * j + i >= end) s[k][i] = -INFINITY;
+        if (t0 + 16 * k + n >= end) {  // (their bytes may stand for NaN)
+          r.v[k] = u32x4{0, 0, 0, 0};
+          r.vs[k] = 127;
+        }
+      }
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const bool in = t0 + 16 * k + n < end;
-      const float sc = in ? __uint_as_float(r.vs[k] << 23) : 1.f;
+      const float sc = __uint_as_float(r.vs[k] << 23);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4 w = values8(in ? r.v[k][i] : 0u, sc);
-        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(
-            vb + (16 * k + n) * 256 + ((2 * j + (i >> 1)) ^ (n & 7)) * 32 + (i & 1) * 16) = w;
-      }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wt ^ (i >> 1) * 32) + k * 4096 + (i & 1) * 16) =
+            values8(r.v[k][i], sc);
     }
-    float mx = vmax3(s[0], s[1], s[2]);
-    mx = vmax3(mx, s[3], s[4]);
-    mx = vmax3(mx, s[5], s[6]);
-    mx = vmax(mx, s[7]);
-    if (__ballot(mx > m + kRescale)) {
+    float mx = vmax3(s[0][0], s[0][1], s[0][2]);
+    mx = vmax3(mx, s[0][3], s[1][0]);
+    mx = vmax3(mx, s[1][1], s[1][2]);
+    mx = vmax(mx, s[1][3]);
+    if (__ballot(mx > m + margin)) {
       mx = vmax(mx, __shfl_xor(mx, 16));
       mx = vmax(mx, __shfl_xor(mx, 32));
-      const float mn = vmax(m, mx), alpha = fast_exp2(m - mn);
-      // (m = -inf: nothing is summed yet)
-      const float f = m == -INFINITY ? 0.f : alpha;
-      m = mn;
-      ref = mn == -INFINITY ? 0.f : mn;
+      const bool none = m == -INFINITY;  // nothing is summed yet
+      m = vmax(m, mx);
+      const float to = m == -INFINITY ? 0.f : m * cs;
+      const float f = none ? 0.f : fast_exp2(ref - to);
+      ref = to;
       l *= f;
 #pragma unroll
       for (int d = 0; d < 8; ++d)
@@ -236,7 +263,8 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     u32x4 pf[NT];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float x = fast_exp2(s[2 * w] - ref), y = fast_exp2(s[2 * w + 1] - ref);
+      float x = fast_exp2(fmaf(s[w >> 1][2 * (w & 1)], cs, -ref));
+      float y = fast_exp2(fmaf(s[w >> 1][2 * (w & 1) + 1], cs, -ref));
       if constexpr (NT == 1) {
         pf[0][w] = Elem<Dt::BF16>::pack2_hw(x, y);
         l = Elem<Dt::BF16>::dot2(pf[0][w], Elem<Dt::BF16>::kOnes, l);
@@ -249,15 +277,15 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
-      const int at = rt * 256 + ((d ^ (rt & 7)) * 32) + 8 * (n & 3);
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + at));
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + at + 16 * 256));
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32)));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32) + 16 * 256));
       const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
       const u32x4 vf = {a0[0], a0[1], a1[0], a1[1]};
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[d] = mfma(vf, pf[t], o[d]);
     }
     asm volatile("" ::: "memory");
+    r = next;
   }
 
   // merge the waves
@@ -270,7 +298,8 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     for (int d = 0; d < 8; ++d)
       *reinterpret_cast<f32x4*>(so + (wave * 16 + n) * kDim + 16 * d + 4 * j) = o[d];
     if (j == 0) {
-      sm_m[wave][n] = m;
+      // the sums' reference; a wave without a token has none
+      sm_m[wave][n] = m == -INFINITY ? -INFINITY : ref;
       sm_l[wave][n] = l;
     }
   }
