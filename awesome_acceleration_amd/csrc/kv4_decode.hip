@@ -59,10 +59,11 @@ struct DecArgs {
   // tile number -> block: (tile * magic) >> shift
   uint64_t magic;
   int32_t shift;
+  int32_t cap_tiles;  // of the tables
 };
 
-__device__ __forceinline__ int context_len(const DecArgs& a, int b) {
-  const int64_t ctx = (int64_t)a.lens[b] + a.lens_add, cap = (int64_t)a.max_blocks * a.c.block_size;
+__device__ __forceinline__ int context_len(const DecArgs& a, int len) {
+  const int64_t ctx = (int64_t)len + a.lens_add, cap = (int64_t)a.max_blocks * a.c.block_size;
   return (int)(ctx < 0 ? 0 : ctx > cap ? cap : ctx);
 }
 __device__ __forceinline__ int parts_of(const DecArgs& a, int ctx) {
@@ -90,22 +91,48 @@ __device__ __forceinline__ u32x4 values8(u32 w, float scale) {
                __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
 }
 
-// one step's codes and scale bytes of a lane, K and V of two tiles
+// One step's codes of a lane, K and V of four tiles, and the scales of one token each.
 struct Raw {
-  u32x4 k[2], v[2];
-  u32 ks[2], vs[2];
+  u32x4 k[4], v[4];
+  u32 ks, vs;
 };
 
-template <Dt DT>
-__global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel(DecArgs a) {
+constexpr int kStep = 64;      // tokens of a step
+constexpr int kLoadAux = 2;  // non-temporal: nothing reads the rows again
+
+// WIDE: block sizes are a multiple of a step, so that a step lies in one block.
+template <Dt DT, bool WIDE>
+__global__ __launch_bounds__(256, DT == Dt::BF16 ? 3 : 2) void kv4_decode_kernel(DecArgs a) {
   constexpr int NT = DT == Dt::BF16 ? 1 : DT == Dt::FP16 ? 2 : 3;
   constexpr int kWaveLds = 32 * 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kWaveLds];
+  __shared__ u32 s_scale[4][2][kStep];
   __shared__ float sm_m[4][16], sm_l[4][16];
   const int h = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ctx = context_len(a, b);
+  // The waves take steps in turn.  A wave's first table entry does not depend on the
+  // context's length, so both are on their way together.
+  typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
+  const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
+  const int beg = part * a.part_tokens, t_first = beg + kStep * wave;
+  const int tpb = a.c.block_size / kTile;
+  constexpr int kLooks = WIDE ? 1 : 4;
+  struct Where {
+    int block[kLooks], row[kLooks];  // of a step's tiles: table entry, first row in the block
+  };
+  auto look = [&](int t0, int tiles, Where& w) {
+#pragma unroll
+    for (int k = 0; k < kLooks; ++k) {
+      const int tile = min(t0 / kTile + k, tiles - 1);  // past the end: the last again
+      const int bi = (int)(((u64)(u32)tile * a.magic) >> a.shift);
+      w.block[k] = table[bi];
+      w.row[k] = (tile - bi * tpb) * kTile;
+    }
+  };
+  Where w;
+  look(t_first, a.cap_tiles, w);
+  const int ctx = context_len(a, ((const cint*)(uintptr_t)a.lens)[b]);
   const int np = parts_of(a, ctx);
   if (part >= np) {  // workgroup-uniform
     if (part == 0) {  // an empty context
@@ -114,21 +141,60 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     }
     return;
   }
-  const int beg = part * a.part_tokens, end = min(ctx, beg + a.part_tokens);
+  const int end = min(ctx, beg + a.part_tokens), n_tiles = (end + kTile - 1) / kTile;
+
+  // A buffer of each tile's pages (K, then V) from the block number, and offsets that each
+  // lane keeps.  Past the end the buffer is empty: the loads are issued all the same, so
+  // that the number in flight is known, and read nothing.
+  const int pb = (int)a.c.page_bytes();
+  const int voff = n * kRowBytes + 16 * j;
+  auto page_of = [&](int block) { return a.c.page((u32)block < (u32)a.c.num_blocks ? (u32)block : 0u, h); };
+  auto load_codes = [&](int t0, const Where& w, int k, bool v) {
+    const __amdgpu_buffer_rsrc_t page = __builtin_amdgcn_make_buffer_rsrc(
+        page_of(w.block[WIDE ? 0 : k]), 0, t0 + (WIDE ? 0 : kTile * k) < end ? 2 * pb : 0, 0x00020000);
+    const int row = WIDE ? w.row[0] + kTile * k : w.row[k];
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                         page, voff, (v ? pb : 0) + row * kRowBytes, kLoadAux));
+  };
+  // lane l: the four scales of token l of the step (of the last tile's past the end)
+  auto load_scales = [&](const Where& w, Raw& r) {
+    uint64_t at = 0;
+#pragma unroll
+    for (int k = 0; k < kLooks; ++k) {
+      const uint64_t t = (uint64_t)page_of(w.block[k]) + (u32)(a.c.block_size * kRowBytes + w.row[k] * kScaleBytes);
+      at = k == 0 || j == k ? t : at;
+    }
+    // (a global address: a flat load would also count as an LDS access)
+    typedef const __attribute__((address_space(1))) u32 gu32;
+    const uint64_t p = at + (u32)((WIDE ? lane : n) * kScaleBytes);
+    r.ks = __builtin_nontemporal_load((gu32*)p);
+    r.vs = __builtin_nontemporal_load((gu32*)(p + (u32)pb));
+  };
+  // One buffer of rows: those of the next step are asked for where this step's have been
+  // taken.
+  Raw r;
+  look(t_first, n_tiles, w);
+  load_scales(w, r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    r.k[k] = load_codes(t_first, w, k, false);
+    r.v[k] = load_codes(t_first, w, k, true);
+  }
 
   // Q operand: query n's dims 32 j + 8 i .. + 7 for product i, in NT terms
-  const bool flip = a.scale_log2 < 0.f;  // -q and -scale: the largest product has the largest score
+  // (a negative scale: -q and -scale, so that the largest product has the largest score)
   const float cs = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: equal scores)
   u32x4 qf[NT][4];
   {
     const bool row = n < a.g;
+    const u32 flip = a.scale_log2 < 0.f ? 0x80000000u : 0u, keep = row ? 0xffffffffu : 0u;
     const int64_t at = (int64_t)b * a.q_stride + (int64_t)(h * a.g + (row ? n : 0)) * kDim + 32 * j;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (DT == Dt::BF16) {
-        u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const u16*>(a.q) + at + 8 * i);
+        const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const u16*>(a.q) + at + 8 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qf[0][i][e] = row ? (flip ? w[e] ^ 0x80008000u : w[e]) : 0u;
+        for (int e = 0; e < 4; ++e) qf[0][i][e] = (w[e] ^ (flip | flip >> 16)) & keep;
       } else {
         float x[8];
         if constexpr (DT == Dt::FP16) {
@@ -143,7 +209,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
           }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = row ? (flip ? -x[e] : x[e]) : 0.f;
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) ^ flip) & keep);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -152,47 +218,12 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     }
   }
 
-  // Addresses are a scalar base for each tile, from the block number, and offsets that
-  // each lane keeps.
-  typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
-  const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
-  const u32 pb = (u32)a.c.page_bytes();
-  const int tpb = a.c.block_size / kTile;
-  const int last_tile = (end - 1) / kTile;
-  const u32 voff = n * kRowBytes + 16 * j, soff = n * kScaleBytes + j;
-  struct Where {
-    int block[2], row[2];  // of two tiles: table entry, first row in the block
-  };
-  auto look = [&](int t0) {
-    Where w;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int tile = min(t0 / kTile + s, last_tile);  // past the end: the last again
-      const int bi = (int)(((u64)(u32)tile * a.magic) >> a.shift);
-      w.block[s] = table[bi];
-      w.row[s] = (tile - bi * tpb) * kTile;
-    }
-    return w;
-  };
-  auto load = [&](const Where& w, Raw& r) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const u32 blk = (u32)w.block[s] < (u32)a.c.num_blocks ? (u32)w.block[s] : 0u;
-      const unsigned char* page = a.c.page(blk, h);
-      const unsigned char* p = page + (u32)w.row[s] * kRowBytes;
-      const unsigned char* ps = page + (u32)(a.c.block_size * kRowBytes + w.row[s] * kScaleBytes);
-      r.k[s] = *reinterpret_cast<const u32x4*>(p + voff);
-      r.v[s] = *reinterpret_cast<const u32x4*>(p + pb + voff);
-      r.ks[s] = ps[soff];
-      r.vs[s] = (ps + pb)[soff];
-    }
-  };
-
   lds_u8* vb = (lds_u8*)lds + wave * kWaveLds;
-  // writes: token n's dims 32 j + 8 i at chunk 2 j + i / 2; reads: this quarter's
-  // tokens 4 j + (n >> 2), dims 16 d + 4 (n & 3)
-  const int wt = n * 256 + ((2 * j ^ (n & 7)) << 5);
-  const int rt = 4 * j + (n >> 2), rd = rt * 256 + ((rt & 7) << 5) + 8 * (n & 3);
+  // writes: token n's dims 32 j + 8 i, 16-byte slot 4 j + i of its row; reads: this
+  // quarter's tokens 4 j + (n >> 2), dims 16 d + 4 (n & 3), slot 2 d + (n & 3) / 2
+  auto swizzle = [](int row) { return ((row & 7) << 1) | (row >> 3); };
+  const int wt = n * 256 + ((4 * j ^ swizzle(n)) << 4);
+  const int rt = 4 * j + (n >> 2), rd = rt * 256 + ((((n & 3) >> 1) ^ swizzle(rt)) << 4) + 8 * (n & 1);
   f32x4 o[8];
 #pragma unroll
   for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -201,51 +232,53 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   float m = -INFINITY, ref = 0.f, l = 0.f;
   const float margin = kRescale / cs;
 
-  Raw r;
-  int t0 = beg + 32 * wave;
-  Where ahead = look(t0);  // (past the end: a tile of the partition all the same)
-  load(ahead, r);
-  ahead = look(t0 + 128);
-  for (; t0 < end; t0 += 128) {
-    Raw next;
-    load(ahead, next);
-    ahead = look(t0 + 256);
-    f32x4 s[2];
+  look(t_first + 4 * kStep, n_tiles, w);
+  // The scales have arrived before the loop: with them among the loads under way at its
+  // entry, the compiler waits for every load at its top (the counts of both ways in
+  // have to agree).
+  asm volatile("" : "+v"(r.ks), "+v"(r.vs));
+  __attribute__((address_space(3))) u32* sc = (__attribute__((address_space(3))) u32*)&s_scale[wave][0][0];
+  const __attribute__((address_space(3))) unsigned char* sc8 =
+      (const __attribute__((address_space(3))) unsigned char*)&s_scale[wave][0][0] + n * kScaleBytes + j;
+  for (int t0 = t_first; t0 < end; t0 += 4 * kStep) {
+    sc[lane] = r.ks;
+    sc[kStep + lane] = r.vs;
+    asm volatile("" ::: "memory");
+    load_scales(w, r);
+    f32x4 s[4];
+    u32 vs[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k) {
       s[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const float sc = __uint_as_float(r.ks[k] << 23);
+      const float ks = __uint_as_float((u32)sc8[k * 64] << 23);
+      vs[k] = sc8[kStep * kScaleBytes + k * 64];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u32x4 kf = values8(r.k[k][i], sc);
+        const u32x4 kf = values8(r.k[k][i], ks);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[k] = mfma(kf, qf[t][i], s[k]);
+        for (int x = 0; x < NT; ++x) s[k] = mfma(kf, qf[x][i], s[k]);
       }
+      // (kept here: asked for earlier, the rows need registers of their own and a copy)
+      __builtin_amdgcn_sched_barrier(0);
+      r.k[k] = load_codes(t0 + 4 * kStep, w, k, false);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (t0 + 32 > end) {  // the last step: rows past the end stand for nothing
+    if (t0 + kStep > end) {  // the last rows: those past the end stand for nothing
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (t0 + 16 * k + 4 * j + i >= end) s[k][i] = -INFINITY;
         if (t0 + 16 * k + n >= end) {  // (their bytes may stand for NaN)
           r.v[k] = u32x4{0, 0, 0, 0};
-          r.vs[k] = 127;
+          vs[k] = 127;
         }
       }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float sc = __uint_as_float(r.vs[k] << 23);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wt ^ (i >> 1) * 32) + k * 4096 + (i & 1) * 16) =
-            values8(r.v[k][i], sc);
-    }
-    float mx = vmax3(s[0][0], s[0][1], s[0][2]);
-    mx = vmax3(mx, s[0][3], s[1][0]);
-    mx = vmax3(mx, s[1][1], s[1][2]);
-    mx = vmax(mx, s[1][3]);
+    float mx = vmax3(vmax3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
+    mx = vmax3(vmax3(mx, s[1][1], s[1][2]), s[1][3], s[2][0]);
+    mx = vmax3(vmax3(mx, s[2][1], s[2][2]), s[2][3], s[3][0]);
+    mx = vmax(vmax3(mx, s[3][1], s[3][2]), s[3][3]);
     if (__ballot(mx > m + margin)) {
       mx = vmax(mx, __shfl_xor(mx, 16));
       mx = vmax(mx, __shfl_xor(mx, 32));
@@ -260,32 +293,49 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[d][i] *= f;
     }
-    u32x4 pf[NT];
+    u32x4 pf[2][NT];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float x = fast_exp2(fmaf(s[w >> 1][2 * (w & 1)], cs, -ref));
-      float y = fast_exp2(fmaf(s[w >> 1][2 * (w & 1) + 1], cs, -ref));
-      if constexpr (NT == 1) {
-        pf[0][w] = Elem<Dt::BF16>::pack2_hw(x, y);
-        l = Elem<Dt::BF16>::dot2(pf[0][w], Elem<Dt::BF16>::kOnes, l);
-      } else {
-        l += x + y;
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) pf[t][w] = take_bf16(x, y);
+      for (int e = 0; e < 2; ++e) {
+        u32x4* const p = pf[k >> 1];
+        const int at = 2 * (k & 1) + e;
+        float x = fast_exp2(fmaf(s[k][2 * e], cs, -ref)), y = fast_exp2(fmaf(s[k][2 * e + 1], cs, -ref));
+        if constexpr (NT == 1) {
+          p[0][at] = Elem<Dt::BF16>::pack2_hw(x, y);
+          l = Elem<Dt::BF16>::dot2(p[0][at], Elem<Dt::BF16>::kOnes, l);
+        } else {
+          l += x + y;
+#pragma unroll
+          for (int c = 0; c < NT; ++c) p[c][at] = take_bf16(x, y);
+        }
       }
-    }
-    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32)));
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32) + 16 * 256));
-      const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
-      const u32x4 vf = {a0[0], a0[1], a1[0], a1[1]};
+    for (int q = 0; q < 2; ++q) {  // 32 tokens
 #pragma unroll
-      for (int t = 0; t < NT; ++t) o[d] = mfma(vf, pf[t], o[d]);
+      for (int k = 0; k < 2; ++k) {
+        const float sv = __uint_as_float(vs[2 * q + k] << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wt ^ i * 16) + k * 4096) =
+              values8(r.v[2 * q + k][i], sv);
+        __builtin_amdgcn_sched_barrier(0);
+        r.v[2 * q + k] = load_codes(t0 + 4 * kStep, w, 2 * q + k, true);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32)));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32) + 16 * 256));
+        const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
+        const u32x4 vf = {a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+        for (int c = 0; c < NT; ++c) o[d] = mfma(vf, pf[q][c], o[d]);
+      }
+      asm volatile("" ::: "memory");
     }
-    asm volatile("" ::: "memory");
-    r = next;
+    look(t0 + 8 * kStep, n_tiles, w);
   }
 
   // merge the waves
@@ -333,7 +383,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
 
 template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArgs a) {
   const int hq = blockIdx.x, b = blockIdx.y;
-  const int np = parts_of(a, context_len(a, b));
+  const int np = parts_of(a, context_len(a, a.lens[b]));
   if (np <= 1) return;
   combine_partitions<DT>(a.ws_o, a.ws_lse, ((int64_t)b * a.hq + hq) * a.n_parts, np, a.out,
                          (int64_t)b * a.out_stride + (int64_t)hq * kDim);
@@ -370,7 +420,11 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
 }
 
 template <Dt DT> static void launch(const DecArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((kv4_decode_kernel<DT>), dim3(a.c.hkv, a.n_parts, a.n_seqs), dim3(256), 0, s, a);
+  const dim3 grid(a.c.hkv, a.n_parts, a.n_seqs);
+  if (a.c.block_size % kStep == 0)
+    hipLaunchKernelGGL((kv4_decode_kernel<DT, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv4_decode_kernel<DT, false>), grid, dim3(256), 0, s, a);
   if (a.n_parts > 1)
     hipLaunchKernelGGL((kv4_reduce_kernel<DT>), dim3(a.hq, a.n_seqs), dim3(256), 0, s, a);
 }
@@ -442,6 +496,7 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* c
   const int l = d == 1 ? 0 : 32 - __builtin_clz(d - 1);
   a.magic = (uint64_t(1) << (27 + l)) / d + 1;
   a.shift = 27 + l;
+  a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, (1 << 27) - 1);
   if (p.ws_bytes) {
     a.ws_o = reinterpret_cast<float*>(workspace);
     a.ws_lse = a.ws_o + (size_t)n_seqs * n_q_heads * p.n_parts * kv4::kDim;
