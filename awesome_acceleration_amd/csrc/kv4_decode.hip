@@ -124,7 +124,9 @@ __global__ __launch_bounds__(256, DT == Dt::BF16 ? 3 : 2) void kv4_decode_kernel
   auto look = [&](int t0, int tiles, Where& w) {
 #pragma unroll
     for (int k = 0; k < kLooks; ++k) {
-      const int tile = min(t0 / kTile + k, tiles - 1);  // past the end: the last again
+      // past the end: the last again (its first tile where one look serves a whole step,
+      // whose rows then all lie in the block)
+      const int tile = min(t0 / kTile + k, WIDE ? (tiles - 1) & ~(kStep / kTile - 1) : tiles - 1);
       const int bi = (int)(((u64)(u32)tile * a.magic) >> a.shift);
       w.block[k] = table[bi];
       w.row[k] = (tile - bi * tpb) * kTile;

@@ -263,6 +263,20 @@ def test_attention_is_the_same_on_every_run_and_stream(gpu):
         assert torch.equal(o, first)
 
 
+def test_attention_ends_with_the_cache(gpu):
+    """Contexts that end inside the pool's last block, whose pages end where the cache does,
+    in a cache of whole 2 MiB pages: what a step asks for past its end lies in the block."""
+    print("case: cache of 34 x 2 MiB", flush=True)
+    n, hkv, bs = 256, 8, 256
+    assert n * hkv * 2 * bs * 68 == 34 << 21
+    cache = torch.zeros((n, hkv, 2, bs * 68), dtype=torch.uint8, device=gpu)
+    tables = torch.arange(n, dtype=torch.int32, device=gpu)[:, None]
+    q = torch.ones((n, 16, 128), dtype=torch.bfloat16, device=gpu)
+    for ctx in (250, 193, 1):
+        out = kv4.decode_paged_kv4(q, cache, tables, torch.full((n,), ctx, dtype=torch.int32, device=gpu))
+        assert (out == 0).all()
+
+
 def test_attention_of_no_sequence(gpu):
     c = _case(gpu, [5], 4, 2, 16, "bf16", 13)
     out = kv4.decode_paged_kv4(c["q"][:0], c["gcache"], c["gtables"][:0], c["ctx"][:0])
