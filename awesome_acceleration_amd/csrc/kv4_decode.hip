@@ -102,7 +102,7 @@ constexpr int kLoadAux = 2;  // non-temporal: nothing reads the rows again
 
 // WIDE: block sizes are a multiple of a step, so that a step lies in one block.
 template <Dt DT, bool WIDE>
-__global__ __launch_bounds__(256, DT == Dt::BF16 ? 3 : 2) void kv4_decode_kernel(DecArgs a) {
+__global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel(DecArgs a) {
   constexpr int NT = DT == Dt::BF16 ? 1 : DT == Dt::FP16 ? 2 : 3;
   constexpr int kWaveLds = 32 * 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kWaveLds];
@@ -314,12 +314,15 @@ __global__ __launch_bounds__(256, DT == Dt::BF16 ? 3 : 2) void kv4_decode_kernel
       }
 #pragma unroll
     for (int q = 0; q < 2; ++q) {  // 32 tokens
+      // (fp16: the addresses formed anew, 16 registers for a third workgroup per CU)
+      int wo = wt, ro = rd;
+      if constexpr (NT == 2) asm volatile("" : "+v"(wo), "+v"(ro));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float sv = __uint_as_float(vs[2 * q + k] << 23);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wt ^ i * 16) + k * 4096) =
+          *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wo ^ i * 16) + k * 4096) =
               values8(r.v[2 * q + k][i], sv);
         __builtin_amdgcn_sched_barrier(0);
         r.v[2 * q + k] = load_codes(t0 + 4 * kStep, w, 2 * q + k, true);
@@ -328,8 +331,8 @@ __global__ __launch_bounds__(256, DT == Dt::BF16 ? 3 : 2) void kv4_decode_kernel
       asm volatile("" ::: "memory");
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32)));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (rd ^ d * 32) + 16 * 256));
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (ro ^ d * 32)));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + (ro ^ d * 32) + 16 * 256));
         const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
         const u32x4 vf = {a0[0], a0[1], a1[0], a1[1]};
 #pragma unroll
@@ -397,24 +400,33 @@ struct Plan {
 };
 
 static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, int32_t max_blocks,
-                 int32_t max_context_len, int32_t part_tokens) {
-  constexpr int kIter = 128;  // tokens of one turn of the workgroup's waves
+                 int32_t max_context_len, int32_t part_tokens, bool fp32) {
+  constexpr int kTurn = 4 * kStep;  // tokens of one turn of the workgroup's waves
   Plan p;
-  int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, INT32_MAX - kIter);
+  int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, INT32_MAX - kTurn);
   if (max_context_len > 0 && max_context_len < cap) cap = max_context_len;
   if (cap < 1) cap = 1;
-  int64_t part = part_tokens > 0 ? cdiv(part_tokens, kIter) * kIter : 0;
-  if (part == 0) {
-    const int64_t items = (int64_t)n_seqs * hkv;
-    part = cap;
-    if (!((items >= 512 && cap <= 4096) || cap <= 2 * kIter)) {
-      for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        part = k * kIter;
-        if (items * cdiv(cap, part) <= 3072 && cdiv(cap, part) <= 64) break;
-      }
-    }
+  int64_t part = part_tokens;
+  if (part <= 0) {
+    // Measured on MI355X (us, graph replay).  A workgroup starts and ends in some 4 us, a
+    // turn of 256 tokens takes 1.2 of latency, and the second launch 2.5.  So no split
+    // up to 768 tokens (32 x 100-600 at 4 heads: 7.8 against 9.5 in 256), nor from 512
+    // (sequence, head) items up to 4096 (256 x 1-2k: 72.5 against 81 in 768 or 1024).  Else
+    // what one round of workgroups (three per CU, fp32 two) makes of the tables, up to
+    // 1024 tokens (24 x 100-2063: 768 15.4, 256 17.4, unsplit 17.3; one of 8000: 256
+    // 8.4, 768 10.6).  Beyond, contexts of different lengths leave a round's end to a
+    // few workgroups: the power of two from a quarter of it on, 1024 to 4096 (200 x 1-6k
+    // at one head: 1024 32.9, 2048 36; 16 x 10-30k at 8: 1024 66.9, 2048 67.7, 6144 80;
+    // 100 x 2-6k at 4: 1024 45.0, 512 48.6, 4096 63; 64 x 16-32k at 8: 8192 272, 4096 276,
+    // 5632 282, 1024 302; 200 x 4-12k at 8: 4096 286, 8192 336).  No more than 64 parts to
+    // combine (2 x 60k at 4: 1024 18.3, 768 20.3; one of 115k in fp16: 2048 30.5, 1024
+    // 34.8, 4096 34.1).
+    const int64_t items = (int64_t)n_seqs * hkv, round = cdiv(cap * items, fp32 ? 512 : 768);
+    part = round <= 1024 ? round : round <= 4096 ? 1024 : round <= 8192 ? 2048 : 4096;
+    part = std::max(part, cdiv(cap, 64));
+    if (cap <= 768 || (items >= 512 && cap <= 4096)) part = cap;
   }
-  part = cdiv(std::min(part, cap), kIter) * kIter;
+  part = cdiv(std::min(part, cap), kTurn) * kTurn;
   p.part_tokens = (int32_t)part;
   p.n_parts = (int32_t)cdiv(cap, part);
   p.ws_bytes = p.n_parts > 1 ? (size_t)n_seqs * hq * p.n_parts * (kDim + 1) * sizeof(float) : 0;
@@ -443,8 +455,12 @@ extern "C" size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_hea
   (void)head_dim;
   if (n_seqs <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
     return 0;
-  return kv4::plan(n_seqs, n_q_heads, n_kv_heads, block_size, max_blocks_per_seq, max_context_len,
-                   partition_tokens).ws_bytes;
+  // the element type is not known here: the larger of the two plans
+  size_t most = 0;
+  for (bool fp32 : {false, true})
+    most = std::max(most, kv4::plan(n_seqs, n_q_heads, n_kv_heads, block_size, max_blocks_per_seq,
+                                    max_context_len, partition_tokens, fp32).ws_bytes);
+  return most;
 }
 
 extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* cache, int64_t num_blocks,
@@ -470,7 +486,7 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* c
   if ((uintptr_t)q % 16 || (q_seq_stride * es) % 16 || (uintptr_t)out % 8 || (out_seq_stride * es) % 8)
     return AAC_ERR_MISALIGNED;
   const kv4::Plan p = kv4::plan(n_seqs, n_q_heads, n_kv_heads, block_size, max_blocks_per_seq,
-                                max_context_len, partition_tokens);
+                                max_context_len, partition_tokens, dtype == AAC_DTYPE_FP32);
   if (p.n_parts > 65535) return AAC_ERR_UNSUPPORTED;
   if (p.ws_bytes) {
     if (!workspace || workspace_bytes < p.ws_bytes) return AAC_ERR_WORKSPACE;

@@ -477,7 +477,7 @@ int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block_size,
  * max_context_len: 0, or a bound on every context (a longer one is cut).  Contexts
  * split over workgroups need aac_kv4_decode_workspace_bytes(...) bytes of workspace,
  * 16-byte aligned, any contents, not shared with a call that may overlap.
- * partition_tokens: 0, or the tokens of a partition (rounded up to 128).
+ * partition_tokens: 0, or the tokens of a partition (rounded up to 256).
  */
 size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
                                       int32_t head_dim, int32_t block_size,
