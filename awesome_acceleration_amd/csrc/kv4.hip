@@ -11,11 +11,14 @@
 // power of two is exact, and v_cvt_scalef32_pk_fp4_f32 does it with the rounding.
 // The bounds of e keep every value a normal number of bfloat16.
 //
-// Sixteen lanes take a row, eight dims each; four of them share a scale, so the
-// maximum takes two DPP steps.  A group of 256 threads takes 16 consecutive tokens of
-// one head, so that where they fall into one tile of the cache (the usual case) the
-// codes go out as 1 KiB in one piece.  Bound by memory: 512 bytes in (16-bit types)
-// and 136 out a token and head.
+// Sixteen lanes take a row, eight dims each, so the maximum takes two or three DPP steps.
+// A group of 256 threads takes 16 consecutive tokens of two heads, so that where they
+// fall into one tile of the cache (the usual case) the codes go out as 1 KiB in one
+// piece.  Bound by memory: 512 bytes in (16-bit types) and 136 out a token and head.
+// Measured: 32,768 tokens of 8 heads in bf16 27 us each way, 6.3 TB/s (rows that a
+// prefill has just made are in the last-level cache); 262,144 tokens 271 us stored, 5.0
+// TB/s, and 238 loaded, 5.7; fp32 5.2 and 7.0.  The load's results go out with
+// non-temporal stores (261 us without).
 #include "kv4.h"
 
 namespace aac {
@@ -32,6 +35,9 @@ struct StoreArgs {
   int32_t max_blocks;
 };
 
+// dpp_ctrl: lane i takes lane i + 4, 8, 12 of its 16 (0 past the last)
+constexpr int kDppRowShl4 = 0x104, kDppRowShl8 = 0x108, kDppRowShl12 = 0x10C;
+
 template <Dt DT> __device__ __forceinline__ float elem_f32(const char* p);
 template <> __device__ __forceinline__ float elem_f32<Dt::BF16>(const char* p) {
   return bf16lo(*reinterpret_cast<const u16*>(p));
@@ -43,75 +49,133 @@ template <> __device__ __forceinline__ float elem_f32<Dt::FP32>(const char* p) {
   return *reinterpret_cast<const float*>(p);
 }
 
-// eight elements of a row as float
-template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load8(const char* p, float* x) {
-  constexpr int es = DT == Dt::FP32 ? 4 : 2;
-  if constexpr (!ALIGNED) {
+// The scale byte of 32 elements whose largest is a (bits without the sign), and the scale.
+__device__ __forceinline__ u32 scale_byte(u32 a) {
+  return a >= 0x7f800000u ? 255u : (u32)min(max((int)((a + 0x200000u) >> 23) - 2, 2), 252);
+}
+template <int CTRL> __device__ __forceinline__ u32 dpp_umax(u32 a) {
+  return max(a, (u32)__builtin_amdgcn_update_dpp(0, (int)a, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ u32 bits_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// How 16 lanes hold a row.  16-bit types: eight dims each, 8 l .. 8 l + 7 of lane l, four
+// lanes a scale.  fp32: 4 l .. and 64 + 4 l .., so that the lanes' 16 bytes lie side by
+// side in each access; eight lanes a scale.
+template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const char* row, int l, float* x) {
+  if constexpr (DT == Dt::FP32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = elem_f32<DT>(p + i * es);
-  } else if constexpr (DT == Dt::FP32) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    for (int q = 0; q < 2; ++q) {
+      const char* p = row + (64 * q + 4 * l) * 4;
+      if constexpr (ALIGNED) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
+        for (int i = 0; i < 4; ++i) x[4 * q + i] = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * q + i] = elem_f32<DT>(p + 4 * i);
+      }
     }
+  } else if constexpr (ALIGNED) {
+    Elem<DT>::unpack8(*reinterpret_cast<const u32x4*>(row + l * 16), x);
   } else {
-    Elem<DT>::unpack8(*reinterpret_cast<const u32x4*>(p), x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = elem_f32<DT>(row + l * 16 + i * 2);
   }
 }
 
-// codes of eight elements; the four lanes of a quad hold the 32 of a scale
-__device__ __forceinline__ u32 quantise8(const float* x, u32* scale_byte) {
-  u32 a = 0;
+// Quantises a row and writes its codes and scales.
+template <Dt DT> __device__ __forceinline__ void write_row(const float* x, int l, unsigned char* codes, u32* scales) {
+  u32 a = 0, s4;
+  if constexpr (DT == Dt::FP32) {
+    u32 b = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
-  a = max(a, (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppQuadXor1, 0xF, 0xF, false));
-  a = max(a, (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppQuadXor2, 0xF, 0xF, false));
-  const bool bad = a >= 0x7f800000u;
-  const int e = min(max((int)((a + 0x200000u) >> 23) - 2, 2), 252);
-  const float s = __uint_as_float((u32)e << 23);
-  u32 w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-  *scale_byte = bad ? 255u : (u32)e;
-  return bad ? 0u : w;
+    for (int i = 0; i < 4; ++i) {
+      a = max(a, bits_of(x[i]));
+      b = max(b, bits_of(x[4 + i]));
+    }
+    a = scale_byte(dpp_umax<kDppRowHalfMirror>(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(a))));
+    b = scale_byte(dpp_umax<kDppRowHalfMirror>(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(b))));
+    const float sa = __uint_as_float(a << 23), sb = __uint_as_float(b << 23);
+    u32 w = 0, z = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], sa, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], sa, 1);
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, x[4], x[5], sb, 0);
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, x[6], x[7], sb, 1);
+    *reinterpret_cast<u16*>(codes + 2 * l) = a == 255u ? 0 : (u16)w;
+    *reinterpret_cast<u16*>(codes + 32 + 2 * l) = b == 255u ? 0 : (u16)z;
+    const u32 both = a | b << 16;  // scales 0 and 2 from lane 0, 1 and 3 from lane 8
+    s4 = both | (u32)__builtin_amdgcn_update_dpp(0, (int)both, kDppRowShl8, 0xF, 0xF, true) << 8;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, bits_of(x[i]));
+    a = scale_byte(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(a)));
+    const float s = __uint_as_float(a << 23);
+    u32 w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+    __builtin_nontemporal_store(a == 255u ? 0u : w, reinterpret_cast<u32*>(codes + 4 * l));
+    // the four scales, from lanes 0, 4, 8 and 12
+    s4 = a;
+    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl4, 0xF, 0xF, true) << 8;
+    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl8, 0xF, 0xF, true) << 16;
+    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl12, 0xF, 0xF, true) << 24;
+  }
+  if (l == 0) *scales = s4;
+}
+
+// Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16,
+// store and load in us: one head 277 and 273, two 271 and 238, four and eight as two).
+constexpr int kHeads = 2;
+
+// (block, row in it) of a cache row
+__device__ __forceinline__ void split_row(const Cache& c, int64_t row, int64_t* blk, int* r) {
+  if (row < 0x80000000ll) {  // (a 64-bit division is some 100 instructions)
+    *blk = (u32)row / (u32)c.block_size;
+  } else {
+    *blk = row / c.block_size;
+  }
+  *r = (int)(row - *blk * c.block_size);
 }
 
 template <Dt DT, bool ALIGNED, bool PAGED>
 __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
-  const int h = blockIdx.x % a.c.hkv;
-  const int64_t t = (int64_t)(blockIdx.x / a.c.hkv) * 16 + (threadIdx.x >> 4);
+  const int groups = (a.c.hkv + kHeads - 1) / kHeads;
+  const int h0 = (int)(blockIdx.x % groups) * kHeads;
+  const int64_t t = (int64_t)(blockIdx.x / groups) * 16 + (threadIdx.x >> 4);
   const int l = threadIdx.x & 15;
   if (t >= a.n_tokens) return;  // whole groups of 16 lanes
-  int64_t row;
+  constexpr int es = DT == Dt::FP32 ? 4 : 2;
+  float x[kHeads][2][8];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // (a head past the last: the last once more, not written)
+      load_row<DT, ALIGNED>(a.src[i] + t * a.stride[i] + (int64_t)min(h0 + h, a.c.hkv - 1) * kDim * es, l, x[h][i]);
+  int64_t blk;
+  int r;
   if constexpr (PAGED) {
     const int p = a.seqlens[t];
     if (p < 0 || p / a.c.block_size >= a.max_blocks) return;
-    const int blk = a.block_tables[t * a.max_blocks + p / a.c.block_size];
+    blk = a.block_tables[t * a.max_blocks + p / a.c.block_size];
+    r = p % a.c.block_size;
     if (blk < 0 || blk >= a.c.num_blocks) return;
-    row = (int64_t)blk * a.c.block_size + p % a.c.block_size;
   } else {
-    row = a.slots[t];
+    const int64_t row = a.slots[t];
     if (row < 0 || row >= a.c.num_blocks * a.c.block_size) return;
+    split_row(a.c, row, &blk, &r);
   }
-  const int64_t blk = row / a.c.block_size;
-  const int r = (int)(row - blk * a.c.block_size);
-  constexpr int es = DT == Dt::FP32 ? 4 : 2;
-  float x[2][8];
+  unsigned char* page = a.c.page(blk, h0);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    load8<DT, ALIGNED>(a.src[i] + t * a.stride[i] + (h * kDim + l * 8) * es, x[i]);
-  unsigned char* page = a.c.page(blk, h);
+  for (int h = 0; h < kHeads; ++h) {
+    if (h0 + h >= a.c.hkv) break;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    u32 sb;
-    const u32 w = quantise8(x[i], &sb);
-    *reinterpret_cast<u32*>(page + r * kRowBytes + l * 4) = w;
-    if ((l & 3) == 0) page[a.c.block_size * kRowBytes + r * kScaleBytes + (l >> 2)] = (unsigned char)sb;
-    page += a.c.page_bytes();
+    for (int i = 0; i < 2; ++i) {
+      write_row<DT>(x[h][i], l, page + r * kRowBytes,
+                    reinterpret_cast<u32*>(page + a.c.block_size * kRowBytes + r * kScaleBytes));
+      page += a.c.page_bytes();
+    }
   }
 }
 
@@ -124,45 +188,63 @@ struct LoadArgs {
 
 template <Dt DT>
 __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
-  const int h = blockIdx.x % a.c.hkv;
-  const int64_t t = (int64_t)(blockIdx.x / a.c.hkv) * 16 + (threadIdx.x >> 4);
+  const int groups = (a.c.hkv + kHeads - 1) / kHeads;
+  const int h0 = (int)(blockIdx.x % groups) * kHeads;
+  const int64_t t = (int64_t)(blockIdx.x / groups) * 16 + (threadIdx.x >> 4);
   const int l = threadIdx.x & 15;
   if (t >= a.n_tokens) return;
   const int64_t row = a.slots[t];
   const bool in = row >= 0 && row < a.c.num_blocks * a.c.block_size;
-  const int64_t blk = in ? row / a.c.block_size : 0;
-  const int r = in ? (int)(row - blk * a.c.block_size) : 0;
-  const unsigned char* page = a.c.page(blk, h);
-  u32 w[2], sb[2];
+  int64_t blk;
+  int r;
+  split_row(a.c, in ? row : 0, &blk, &r);
+  u32 w[kHeads][2], sb[kHeads][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const unsigned char* p = page + i * a.c.page_bytes();
-    w[i] = *reinterpret_cast<const u32*>(p + r * kRowBytes + l * 4);
-    sb[i] = p[a.c.block_size * kRowBytes + r * kScaleBytes + (l >> 2)];
+  for (int h = 0; h < kHeads; ++h) {
+    const unsigned char* p = a.c.page(blk, min(h0 + h, a.c.hkv - 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned char* codes = p + r * kRowBytes;
+      const unsigned char* scales = p + a.c.block_size * kRowBytes + r * kScaleBytes;
+      if constexpr (DT == Dt::FP32) {
+        w[h][i] = *reinterpret_cast<const u16*>(codes + 2 * l) | (u32)*reinterpret_cast<const u16*>(codes + 32 + 2 * l) << 16;
+        sb[h][i] = scales[l >> 3] | (u32)scales[2 + (l >> 3)] << 8;
+      } else {
+        w[h][i] = *reinterpret_cast<const u32*>(codes + l * 4);
+        sb[h][i] = scales[l >> 2] * 0x101u;
+      }
+      p += a.c.page_bytes();
+    }
   }
-  const int64_t at = (t * a.c.hkv + h) * kDim + l * 8;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float s = __uint_as_float(sb[i] << 23);
-    typedef __attribute__((ext_vector_type(2))) float f2;
-    f2 f[4];
-    f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 0);
-    f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 1);
-    f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 2);
-    f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 3);
-    float x[8];
+  for (int h = 0; h < kHeads; ++h) {
+    if (h0 + h >= a.c.hkv) break;
+    const int64_t at = (t * a.c.hkv + h0 + h) * kDim;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = !in ? 0.f : sb[i] == 255u ? __uint_as_float(0x7fc00000u) : f[e >> 1][e & 1];
-    if constexpr (DT == Dt::FP32) {
-      f32x4* d = reinterpret_cast<f32x4*>(a.dst[i] + at * 4);
-      d[0] = f32x4{x[0], x[1], x[2], x[3]};
-      d[1] = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
-      u32x4 o;
+    for (int i = 0; i < 2; ++i) {
+      // (the scale of the first four values and of the last)
+      const u32 b0 = sb[h][i] & 255u, b1 = sb[h][i] >> 8;
+      const float s0 = __uint_as_float(b0 << 23), s1 = __uint_as_float(b1 << 23);
+      typedef __attribute__((ext_vector_type(2))) float f2;
+      f2 f[4];
+      f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h][i], s0, 0);
+      f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h][i], s0, 1);
+      f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h][i], s1, 2);
+      f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h][i], s1, 3);
+      float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = Elem<DT>::pack2_hw(x[2 * e], x[2 * e + 1]);
-      *reinterpret_cast<u32x4*>(a.dst[i] + at * 2) = o;
+      for (int e = 0; e < 8; ++e)
+        x[e] = !in ? 0.f : (e < 4 ? b0 : b1) == 255u ? __uint_as_float(0x7fc00000u) : f[e >> 1][e & 1];
+      if constexpr (DT == Dt::FP32) {
+        f32x4* d = reinterpret_cast<f32x4*>(a.dst[i] + at * 4);
+        __builtin_nontemporal_store((f32x4{x[0], x[1], x[2], x[3]}), d + l);
+        __builtin_nontemporal_store((f32x4{x[4], x[5], x[6], x[7]}), d + 16 + l);
+      } else {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = Elem<DT>::pack2_hw(x[2 * e], x[2 * e + 1]);
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(a.dst[i] + at * 2) + l);
+      }
     }
   }
 }
@@ -172,7 +254,7 @@ static int elem_bytes(int32_t dtype) {
 }
 
 template <Dt DT, bool PAGED> static void launch_store_t(const StoreArgs& a, bool aligned, hipStream_t s) {
-  const dim3 grid((unsigned)(cdiv(a.n_tokens, 16) * a.c.hkv));
+  const dim3 grid((unsigned)(cdiv(a.n_tokens, 16) * cdiv(a.c.hkv, kHeads)));
   if (aligned)
     hipLaunchKernelGGL((kv4_store_kernel<DT, true, PAGED>), grid, dim3(256), 0, s, a);
   else
@@ -261,7 +343,7 @@ extern "C" int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block
   a.slots = slot_mapping;
   a.dst[0] = (char*)k_out;
   a.dst[1] = (char*)v_out;
-  const dim3 grid((unsigned)(cdiv(n_tokens, 16) * n_kv_heads));
+  const dim3 grid((unsigned)(cdiv(n_tokens, 16) * cdiv(n_kv_heads, kv4::kHeads)));
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case AAC_DTYPE_BF16: hipLaunchKernelGGL((kv4::kv4_load_kernel<Dt::BF16>), grid, dim3(256), 0, s, a); break;
