@@ -99,8 +99,8 @@ SIGNATURES: dict[str, tuple] = {
     "aac_kv4_decode_workspace_bytes": (_size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "aac_kv4_decode": (
         _c_int,
-        [_p, _i64, _p, _i64, _i32, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p,
-         _i64, _p, _size, _i32, _i32, _p]),
+        [_p, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32,
+         _f32, _p, _i64, _p, _size, _i32, _i32, _p]),
     "aac_step_maps": (
         _c_int, [_p, _p, _p, _i32, _i32, _i32, _p, _i32, _i64, _p, _p, _p, _p, _p, _p]),
     "aac_logprobs_workspace_bytes": (_size, [_i64, _i64, _i32]),
@@ -156,15 +156,18 @@ raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def launch(name: str, device_index: int, *args) -> None:
     """Call entry point ``name`` with ``args`` and the current stream of that
     device; a device that is not the current one is made so for the call (a
     null stream is the current device's).  Raises as ``check``."""
-    fn = getattr(lib(), name)
-    if device_index == torch.cuda.current_device():
+    fn = getattr(_lib or lib(), name)
+    if device_index == _current_device():
         rc = fn(*args, raw_stream(device_index))
     else:
         with torch.cuda.device(device_index):
             rc = fn(*args, raw_stream(device_index))
-    if rc != 0:
+    if rc:
         check(rc, name)

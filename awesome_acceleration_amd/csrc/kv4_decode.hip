@@ -463,10 +463,10 @@ extern "C" size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_hea
   return most;
 }
 
-extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* cache, int64_t num_blocks,
+extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k, const void* v,
+                              int64_t k_seq_stride, int64_t v_seq_stride, void* cache, int64_t num_blocks,
                               int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
-                              const int32_t* context_lens, int32_t lens_add, int32_t n_seqs,
-                              int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads,
+                              const int32_t* context_lens, int32_t n_seqs, int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads,
                               int32_t head_dim, float scale, void* out, int64_t out_seq_stride,
                               void* workspace, size_t workspace_bytes, int32_t partition_tokens,
                               int32_t dtype, void* stream) {
@@ -492,14 +492,20 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* c
     if (!workspace || workspace_bytes < p.ws_bytes) return AAC_ERR_WORKSPACE;
     if ((uintptr_t)workspace % 16) return AAC_ERR_MISALIGNED;
   }
+  if ((k == nullptr) != (v == nullptr)) return AAC_ERR_INVALID_ARGUMENT;
+  if (k) {  // all rows are written before any is read
+    const int arc = aac_kv4_append(k, v, k_seq_stride, v_seq_stride, cache, num_blocks, block_size, block_tables,
+                                   max_blocks_per_seq, context_lens, n_seqs, n_kv_heads, head_dim, dtype, stream);
+    if (arc != AAC_OK) return arc;
+  }
   kv4::DecArgs a = {};
   a.q = q;
   a.q_stride = q_seq_stride;
-  a.c = {(unsigned char*)const_cast<void*>(cache), num_blocks, block_size, n_kv_heads};
+  a.c = {(unsigned char*)cache, num_blocks, block_size, n_kv_heads};
   a.block_tables = block_tables;
   a.max_blocks = max_blocks_per_seq;
   a.lens = context_lens;
-  a.lens_add = lens_add;
+  a.lens_add = k ? 1 : 0;
   a.n_seqs = n_seqs;
   a.hq = n_q_heads;
   a.g = n_q_heads / n_kv_heads;

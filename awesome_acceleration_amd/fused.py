@@ -3,6 +3,7 @@ RMSNorm + RoPE + KV store, SiLU * up).  Device tensors only; every op runs on
 the current stream and fails loudly without the HIP library."""
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -252,29 +253,44 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     (with ``AAC_CHECK=1`` an ``IndexError``, at one device sync).  A row with a NaN
     or +inf, or masked to -inf throughout, gets NaN, as ``log_softmax`` gives."""
     _on_gpu(logits, tokens)
-    _req(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-         "logits must be [rows, cols] with contiguous rows")
-    _req(logits.dtype in _lib.AAC_DTYPE, f"unsupported dtype {logits.dtype}")
+    if logits.dim() != 2:
+        raise RuntimeError("logits must be [rows, cols]")
     rows, cols = logits.shape
-    _req(tokens.dtype == torch.int64 and tokens.shape == (rows,) and tokens.is_contiguous(),
-         "tokens must be contiguous int64 [rows]")
-    _req(cols > 0, "logits must have a column")
-    _req(0 <= top_k <= min(MAX_TOP_LOGPROBS, cols),
-         f"top_k must be within [0, {min(MAX_TOP_LOGPROBS, cols)}]")
+    stride, one = logits.stride()
+    if one != 1 and cols != 1:
+        raise RuntimeError("logits must be [rows, cols] with contiguous rows")
+    code = _lib.AAC_DTYPE.get(logits.dtype)
+    if code is None:
+        raise RuntimeError(f"unsupported dtype {logits.dtype}")
+    if tokens.dtype is not torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous():
+        raise RuntimeError("tokens must be contiguous int64 [rows]")
+    if cols <= 0:
+        raise RuntimeError("logits must have a column")
+    if not 0 <= top_k <= min(MAX_TOP_LOGPROBS, cols):
+        raise RuntimeError(f"top_k must be within [0, {min(MAX_TOP_LOGPROBS, cols)}]")
+    if rows <= 1:
+        stride = cols
+    elif stride < cols:
+        raise RuntimeError("rows of logits must not overlap")
     if check_mode() and rows and int(tokens.max()) >= cols:
         raise IndexError(f"index {int(tokens.max())} is out of bounds for dimension 1 with size {cols}")
     dev = logits.device
-    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
-    out = TokenLogprobs(both[0], both[1], top, ids)
+    out = TokenLogprobs(lp, ent, top, ids)
     if rows == 0:
         return out
-    nbytes = _lib.lib().aac_logprobs_workspace_bytes(rows, cols, top_k)
+    nbytes = _logprobs_ws(rows, cols, top_k)
+    # from the allocator, in stream order: a captured call's belongs to its graph
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    stride = logits.stride(0) if rows > 1 else cols
-    _req(stride >= cols, "rows of logits must not overlap")
     _lib.launch("aac_token_logprobs", logits.get_device(), logits.data_ptr(), stride, rows, cols,
-                tokens.data_ptr(), top_k, both.data_ptr(), both.data_ptr() + 4 * rows,
-                top.data_ptr(), ids.data_ptr(), ws.data_ptr(), nbytes, _lib.AAC_DTYPE[logits.dtype])
+                tokens.data_ptr(), top_k, lp.data_ptr(), ent.data_ptr(), top.data_ptr(), ids.data_ptr(),
+                ws.data_ptr(), nbytes, code)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _logprobs_ws(*args: int) -> int:
+    """aac_logprobs_workspace_bytes: host arithmetic on its integer arguments."""
+    return _lib.lib().aac_logprobs_workspace_bytes(*args)

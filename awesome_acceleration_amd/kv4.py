@@ -21,8 +21,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .flash_attn_interface import (_check_slots, _dtype_code, _on_gpu, _require, _scale,
-                                   _token_rows)
+from .flash_attn_interface import (_check_slots, _on_gpu, _require, _scale, _token_rows,
+                                   check_mode)
 
 __all__ = ["alloc_kv4_cache", "kv4_store", "kv4_load", "decode_paged_kv4",
            "flash_attn_with_kv4cache", "BYTES_PER_TOKEN"]
@@ -58,9 +58,16 @@ def _cache(kv_cache: torch.Tensor) -> tuple[int, int, int]:
 
 
 def _slots(slot_mapping: torch.Tensor, n: Optional[int]) -> None:
-    _require(slot_mapping.dtype == torch.int64 and slot_mapping.dim() == 1
-             and slot_mapping.is_contiguous() and (n is None or slot_mapping.shape[0] == n),
-             "slot_mapping must be contiguous int64 [N]")
+    if (slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1
+            or not slot_mapping.is_contiguous() or (n is not None and slot_mapping.shape[0] != n)):
+        raise RuntimeError("slot_mapping must be contiguous int64 [N]")
+
+
+def _code(dtype: torch.dtype) -> int:
+    code = _lib.AAC_DTYPE.get(dtype)
+    if code is None:
+        raise RuntimeError(f"unsupported dtype {dtype}")
+    return code
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
@@ -72,13 +79,17 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
     _on_gpu(k, v, kv_cache, slot_mapping)
     nb, bs, hkv = _cache(kv_cache)
     ks, vs = _token_rows(k, "k"), _token_rows(v, "v")
-    _require(k.shape == v.shape and k.dtype == v.dtype, "k and v must have one shape and dtype")
-    _require(tuple(k.shape[1:]) == (hkv, HEAD_DIM), "row shape != [Hkv, 128]")
-    _slots(slot_mapping, k.shape[0])
-    _check_slots(slot_mapping, nb * bs)
+    shape = k.shape
+    if shape != v.shape or k.dtype is not v.dtype:
+        raise RuntimeError("k and v must have one shape and dtype")
+    if shape[1] != hkv or shape[2] != HEAD_DIM:
+        raise RuntimeError("row shape != [Hkv, 128]")
+    _slots(slot_mapping, shape[0])
+    if check_mode():
+        _check_slots(slot_mapping, nb * bs)
     _lib.launch("aac_kv4_store", k.get_device(), k.data_ptr(), v.data_ptr(), ks, vs,
-                kv_cache.data_ptr(), nb, bs, slot_mapping.data_ptr(), k.shape[0], hkv, HEAD_DIM,
-                _dtype_code(k))
+                kv_cache.data_ptr(), nb, bs, slot_mapping.data_ptr(), shape[0], hkv, HEAD_DIM,
+                _code(k.dtype))
 
 
 def kv4_load(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -88,13 +99,12 @@ def kv4_load(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     _on_gpu(kv_cache, slot_mapping)
     nb, bs, hkv = _cache(kv_cache)
     _slots(slot_mapping, None)
+    code = _code(dtype)
     n = slot_mapping.shape[0]
-    _require(dtype in _lib.AAC_DTYPE, f"unsupported dtype {dtype}")
     k = torch.empty((n, hkv, HEAD_DIM), dtype=dtype, device=kv_cache.device)
     v = torch.empty_like(k)
     _lib.launch("aac_kv4_load", kv_cache.get_device(), kv_cache.data_ptr(), nb, bs,
-                slot_mapping.data_ptr(), n, hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(),
-                _lib.AAC_DTYPE[dtype])
+                slot_mapping.data_ptr(), n, hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(), code)
     return k, v
 
 
@@ -104,16 +114,16 @@ def _ws_bytes(*args: int) -> int:
     return _lib.lib().aac_kv4_decode_workspace_bytes(*args)
 
 
-def _decode(q, q_stride, n, hq, kv_cache, cache, tables, lens, lens_add, scale, mcl, part, out):
+def _decode(q, q_stride, n, hq, kv_cache, cache, tables, lens, k, v, ks, vs, scale, mcl, part, out,
+            out_stride):
     nb, bs, hkv = cache
     mb = tables.shape[1]
     nbytes = _ws_bytes(n, hq, hkv, HEAD_DIM, bs, mb, mcl, part)
     # from the allocator, in stream order: a captured call's belongs to its graph
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.launch("aac_kv4_decode", q.get_device(), q.data_ptr(), q_stride, kv_cache.data_ptr(), nb, bs,
-                tables.data_ptr(), mb, lens.data_ptr(), lens_add, n, mcl, hq, hkv, HEAD_DIM, scale,
-                out.data_ptr(), out.stride(0) if n > 1 else hq * HEAD_DIM,
-                None if ws is None else ws.data_ptr(), nbytes, part, _dtype_code(q))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    _lib.launch("aac_kv4_decode", q.get_device(), q.data_ptr(), q_stride, k, v, ks, vs,
+                kv_cache.data_ptr(), nb, bs, tables.data_ptr(), mb, lens.data_ptr(), n, mcl, hq, hkv,
+                HEAD_DIM, scale, out.data_ptr(), out_stride, ws, nbytes, part, _code(q.dtype))
 
 
 def _heads(hq: int, hkv: int, d: int) -> None:
@@ -139,20 +149,27 @@ def decode_paged_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torc
     the cache stands for; a sequence of none gets zeros.  1 to 16 query heads a KV head."""
     _on_gpu(q, kv_cache, block_tables, context_lens, out)
     cache = _cache(kv_cache)
-    _require(q.dim() == 3, "q must be [B, Hq, 128]")
+    if q.dim() != 3:
+        raise RuntimeError("q must be [B, Hq, 128]")
     n, hq, d = q.shape
     _heads(hq, cache[2], d)
-    _require(q.stride(2) == 1 and q.stride(1) == d, "q heads/head_dim must be contiguous")
+    qst = q.stride()
+    if qst[2] != 1 or qst[1] != d:
+        raise RuntimeError("q heads/head_dim must be contiguous")
     _table(block_tables, n)
-    _require(context_lens.dtype == torch.int32 and context_lens.shape == (n,)
-             and context_lens.is_contiguous(), "context_lens must be contiguous int32 [B]")
+    if (context_lens.dtype is not torch.int32 or context_lens.shape != (n,)
+            or not context_lens.is_contiguous()):
+        raise RuntimeError("context_lens must be contiguous int32 [B]")
+    row = hq * d
     if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        out, ost = torch.empty((n, hq, d), dtype=q.dtype, device=q.device), row
     else:
-        _require(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-                 and out.stride(1) == d, "out must be [B, Hq, 128] like q")
-    _decode(q, q.stride(0) if n > 1 else hq * d, n, hq, kv_cache, cache, block_tables, context_lens, 0,
-            _scale(softmax_scale, d), int(max_context_len or 0), int(partition_tokens), out)
+        st = out.stride()
+        if out.shape != q.shape or out.dtype is not q.dtype or st[2] != 1 or st[1] != d:
+            raise RuntimeError("out must be [B, Hq, 128] like q")
+        ost = st[0] if n > 1 else row
+    _decode(q, qst[0] if n > 1 else row, n, hq, kv_cache, cache, block_tables, context_lens, None, None, 0,
+            0, _scale(softmax_scale, d), int(max_context_len or 0), int(partition_tokens), out, ost)
     return out
 
 
@@ -175,29 +192,35 @@ def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
         raise RuntimeError("k and v must be given together")
     _on_gpu(q, kv_cache, k, v, cache_seqlens, block_table)
     cache = _cache(kv_cache)
-    nb, bs, hkv = cache
+    hkv = cache[2]
     _heads(hq, hkv, d)
     _table(block_table, n)
     if (cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (n,)
             or not cache_seqlens.is_contiguous()):
         raise RuntimeError("cache_seqlens must be contiguous int32 [B]")
-    if q.stride(3) != 1 or q.stride(2) != d:
+    qst = q.stride()
+    if qst[3] != 1 or qst[2] != d:
         q = q.contiguous()
+        qst = q.stride()
     out = torch.empty((n, 1, hq, d), dtype=q.dtype, device=q.device)
+    kp = vp = None
+    ks = vs = 0
     if k is not None:
         if k.shape != v.shape or k.shape != (n, 1, hkv, d):
             raise RuntimeError("k/v must be [B, 1, Hkv, 128]")
         if k.dtype is not q.dtype or v.dtype is not q.dtype:
             raise RuntimeError("k/v dtype mismatch")
-        if k.stride(3) != 1 or k.stride(2) != d:
+        kst, vst = k.stride(), v.stride()
+        if kst[3] != 1 or kst[2] != d:
             k = k.contiguous()
-        if v.stride(3) != 1 or v.stride(2) != d:
+            kst = k.stride()
+        if vst[3] != 1 or vst[2] != d:
             v = v.contiguous()
+            vst = v.stride()
         row = hkv * d
-        _lib.launch("aac_kv4_append", q.get_device(), k.data_ptr(), v.data_ptr(),
-                    k.stride(0) if n > 1 else row, v.stride(0) if n > 1 else row,
-                    kv_cache.data_ptr(), nb, bs, block_table.data_ptr(), block_table.shape[1],
-                    cache_seqlens.data_ptr(), n, hkv, d, _dtype_code(q))
-    _decode(q, q.stride(0) if n > 1 else hq * d, n, hq, kv_cache, cache, block_table, cache_seqlens,
-            0 if k is None else 1, _scale(softmax_scale, d), int(max_context_len or 0), 0, out)
+        kp, vp = k.data_ptr(), v.data_ptr()
+        ks, vs = (kst[0], vst[0]) if n > 1 else (row, row)
+    row = hq * d
+    _decode(q, qst[0] if n > 1 else row, n, hq, kv_cache, cache, block_table, cache_seqlens, kp, vp, ks, vs,
+            _scale(softmax_scale, d), int(max_context_len or 0), 0, out, row)
     return out

@@ -290,37 +290,35 @@ def build_step_maps(new_lens: torch.Tensor, cached_lens: torch.Tensor | None,
     sequence by sequence, and written into ``block_tables``; ``blocks_taken`` tells how
     many were asked for (more than the list holds: the missing ones are -1).  The
     lengths and the list are not modified.  Nothing synchronises."""
-    req = lambda c, m: None if c else _raise(m)  # noqa: E731
-    ints = dict(new_lens=new_lens, cached_lens=cached_lens, free_blocks=free_blocks)
     dev = new_lens.get_device()
-    for name, t in ints.items():
+    for t in (new_lens, cached_lens, free_blocks):
         if t is not None:
-            req(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(),
-                f"{name} must be contiguous int32, one-dimensional")
-            req(t.get_device() == dev and dev >= 0, "all tensors must be on the same GPU")
+            if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+                raise RuntimeError("new_lens, cached_lens and free_blocks must be contiguous int32, "
+                                   "one-dimensional")
+            if dev < 0 or t.get_device() != dev:
+                raise RuntimeError("all tensors must be on the same GPU")
     n = new_lens.shape[0]
-    req(n <= MAX_MAP_SEQS, f"at most {MAX_MAP_SEQS} sequences")
-    req(cached_lens is None or cached_lens.shape[0] == n, "one cached length per sequence")
-    req(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == n
-        and block_tables.shape[1] > 0 and block_tables.is_contiguous()
-        and block_tables.get_device() == dev, "block_tables must be contiguous int32 [n, width] "
-        "on the lengths' GPU")
-    req(block_size > 0, "block_size must be positive")
-    req(0 <= n_tokens < 1 << 31, "n_tokens must be within [0, 2^31)")
-    # one allocation: positions and slots, then the 32-bit results
-    both = torch.empty((2, n_tokens), dtype=torch.int64, device=new_lens.device)
-    small = torch.empty(2 * n + 2, dtype=torch.int32, device=new_lens.device)
-    p, at = both.data_ptr(), small.data_ptr()
-    out = StepMaps(small[:n + 1], both[0], both[1], small[n + 2:], small[n + 1:n + 2])
-    n_free = 0 if free_blocks is None else free_blocks.shape[0]
-    # an empty list is a list: every block asked of it is missing
-    free = 0 if free_blocks is None else free_blocks.data_ptr() or at
+    if n > MAX_MAP_SEQS:
+        raise RuntimeError(f"at most {MAX_MAP_SEQS} sequences")
+    if cached_lens is not None and cached_lens.shape[0] != n:
+        raise RuntimeError("one cached length per sequence")
+    if (block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != n
+            or block_tables.shape[1] == 0 or not block_tables.is_contiguous()
+            or block_tables.get_device() != dev):
+        raise RuntimeError("block_tables must be contiguous int32 [n, width] on the lengths' GPU")
+    if block_size <= 0:
+        raise RuntimeError("block_size must be positive")
+    if not 0 <= n_tokens < 1 << 31:
+        raise RuntimeError("n_tokens must be within [0, 2^31)")
+    pos, slots = torch.empty((2, n_tokens), dtype=torch.int64, device=new_lens.device).unbind()
+    cu, ctx, taken = torch.empty(2 * n + 2, dtype=torch.int32, device=new_lens.device).split((n + 1, n, 1))
+    at = cu.data_ptr()
+    n_free = free = 0
+    if free_blocks is not None:  # (an empty list is a list: every block asked of it is missing)
+        n_free, free = free_blocks.shape[0], free_blocks.data_ptr() or at
     _lib.launch("aac_step_maps", dev, new_lens.data_ptr(),
                 None if cached_lens is None else cached_lens.data_ptr(), block_tables.data_ptr(), n,
-                block_tables.shape[1], block_size, free or None, n_free, n_tokens, at, p,
-                p + 8 * n_tokens, at + 4 * (n + 2), at + 4 * (n + 1))
-    return out
-
-
-def _raise(message: str):
-    raise RuntimeError(message)
+                block_tables.shape[1], block_size, free or None, n_free, n_tokens, at, pos.data_ptr(),
+                slots.data_ptr(), at + 4 * (n + 1), at + 4 * (2 * n + 1))
+    return StepMaps(cu, pos, slots, ctx, taken)

@@ -470,23 +470,27 @@ int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block_size,
                  void* k_out, void* v_out, int32_t dtype, void* stream);
 
 /*
- * Attend-only decode over the 4-bit cache: out[b] = softmax(scale q[b] K^T) V over the
- * first context_lens[b] + lens_add tokens of sequence b (at most the table's capacity;
- * none: zeros), read through block_tables as aac_decode_paged reads them.
+ * Decode over the 4-bit cache: out[b] = softmax(scale q[b] K^T) V over the first
+ * context_lens[b] tokens of sequence b (at most the table's capacity; none: zeros), read
+ * through block_tables as aac_decode_paged reads them.  With k and v (one row of
+ * n_kv_heads * 128 a sequence, dtype as q's) they are appended first, at position
+ * context_lens[b], as aac_kv4_append does, and the call attends over one token more; all
+ * rows are written before any is read.  Both null: attend only.
  * q, out [n_seqs, n_q_heads, 128] BF16, FP16 or FP32; n_q_heads / n_kv_heads from 1 to 16.
- * max_context_len: 0, or a bound on every context (a longer one is cut).  Contexts
- * split over workgroups need aac_kv4_decode_workspace_bytes(...) bytes of workspace,
- * 16-byte aligned, any contents, not shared with a call that may overlap.
+ * max_context_len: 0, or a bound on every context (what lies past it may be left out).
+ * Contexts split over workgroups need aac_kv4_decode_workspace_bytes(...) bytes of
+ * workspace, 16-byte aligned, any contents, not shared with a call that may overlap.
  * partition_tokens: 0, or the tokens of a partition (rounded up to 256).
  */
 size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
                                       int32_t head_dim, int32_t block_size,
                                       int32_t max_blocks_per_seq, int32_t max_context_len,
                                       int32_t partition_tokens);
-int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* cache, int64_t num_blocks,
+int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k, const void* v,
+                   int64_t k_seq_stride, int64_t v_seq_stride, void* cache, int64_t num_blocks,
                    int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
-                   const int32_t* context_lens, int32_t lens_add, int32_t n_seqs,
-                   int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                   const int32_t* context_lens, int32_t n_seqs, int32_t max_context_len,
+                   int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                    float scale, void* out, int64_t out_seq_stride, void* workspace,
                    size_t workspace_bytes, int32_t partition_tokens, int32_t dtype, void* stream);
 

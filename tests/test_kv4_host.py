@@ -99,9 +99,10 @@ def test_load_refusals(change, code):
     (dict(d=64), -2), (dict(dt=3), -2), (dict(n=70000), -2), (dict(qs=1000), -5), (dict(os=1000), -5),
     (dict(q=P + 8), -3), (dict(qs=2052), -3), (dict(o=P + 4), -3), (dict(bs=17), -5), (dict(c=P + 8), -3),
     (dict(part=128, w=64), -4), (dict(part=128, w=64, ws=P, wsb=1 << 10), -4),
-    (dict(part=128, w=64, ws=P + 8, wsb=1 << 30), -3), (dict(n=0), 0)])
+    (dict(part=128, w=64, ws=P + 8, wsb=1 << 30), -3), (dict(n=0), 0), (dict(k=P), -1), (dict(v=P), -1),
+    (dict(k=P, v=P, ks=1000, vs=1024), -5), (dict(k=P + 1, v=P, ks=1024, vs=1024), -3)])
 def test_decode_refusals(change, code):
-    a = dict(q=P, qs=2048, c=P, nb=4, bs=16, t=P, w=3, l=P, add=0, n=4, mcl=0, hq=16, h=8, d=128,
+    a = dict(q=P, qs=2048, k=None, v=None, ks=0, vs=0, c=P, nb=4, bs=16, t=P, w=3, l=P, n=4, mcl=0, hq=16, h=8, d=128,
              scale=1.0, o=P, os=2048, ws=None, wsb=0, part=0, dt=0)
     a.update(change)
     assert _lib.lib().aac_kv4_decode(*a.values(), None) == code
