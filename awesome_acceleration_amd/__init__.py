@@ -16,8 +16,11 @@ from .kv4 import (  # noqa: F401
     alloc_kv4_cache,
     decode_paged_kv4,
     flash_attn_with_kv4cache,
+    kv4_export,
+    kv4_import,
     kv4_load,
     kv4_store,
+    qk_norm_rope_store_kv4,
 )
 from .paged import BlockAllocator, SlotCacheManager  # noqa: F401
 

@@ -101,6 +101,10 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_p, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32,
          _f32, _p, _i64, _p, _size, _i32, _i32, _p]),
+    "aac_qk_norm_rope_store_kv4": (
+        _c_int,
+        [_p, _i64, _i64, _i32, _i32, _i32, _p, _p, _f32, _p, _p, _i32, _p, _p, _p, _p, _i64, _i32, _p,
+         _p, _i32, _p, _i32, _p]),
     "aac_step_maps": (
         _c_int, [_p, _p, _p, _i32, _i32, _i32, _p, _i32, _i64, _p, _p, _p, _p, _p, _p]),
     "aac_logprobs_workspace_bytes": (_size, [_i64, _i64, _i32]),

@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kv4_quant.h"
 #include "qk_head.h"
 
 namespace aac {
@@ -91,11 +92,42 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const u16* x, int64_t x_st
   }
 }
 
+// The same with the K and V rows quantised into the 4-bit cache: the 16 lanes of a head
+// hold its row as the quantiser takes it.  The rounding of k to the activation type
+// stays, so the cache holds what a store of the returned k would write.  Bound by memory
+// from some thousand tokens on; us in bf16, 16/8 heads, here / the 16-bit store above /
+// norm and aac_kv4_store one after the other: 1 token 2.7 / 2.6 / 4.6, 256: 3.5 / 3.3 /
+// 5.4, 16,000: 44.0 (5.6 TB/s) / 50.1 / 52.5, 40,000: 112 / 124 / 126.
+struct Qk4Args : QkArgs {
+  kv4::Cache c;
+};
+template <Dt DT, bool NT = false>
+__device__ __forceinline__ void norm_rope_head(const Qk4Args& a, int64_t t, int hh, int li, const u32x4& xr,
+                                               int64_t crow, const float* wf, const float* cf, const float* sf) {
+  const bool value = hh >= a.hq + a.hkv;
+  const u32x4 packed = value ? xr : norm_rope_row<DT>(xr, a.eps, wf, cf, sf);
+  if (hh < a.hq) {
+    put16<NT>(a.q_out + (t * a.hq + hh) * kHeadDimFused + li * 8, packed);
+    return;
+  }
+  const int kh = hh - a.hq - (value ? a.hkv : 0);
+  if (!value && a.k_out != nullptr) put16<NT>(a.k_out + (t * a.hkv + kh) * kHeadDimFused + li * 8, packed);
+  if (crow < 0) return;
+  int64_t blk;
+  int r;
+  kv4::split_row(a.c, crow, &blk, &r);
+  unsigned char* page = a.c.page(blk, kh) + (value ? a.c.page_bytes() : 0);
+  float x[8];
+  unpack8<DT>(packed, x);
+  kv4::write_row<DT>(x, li, page + r * kv4::kRowBytes,
+                     reinterpret_cast<u32*>(page + a.c.block_size * kv4::kRowBytes + r * kv4::kScaleBytes));
+}
+
 // Few tokens (a decode step): one 16-lane DPP row per (token, head), the
 // most parallel mapping.  Heads 0..hq-1 are query heads, hq..hq+hkv-1 key
 // heads, then value heads.
-template <Dt DT>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a) {
+template <Dt DT, typename Args>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(Args a) {
   const int lane = threadIdx.x & 63;
   const int li = lane & 15;
   const int heads = a.hq + 2 * a.hkv;
@@ -122,8 +154,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a) {
 // and a row loads a group of its heads before it processes the first.  (fp16 takes
 // 82 registers; held to 80 by three heads a group or a launch bound 16,000 tokens
 // take 51.5 us against 50.3, 24,000 88 against 85.)
-template <Dt DT, bool NT>
-__global__ __launch_bounds__(256) void qk_norm_rope_tok_kernel(QkArgs a) {
+template <Dt DT, bool NT, typename Args>
+__global__ __launch_bounds__(256) void qk_norm_rope_tok_kernel(Args a) {
   const int lane = threadIdx.x & 63;
   const int li = lane & 15, r = lane >> 4;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -341,6 +373,24 @@ extern "C" int aac_rmsnorm(const void* x, int64_t x_row_stride, const void* resi
   return fz_status();
 }
 
+template <Dt DT, typename Args> static void launch_qk_t(const Args& a, hipStream_t s) {
+  if (a.n_tokens >= kQkTokenKernelMin) {  // one wavefront per token
+    const dim3 grid((unsigned)cdiv(a.n_tokens, 4));
+    if (a.n_tokens * (4 * a.hq + 8 * a.hkv) * kHeadDimFused >= kNtBytes)
+      hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<DT, true, Args>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<DT, false, Args>), grid, dim3(256), 0, s, a);
+  } else {  // one 16-lane row per (token, head)
+    const dim3 grid((unsigned)cdiv(a.n_tokens * (a.hq + 2 * a.hkv) * 16, 256));
+    hipLaunchKernelGGL((fz::qk_norm_rope_kernel<DT, Args>), grid, dim3(256), 0, s, a);
+  }
+}
+template <typename Args> static int launch_qk(const Args& a, Dt dt, hipStream_t s) {
+  if (dt == Dt::BF16) launch_qk_t<Dt::BF16>(a, s);
+  else launch_qk_t<Dt::FP16>(a, s);
+  return fz_status();
+}
+
 extern "C" int aac_qk_norm_rope_store(
     const void* qkv, int64_t qkv_tok_stride, int64_t n_tokens, int32_t n_q_heads,
     int32_t n_kv_heads, int32_t head_dim, const void* q_norm_weight, const void* k_norm_weight,
@@ -394,26 +444,55 @@ extern "C" int aac_qk_norm_rope_store(
   a.cache_seqlens = cache_seqlens;
   a.block_size = block_size;
   a.num_blocks = block_size > 0 ? num_cache_rows / block_size : 0;
-  hipStream_t s = (hipStream_t)stream;
-  if (n_tokens >= kQkTokenKernelMin) {  // one wavefront per token
-    const dim3 grid((unsigned)cdiv(n_tokens, 4));
-    const bool nt = n_tokens * (4 * n_q_heads + 8 * n_kv_heads) * head_dim >= kNtBytes;
-    if (dt == Dt::BF16) {
-      if (nt) hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<Dt::BF16, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<Dt::BF16, false>), grid, dim3(256), 0, s, a);
-    } else {
-      if (nt) hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<Dt::FP16, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((fz::qk_norm_rope_tok_kernel<Dt::FP16, false>), grid, dim3(256), 0, s, a);
-    }
-  } else {  // one 16-lane row per (token, head)
-    const int64_t items = n_tokens * (n_q_heads + 2 * n_kv_heads);
-    const dim3 grid((unsigned)cdiv(items * 16, 256));
-    if (dt == Dt::BF16)
-      hipLaunchKernelGGL((fz::qk_norm_rope_kernel<Dt::BF16>), grid, dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((fz::qk_norm_rope_kernel<Dt::FP16>), grid, dim3(256), 0, s, a);
-  }
-  return fz_status();
+  return launch_qk(a, dt, (hipStream_t)stream);
+}
+
+extern "C" int aac_qk_norm_rope_store_kv4(
+    const void* qkv, int64_t qkv_tok_stride, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+    int32_t head_dim, const void* q_norm_weight, const void* k_norm_weight, float eps,
+    const void* cos_table, const void* sin_table, int32_t max_position, const int32_t* positions,
+    void* q_out, void* k_out, void* cache, int64_t num_blocks, int32_t block_size,
+    const int64_t* slot_mapping, const int32_t* block_tables, int32_t max_blocks_per_seq,
+    const int32_t* cache_seqlens, int32_t dtype, void* stream) {
+  Dt dt;
+  if (!fz_dtype(dtype, &dt)) return AAC_ERR_UNSUPPORTED;
+  if (n_tokens < 0 || n_q_heads <= 0 || max_position <= 0) return AAC_ERR_INVALID_ARGUMENT;
+  if (n_tokens == 0) return AAC_OK;
+  const int rc = kv4::check_cache(cache, num_blocks, block_size, n_kv_heads, head_dim);
+  if (rc != AAC_OK) return rc;
+  if (qkv_tok_stride < (int64_t)(n_q_heads + 2 * n_kv_heads) * head_dim) return AAC_ERR_SHAPE;
+  if (!qkv || !q_norm_weight || !k_norm_weight || !cos_table || !sin_table || !positions || !q_out)
+    return AAC_ERR_INVALID_ARGUMENT;
+  if (!slot_mapping && (!block_tables || !cache_seqlens || max_blocks_per_seq <= 0))
+    return AAC_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_norm_weight |
+       (uintptr_t)k_norm_weight | (uintptr_t)cos_table | (uintptr_t)sin_table) % 16 || qkv_tok_stride % 8)
+    return AAC_ERR_MISALIGNED;
+  fz::Qk4Args a = {};
+  a.c = {(unsigned char*)cache, num_blocks, block_size, n_kv_heads};
+  a.qkv = (const u16*)qkv;
+  a.qkv_stride = qkv_tok_stride;
+  a.n_tokens = n_tokens;
+  a.hq = n_q_heads;
+  a.hkv = n_kv_heads;
+  a.qw = (const u16*)q_norm_weight;
+  a.kw = (const u16*)k_norm_weight;
+  a.eps = eps;
+  a.cos = (const u16*)cos_table;
+  a.sin = (const u16*)sin_table;
+  a.positions = positions;
+  a.max_pos = max_position;
+  a.q_out = (u16*)q_out;
+  a.k_out = (u16*)k_out;
+  a.v_cache = (u16*)cache;  // (cache_row: there is a store)
+  a.slot_mapping = slot_mapping;
+  a.num_rows = num_blocks * block_size;
+  a.block_tables = block_tables;
+  a.max_blocks = max_blocks_per_seq;
+  a.cache_seqlens = cache_seqlens;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  return launch_qk(a, dt, (hipStream_t)stream);
 }
 
 extern "C" int aac_silu_mul(const void* gate_up, void* out, int64_t n_rows, int32_t intermediate,

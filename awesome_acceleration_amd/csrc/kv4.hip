@@ -19,7 +19,7 @@
 // prefill has just made are in the last-level cache); 262,144 tokens 271 us stored, 5.0
 // TB/s, and 238 loaded, 5.7; fp32 5.2 and 7.0.  The load's results go out with
 // non-temporal stores (261 us without).
-#include "kv4.h"
+#include "kv4_quant.h"
 
 namespace aac {
 namespace kv4 {
@@ -35,9 +35,6 @@ struct StoreArgs {
   int32_t max_blocks;
 };
 
-// dpp_ctrl: lane i takes lane i + 4, 8, 12 of its 16 (0 past the last)
-constexpr int kDppRowShl4 = 0x104, kDppRowShl8 = 0x108, kDppRowShl12 = 0x10C;
-
 template <Dt DT> __device__ __forceinline__ float elem_f32(const char* p);
 template <> __device__ __forceinline__ float elem_f32<Dt::BF16>(const char* p) {
   return bf16lo(*reinterpret_cast<const u16*>(p));
@@ -49,18 +46,7 @@ template <> __device__ __forceinline__ float elem_f32<Dt::FP32>(const char* p) {
   return *reinterpret_cast<const float*>(p);
 }
 
-// The scale byte of 32 elements whose largest is a (bits without the sign), and the scale.
-__device__ __forceinline__ u32 scale_byte(u32 a) {
-  return a >= 0x7f800000u ? 255u : (u32)min(max((int)((a + 0x200000u) >> 23) - 2, 2), 252);
-}
-template <int CTRL> __device__ __forceinline__ u32 dpp_umax(u32 a) {
-  return max(a, (u32)__builtin_amdgcn_update_dpp(0, (int)a, CTRL, 0xF, 0xF, false));
-}
-__device__ __forceinline__ u32 bits_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-// How 16 lanes hold a row.  16-bit types: eight dims each, 8 l .. 8 l + 7 of lane l, four
-// lanes a scale.  fp32: 4 l .. and 64 + 4 l .., so that the lanes' 16 bytes lie side by
-// side in each access; eight lanes a scale.
+// A row in the layout of write_row (kv4_quant.h).
 template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const char* row, int l, float* x) {
   if constexpr (DT == Dt::FP32) {
 #pragma unroll
@@ -83,61 +69,9 @@ template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const ch
   }
 }
 
-// Quantises a row and writes its codes and scales.
-template <Dt DT> __device__ __forceinline__ void write_row(const float* x, int l, unsigned char* codes, u32* scales) {
-  u32 a = 0, s4;
-  if constexpr (DT == Dt::FP32) {
-    u32 b = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a = max(a, bits_of(x[i]));
-      b = max(b, bits_of(x[4 + i]));
-    }
-    a = scale_byte(dpp_umax<kDppRowHalfMirror>(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(a))));
-    b = scale_byte(dpp_umax<kDppRowHalfMirror>(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(b))));
-    const float sa = __uint_as_float(a << 23), sb = __uint_as_float(b << 23);
-    u32 w = 0, z = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], sa, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], sa, 1);
-    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, x[4], x[5], sb, 0);
-    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, x[6], x[7], sb, 1);
-    *reinterpret_cast<u16*>(codes + 2 * l) = a == 255u ? 0 : (u16)w;
-    *reinterpret_cast<u16*>(codes + 32 + 2 * l) = b == 255u ? 0 : (u16)z;
-    const u32 both = a | b << 16;  // scales 0 and 2 from lane 0, 1 and 3 from lane 8
-    s4 = both | (u32)__builtin_amdgcn_update_dpp(0, (int)both, kDppRowShl8, 0xF, 0xF, true) << 8;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = max(a, bits_of(x[i]));
-    a = scale_byte(dpp_umax<kDppQuadXor2>(dpp_umax<kDppQuadXor1>(a)));
-    const float s = __uint_as_float(a << 23);
-    u32 w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-    __builtin_nontemporal_store(a == 255u ? 0u : w, reinterpret_cast<u32*>(codes + 4 * l));
-    // the four scales, from lanes 0, 4, 8 and 12
-    s4 = a;
-    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl4, 0xF, 0xF, true) << 8;
-    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl8, 0xF, 0xF, true) << 16;
-    s4 |= (u32)__builtin_amdgcn_update_dpp(0, (int)a, kDppRowShl12, 0xF, 0xF, true) << 24;
-  }
-  if (l == 0) *scales = s4;
-}
-
 // Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16,
 // store and load in us: one head 277 and 273, two 271 and 238, four and eight as two).
 constexpr int kHeads = 2;
-
-// (block, row in it) of a cache row
-__device__ __forceinline__ void split_row(const Cache& c, int64_t row, int64_t* blk, int* r) {
-  if (row < 0x80000000ll) {  // (a 64-bit division is some 100 instructions)
-    *blk = (u32)row / (u32)c.block_size;
-  } else {
-    *blk = row / c.block_size;
-  }
-  *r = (int)(row - *blk * c.block_size);
-}
 
 template <Dt DT, bool ALIGNED, bool PAGED>
 __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {

@@ -240,6 +240,7 @@ class TokenLogprobs(NamedTuple):
 
 
 MAX_TOP_LOGPROBS = 32
+MAX_LOGPROB_COLS = 1 << 20
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:

@@ -25,7 +25,8 @@ from .flash_attn_interface import (_check_slots, _on_gpu, _require, _scale, _tok
                                    check_mode)
 
 __all__ = ["alloc_kv4_cache", "kv4_store", "kv4_load", "decode_paged_kv4",
-           "flash_attn_with_kv4cache", "BYTES_PER_TOKEN"]
+           "flash_attn_with_kv4cache", "qk_norm_rope_store_kv4", "kv4_export", "kv4_import",
+           "BYTES_PER_TOKEN"]
 
 HEAD_DIM = 128
 PAGE_BYTES = 68        # of a token's K or V row of one head: 64 of codes, 4 of scales
@@ -106,6 +107,90 @@ def kv4_load(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     _lib.launch("aac_kv4_load", kv_cache.get_device(), kv_cache.data_ptr(), nb, bs,
                 slot_mapping.data_ptr(), n, hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(), code)
     return k, v
+
+
+def qk_norm_rope_store_kv4(qkv: torch.Tensor, n_q_heads: int, q_norm_weight: torch.Tensor,
+                           k_norm_weight: torch.Tensor, eps: float, cos: torch.Tensor,
+                           sin: torch.Tensor, positions: torch.Tensor, kv_cache: torch.Tensor, *,
+                           slot_mapping: Optional[torch.Tensor] = None,
+                           block_tables: Optional[torch.Tensor] = None,
+                           cache_seqlens: Optional[torch.Tensor] = None, want_k: bool = True):
+    """``fused.qk_norm_rope_store`` with the 4-bit cache: q/k RMSNorm + RoPE of the fused
+    projection ``qkv`` ``[T, (Hq + 2 Hkv) * 128]`` (bf16 or fp16), and the K and V rows
+    quantised into the rows of ``slot_mapping`` or appended at ``cache_seqlens`` of
+    ``block_tables``, in one launch.  Returns ``(q [T, Hq, 128], k [T, Hkv, 128] or None)``;
+    the cache holds what ``kv4_store`` of ``k`` and ``v`` would write."""
+    _on_gpu(qkv, q_norm_weight, k_norm_weight, cos, sin, positions, kv_cache, slot_mapping, block_tables,
+            cache_seqlens)
+    nb, bs, hkv = _cache(kv_cache)
+    _require(qkv.dim() == 2 and qkv.stride(1) == 1
+             and qkv.shape[1] == (n_q_heads + 2 * hkv) * HEAD_DIM, "qkv must be [T, (Hq + 2 Hkv) * 128]")
+    n, dt = qkv.shape[0], qkv.dtype
+    _require(dt in (torch.bfloat16, torch.float16), "bf16 and fp16 only")
+    for t in (q_norm_weight, k_norm_weight):
+        _require(t.dtype is dt and t.shape == (HEAD_DIM,) and t.is_contiguous(), "norm weights must be [128]")
+    _require(cos.dim() == 2 and cos.shape[1] == HEAD_DIM and sin.shape == cos.shape and cos.dtype is dt
+             and sin.dtype is dt and cos.is_contiguous() and sin.is_contiguous(), "cos/sin must be [P, 128]")
+    _require(positions.dtype is torch.int32 and positions.shape == (n,) and positions.is_contiguous(),
+             "positions must be contiguous int32 [T]")
+    slots = tables = lens = None
+    mb = 0
+    if slot_mapping is not None:
+        _slots(slot_mapping, n)
+        if check_mode():
+            _check_slots(slot_mapping, nb * bs)
+        slots = slot_mapping.data_ptr()
+    else:
+        _require(block_tables is not None and cache_seqlens is not None,
+                 "append needs block_tables and cache_seqlens")
+        _table(block_tables, n)
+        _require(cache_seqlens.dtype is torch.int32 and cache_seqlens.shape == (n,)
+                 and cache_seqlens.is_contiguous(), "cache_seqlens must be contiguous int32 [T]")
+        tables, lens, mb = block_tables.data_ptr(), cache_seqlens.data_ptr(), block_tables.shape[1]
+    q = torch.empty((n, n_q_heads, HEAD_DIM), dtype=dt, device=qkv.device)
+    k = torch.empty((n, hkv, HEAD_DIM), dtype=dt, device=qkv.device) if want_k else None
+    _lib.launch("aac_qk_norm_rope_store_kv4", qkv.get_device(), qkv.data_ptr(),
+                qkv.stride(0) if n > 1 else qkv.shape[1], n, n_q_heads, hkv, HEAD_DIM,
+                q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(eps), cos.data_ptr(),
+                sin.data_ptr(), cos.shape[0], positions.data_ptr(), q.data_ptr(),
+                None if k is None else k.data_ptr(), kv_cache.data_ptr(), nb, bs, slots, tables, mb, lens,
+                _code(dt))
+    return q, k
+
+
+def kv4_export(storage: torch.Tensor, block_table, length: int,
+               dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The first ``length`` tokens of one sequence in every layer of ``storage`` (``[n_layers,
+    num_blocks, Hkv, 2, block_size * 68]``): K and V ``[n_layers, length, Hkv, 128]`` in
+    ``dtype`` (bf16 and fp32 hold every value of the cache exactly), zeros where a block is
+    outside the pool."""
+    k, v = kv4_load(storage.flatten(0, 1), _layer_slots(storage, block_table, length), dtype)
+    return k.unflatten(0, (storage.shape[0], length)), v.unflatten(0, (storage.shape[0], length))
+
+
+def kv4_import(k: torch.Tensor, v: torch.Tensor, storage: torch.Tensor, block_table) -> None:
+    """The reverse of ``kv4_export``: quantises ``k`` and ``v`` ``[n_layers, length, Hkv, 128]``
+    into the sequence's blocks; those outside the pool are skipped.  Rows exported in bf16 or
+    fp32 come back as they were held, byte for byte."""
+    _require(k.dim() == 4 and k.shape == v.shape and k.shape[0] == storage.shape[0],
+             "k and v must be [n_layers, length, Hkv, 128]")
+    kv4_store(k.flatten(0, 1), v.flatten(0, 1), storage.flatten(0, 1),
+              _layer_slots(storage, block_table, k.shape[1]))
+
+
+def _layer_slots(storage: torch.Tensor, block_table, length: int) -> torch.Tensor:
+    """Rows of the sequence in each layer of the storage taken as one cache; -1 where the
+    block is outside the pool."""
+    _require(storage.dim() == 5 and storage.is_contiguous(),
+             "KV storage must be contiguous [n_layers, num_blocks, Hkv, 2, block_size * 68]")
+    nb, bs, _ = _cache(storage[0])
+    table = torch.as_tensor(block_table, device=storage.device).reshape(-1).long()
+    _require(0 <= length <= table.numel() * bs, "the block table is too short for the length")
+    at = torch.arange(length, device=storage.device)
+    blk = table[at // bs]
+    row = torch.where((blk >= 0) & (blk < nb), blk * bs + at % bs, -1)
+    first = torch.arange(storage.shape[0], device=storage.device)[:, None] * (nb * bs)
+    return torch.where(row >= 0, first + row, -1).reshape(-1)
 
 
 @functools.lru_cache(maxsize=4096)

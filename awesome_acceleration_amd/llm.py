@@ -43,8 +43,9 @@ import numpy as np
 import torch
 
 from . import fused as fz
-from .paged import BlockAllocator, build_prefill_metadata, pad_block_tables
-from .qwen3 import PagedKVCache, Qwen3Config, Qwen3ForCausalLM, StepMeta
+from .paged import (MAX_MAP_SEQS, BlockAllocator, blocks_needed, build_prefill_metadata,
+                    build_step_maps, pad_block_tables)
+from .qwen3 import PagedKV4Cache, PagedKVCache, Qwen3Config, Qwen3ForCausalLM, StepMeta
 
 __all__ = ["LLM", "GenerationOutput"]
 
@@ -56,6 +57,10 @@ class GenerationOutput:
     token_ids: list[int]
     prompt_tokens: int = 0
     generated_tokens: int = 0
+    # of generate(logprobs=k), one entry per generated token
+    logprobs: Optional[list[float]] = None
+    entropies: Optional[list[float]] = None
+    top_logprobs: Optional[list[list[tuple[int, float]]]] = None  # (token id, log probability)
 
 
 @dataclass
@@ -68,6 +73,7 @@ class _Request:
     future: concurrent.futures.Future
     results: list = field(default_factory=list)
     pending_indices: list = field(default_factory=list)
+    logprobs: Optional[int] = None
 
 
 @dataclass
@@ -79,6 +85,7 @@ class _Seq:
     tokens: list[int]        # generated so far
     pos: int                 # position of the next token to feed
     done: bool = False       # finished (a step launched ahead may still hold its row)
+    scores: list = field(default_factory=list)  # (log probability, entropy, alternatives) of each token
 
 
 class LLM:
@@ -86,14 +93,18 @@ class LLM:
 
     ``max_num_seqs`` bounds the decode batch (the reference's slot count);
     ``num_blocks`` defaults to enough blocks for ``max_num_seqs`` sequences
-    of ``max_seq_len`` tokens.
+    of ``max_seq_len`` tokens.  ``kv_cache_dtype`` "mxfp4" keeps K and V in four bits
+    (``PagedKV4Cache``; head_dim 128, blocks of a multiple of 16 tokens), in 27 % of the
+    memory; ``None`` in ``dtype``.
     """
 
     def __init__(self, config: Optional[Qwen3Config] = None, max_num_seqs: int = 32,
                  max_seq_len: int = 4096, dtype=torch.bfloat16, block_size: int = 256,
                  num_blocks: Optional[int] = None, seed: int = 0, device="cuda",
                  decode_fn: Optional[Callable[[list[int]], str]] = None, use_graphs: bool = True,
-                 fused: bool = True):
+                 fused: bool = True, kv_cache_dtype: Optional[str] = None):
+        if kv_cache_dtype not in (None, "mxfp4"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: None or \"mxfp4\"")
         self.device = torch.device(device)
         self.dtype = dtype
         self.config = config or Qwen3Config()
@@ -107,7 +118,12 @@ class LLM:
         self.model = Qwen3ForCausalLM(self.config, self.device, dtype, seed, fused=fused)
         # block 0 is a scratch block: padding rows of a graph-captured decode
         # step append into it, so they never touch a live sequence's cache
-        self.cache = PagedKVCache(self.config, num_blocks + 1, block_size, self.device, dtype)
+        if kv_cache_dtype is None:
+            self.cache = PagedKVCache(self.config, num_blocks + 1, block_size, self.device, dtype)
+        else:
+            if self.model.hq > 16 * self.model.hkv:
+                raise ValueError("the 4-bit cache takes up to 16 query heads a KV head")
+            self.cache = PagedKV4Cache(self.config, num_blocks + 1, block_size, self.device)
         self.allocator = BlockAllocator(num_blocks + 1)
         self.allocator.allocate(1)
         self.use_graphs = use_graphs
@@ -128,11 +144,22 @@ class LLM:
 
     # ------------------------------------------------------------------ API
     def generate(self, prompts: list[list[int]], max_tokens: int = 100, temperature: float = 0.0,
-                 ignore_eos: bool = False) -> concurrent.futures.Future:
+                 ignore_eos: bool = False, logprobs: Optional[int] = None) -> concurrent.futures.Future:
         """Submit token-id prompts; the future resolves to ``list[GenerationOutput]``
-        in prompt order (llm.py:225-264)."""
+        in prompt order (llm.py:225-264).
+
+        With ``logprobs`` = k (0 to 32) each output holds, for every generated token,
+        its log probability, the entropy of its distribution and the k most likely
+        tokens with theirs, all of the model's distribution (the softmax of the logits
+        as they are, at any ``temperature``)."""
         if not prompts:
             raise ValueError("no prompts")
+        if logprobs is not None:
+            most = min(fz.MAX_TOP_LOGPROBS, self.config.vocab_size)
+            if not isinstance(logprobs, int) or not 0 <= logprobs <= most:
+                raise ValueError(f"logprobs must be within [0, {most}]")
+            if self.config.vocab_size > fz.MAX_LOGPROB_COLS:
+                raise ValueError(f"log probabilities are of up to {fz.MAX_LOGPROB_COLS} tokens")
         pool = self.allocator.num_blocks - 1  # block 0 is the scratch block
         for p in prompts:
             if not p:
@@ -150,7 +177,8 @@ class LLM:
         fut: concurrent.futures.Future = concurrent.futures.Future()
         req = _Request(token_ids=[list(map(int, p)) for p in prompts], max_tokens=max_tokens,
                        temperature=temperature, ignore_eos=ignore_eos, future=fut,
-                       results=[None] * len(prompts), pending_indices=list(range(len(prompts))))
+                       results=[None] * len(prompts), pending_indices=list(range(len(prompts))),
+                       logprobs=logprobs)
         self._request_queue.put(req)
         return fut
 
@@ -174,22 +202,70 @@ class LLM:
             self._loop_thread.start()
 
     # ------------------------------------------------------------ core steps
-    def _sample(self, logits: torch.Tensor, temperature: float) -> list[int]:
+    def _sample(self, logits: torch.Tensor, temperature: float) -> torch.Tensor:
+        """The sampled token of each row (int64)."""
         if temperature == 0:
-            return fz.argmax(logits).tolist()
+            return fz.argmax(logits)
         probs = torch.softmax(logits.float() / temperature, dim=-1)
-        return torch.multinomial(probs, 1).squeeze(-1).tolist()
+        return torch.multinomial(probs, 1).squeeze(-1)
+
+    @staticmethod
+    def _alternatives(seqs: list[_Seq]) -> Optional[int]:
+        """How many alternatives a step of these sequences records; None: no scores."""
+        return max((s.req.logprobs for s in seqs if s.req.logprobs is not None), default=None)
+
+    def _scores(self, logits: torch.Tensor, tok: torch.Tensor, top: Optional[int]):
+        """Log probability, entropy and ``top`` alternatives of each row, on their way to
+        pinned host memory (whole once the stream has come here); None without ``top``."""
+        if top is None:
+            return None
+        return [torch.empty(t.shape, dtype=t.dtype, pin_memory=True).copy_(t, non_blocking=True)
+                for t in fz.token_logprobs(logits, tok, top)]
+
+    @staticmethod
+    def _record(seqs: list[_Seq], scores) -> None:
+        """Append the scores of a step, whose row i is sequence i, to those who asked."""
+        if scores is None:
+            return
+        lp, ent, top, ids = (t.tolist() for t in scores)
+        for i, s in enumerate(seqs):
+            k = s.req.logprobs
+            if k is not None and not s.done:
+                s.scores.append((lp[i], ent[i], list(zip(ids[i][:k], top[i][:k]))))
+
+    def _sample_step(self, seqs: list[_Seq], logits: torch.Tensor, temperature: float) -> list[int]:
+        """The sampled tokens of a step on the host, its scores recorded."""
+        tok = self._sample(logits, temperature)
+        scores = self._scores(logits, tok, self._alternatives(seqs))
+        out = tok.tolist()  # (waits for the stream)
+        self._record(seqs, scores)
+        return out
+
+    def _prefill_maps(self, lens: list[int], seqs: list[_Seq]):
+        """(cu_seqlens, positions, slot_mapping) of a prefill of whole prompts.  Built on
+        the GPU from the lengths and block tables, which go there in one copy; a block
+        outside the cache raises IndexError here, before any launch, as the reference's
+        index_copy_ store does (llm.py:171-174)."""
+        tables = pad_block_tables([s.blocks for s in seqs], self.blocks_per_seq)
+        n, rows = len(seqs), self.cache.num_blocks * self.block_size
+        if n > MAX_MAP_SEQS:
+            return build_prefill_metadata(lens, tables, self.block_size, self.device,
+                                          num_cache_rows=rows)
+        for L, s in zip(lens, seqs):
+            used = s.blocks[:blocks_needed(L, self.block_size)]
+            if min(used) < 0 or max(used) >= self.cache.num_blocks:
+                raise IndexError(f"prefill store outside the KV cache ({self.cache.num_blocks} blocks "
+                                 f"of {self.block_size})")
+        packed = torch.from_numpy(np.concatenate((np.asarray(lens, np.int32), tables.reshape(-1))))
+        d = packed.to(self.device)
+        maps = build_step_maps(d[:n], None, d[n:].view(n, -1), self.block_size, sum(lens))
+        return maps[:3]
 
     def _prefill(self, seqs: list[_Seq]) -> torch.Tensor:
         """Packed varlen prefill of newly admitted sequences (llm.py:116-208)."""
         prompts = [s.req.token_ids[s.prompt_idx] for s in seqs]
         lens = [len(p) for p in prompts]
-        tables = pad_block_tables([s.blocks for s in seqs], self.blocks_per_seq)
-        # a slot outside the cache raises IndexError here, before any launch,
-        # as the reference's index_copy_ store does (llm.py:171-174)
-        cu, positions, slots = build_prefill_metadata(
-            lens, tables, self.block_size, self.device,
-            num_cache_rows=self.cache.num_blocks * self.block_size)
+        cu, positions, slots = self._prefill_maps(lens, seqs)
         ids = torch.from_numpy(np.fromiter((t for p in prompts for t in p), dtype=np.int64,
                                            count=sum(lens))).to(self.device)
         last = (cu[1:] - 1).long()
@@ -247,20 +323,17 @@ class LLM:
     def _bucket(self, n: int) -> int:
         return min(1 << (n - 1).bit_length(), self.max_num_seqs) if self.use_graphs else n
 
-    def _sample_ahead(self, n: int, temperature: float):
+    def _sample_ahead(self, n: int, temperature: float, top: Optional[int] = None):
         """After a graph step of n sequences: sample every row on the device,
         make the samples the next step's input ids, advance the live rows'
         positions and cache lengths by one (the device-side state of the
         next step, whose block tables are unchanged: blocks are reserved at
-        admission), and copy the samples to pinned host memory.  Returns the
-        handle ``_tokens`` waits on."""
+        admission), and copy the samples (and with ``top`` their scores) to pinned
+        host memory.  Returns the handle ``_tokens`` waits on."""
         B, W = self._bucket(n), self.blocks_per_seq
         logits = self._graphs[B][1]
-        if temperature == 0:
-            tok = fz.argmax(logits)
-        else:
-            tok = torch.multinomial(torch.softmax(logits.float() / temperature, dim=-1), 1)
-            tok = tok.squeeze(-1)
+        tok = self._sample(logits, temperature)
+        scores = self._scores(logits, tok, top)
         d = self._dev
         d[:B].copy_(tok)
         d[B:4 * B].view(3, B).add_(d[4 * B + B * W:5 * B + B * W].view(1, B))
@@ -269,17 +342,18 @@ class LLM:
         buf[:B].copy_(d[:B], non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
-        return n, ev, buf
+        return n, ev, buf, scores
 
     def _step_ahead(self, n: int):
         """Replay the graph of the last batch from the device-side state."""
         self.stats["decode_steps"] += 1
         self._graphs[self._bucket(n)][0].replay()
 
-    @staticmethod
-    def _tokens(handle) -> list[int]:
-        n, ev, buf = handle
+    def _tokens(self, handle, seqs: list[_Seq]) -> list[int]:
+        """The tokens of a step sampled ahead, its scores recorded."""
+        n, ev, buf, scores = handle
         ev.synchronize()
+        self._record(seqs, scores)
         return buf[:n].tolist()
 
     def _capture(self, B: int):
@@ -306,8 +380,10 @@ class LLM:
         req = s.req
         s.done = True
         text = self.decode_fn(s.tokens) if self.decode_fn else ""
-        req.results[s.prompt_idx] = GenerationOutput(
-            text, list(s.tokens), len(req.token_ids[s.prompt_idx]), len(s.tokens))
+        out = GenerationOutput(text, list(s.tokens), len(req.token_ids[s.prompt_idx]), len(s.tokens))
+        if req.logprobs is not None:
+            out.logprobs, out.entropies, out.top_logprobs = map(list, zip(*s.scores))
+        req.results[s.prompt_idx] = out
         self.allocator.free(s.blocks)
         bisect.insort(free_rows, s.row)
         if all(r is not None for r in req.results):
@@ -369,7 +445,7 @@ class LLM:
                         break
                 # Phase 3: prefill the admitted prompts, sample their first token
                 if new:
-                    sampled = self._sample(self._prefill(new), new[0].req.temperature)
+                    sampled = self._sample_step(new, self._prefill(new), new[0].req.temperature)
                     for s, tok in zip(new, sampled):
                         s.tokens.append(tok)
                         if 1 >= s.req.max_tokens or (not s.req.ignore_eos
@@ -383,8 +459,8 @@ class LLM:
                 seqs = [active[r] for r in sorted(active)]
                 temp = seqs[0].req.temperature
                 if not self.use_graphs:
-                    self._retire(seqs, self._sample(self._decode_step(seqs), temp), active,
-                                 free_rows)  # Phase 5: bookkeeping
+                    self._retire(seqs, self._sample_step(seqs, self._decode_step(seqs), temp),
+                                 active, free_rows)  # Phase 5: bookkeeping
                     continue
                 # With graphs the next step of the same batch is launched from
                 # the device-side state before the host reads this step's
@@ -395,18 +471,19 @@ class LLM:
                 # batch is rebuilt on the host once rows finish or a waiting
                 # request may be admitted.
                 self._decode_step(seqs)
-                h = self._sample_ahead(len(seqs), temp)
+                top = self._alternatives(seqs)
+                h = self._sample_ahead(len(seqs), temp, top)
                 while True:
                     ahead = None
                     if self._request_queue.empty() and (not pending or not free_rows):
                         self._step_ahead(len(seqs))
-                        ahead = self._sample_ahead(len(seqs), temp)
-                    finished = self._retire(seqs, self._tokens(h), active, free_rows)
+                        ahead = self._sample_ahead(len(seqs), temp, top)
+                    finished = self._retire(seqs, self._tokens(h, seqs), active, free_rows)
                     if ahead is None:
                         break
                     h = ahead
                     if finished or not self._loop_running:
-                        self._retire(seqs, self._tokens(h), active, free_rows)
+                        self._retire(seqs, self._tokens(h, seqs), active, free_rows)
                         break
         except BaseException as e:  # surface failures to every waiting caller
             for s in active.values():

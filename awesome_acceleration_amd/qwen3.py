@@ -33,10 +33,11 @@ import torch.nn.functional as F
 
 from . import flash_attn_interface as fai
 from . import fused as fz
+from . import kv4
 from . import kv_transfer
 from . import paged
 
-__all__ = ["Qwen3Config", "Qwen3ForCausalLM", "PagedKVCache", "StepMeta"]
+__all__ = ["Qwen3Config", "Qwen3ForCausalLM", "PagedKVCache", "PagedKV4Cache", "StepMeta"]
 
 
 # Where the forms of a decode step change hands, in sequences (us a step of 14
@@ -142,6 +143,53 @@ class PagedKVCache:
         return kv_transfer.import_request_kv(self.storage, block_table, payload, length)
 
 
+class PagedKV4Cache:
+    """The paged cache in four bits (``kv4``), zero-filled, in one storage ``[n_layers,
+    num_blocks, Hkv, 2, block_size * 68]``: 136 bytes a token, layer and KV head against
+    512 in 16 bits.  A prefill attends to its own K and V as they are; decode steps read
+    what the cache holds of them.  A decode step of Qwen3-0.6B on MI355X, us, 16 bits /
+    4 bits: 1 sequence of 4,096 tokens 861 / 859, 32 of 2,048 2479 / 1549, 256 of 1,024
+    6264 / 2811, 256 of 4,096 19830 / 6393."""
+
+    def __init__(self, cfg: Qwen3Config, num_blocks: int, block_size: int, device):
+        self.num_blocks = num_blocks
+        self.block_size = block_size
+        self.storage = kv4.alloc_kv4_cache(num_blocks, block_size, cfg.num_key_value_heads, cfg.head_dim,
+                                           device=device, n_layers=cfg.num_hidden_layers)
+
+    def layer(self, layer: int) -> torch.Tensor:
+        return self.storage[layer]
+
+    @property
+    def nbytes(self) -> int:
+        return self.storage.untyped_storage().nbytes()
+
+    def export_request_kv(self, block_table, length: int, seqlen: int) -> dict:
+        """``PagedKVCache.export_request_kv``'s payload, in bf16, which holds every value
+        of the cache exactly."""
+        k, v = kv4.kv4_export(self.storage, block_table, length)
+        host = torch.empty((2, *k.shape), dtype=k.dtype, pin_memory=True)
+        host[0].copy_(k, non_blocking=True)
+        host[1].copy_(v, non_blocking=True)
+        torch.cuda.current_stream(k.device).synchronize()
+        return {"layers": [{"k": host[0, i], "v": host[1, i], "seqlen": int(seqlen)}
+                           for i in range(k.shape[0])]}
+
+    def import_request_kv(self, block_table, payload: dict, length: int) -> int:
+        """The payload of either cache, of one dtype, into the blocks ``block_table``;
+        returns the payload's seqlen."""
+        layers = payload["layers"]
+        if len(layers) != self.storage.shape[0]:
+            raise ValueError(f"Layer count mismatch: payload has {len(layers)}, model has "
+                             f"{self.storage.shape[0]}")
+        seqlens = {int(lp["seqlen"]) for lp in layers}
+        if len(seqlens) != 1:
+            raise RuntimeError("payload layers disagree on seqlen")
+        k, v = (torch.stack([lp[n][:length] for lp in layers]).to(self.storage.device) for n in "kv")
+        kv4.kv4_import(k, v, self.storage, block_table)
+        return seqlens.pop()
+
+
 @dataclass
 class StepMeta:
     """Device-side metadata of one forward pass.
@@ -239,13 +287,15 @@ class Qwen3ForCausalLM:
         I = self.cfg.intermediate_size
         return F.linear(F.silu(gu[:, :I]) * gu[:, I:], L["down"])
 
-    def _layer(self, li, h, meta: StepMeta, cache: PagedKVCache, prefill: bool):
+    def _layer(self, li, h, meta: StepMeta, cache, prefill: bool):
         L = self.layers[li]
         eps = self.cfg.rms_norm_eps
         res = h
         x = rms_norm(h, L["ln1"], eps)
         q, k, v = self._qkv(L, x, meta.positions)
-        if prefill:
+        if isinstance(cache, PagedKV4Cache):
+            attn = self._attend_kv4(li, q, k, v, meta, cache, prefill)
+        elif prefill:
             # store K/V through slot_mapping and attend (llm.py:171-184)
             attn = fai.varlen_prefill_with_kvcache(
                 q, k, v, meta.cu_seqlens, meta.max_seqlen, cache.k(li), cache.v(li),
@@ -263,15 +313,28 @@ class Qwen3ForCausalLM:
         h = res + self._mlp(L, rms_norm(h, L["ln2"], eps))
         return h
 
-    def _forward_fused(self, input_ids, meta: StepMeta, cache: PagedKVCache, prefill: bool):
+    def _attend_kv4(self, li, q, k, v, meta: StepMeta, cache: PagedKV4Cache, prefill: bool):
+        if prefill:
+            kv4.kv4_store(k, v, cache.layer(li), meta.slot_mapping)
+            return fai.flash_attn_varlen_func(q, k, v, meta.cu_seqlens, meta.cu_seqlens,
+                                              meta.max_seqlen, meta.max_seqlen,
+                                              softmax_scale=self.scale, causal=True)
+        B = q.shape[0]
+        return kv4.flash_attn_with_kv4cache(
+            q.view(B, 1, self.hq, self.d), cache.layer(li), k=k.view(B, 1, self.hkv, self.d),
+            v=v.view(B, 1, self.hkv, self.d), cache_seqlens=meta.cache_seqlens,
+            block_table=meta.block_tables, softmax_scale=self.scale,
+            max_context_len=meta.max_context_len)
+
+    def _forward_fused(self, input_ids, meta: StepMeta, cache, prefill: bool):
         """The same layer with the fused call-site kernels: residual add +
         RMSNorm, q/k RMSNorm + RoPE + KV store/append, SiLU * up are one launch
         each, and the residual add of each block is folded into the next norm.
         A decode step's projections (one row per sequence) run on the
         decode-batch GEMM, gate/up with SiLU * up in its epilogue; the q/k norm,
         RoPE and KV append run in the attention launch or, from
-        QKV_ATTENTION_ROWS on, in QKV's epilogue; prefill steps (many rows) keep
-        the library GEMMs."""
+        QKV_ATTENTION_ROWS on, in QKV's epilogue (with the 4-bit cache in a launch of
+        their own); prefill steps (many rows) keep the library GEMMs."""
         eps = self.cfg.rms_norm_eps
         I = self.cfg.intermediate_size
         h = F.embedding(input_ids, self.embed)
@@ -281,7 +344,8 @@ class Qwen3ForCausalLM:
         small = not prefill and T <= self.small_gemm_rows
         lin = fz.linear if small else F.linear
         merged = small and T <= self.norm_gemm_rows
-        epilogue = small and T > QKV_ATTENTION_ROWS
+        four = isinstance(cache, PagedKV4Cache)
+        epilogue = small and T > QKV_ATTENTION_ROWS and not four
         for li, L in enumerate(self.layers):
             if merged:  # norm and projection in one launch
                 qkv, r = fz.rmsnorm_linear(res if delta is None else delta, L["ln1"], eps, L["qkv"],
@@ -295,13 +359,26 @@ class Qwen3ForCausalLM:
                 if not epilogue:
                     qkv = lin(x, L["qkv"])
             if prefill:
-                q, k = fz.qk_norm_rope_store(
-                    qkv, self.hq, self.hkv, L["q_norm"], L["k_norm"], eps, self.rope.cos,
-                    self.rope.sin, pos, cache.k(li), cache.v(li), slot_mapping=meta.slot_mapping)
+                if four:
+                    q, k = kv4.qk_norm_rope_store_kv4(
+                        qkv, self.hq, L["q_norm"], L["k_norm"], eps, self.rope.cos, self.rope.sin,
+                        pos, cache.layer(li), slot_mapping=meta.slot_mapping)
+                else:
+                    q, k = fz.qk_norm_rope_store(
+                        qkv, self.hq, self.hkv, L["q_norm"], L["k_norm"], eps, self.rope.cos,
+                        self.rope.sin, pos, cache.k(li), cache.v(li), slot_mapping=meta.slot_mapping)
                 v = qkv[:, self.q_size + self.kv_size:].view(T, self.hkv, self.d)
                 attn = fai.flash_attn_varlen_func(q, k, v, meta.cu_seqlens, meta.cu_seqlens,
                                                   meta.max_seqlen, meta.max_seqlen,
                                                   softmax_scale=self.scale, causal=True)
+            elif four:
+                q, _ = kv4.qk_norm_rope_store_kv4(
+                    qkv, self.hq, L["q_norm"], L["k_norm"], eps, self.rope.cos, self.rope.sin, pos,
+                    cache.layer(li), block_tables=meta.block_tables,
+                    cache_seqlens=meta.cache_seqlens, want_k=False)
+                attn = kv4.decode_paged_kv4(q, cache.layer(li), meta.block_tables, meta.context_lens,
+                                            softmax_scale=self.scale,
+                                            max_context_len=meta.max_context_len)
             elif T > QKV_ATTENTION_ROWS:
                 # q/k norm + RoPE and the KV append, in the projection's launch
                 # where the decode-batch GEMM takes it
@@ -340,7 +417,7 @@ class Qwen3ForCausalLM:
         return F.linear(h, self.embed)
 
     @torch.no_grad()
-    def forward(self, input_ids: torch.Tensor, meta: StepMeta, cache: PagedKVCache,
+    def forward(self, input_ids: torch.Tensor, meta: StepMeta, cache,
                 prefill: bool) -> torch.Tensor:
         """Logits for the last token of every sequence: prefill takes packed
         tokens (llm.py:116-208), decode one token per sequence

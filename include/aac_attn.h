@@ -470,6 +470,21 @@ int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block_size,
                  void* k_out, void* v_out, int32_t dtype, void* stream);
 
 /*
+ * aac_qk_norm_rope_store with the 4-bit cache in the place of the 16-bit caches: q/k
+ * RMSNorm + RoPE of the fused projection, and k (rounded to dtype) and v quantised into
+ * the rows slot_mapping names or, where it is null, appended at cache_seqlens of
+ * block_tables.  q_out [n_tokens, n_q_heads, 128]; k_out [n_tokens, n_kv_heads, 128] or
+ * null.  The cache holds what aac_kv4_store of k_out and v would write.  BF16 or FP16.
+ */
+int aac_qk_norm_rope_store_kv4(
+    const void* qkv, int64_t qkv_tok_stride, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+    int32_t head_dim, const void* q_norm_weight, const void* k_norm_weight, float eps,
+    const void* cos_table, const void* sin_table, int32_t max_position, const int32_t* positions,
+    void* q_out, void* k_out, void* cache, int64_t num_blocks, int32_t block_size,
+    const int64_t* slot_mapping, const int32_t* block_tables, int32_t max_blocks_per_seq,
+    const int32_t* cache_seqlens, int32_t dtype, void* stream);
+
+/*
  * Decode over the 4-bit cache: out[b] = softmax(scale q[b] K^T) V over the first
  * context_lens[b] tokens of sequence b (at most the table's capacity; none: zeros), read
  * through block_tables as aac_decode_paged reads them.  With k and v (one row of

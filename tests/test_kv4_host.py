@@ -167,3 +167,23 @@ def test_every_surface_refuses_host_tensors():
 def test_top_orders_ties_nan_and_signed_zeros():
     x = np.array([[1.0, np.nan, 1.0, -0.0, 0.0, -np.inf]])
     assert oracle4.top(x, 6).tolist() == [[1, 0, 2, 3, 4, 5]]
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(x=None), -1), (dict(qw=None), -1), (dict(kw=None), -1), (dict(cos=None), -1), (dict(sin=None), -1),
+    (dict(pos=None), -1), (dict(q=None), -1), (dict(c=None), -1), (dict(s=None), -1), (dict(n=-1), -1),
+    (dict(hq=0), -1), (dict(h=0), -1), (dict(maxp=0), -1), (dict(nb=0), -1), (dict(d=64), -2), (dict(dt=2), -2),
+    (dict(dt=7), -2), (dict(bs=24), -5), (dict(xs=4095), -5), (dict(xs=4100), -3), (dict(c=P + 16), -3),
+    (dict(x=P + 8), -3), (dict(k=P + 8), -3), (dict(qw=P + 2), -3), (dict(s=None, t=P, l=P, w=0), -1),
+    (dict(s=None, t=P, w=2), -1), (dict(s=None, l=P, w=2), -1), (dict(n=0, x=None), 0)])
+def test_fused_store_refusals(change, code):
+    a = dict(x=P, xs=4096, n=4, hq=16, h=8, d=128, qw=P, kw=P, eps=1e-6, cos=P, sin=P, maxp=100, pos=P, q=P,
+             k=None, c=P, nb=4, bs=16, s=P, t=None, w=0, l=None, dt=0)
+    a.update(change)
+    assert _lib.lib().aac_qk_norm_rope_store_kv4(*a.values(), None) == code
+
+
+def test_engine_refuses_an_unknown_cache_type():
+    from awesome_acceleration_amd.llm import LLM
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        LLM(kv_cache_dtype="int8")
