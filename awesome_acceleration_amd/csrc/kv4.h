@@ -21,6 +21,7 @@ constexpr int kDim = 128;
 constexpr int kRowBytes = 64;    // codes of a token and head
 constexpr int kScaleBytes = 4;
 constexpr int kTile = 16;        // tokens of a tile; block sizes are multiples of it
+constexpr int kMaxBlock = 1 << 23;  // tokens of a block: offsets in its K and V pages are 32 bits
 
 struct Cache {
   unsigned char* base;
@@ -39,7 +40,7 @@ struct Cache {
 inline int check_cache(const void* cache, int64_t num_blocks, int32_t block_size, int32_t hkv,
                        int32_t head_dim) {
   if (num_blocks <= 0 || block_size <= 0 || hkv <= 0) return AAC_ERR_INVALID_ARGUMENT;
-  if (head_dim != kDim) return AAC_ERR_UNSUPPORTED;
+  if (head_dim != kDim || block_size > kMaxBlock) return AAC_ERR_UNSUPPORTED;
   if (block_size % kTile) return AAC_ERR_SHAPE;
   if (!cache) return AAC_ERR_INVALID_ARGUMENT;
   if ((uintptr_t)cache % 64) return AAC_ERR_MISALIGNED;

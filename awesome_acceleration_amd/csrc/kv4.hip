@@ -72,6 +72,7 @@ template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const ch
 // Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16,
 // store and load in us: one head 277 and 273, two 271 and 238, four and eight as two).
 constexpr int kHeads = 2;
+constexpr int64_t kMaxGroups = 1 << 24;  // a launch's threads are numbered in 32 bits
 
 template <Dt DT, bool ALIGNED, bool PAGED>
 __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
@@ -203,7 +204,7 @@ static int store_common(const void* k, const void* v, int64_t k_stride, int64_t 
   if (!k || !v) return AAC_ERR_INVALID_ARGUMENT;
   if (k_stride < width || v_stride < width) return AAC_ERR_SHAPE;
   if (((uintptr_t)k | (uintptr_t)v) % es) return AAC_ERR_MISALIGNED;
-  if (cdiv(a.n_tokens, 16) * a.c.hkv > 0x7fffffff) return AAC_ERR_SHAPE;
+  if (cdiv(a.n_tokens, 16) * cdiv(a.c.hkv, kHeads) >= kMaxGroups) return AAC_ERR_UNSUPPORTED;
   a.src[0] = (const char*)k;
   a.src[1] = (const char*)v;
   a.stride[0] = k_stride * es;
@@ -270,7 +271,7 @@ extern "C" int aac_kv4_load(const void* cache, int64_t num_blocks, int32_t block
   if (rc != AAC_OK) return rc;
   if (!slot_mapping || !k_out || !v_out) return AAC_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return AAC_ERR_MISALIGNED;
-  if (cdiv(n_tokens, 16) * n_kv_heads > 0x7fffffff) return AAC_ERR_SHAPE;
+  if (cdiv(n_tokens, 16) * cdiv(n_kv_heads, kv4::kHeads) >= kv4::kMaxGroups) return AAC_ERR_UNSUPPORTED;
   kv4::LoadArgs a = {};
   a.c = {(unsigned char*)const_cast<void*>(cache), num_blocks, block_size, n_kv_heads};
   a.n_tokens = n_tokens;

@@ -3,9 +3,10 @@
 //   out[b, hq] = sum_t softmax_t(scale q[b, hq] . k_t) v_t,   t < context of b
 //
 // A workgroup takes one KV head's group of G <= 16 query heads over one partition of
-// a sequence's tokens; its four waves take steps of 32 tokens in turn and keep an
+// a sequence's tokens; its four waves take steps of 64 tokens in turn and keep an
 // online softmax each (log2 domain), merged at the end; partitions are combined by
-// a second launch.
+// a second launch.  Steps in turn, not a quarter of the partition each: the workgroup
+// then reads pages in order, and the waves end together.
 //
 // Both products run on v_mfma_f32_16x16x32_bf16.  A cached value is a 2-bit significand
 // times a power of two, so its bfloat16 is exact (v_cvt_scalef32_pk_bf16_fp4: two
@@ -23,8 +24,20 @@
 // operand of O^T += V^T P^T with tokens in the order (tile, 4 j + i).  V^T needs four
 // tokens of one dim a lane: V is converted in token order like K, written to the
 // wave's own 8 KiB of LDS as bf16 and read back with the transposing load
-// ds_read_b64_tr_b16.  Chunks of 32 bytes sit at c ^ (t & 7), which spreads the
-// four rows a quarter-wave reads, and the eight a b128 write covers, over the banks.
+// ds_read_b64_tr_b16.  Slots of 16 bytes sit at slot ^ (2 (row & 7) | row >> 3), with
+// which neither the b128 writes nor the transposing reads meet a bank twice.  Scales
+// (256 bytes of K and of V a step) go through LDS too: one dword a lane and page
+// instead of a byte a lane for each tile.
+//
+// Bound by the way the rows arrive: with the arithmetic left out, the loads alone take
+// 69.7, 276 and 28 us of the cases below, and the arithmetic alone (rows held) 50, 198.
+// So rows are asked for where the last ones have been taken, a step ahead of their use
+// (deeper rings spill or lose a workgroup a CU, and gained nothing), as non-temporal buffer loads, whose
+// bounds stand for the branch at a partition's end, 1 KiB of codes in one piece each.
+// Measured on MI355X (GPU time): bf16, 256 sequences of 1,024 to 2,048 tokens, 16/8 heads
+// 72.5 us (the bytes alone, at the 7.0 TB/s of a large copy: 60); 64 of 16,384 to 32,768
+// 278 (245); fp16, one of 115,000 31 (19), of which the second launch is 3; fp32, 4 of up
+// to 400 tokens 7.6, where latency alone counts.
 #include <algorithm>
 #include <climits>
 
@@ -39,6 +52,7 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 typedef unsigned long long u64;
 
+constexpr int64_t kMaxContext = (int64_t(1) << 31) - 1024;  // tokens: the steps' numbers stay within 31 bits
 constexpr float kRescale = 8.f;  // probabilities up to 2^8 before the reference moves
 
 struct DecArgs {
@@ -63,7 +77,8 @@ struct DecArgs {
 };
 
 __device__ __forceinline__ int context_len(const DecArgs& a, int len) {
-  const int64_t ctx = (int64_t)len + a.lens_add, cap = (int64_t)a.max_blocks * a.c.block_size;
+  const int64_t ctx = (int64_t)len + a.lens_add;
+  const int64_t cap = min((int64_t)a.max_blocks * a.c.block_size, kMaxContext);
   return (int)(ctx < 0 ? 0 : ctx > cap ? cap : ctx);
 }
 __device__ __forceinline__ int parts_of(const DecArgs& a, int ctx) {
@@ -143,7 +158,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     }
     return;
   }
-  const int end = min(ctx, beg + a.part_tokens), n_tiles = (end + kTile - 1) / kTile;
+  const int end = beg + min(ctx - beg, a.part_tokens), n_tiles = (end + kTile - 1) / kTile;
 
   // A buffer of each tile's pages (K, then V) from the block number, and offsets that each
   // lane keeps.  Past the end the buffer is empty: the loads are issued all the same, so
@@ -403,7 +418,7 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
                  int32_t max_context_len, int32_t part_tokens, bool fp32) {
   constexpr int kTurn = 4 * kStep;  // tokens of one turn of the workgroup's waves
   Plan p;
-  int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, INT32_MAX - kTurn);
+  int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, kMaxContext);
   if (max_context_len > 0 && max_context_len < cap) cap = max_context_len;
   if (cap < 1) cap = 1;
   int64_t part = part_tokens;
@@ -466,8 +481,8 @@ extern "C" size_t aac_kv4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_hea
 extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k, const void* v,
                               int64_t k_seq_stride, int64_t v_seq_stride, void* cache, int64_t num_blocks,
                               int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
-                              const int32_t* context_lens, int32_t n_seqs, int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads,
-                              int32_t head_dim, float scale, void* out, int64_t out_seq_stride,
+                              const int32_t* context_lens, int32_t n_seqs, int32_t max_context_len,
+                              int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale, void* out, int64_t out_seq_stride,
                               void* workspace, size_t workspace_bytes, int32_t partition_tokens,
                               int32_t dtype, void* stream) {
   if (n_seqs < 0 || n_q_heads <= 0 || max_blocks_per_seq <= 0 || q_seq_stride < 0 || out_seq_stride < 0)
@@ -514,13 +529,12 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k
   a.out_stride = out_seq_stride;
   a.n_parts = p.n_parts;
   a.part_tokens = p.part_tokens;
-  // Granlund and Montgomery 1994, Theorem 4.2, for tile numbers below 2^27 (a
-  // context is below 2^31 tokens): magic = floor(2^(27 + l) / d) + 1, l = ceil(log2 d)
+  // Granlund and Montgomery 1994, Theorem 4.2, for tile numbers below 2^27: magic = floor(2^(27 + l) / d) + 1, l = ceil(log2 d)
   const u32 d = (u32)(block_size / kv4::kTile);
   const int l = d == 1 ? 0 : 32 - __builtin_clz(d - 1);
   a.magic = (uint64_t(1) << (27 + l)) / d + 1;
   a.shift = 27 + l;
-  a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, (1 << 27) - 1);
+  a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, kv4::kMaxContext / kv4::kTile);
   if (p.ws_bytes) {
     a.ws_o = reinterpret_cast<float*>(workspace);
     a.ws_lse = a.ws_o + (size_t)n_seqs * n_q_heads * p.n_parts * kv4::kDim;

@@ -639,7 +639,7 @@ extern "C" int aac_token_logprobs(const void* logits, int64_t row_stride, int64_
   a.cols = (int32_t)n_cols;
   a.top = top_k;
   a.n_seg = lp::seg_of(n_cols, es);
-  if (n_rows * a.n_seg > INT_MAX) return AAC_ERR_UNSUPPORTED;
+  if (n_rows * a.n_seg >= (1 << 24)) return AAC_ERR_UNSUPPORTED;  // (a launch numbers its threads in 32 bits)
   a.tokens = tokens;
   a.logp = logprobs;
   a.entropy = entropy;

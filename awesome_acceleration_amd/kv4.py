@@ -96,7 +96,8 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
 def kv4_load(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """The K and V rows ``[N, Hkv, 128]`` that the cache holds at ``slot_mapping`` (int64
-    ``[N]``), in ``dtype``; zeros for a slot outside the cache."""
+    ``[N]``), in ``dtype`` (bf16 and fp32 hold them exactly, fp16 those within its range);
+    zeros for a slot outside the cache."""
     _on_gpu(kv_cache, slot_mapping)
     nb, bs, hkv = _cache(kv_cache)
     _slots(slot_mapping, None)

@@ -440,7 +440,7 @@ int aac_kv_import_paged(const void* src, void* kv_cache, int64_t layer_stride, i
 
 /*
  * The paged KV cache in four bits.  cache: uint8 [num_blocks][n_kv_heads][K, V]
- * [block_size * 68], 64-byte aligned, block_size a multiple of 16, head_dim 128.  A
+ * [block_size * 68], 64-byte aligned, block_size a multiple of 16 (to 2^23), head_dim 128.  A
  * page holds block_size rows of 64 bytes (E2M1 codes, dim 2 i in the low nibble of
  * byte i), then block_size rows of 4 scale bytes (E8M0, one for 32 dims): an element
  * is code * 2^(byte - 127), NaN where the byte is 255.  With a = max |x| of 32 dims, the
@@ -486,8 +486,8 @@ int aac_qk_norm_rope_store_kv4(
 
 /*
  * Decode over the 4-bit cache: out[b] = softmax(scale q[b] K^T) V over the first
- * context_lens[b] tokens of sequence b (at most the table's capacity; none: zeros), read
- * through block_tables as aac_decode_paged reads them.  With k and v (one row of
+ * context_lens[b] tokens of sequence b (at most the table's capacity and 2^31 - 1024;
+ * none: zeros), read through block_tables as aac_decode_paged reads them.  With k and v (one row of
  * n_kv_heads * 128 a sequence, dtype as q's) they are appended first, at position
  * context_lens[b], as aac_kv4_append does, and the call attends over one token more; all
  * rows are written before any is read.  Both null: attend only.

@@ -418,3 +418,23 @@ def test_python_surface_refuses(gpu):
     no("mismatch", kv4.flash_attn_with_kv4cache, q[:, None], cache, k=k[:, None].half(), v=k[:, None].half(), **a)
     no("k/v must", kv4.flash_attn_with_kv4cache, q[:, None], cache, k=k[:, None, :1], v=k[:, None, :1], **a)
     no("cache_seqlens", kv4.flash_attn_with_kv4cache, q[:, None], cache, cache_seqlens=ctx.long(), block_table=t)
+
+
+def test_contexts_to_the_last_token_of_31_bits(gpu):
+    """A table of 2^31 tokens (one block again and again) and lengths at its end and past
+    the largest that is read: equal scores of equal values, so their average is exact."""
+    print("case: context of 2^31 tokens", flush=True)
+    bs = 1 << 20
+    cache = kv4.alloc_kv4_cache(1, bs, 1, device=gpu)
+    rows = torch.zeros((bs, 1, 128), dtype=torch.bfloat16, device=gpu)
+    kv4.kv4_store(rows, rows + 1, cache, torch.arange(bs, device=gpu))
+    tables = torch.zeros((2, 2048), dtype=torch.int32, device=gpu)
+    lens = torch.tensor([2 ** 31 - 1, 5], dtype=torch.int32, device=gpu)
+    q = torch.ones((2, 1, 128), dtype=torch.bfloat16, device=gpu)
+    print("attend", flush=True)
+    out = kv4.decode_paged_kv4(q, cache, tables, lens)
+    assert (out == 1).all()
+    print("append and attend", flush=True)
+    kv = torch.zeros((2, 1, 1, 128), dtype=torch.bfloat16, device=gpu)
+    out = kv4.flash_attn_with_kv4cache(q[:, None], cache, k=kv, v=kv + 1, cache_seqlens=lens, block_table=tables)
+    assert (out == 1).all()

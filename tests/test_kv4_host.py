@@ -187,3 +187,17 @@ def test_engine_refuses_an_unknown_cache_type():
     from awesome_acceleration_amd.llm import LLM
     with pytest.raises(ValueError, match="kv_cache_dtype"):
         LLM(kv_cache_dtype="int8")
+
+
+def test_sizes_past_32_bit_offsets_are_refused():
+    big = 1 << 23
+    assert _store(bs=2 * big) == _store(bs=big + 16) == -2 and _store(bs=big, n=0) == 0
+    # 2^24 workgroups of 256 threads: 16 tokens of two heads each
+    assert _store(n=16 << 24, h=1) == _store(n=4 << 24, h=8) == -2
+    L = _lib.lib()
+    assert L.aac_kv4_load(P, 4, 16, P, 4 << 24, 8, 128, P, P, 0, None) == -2
+    a = (P, 1 << 26, 16, 8, 128, P, P, 1e-6, P, P, 100, P, P, None, P, 4, 16, P, None, 0, None, 0, None)
+    assert L.aac_qk_norm_rope_store_kv4(P, 4096, *a[1:]) == -2
+    assert L.aac_token_logprobs(P, 100, 1 << 24, 100, P, 0, P, P, P, P, P, 1 << 40, 0, None) == -2
+    # a table's capacity passes 2^31 tokens: the plan stays within it (64 partitions of 2^25)
+    assert L.aac_kv4_decode_workspace_bytes(1, 1, 1, 128, big, 1 << 20, 0, 0) == 64 * 129 * 4
