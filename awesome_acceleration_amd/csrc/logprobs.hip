@@ -259,11 +259,39 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_segment_kernel(Args a) {
         f32x4{m, S, T, residue<DT>(m)};
 }
 
-// The wave's k-th and j-th largest of 64 keys (0 where it has fewer above 0), bit by bit.
-__device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, int bits, int drop) {
-  u32 tk = 0, tj = 0;
+template <int CTRL> __device__ __forceinline__ u32 dpp_u(u32 x) {
+  return (u32)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
+}
+// The smallest and the largest key of the wave.
+__device__ __forceinline__ uint2 wave_range(u32 key) {
+  u32 lo = key, hi = key;
+#define AAC_STEP(c) lo = min(lo, dpp_u<c>(lo)), hi = max(hi, dpp_u<c>(hi))
+  AAC_STEP(kDppQuadXor1);
+  AAC_STEP(kDppQuadXor2);
+  AAC_STEP(kDppRowHalfMirror);
+  AAC_STEP(kDppRowMirror);
+#undef AAC_STEP
+  u32 l = 0xffffffffu, h = 0;
+#pragma unroll
+  for (int r = 0; r < 64; r += 16) {
+    l = min(l, (u32)__builtin_amdgcn_readlane((int)lo, r));
+    h = max(h, (u32)__builtin_amdgcn_readlane((int)hi, r));
+  }
+  return make_uint2(l, h);
+}
+
+// The wave's k-th and j-th largest of 64 keys, bit by bit, `depth` of the bits in which the
+// keys differ; those below are left at 0, so that the result is at most that key.  A
+// step takes some 130 cycles, of counts that only the scalar unit takes (two bits a step
+// cost more: three counts for each key's two bits).
+__device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, int depth) {
+  const uint2 range = wave_range(key);
+  const int top = 32 - __builtin_clz(range.x ^ range.y | 1u);  // bits from here up are alike
+  u32 tk = top < 32 ? range.y >> top << top : 0, tj = tk;
+  const int end = max(top - depth, 0);
 #pragma unroll 1
-  for (u32 bit = 1u << (bits - 1); bit >> drop; bit >>= 1) {
+  for (int s = top - 1; s >= end; --s) {
+    const u32 bit = 1u << s;
     if ((int)__popcll(__ballot(key >= (tk | bit))) >= k) tk |= bit;
     if ((int)__popcll(__ballot(key >= (tj | bit))) >= j) tj |= bit;
   }
@@ -279,27 +307,32 @@ __device__ __forceinline__ u64 entry(u32 key, u32 index) { return (u64)key << 32
 __device__ __forceinline__ u32 index_of(u64 e) { return ~(u32)e; }
 
 // Hands each of the list's n entries that is among the k largest to put(rank, entry).
-// The list is read eight entries at a time, so that the reads overlap: entries n to the
-// next multiple of eight are set to 0 first, which is below every entry.
+// Four lanes an entry, each against eight entries at a time, so that the reads overlap:
+// entries n to the next multiple of 32 are set to 0 first, which is below every entry.
+constexpr int kListPad = 32;
 template <typename F> __device__ __forceinline__ void ranked(u64* list, int n, int k, F put) {
-  if ((int)threadIdx.x < 8) list[n + threadIdx.x] = 0;
+  if ((int)threadIdx.x < kListPad) list[n + threadIdx.x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  const int part = threadIdx.x & 3;
+  for (int i = threadIdx.x >> 2; i < n; i += kThreads / 4) {
     const u64 c = list[i];
     int rank = 0;
-    for (int j = 0; j < n; j += 8) {
+    for (int j = 0; j < n; j += kListPad) {
 #pragma unroll
-      for (int z = 0; z < 8; ++z) rank += list[j + z] > c;
+      for (int z = 0; z < 8; ++z) rank += list[j + 8 * part + z] > c;
     }
-    if (rank < k) put(rank, c);
+    rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor1, 0xF, 0xF, false);
+    rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor2, 0xF, 0xF, false);
+    if (part == 0 && rank < k) put(rank, c);
   }
 }
 
 // Entries a list has to hold in the ordered search: in each of the four waves fewer than k
 // lanes have a key above the bound, `per` entries each, and k entries equal to it are kept.
-__host__ __device__ inline int list_cap(int k, int per) { return 4 * ((k - 1) * per + k) + 8; }
+__host__ __device__ inline int list_cap(int k, int per) { return 4 * ((k - 1) * per + k) + kListPad; }
 constexpr int kFast = 512;      // entries the list holds in the plain search
 constexpr int kFastGroups = 64;
+constexpr int kHeld = 6;  // group maxima a thread keeps
 
 // (m, S, T) of one part of a row, joined with others' about the row's m.  r: d of x = m.
 struct Sums {
@@ -325,12 +358,13 @@ __device__ __forceinline__ float finish_sums(const Args& a, int64_t row, const S
   return log_s;
 }
 
-// The top k of a row from its group maxima, by a workgroup of four waves.
+// The top k of a row from its group maxima, by a workgroup of four waves.  own: those
+// of groups threadIdx.x + 256 i.
 template <Dt DT>
 __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums& sums, float log_s,
-                                          const float* gmax, int n_groups, u64* list) {
+                                          const float* gmax, const float* own, int n_groups, u64* list) {
   typedef Row<DT> R;
-  constexpr int E = R::kE, kShift = R::kKeyShift, kBits = 32 - kShift;
+  constexpr int E = R::kE, kShift = R::kKeyShift;
   __shared__ uint2 s_tau[4];
   __shared__ u32 s_n[4];
   __shared__ u32 s_group[kMaxTop], s_sorted[kMaxTop];
@@ -374,12 +408,10 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   }
 
   if (tid < 4) s_n[tid] = 0;
-  constexpr int kHeld = 6;  // group maxima a thread keeps
   u32 held[kHeld], best = 0;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    const int g = tid + i * kThreads;
-    held[i] = g < n_groups ? key_of(gmax[g]) : 0;
+    held[i] = tid + i * kThreads < n_groups ? key_of(own[i]) : 0;
     best = max(best, held[i]);
   }
   for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) best = max(best, key_of(gmax[g]));
@@ -388,9 +420,9 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   // largest has k entries at or above it, so the largest of the waves' holds; and so does
   // the smallest of the (k / n)-th largest of n waves, which lies higher for values in no
   // order (top 20 of four waves: some 30 of 256 lanes are above it, not 80).  The first
-  // keeps the lists short whatever the order.  `drop` low bits of the keys are left at 0.
-  auto bound = [&](u32 key, int n, int drop) {
-    const uint2 t = kth_of_wave(key, k, (k + n - 1) / n, kBits, drop);
+  // keeps the lists short whatever the order.
+  auto bound = [&](u32 key, int n, int depth) {
+    const uint2 t = kth_of_wave(key, k, (k + n - 1) / n, depth);
     if (lane == 0) s_tau[wave] = t;
     __syncthreads();
     u32 hi = 0, lo = 0xffffffffu;
@@ -402,49 +434,79 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
     return max(hi, lo);
   };
 
-  // Plain search: a bound to 16 bits, every group that reaches it, every value of those
+  // Plain search: a bound to 8 bits of the lanes' range, every group that reaches it, every value of those
   // that reaches it, their ranks.  Some 1.5 k groups and 2 k values of a row in no order.
-  u32 tau = bound(best, min(4, n_groups / 64), kBits - 16);
-  auto list_group = [&](u32 key, u32 g) {
-    if (key >= tau) {
-      const u32 at = atomicAdd(&s_n[0], 1u);
-      if (at < (u32)kFastGroups) list[at] = g;
-    }
-  };
+  u32 tau = bound(best, min(4, n_groups / 64), 8);
+  // A bit for each hit, one atomic a lane and a loop over its bits: a branch for each
+  // value would cost most of what the row's workgroup takes.  (The counter's address as
+  // one that may differ between lanes: of one that does not, the compiler adds up the
+  // lanes' counts itself, lane after lane.)
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  u32 hits = 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i)
-    if (__ballot(held[i] >= tau)) list_group(held[i], tid + i * kThreads);
-  for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) list_group(key_of(gmax[g]), g);
+  for (int i = 0; i < kHeld; ++i) hits |= held[i] >= tau ? 1u << i : 0u;
+  if (hits) {
+    u32 at = atomicAdd(&s_n[zero], (u32)__popc(hits));
+    for (; hits && at < (u32)kFastGroups; hits &= hits - 1) list[at++] = tid + (__ffs(hits) - 1) * kThreads;
+  }
+  for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) {
+    if (key_of(gmax[g]) < tau) continue;
+    const u32 at = atomicAdd(&s_n[0], 1u);
+    if (at < (u32)kFastGroups) list[at] = g;
+  }
   __syncthreads();
   const int mis = (int)((uintptr_t)x & 15) / R::kEs;
   const u32 n_listed = s_n[0];
   if (n_listed <= (u32)kFastGroups) {
     constexpr int kFastPer = kFastGroups * kGroup / kThreads;
     u32x4 w[kFastPer];
-    int64_t i0[kFastPer];
+    int i0[kFastPer];
 #pragma unroll
     for (int q = 0; q < kFastPer; ++q) {
       const u32 c = tid + q * kThreads;
       i0[q] = INT_MAX;
       if (c / kGroup < n_listed) {
-        const int64_t ch = (int64_t)list[c / kGroup] * kGroup + c % kGroup;
+        const int ch = (int)list[c / kGroup] * kGroup + c % kGroup;
         i0[q] = ch * E - mis;
         w[q] = R::chunk(x, mis, a.cols, ch);
       }
     }
     __syncthreads();
+    // (as floats: there is no NaN, and -0 is not below 0)
+    const u32 none = key_of(-INFINITY);
+    const float least = tau <= none ? -INFINITY : key_float(tau, kShift);
+    static_assert(kFastPer * E <= 32, "a bit for each value");
+    u32 hit = 0;
 #pragma unroll
     for (int q = 0; q < kFastPer; ++q) {
       if (q * (kThreads / kGroup) >= (int)n_listed) break;  // workgroup-uniform
       float v[E];
       R::unpack(w[q], v);
+      u32 in = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const u32 key = key_of(v[e]);
-        if (key >= tau && i0[q] + e >= 0 && i0[q] + e < a.cols) {
-          const u32 at = atomicAdd(&s_n[1], 1u);
-          if (at < (u32)kFast) list[at] = entry(key, (u32)(i0[q] + e));
+      for (int e = 0; e < E; ++e) in |= v[e] >= least ? 1u << e : 0u;
+      // (what lies outside the row, and where no chunk was read, is not in)
+      const int lo = max(-i0[q], 0), hi = min(a.cols - i0[q], E);
+      hit |= (hi <= 0 ? 0u : in & ((1u << hi) - 1u) & ~((1u << lo) - 1u)) << (q * E);
+    }
+    if (hit) {
+      u32 at = atomicAdd(&s_n[zero + 1], (u32)__popc(hit));
+      for (; hit && at < (u32)kFast; hit &= hit - 1) {
+        const int bit = __ffs(hit) - 1, q = bit / E, d = bit % E * R::kEs / 4;
+        u32 pair = 0;
+        int i = 0;
+#pragma unroll
+        for (int y = 0; y < kFastPer; ++y) {
+          const u32 x01 = d & 1 ? w[y][1] : w[y][0], x23 = d & 1 ? w[y][3] : w[y][2];
+          pair = q == y ? (d & 2 ? x23 : x01) : pair;
+          i = q == y ? i0[y] : i;
         }
+        float v;
+        if constexpr (DT == Dt::FP32) v = __uint_as_float(pair);
+        else if constexpr (DT == Dt::BF16) v = bit & 1 ? bf16hi(pair) : bf16lo(pair);
+        else v = bit & 1 ? f16hi(pair) : f16lo(pair);
+        list[at++] = entry(key_of(v), (u32)(i + bit % E));
       }
     }
     __syncthreads();
@@ -458,7 +520,7 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   // Ordered search, for rows with many equal values (a mask of -inf) or values in order:
   // exact bounds, and of the entries equal to a bound only the first k of each wave.
   __syncthreads();
-  tau = bound(best, min(4, n_groups / 64), 0);
+  tau = bound(best, min(4, n_groups / 64), 32);
   // This wave's entries above the bound go to the list in any order, of those equal to it
   // the first k in index order (group g0 + lane, g0 rising).
   auto each_group = [&](auto f) {
@@ -520,7 +582,7 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
         if (i0[q] + e >= 0 && i0[q] + e < a.cols) best = max(best, key_of(v[e]));
     }
   }
-  tau = bound(best, min(4, (k * kGroup + 63) / 64), 0);
+  tau = bound(best, min(4, (k * kGroup + 63) / 64), 32);
   // Per lane: values above the bound (11 bits), ties in each of the two chunks (10 bits
   // each, of at most 8 x 64); one scan over the wave gives every lane its places.
   static_assert(kPer <= 2, "two counts of ties");
@@ -575,17 +637,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
   const int lane = threadIdx.x & 63;
   const int n_groups = a.n_seg * (kSegChunks / kGroup);
   const int64_t token = a.tokens[row];
-  const float xt = R::one(a.x + row * a.stride + (token >= 0 && token < a.cols ? token : 0) * R::kEs);
+  // All that the row's chain of steps starts from is asked for at once.
+  const float* gmax = a.ws_max + row * n_groups;
+  float own[kHeld];
+  if (a.top > 0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) own[i] = gmax[min((int)threadIdx.x + i * kThreads, n_groups - 1)];
+  }
   // every wave joins the sums for itself
   const f32x4* parts = reinterpret_cast<const f32x4*>(a.ws_sum) + row * a.n_seg * 4;
+  const int n_parts = a.n_seg * 4;
+  f32x4 first = parts[min(lane, n_parts - 1)];
+  const float xt = R::one(a.x + row * a.stride + (token >= 0 && token < a.cols ? token : 0) * R::kEs);
+  if (lane >= n_parts) first = f32x4{-INFINITY, 0.f, 0.f, 0.f};
   Sums s;
-  for (int i = lane; i < a.n_seg * 4; i += 64) s.m = fmaxf(s.m, parts[i][0]);
+  s.m = first[0];
+  for (int i = lane + 64; i < n_parts; i += 64) s.m = fmaxf(s.m, parts[i][0]);
   s.m = wave_max(s.m);
-  for (int i = lane; i < a.n_seg * 4; i += 64) join(s, parts[i]);
+  join(s, first);
+  for (int i = lane + 64; i < n_parts; i += 64) join(s, parts[i]);
   s.S = wave_sum(s.S);
   s.T = wave_sum(s.T);
   const float log_s = finish_sums<DT>(a, row, s, token, xt);
-  if (a.top > 0) write_top<DT>(a, row, s, log_s, a.ws_max + row * n_groups, n_groups, list);
+  if (a.top > 0) write_top<DT>(a, row, s, log_s, gmax, own, n_groups, list);
 }
 
 static int seg_of(int64_t cols, int es) {
@@ -598,7 +672,7 @@ template <Dt DT> static void launch(const Args& a, hipStream_t s) {
   // group maxima a lane of the second launch goes through, or its chunks' elements
   const int per = std::max(a.n_seg * (kSegChunks / kGroup) / kThreads + 1,
                            kMaxTop * kGroup / kThreads * Row<DT>::kE);
-  const size_t lds = a.top ? (size_t)std::max(list_cap(a.top, per), kFast + 8) * sizeof(u64) : 0;
+  const size_t lds = a.top ? (size_t)std::max(list_cap(a.top, per), kFast + kListPad) * sizeof(u64) : 0;
   hipLaunchKernelGGL((logprobs_segment_kernel<DT>), dim3((unsigned)(a.n_rows * a.n_seg)), dim3(kThreads), 0, s, a);
   hipLaunchKernelGGL((logprobs_merge_kernel<DT>), dim3((unsigned)a.n_rows), dim3(kThreads), lds, s, a);
 }
