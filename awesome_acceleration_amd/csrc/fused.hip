@@ -117,9 +117,7 @@ __device__ __forceinline__ void norm_rope_head(const Qk4Args& a, int64_t t, int 
   int r;
   kv4::split_row(a.c, crow, &blk, &r);
   unsigned char* page = a.c.page(blk, kh) + (value ? a.c.page_bytes() : 0);
-  float x[8];
-  unpack8<DT>(packed, x);
-  kv4::write_row<DT>(x, li, page + r * kv4::kRowBytes,
+  kv4::write_row<DT>({packed}, li, page + r * kv4::kRowBytes,
                      reinterpret_cast<u32*>(page + a.c.block_size * kv4::kRowBytes + r * kv4::kScaleBytes));
 }
 

@@ -16,8 +16,8 @@
 // fall into one tile of the cache (the usual case) the codes go out as 1 KiB in one
 // piece.  Bound by memory: 512 bytes in (16-bit types) and 136 out a token and head.
 // Measured: 32,768 tokens of 8 heads in bf16 27 us each way, 6.3 TB/s (rows that a
-// prefill has just made are in the last-level cache); 262,144 tokens 271 us stored, 5.0
-// TB/s, and 238 loaded, 5.7; fp32 5.2 and 7.0.  The load's results go out with
+// prefill has just made are in the last-level cache); 262,144 tokens 258 us stored, 5.3
+// TB/s, and 238 loaded, 5.7; fp32 5.9 and 7.0.  The load's results go out with
 // non-temporal stores (261 us without).
 #include "kv4_quant.h"
 
@@ -35,38 +35,37 @@ struct StoreArgs {
   int32_t max_blocks;
 };
 
-template <Dt DT> __device__ __forceinline__ float elem_f32(const char* p);
-template <> __device__ __forceinline__ float elem_f32<Dt::BF16>(const char* p) {
-  return bf16lo(*reinterpret_cast<const u16*>(p));
-}
-template <> __device__ __forceinline__ float elem_f32<Dt::FP16>(const char* p) {
-  return (float)*reinterpret_cast<const _Float16*>(p);
-}
-template <> __device__ __forceinline__ float elem_f32<Dt::FP32>(const char* p) {
-  return *reinterpret_cast<const float*>(p);
-}
+// How a store reads its rows: one element at a time (any alignment), 16 bytes, or 16 bytes
+// past the caches.
+enum class Read { Elements, Wide, Stream };
 
-// A row in the layout of write_row (kv4_quant.h).
-template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const char* row, int l, float* x) {
+// A lane's piece of a row.
+template <typename V, Read R> __device__ __forceinline__ V get(const V* p) {
+  if constexpr (R == Read::Stream) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <Dt DT, Read R> __device__ __forceinline__ Piece<DT> load_piece(const char* row, int l) {
+  Piece<DT> x;
   if constexpr (DT == Dt::FP32) {
+    const float* p = reinterpret_cast<const float*>(row) + 4 * l;
+    if constexpr (R != Read::Elements) {
+      x.a = get<f32x4, R>(reinterpret_cast<const f32x4*>(p));
+      x.b = get<f32x4, R>(reinterpret_cast<const f32x4*>(p + 64));
+    } else {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const char* p = row + (64 * q + 4 * l) * 4;
-      if constexpr (ALIGNED) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * q + i] = v[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * q + i] = elem_f32<DT>(p + 4 * i);
+      for (int i = 0; i < 4; ++i) {
+        x.a[i] = p[i];
+        x.b[i] = p[64 + i];
       }
     }
-  } else if constexpr (ALIGNED) {
-    Elem<DT>::unpack8(*reinterpret_cast<const u32x4*>(row + l * 16), x);
+  } else if constexpr (R != Read::Elements) {
+    x.w = get<u32x4, R>(reinterpret_cast<const u32x4*>(row) + l);
   } else {
+    const u16* p = reinterpret_cast<const u16*>(row) + 8 * l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = elem_f32<DT>(row + l * 16 + i * 2);
+    for (int i = 0; i < 4; ++i) x.w[i] = p[2 * i] | (u32)p[2 * i + 1] << 16;
   }
+  return x;
 }
 
 // Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16,
@@ -74,7 +73,7 @@ template <Dt DT, bool ALIGNED> __device__ __forceinline__ void load_row(const ch
 constexpr int kHeads = 2;
 constexpr int64_t kMaxGroups = 1 << 24;  // a launch's threads are numbered in 32 bits
 
-template <Dt DT, bool ALIGNED, bool PAGED>
+template <Dt DT, Read R, bool PAGED>
 __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   const int groups = (a.c.hkv + kHeads - 1) / kHeads;
   const int h0 = (int)(blockIdx.x % groups) * kHeads;
@@ -82,12 +81,12 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   const int l = threadIdx.x & 15;
   if (t >= a.n_tokens) return;  // whole groups of 16 lanes
   constexpr int es = DT == Dt::FP32 ? 4 : 2;
-  float x[kHeads][2][8];
+  Piece<DT> x[kHeads][2];
 #pragma unroll
   for (int h = 0; h < kHeads; ++h)
 #pragma unroll
     for (int i = 0; i < 2; ++i)  // (a head past the last: the last once more, not written)
-      load_row<DT, ALIGNED>(a.src[i] + t * a.stride[i] + (int64_t)min(h0 + h, a.c.hkv - 1) * kDim * es, l, x[h][i]);
+      x[h][i] = load_piece<DT, R>(a.src[i] + t * a.stride[i] + (int64_t)min(h0 + h, a.c.hkv - 1) * kDim * es, l);
   int64_t blk;
   int r;
   if constexpr (PAGED) {
@@ -188,12 +187,24 @@ static int elem_bytes(int32_t dtype) {
   return dtype == AAC_DTYPE_FP32 ? 4 : dtype == AAC_DTYPE_BF16 || dtype == AAC_DTYPE_FP16 ? 2 : 0;
 }
 
+// Bytes of rows from which a store reads past the caches: rows that a prefill has just made
+// are partly in the 256 MiB last-level cache (bf16, 8 heads, us: 32,768 tokens 26.9 and
+// 31.5 past it, 262,144 273 and 258; 131,072 of fp32 234 and 207).
+constexpr int64_t kStreamBytes = int64_t(512) << 20;
+
 template <Dt DT, bool PAGED> static void launch_store_t(const StoreArgs& a, bool aligned, hipStream_t s) {
   const dim3 grid((unsigned)(cdiv(a.n_tokens, 16) * cdiv(a.c.hkv, kHeads)));
-  if (aligned)
-    hipLaunchKernelGGL((kv4_store_kernel<DT, true, PAGED>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((kv4_store_kernel<DT, false, PAGED>), grid, dim3(256), 0, s, a);
+  if (!aligned) {
+    hipLaunchKernelGGL((kv4_store_kernel<DT, Read::Elements, PAGED>), grid, dim3(256), 0, s, a);
+    return;
+  }
+  if constexpr (!PAGED) {  // (an append is of one token a sequence)
+    if (a.n_tokens * a.c.hkv * kDim * 2 * (DT == Dt::FP32 ? 4 : 2) >= kStreamBytes) {
+      hipLaunchKernelGGL((kv4_store_kernel<DT, Read::Stream, PAGED>), grid, dim3(256), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((kv4_store_kernel<DT, Read::Wide, PAGED>), grid, dim3(256), 0, s, a);
 }
 
 template <bool PAGED>

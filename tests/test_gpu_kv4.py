@@ -438,3 +438,27 @@ def test_contexts_to_the_last_token_of_31_bits(gpu):
     kv = torch.zeros((2, 1, 1, 128), dtype=torch.bfloat16, device=gpu)
     out = kv4.flash_attn_with_kv4cache(q[:, None], cache, k=kv, v=kv + 1, cache_seqlens=lens, block_table=tables)
     assert (out == 1).all()
+
+
+@pytest.mark.parametrize("dtype, step", [("bf16", 12), ("fp16", 96)])
+def test_store_of_every_16_bit_value(gpu, dtype, step):
+    """Blocks of 32 patterns over three powers of two, from every pattern on: each value,
+    subnormal, infinite and NaN ones too, under every scale that gives it a code."""
+    rs = np.random.RandomState(40)
+    first = np.arange(1 << 15)[:, None]
+    bits = np.minimum(first + step * np.arange(32), 0x7fff) | rs.randint(0, 2, (1 << 15, 32)) << 15
+    bits = np.take_along_axis(bits, rs.rand(1 << 15, 32).argsort(1), 1).astype(np.uint16)
+    k = torch.from_numpy(bits.view(np.int16).reshape(-1, 1, 128)).view(DTYPES[dtype])
+    n = len(k)
+    want = np.zeros((n // 256, 1, 2, 256 * 68), np.uint8)
+    with np.errstate(all="ignore"):
+        oracle4.store(want, 256, f64(k), f64(k), range(n))
+    cache = torch.from_numpy(np.full_like(want, 99)).to(gpu)
+    kv4.kv4_store(k.to(gpu), k.to(gpu), cache, torch.arange(n, device=gpu))
+    assert np.array_equal(_cache_np(cache), want)
+    # and where rows start off 16 bytes
+    odd = torch.zeros((n, 130), dtype=k.dtype, device=gpu)[:, 1:129].view(n, 1, 128)
+    odd.copy_(k)
+    again = torch.zeros_like(cache)
+    kv4.kv4_store(odd, odd, again, torch.arange(n, device=gpu))
+    assert torch.equal(again, cache)
