@@ -31,8 +31,8 @@ template <> struct Piece<Dt::FP32> {
 
 // Quantises a row and writes its codes and scales.  The 16-bit types stay as they are:
 // their bit patterns, without the sign, are in order of size, two in an instruction, and
-// the conversion takes them in pairs (unpacked to floats first: 262,144 tokens of 8 heads
-// 271 us against AAA).
+// the conversion takes them in pairs (unpacked to floats first 4,096 tokens of 8 heads
+// take 4.6 us against 4.4, and 16,000 in the fused store 44.0 against 42.8).
 template <Dt DT>
 __device__ __forceinline__ void write_row(const Piece<DT>& x, int l, unsigned char* codes, u32* scales) {
   u32 s4;

@@ -15,9 +15,10 @@
 // the 16 lanes of a DPP row hold.  The second, a workgroup a row, joins the sums and
 // finds the top k from the group maxima: a value above a bound that k groups reach
 // lies in a group that reaches it, so only some k groups of 256 bytes are read again.
-// Bound by the read of the logits (bf16, us): 256 x 151,936 17 of the first launch and
-// 3 (no alternatives) to 10 (20) of the second, whose chain of small steps is its
-// cost; 1500 rows 76, 6.0 TB/s (fp32 6.5).  Tried instead: candidates collected in the
+// Bound by the read of the logits (bf16, us): 256 x 151,936 16.6 of the first launch and
+// 5.4 (top 20) of the second, whose chain of small steps is its cost (cycles of a row's
+// workgroup: 2.8k until the sums are there, 1.5k for the bound, 0.9k and 2.9k for the
+// groups, 2k for the values, 1.1k for the ranks); 1500 rows 76, 6.0 TB/s (fp32 6.5).  Tried instead: candidates collected in the
 // first launch, where every wave goes through nearly all of its values again (197
 // against 17); one launch with a workgroup of 16 waves a row, maxima in LDS (as fast at
 // 256 rows, 30% slower at 300, 512 and 3900, where rows do not fill the GPU evenly

@@ -201,3 +201,42 @@ def test_sizes_past_32_bit_offsets_are_refused():
     assert L.aac_token_logprobs(P, 100, 1 << 24, 100, P, 0, P, P, P, P, P, 1 << 40, 0, None) == -2
     # a table's capacity passes 2^31 tokens: the plan stays within it (64 partitions of 2^25)
     assert L.aac_kv4_decode_workspace_bytes(1, 1, 1, 128, big, 1 << 20, 0, 0) == 64 * 129 * 4
+
+
+def test_oracle_decode_is_torchs_attention_over_the_values():
+    rs = np.random.RandomState(2)
+    bs, hkv, hq, lens = 16, 2, 6, [5, 33, 0]
+    tables = rs.permutation(9).reshape(3, 3)
+    cache = np.full((9, hkv, 2, bs * 68), 255, np.uint8)
+    kv = {}
+    for b, n in enumerate(lens):
+        p = np.arange(n)
+        kv[b] = rs.standard_normal((2, n, hkv, 128))
+        oracle4.store(cache, bs, *kv[b], tables[b, p // bs] * bs + p % bs)
+    q = rs.standard_normal((3, hq, 128))
+    out, absv, _ = oracle4.decode(q, cache, bs, tables, lens, 0.09)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        k, v = (torch.from_numpy(oracle4.values(*oracle4.quantise(x))).transpose(0, 1).repeat_interleave(3, 0)
+                for x in kv[b])
+        att = lambda v: torch.nn.functional.scaled_dot_product_attention(  # noqa: E731
+            torch.from_numpy(q[b])[:, None], k, v, scale=0.09)[:, 0].numpy()
+        assert np.allclose(out[b], att(v), rtol=1e-12, atol=1e-13)
+        assert np.allclose(absv[b], att(v.abs()), rtol=1e-12, atol=1e-13)
+
+
+def test_oracle_scores_are_torchs():
+    rs = np.random.RandomState(3)
+    x = rs.standard_normal((6, 200)) * 5
+    x[1, :150] = -np.inf
+    x[2] = np.round(x[2])  # equal values
+    t = torch.from_numpy(x)
+    assert np.allclose(oracle4.log_softmax(x), torch.log_softmax(t, -1).numpy(), rtol=1e-13)
+    assert np.allclose(oracle4.entropy(x), torch.distributions.Categorical(logits=t).entropy().numpy(), rtol=1e-12)
+    # the first index first among equals: a stable sort
+    order = torch.sort(t, dim=-1, descending=True, stable=True).indices.numpy()
+    assert np.array_equal(oracle4.top(x, 20), order[:, :20])
+    x[4, 7] = np.nan
+    assert oracle4.top(x, 1)[4, 0] == 7 == int(torch.from_numpy(x[4]).argmax())
