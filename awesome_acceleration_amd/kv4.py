@@ -171,8 +171,9 @@ def kv4_export(storage: torch.Tensor, block_table, length: int,
 
 def kv4_import(k: torch.Tensor, v: torch.Tensor, storage: torch.Tensor, block_table) -> None:
     """The reverse of ``kv4_export``: quantises ``k`` and ``v`` ``[n_layers, length, Hkv, 128]``
-    into the sequence's blocks; those outside the pool are skipped.  Rows exported in bf16 or
-    fp32 come back as they were held, byte for byte."""
+    into the sequence's blocks; those outside the pool are skipped (``IndexError`` for them
+    with ``AAC_CHECK=1``).  Rows exported in bf16 or fp32 come back as they were held, byte
+    for byte."""
     _require(k.dim() == 4 and k.shape == v.shape and k.shape[0] == storage.shape[0],
              "k and v must be [n_layers, length, Hkv, 128]")
     kv4_store(k.flatten(0, 1), v.flatten(0, 1), storage.flatten(0, 1),
@@ -255,7 +256,7 @@ def decode_paged_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torc
             raise RuntimeError("out must be [B, Hq, 128] like q")
         ost = st[0] if n > 1 else row
     _decode(q, qst[0] if n > 1 else row, n, hq, kv_cache, cache, block_tables, context_lens, None, None, 0,
-            0, _scale(softmax_scale, d), int(max_context_len or 0), int(partition_tokens), out, ost)
+            0, _scale(softmax_scale, d), min(int(max_context_len or 0), 0x7fffffff), int(partition_tokens), out, ost)
     return out
 
 
@@ -308,5 +309,5 @@ def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
         ks, vs = (kst[0], vst[0]) if n > 1 else (row, row)
     row = hq * d
     _decode(q, qst[0] if n > 1 else row, n, hq, kv_cache, cache, block_table, cache_seqlens, kp, vp, ks, vs,
-            _scale(softmax_scale, d), int(max_context_len or 0), 0, out, row)
+            _scale(softmax_scale, d), min(int(max_context_len or 0), 0x7fffffff), 0, out, row)
     return out

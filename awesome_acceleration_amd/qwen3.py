@@ -185,6 +185,8 @@ class PagedKV4Cache:
         seqlens = {int(lp["seqlen"]) for lp in layers}
         if len(seqlens) != 1:
             raise RuntimeError("payload layers disagree on seqlen")
+        if length < 0 or any(lp[n].shape[0] < length for lp in layers for n in "kv"):
+            raise RuntimeError(f"payload layers hold fewer than {length} tokens")
         k, v = (torch.stack([lp[n][:length] for lp in layers]).to(self.storage.device) for n in "kv")
         kv4.kv4_import(k, v, self.storage, block_table)
         return seqlens.pop()

@@ -154,6 +154,9 @@ def test_payload_moves_between_the_caches(gpu):
     assert again.import_request_kv([0, 7, 3], out, 70) == 71
     assert torch.equal(again.storage, four.storage)
     assert wide.import_request_kv([5, 1, 2], out, 70) == 71
+    for length in (71, -1):
+        with pytest.raises(RuntimeError, match="tokens"):
+            four.import_request_kv([0, 7, 3], out, length)
     with pytest.raises(ValueError, match="Layer count"):
         four.import_request_kv([0], {"layers": out["layers"][:1]}, 1)
     assert four.nbytes * 512 == wide.storage.numel() * 2 * 136
