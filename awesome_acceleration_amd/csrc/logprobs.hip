@@ -281,20 +281,21 @@ __device__ __forceinline__ uint2 wave_range(u32 key) {
   return make_uint2(l, h);
 }
 
-// The wave's k-th and j-th largest of 64 keys, bit by bit, `depth` of the bits in which the
-// keys differ; those below are left at 0, so that the result is at most that key.  A
-// step takes some 130 cycles, of counts that only the scalar unit takes (two bits a step
-// cost more: three counts for each key's two bits).
-__device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, int depth) {
+// The wave's k-th and j-th largest of 64 keys, bit by bit from the first in which the keys
+// differ; near: down to a 16th of the way from there to the largest key, the rest left
+// at 0, so that the result is at most that key.  A step takes some 130 cycles, of counts
+// that only the scalar unit takes (two bits a step cost more: three counts for each key's
+// two bits).
+__device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, bool near) {
   const uint2 range = wave_range(key);
   const int top = 32 - __builtin_clz(range.x ^ range.y | 1u);  // bits from here up are alike
   u32 tk = top < 32 ? range.y >> top << top : 0, tj = tk;
-  const int end = max(top - depth, 0);
 #pragma unroll 1
-  for (int s = top - 1; s >= end; --s) {
+  for (int s = top - 1; s >= 0; --s) {
     const u32 bit = 1u << s;
     if ((int)__popcll(__ballot(key >= (tk | bit))) >= k) tk |= bit;
     if ((int)__popcll(__ballot(key >= (tj | bit))) >= j) tj |= bit;
+    if (near && (range.y - tk) >> s >= 16) break;
   }
   return make_uint2(tk, tj);
 }
@@ -332,7 +333,7 @@ template <typename F> __device__ __forceinline__ void ranked(u64* list, int n, i
 // lanes have a key above the bound, `per` entries each, and k entries equal to it are kept.
 __host__ __device__ inline int list_cap(int k, int per) { return 4 * ((k - 1) * per + k) + kListPad; }
 constexpr int kFast = 512;      // entries the list holds in the plain search
-constexpr int kFastGroups = 64;
+constexpr int kFastGroups = 128;  // groups it takes, 64 at a time
 constexpr int kHeld = 6;  // group maxima a thread keeps
 
 // (m, S, T) of one part of a row, joined with others' about the row's m.  r: d of x = m.
@@ -368,7 +369,7 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   constexpr int E = R::kE, kShift = R::kKeyShift;
   __shared__ uint2 s_tau[4];
   __shared__ u32 s_n[4];
-  __shared__ u32 s_group[kMaxTop], s_sorted[kMaxTop];
+  __shared__ u32 s_group[kMaxTop], s_sorted[kMaxTop], s_list[kFastGroups];
   __shared__ u64 s_best[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const char* x = a.x + row * a.stride;
@@ -422,8 +423,8 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   // the smallest of the (k / n)-th largest of n waves, which lies higher for values in no
   // order (top 20 of four waves: some 30 of 256 lanes are above it, not 80).  The first
   // keeps the lists short whatever the order.
-  auto bound = [&](u32 key, int n, int depth) {
-    const uint2 t = kth_of_wave(key, k, (k + n - 1) / n, depth);
+  auto bound = [&](u32 key, int n, bool near) {
+    const uint2 t = kth_of_wave(key, k, (k + n - 1) / n, near);
     if (lane == 0) s_tau[wave] = t;
     __syncthreads();
     u32 hi = 0, lo = 0xffffffffu;
@@ -435,79 +436,107 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
     return max(hi, lo);
   };
 
-  // Plain search: a bound to 8 bits of the lanes' range, every group that reaches it, every value of those
-  // that reaches it, their ranks.  Some 1.5 k groups and 2 k values of a row in no order.
-  u32 tau = bound(best, min(4, n_groups / 64), 8);
+  // Plain search: a bound, every group that reaches it, every value of those that reaches
+  // it, their ranks.  Some 1.5 k groups and 2 k values of a row in no order.  A row of few
+  // groups is read whole, and the bound comes from the lanes' values: of some k groups
+  // the k-th largest maximum says little.  (256 rows, us against the ordered search below:
+  // 2,048 columns top 20 10.0 and 14.2; 32,000, where more than 64 groups are listed in
+  // some row, top 32 13.8 and 17.9.)
+  constexpr int kRound = 64;
+  const int mis = (int)((uintptr_t)x & 15) / R::kEs;
+  const int in_row = (a.cols + mis + kGroup * E - 1) / (kGroup * E);
+  const bool few = in_row <= kRound;
   // A bit for each hit, one atomic a lane and a loop over its bits: a branch for each
   // value would cost most of what the row's workgroup takes.  (The counter's address as
   // one that may differ between lanes: of one that does not, the compiler adds up the
   // lanes' counts itself, lane after lane.)
   int zero = 0;
   asm volatile("" : "+v"(zero));
-  u32 hits = 0;
+  u32 tau = 0;
+  if (!few) {
+    tau = bound(best, min(4, n_groups / 64), true);
+    u32 hits = 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) hits |= held[i] >= tau ? 1u << i : 0u;
-  if (hits) {
-    u32 at = atomicAdd(&s_n[zero], (u32)__popc(hits));
-    for (; hits && at < (u32)kFastGroups; hits &= hits - 1) list[at++] = tid + (__ffs(hits) - 1) * kThreads;
-  }
-  for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) {
-    if (key_of(gmax[g]) < tau) continue;
-    const u32 at = atomicAdd(&s_n[0], 1u);
-    if (at < (u32)kFastGroups) list[at] = g;
+    for (int i = 0; i < kHeld; ++i) hits |= held[i] >= tau ? 1u << i : 0u;
+    if (hits) {
+      u32 at = atomicAdd(&s_n[zero], (u32)__popc(hits));
+      for (; hits && at < (u32)kFastGroups; hits &= hits - 1) s_list[at++] = tid + (__ffs(hits) - 1) * kThreads;
+    }
+    for (int g = tid + kHeld * kThreads; g < n_groups; g += kThreads) {
+      if (key_of(gmax[g]) < tau) continue;
+      const u32 at = atomicAdd(&s_n[0], 1u);
+      if (at < (u32)kFastGroups) s_list[at] = g;
+    }
+  } else if (tid < in_row) {
+    s_list[tid] = tid;
   }
   __syncthreads();
-  const int mis = (int)((uintptr_t)x & 15) / R::kEs;
-  const u32 n_listed = s_n[0];
+  const u32 n_listed = few ? in_row : s_n[0];
   if (n_listed <= (u32)kFastGroups) {
-    constexpr int kFastPer = kFastGroups * kGroup / kThreads;
-    u32x4 w[kFastPer];
-    int i0[kFastPer];
+    constexpr int kFastPer = kRound * kGroup / kThreads;
+#pragma unroll 1
+    for (u32 g0 = 0; g0 < n_listed; g0 += kRound) {
+      u32x4 w[kFastPer];
+      int i0[kFastPer];
 #pragma unroll
-    for (int q = 0; q < kFastPer; ++q) {
-      const u32 c = tid + q * kThreads;
-      i0[q] = INT_MAX;
-      if (c / kGroup < n_listed) {
-        const int ch = (int)list[c / kGroup] * kGroup + c % kGroup;
-        i0[q] = ch * E - mis;
-        w[q] = R::chunk(x, mis, a.cols, ch);
-      }
-    }
-    __syncthreads();
-    // (as floats: there is no NaN, and -0 is not below 0)
-    const u32 none = key_of(-INFINITY);
-    const float least = tau <= none ? -INFINITY : key_float(tau, kShift);
-    static_assert(kFastPer * E <= 32, "a bit for each value");
-    u32 hit = 0;
-#pragma unroll
-    for (int q = 0; q < kFastPer; ++q) {
-      if (q * (kThreads / kGroup) >= (int)n_listed) break;  // workgroup-uniform
-      float v[E];
-      R::unpack(w[q], v);
-      u32 in = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) in |= v[e] >= least ? 1u << e : 0u;
-      // (what lies outside the row, and where no chunk was read, is not in)
-      const int lo = max(-i0[q], 0), hi = min(a.cols - i0[q], E);
-      hit |= (hi <= 0 ? 0u : in & ((1u << hi) - 1u) & ~((1u << lo) - 1u)) << (q * E);
-    }
-    if (hit) {
-      u32 at = atomicAdd(&s_n[zero + 1], (u32)__popc(hit));
-      for (; hit && at < (u32)kFast; hit &= hit - 1) {
-        const int bit = __ffs(hit) - 1, q = bit / E, d = bit % E * R::kEs / 4;
-        u32 pair = 0;
-        int i = 0;
-#pragma unroll
-        for (int y = 0; y < kFastPer; ++y) {
-          const u32 x01 = d & 1 ? w[y][1] : w[y][0], x23 = d & 1 ? w[y][3] : w[y][2];
-          pair = q == y ? (d & 2 ? x23 : x01) : pair;
-          i = q == y ? i0[y] : i;
+      for (int q = 0; q < kFastPer; ++q) {
+        const u32 c = tid + q * kThreads;
+        i0[q] = INT_MAX;
+        if (g0 + c / kGroup < n_listed) {
+          const int ch = (int)s_list[g0 + c / kGroup] * kGroup + c % kGroup;
+          i0[q] = ch * E - mis;
+          w[q] = R::chunk(x, mis, a.cols, ch);
         }
-        float v;
-        if constexpr (DT == Dt::FP32) v = __uint_as_float(pair);
-        else if constexpr (DT == Dt::BF16) v = bit & 1 ? bf16hi(pair) : bf16lo(pair);
-        else v = bit & 1 ? f16hi(pair) : f16lo(pair);
-        list[at++] = entry(key_of(v), (u32)(i + bit % E));
+      }
+      if (few) {
+        u32 mine = 0;
+#pragma unroll
+        for (int q = 0; q < kFastPer; ++q) {
+          if (i0[q] == INT_MAX) continue;
+          float v[E];
+          R::unpack(w[q], v);
+          float m = v[0];
+#pragma unroll
+          for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+          mine = max(mine, key_of(m));
+        }
+        tau = bound(mine, min(4, max(1, in_row * kGroup / 64)), true);
+      }
+      // (as floats: there is no NaN, and -0 is not below 0)
+      const u32 none = key_of(-INFINITY);
+      const float least = tau <= none ? -INFINITY : key_float(tau, kShift);
+      static_assert(kFastPer * E <= 32, "a bit for each value");
+      u32 hit = 0;
+#pragma unroll
+      for (int q = 0; q < kFastPer; ++q) {
+        if (g0 + q * (kThreads / kGroup) >= n_listed) break;  // workgroup-uniform
+        float v[E];
+        R::unpack(w[q], v);
+        u32 in = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) in |= v[e] >= least ? 1u << e : 0u;
+        // (what lies outside the row, and where no chunk was read, is not in)
+        const int lo = max(-i0[q], 0), hi = min(a.cols - i0[q], E);
+        hit |= (hi <= 0 ? 0u : in & ((1u << hi) - 1u) & ~((1u << lo) - 1u)) << (q * E);
+      }
+      if (hit) {
+        u32 at = atomicAdd(&s_n[zero + 1], (u32)__popc(hit));
+        for (; hit && at < (u32)kFast; hit &= hit - 1) {
+          const int bit = __ffs(hit) - 1, q = bit / E, d = bit % E * R::kEs / 4;
+          u32 pair = 0;
+          int i = 0;
+#pragma unroll
+          for (int y = 0; y < kFastPer; ++y) {
+            const u32 x01 = d & 1 ? w[y][1] : w[y][0], x23 = d & 1 ? w[y][3] : w[y][2];
+            pair = q == y ? (d & 2 ? x23 : x01) : pair;
+            i = q == y ? i0[y] : i;
+          }
+          float v;
+          if constexpr (DT == Dt::FP32) v = __uint_as_float(pair);
+          else if constexpr (DT == Dt::BF16) v = bit & 1 ? bf16hi(pair) : bf16lo(pair);
+          else v = bit & 1 ? f16hi(pair) : f16lo(pair);
+          list[at++] = entry(key_of(v), (u32)(i + bit % E));
+        }
       }
     }
     __syncthreads();
@@ -521,7 +550,7 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
   // Ordered search, for rows with many equal values (a mask of -inf) or values in order:
   // exact bounds, and of the entries equal to a bound only the first k of each wave.
   __syncthreads();
-  tau = bound(best, min(4, n_groups / 64), 32);
+  tau = bound(best, min(4, n_groups / 64), false);
   // This wave's entries above the bound go to the list in any order, of those equal to it
   // the first k in index order (group g0 + lane, g0 rising).
   auto each_group = [&](auto f) {
@@ -583,7 +612,7 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t row, const Sums
         if (i0[q] + e >= 0 && i0[q] + e < a.cols) best = max(best, key_of(v[e]));
     }
   }
-  tau = bound(best, min(4, (k * kGroup + 63) / 64), 32);
+  tau = bound(best, min(4, (k * kGroup + 63) / 64), false);
   // Per lane: values above the bound (11 bits), ties in each of the two chunks (10 bits
   // each, of at most 8 x 64); one scan over the wave gives every lane its places.
   static_assert(kPer <= 2, "two counts of ties");

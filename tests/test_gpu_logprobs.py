@@ -177,3 +177,20 @@ def test_captured_replayed_and_on_another_stream(gpu):
         for a, b, c in zip(m, eager, other):
             assert torch.equal(a, b) and torch.equal(c, b)
     _check(x, t, 7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_about_the_most_groups_read_whole(gpu, dtype):
+    """Columns about 64 and 128 groups of maxima, from every place of a 16-byte boundary on,
+    and values whose largest lie in one group or in every one."""
+    rs = np.random.RandomState(30)
+    group = 64 if dtype == "fp32" else 128
+    for cols in (64 * group, 128 * group):
+        for off in (0, 1, 3, 7):
+            n = cols + int(rs.randint(-9, 10))
+            wide = _rows(gpu, rs, 3, n + 16, dtype)
+            x = wide[:, off:off + n]
+            x[1, 700:732] += 30.0                 # the top within one group and its neighbour
+            x[2, ::group] += 30.0                 # a large one in each
+            for k in (1, 20, 32):
+                _check(x, _tokens(gpu, rs, 3, n), k, f"{n} columns from {off}, top {k}")
