@@ -240,3 +240,13 @@ def test_oracle_scores_are_torchs():
     assert np.array_equal(oracle4.top(x, 20), order[:, :20])
     x[4, 7] = np.nan
     assert oracle4.top(x, 1)[4, 0] == 7 == int(torch.from_numpy(x[4]).argmax())
+
+
+def test_limits_are_the_headers():
+    import re
+    from pathlib import Path
+    text = (Path(__file__).parent.parent / "include" / "aac_attn.h").read_text()
+    limit = lambda name: eval(re.search(rf"#define {name} (.+)", text)[1])  # noqa: E731
+    assert limit("AAC_STEP_MAPS_MAX_SEQS") == paged.MAX_MAP_SEQS
+    assert limit("AAC_LOGPROBS_MAX_TOP") == fused.MAX_TOP_LOGPROBS
+    assert limit("AAC_LOGPROBS_MAX_COLS") == fused.MAX_LOGPROB_COLS
