@@ -276,9 +276,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     if check_mode() and rows and int(tokens.max()) >= cols:
         raise IndexError(f"index {int(tokens.max())} is out of bounds for dimension 1 with size {cols}")
     dev = logits.device
-    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
+    lp = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lp)
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    ids = torch.empty_like(top, dtype=torch.int64)
     out = TokenLogprobs(lp, ent, top, ids)
     if rows == 0:
         return out

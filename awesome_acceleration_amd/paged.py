@@ -311,7 +311,8 @@ def build_step_maps(new_lens: torch.Tensor, cached_lens: torch.Tensor | None,
         raise RuntimeError("block_size must be positive")
     if not 0 <= n_tokens < 1 << 31:
         raise RuntimeError("n_tokens must be within [0, 2^31)")
-    pos, slots = torch.empty((2, n_tokens), dtype=torch.int64, device=new_lens.device).unbind()
+    pos = torch.empty(n_tokens, dtype=torch.int64, device=new_lens.device)
+    slots = torch.empty_like(pos)
     cu, ctx, taken = torch.empty(2 * n + 2, dtype=torch.int32, device=new_lens.device).split((n + 1, n, 1))
     at = cu.data_ptr()
     n_free = free = 0
