@@ -74,6 +74,7 @@ struct DecArgs {
   uint64_t magic;
   int32_t shift;
   int32_t cap_tiles;  // of the tables
+  int32_t alone;      // the longest context that one wave takes
 };
 
 __device__ __forceinline__ int context_len(const DecArgs& a, int len) {
@@ -123,14 +124,16 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kWaveLds];
   __shared__ u32 s_scale[4][2][kStep];
   __shared__ float sm_m[4][16], sm_l[4][16];
-  const int h = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
+  const int part = blockIdx.y, b = blockIdx.z;
+  int h = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // The waves take steps in turn.  A wave's first table entry does not depend on the
   // context's length, so both are on their way together.
   typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
   const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
-  const int beg = part * a.part_tokens, t_first = beg + kStep * wave;
+  const int beg = part * a.part_tokens;
+  int t_first = beg + kStep * wave, stride = 4 * kStep;
   const int tpb = a.c.block_size / kTile;
   constexpr int kLooks = WIDE ? 1 : 4;
   struct Where {
@@ -157,6 +160,17 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
         store_out2<DT>(a.out, (int64_t)b * a.out_stride + (int64_t)h * a.g * kDim + 2 * i, 0.f, 0.f);
     }
     return;
+  }
+  // A short context of many: each of the group's waves takes a head to itself, and three of
+  // four workgroups end here.  Which one stays moves on from sequence to sequence, and
+  // once more every fourth: workgroups go round the XCDs and their shader engines in turn,
+  // and every fourth would meet the same engine.
+  const bool alone = ctx <= a.alone;
+  if (alone) {
+    if ((h ^ (b + (b >> 2))) & 3) return;
+    h = (h & ~3) + wave;
+    t_first = 0;
+    stride = kStep;
   }
   const int end = beg + min(ctx - beg, a.part_tokens), n_tiles = (end + kTile - 1) / kTile;
 
@@ -249,7 +263,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   float m = -INFINITY, ref = 0.f, l = 0.f;
   const float margin = kRescale / cs;
 
-  look(t_first + 4 * kStep, n_tiles, w);
+  look(t_first + stride, n_tiles, w);
   // The scales have arrived before the loop: with them among the loads under way at its
   // entry, the compiler waits for every load at its top (the counts of both ways in
   // have to agree).
@@ -257,7 +271,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   __attribute__((address_space(3))) u32* sc = (__attribute__((address_space(3))) u32*)&s_scale[wave][0][0];
   const __attribute__((address_space(3))) unsigned char* sc8 =
       (const __attribute__((address_space(3))) unsigned char*)&s_scale[wave][0][0] + n * kScaleBytes + j;
-  for (int t0 = t_first; t0 < end; t0 += 4 * kStep) {
+  for (int t0 = t_first; t0 < end; t0 += stride) {
     sc[lane] = r.ks;
     sc[kStep + lane] = r.vs;
     asm volatile("" ::: "memory");
@@ -277,7 +291,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
       }
       // (kept here: asked for earlier, the rows need registers of their own and a copy)
       __builtin_amdgcn_sched_barrier(0);
-      r.k[k] = load_codes(t0 + 4 * kStep, w, k, false);
+      r.k[k] = load_codes(t0 + stride, w, k, false);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (t0 + kStep > end) {  // the last rows: those past the end stand for nothing
@@ -340,7 +354,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
           *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(vb + (wo ^ i * 16) + k * 4096) =
               values8(r.v[2 * q + k][i], sv);
         __builtin_amdgcn_sched_barrier(0);
-        r.v[2 * q + k] = load_codes(t0 + 4 * kStep, w, 2 * q + k, true);
+        r.v[2 * q + k] = load_codes(t0 + stride, w, 2 * q + k, true);
         __builtin_amdgcn_sched_barrier(0);
       }
       asm volatile("" ::: "memory");
@@ -355,12 +369,24 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
       }
       asm volatile("" ::: "memory");
     }
-    look(t0 + 8 * kStep, n_tiles, w);
+    look(t0 + 2 * stride, n_tiles, w);
   }
 
-  // merge the waves
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  if (alone) {
+    if (n < a.g) {
+      const float inv = 1.f / l;
+      const int64_t at = (int64_t)b * a.out_stride + (int64_t)(h * a.g + n) * kDim + 4 * j;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        store_out2<DT>(a.out, at + 16 * d, o[d][0] * inv, o[d][1] * inv);
+        store_out2<DT>(a.out, at + 16 * d + 2, o[d][2] * inv, o[d][3] * inv);
+      }
+    }
+    return;
+  }
+  // merge the waves
   __syncthreads();
   float* so = reinterpret_cast<float*>(lds);  // [wave][query][128]
   if (n < a.g) {
@@ -407,6 +433,15 @@ template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArg
   if (np <= 1) return;
   combine_partitions<DT>(a.ws_o, a.ws_lse, ((int64_t)b * a.hq + hq) * a.n_parts, np, a.out,
                          (int64_t)b * a.out_stride + (int64_t)hq * kDim);
+}
+
+// The longest context that one wave takes, from four rounds of workgroups on (three per
+// CU, fp32 two; us, one wave / four: 512 x 1-64 at 8 heads 17.6 / 26.1, 129-256 31.0 /
+// 32.5, 2000 x 10-300 93 / 114; fp32 20.0 / 43.0, 37.3 / 49.0, 137 / 191, 256 x 1-256 21.4
+// / 25.3).  Below that four waves a head are done sooner: bf16, 256 x 1-256 18.4 / 17.4, 128
+// x 1-200 15.4 / 10.6.
+static int32_t one_wave_context(int32_t n_seqs, int32_t hkv, bool fp32) {
+  return hkv % 4 == 0 && (int64_t)n_seqs * hkv >= 4 * (fp32 ? 512 : 768) ? 4 * kStep : 0;
 }
 
 struct Plan {
@@ -535,6 +570,7 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k
   a.magic = (uint64_t(1) << (27 + l)) / d + 1;
   a.shift = 27 + l;
   a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, kv4::kMaxContext / kv4::kTile);
+  a.alone = kv4::one_wave_context(n_seqs, n_kv_heads, dtype == AAC_DTYPE_FP32);
   if (p.ws_bytes) {
     a.ws_o = reinterpret_cast<float*>(workspace);
     a.ws_lse = a.ws_o + (size_t)n_seqs * n_q_heads * p.n_parts * kv4::kDim;

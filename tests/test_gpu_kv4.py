@@ -462,3 +462,21 @@ def test_store_of_every_16_bit_value(gpu, dtype, step):
     again = torch.zeros_like(cache)
     kv4.kv4_store(odd, odd, again, torch.arange(n, device=gpu))
     assert torch.equal(again, cache)
+
+
+@pytest.mark.parametrize("dtype, n, hq, hkv, bs", [
+    ("bf16", 400, 16, 8, 16), ("bf16", 770, 12, 4, 64), ("fp16", 390, 8, 8, 256), ("fp16", 260, 48, 12, 48),
+    ("fp32", 260, 16, 8, 16), ("fp32", 130, 64, 16, 64)])
+def test_attention_of_many_short_contexts(gpu, dtype, n, hq, hkv, bs):
+    """Enough (sequence, head) items that one wave takes a context of up to 256 tokens, with
+    longer ones and empty ones among them."""
+    _say("many", dtype, n, hq, hkv, bs)
+    rs = np.random.RandomState(n)
+    lens = rs.choice([0, 1, 15, 63, 64, 65, 128, 200, 255, 256, 257, 300, 520], n).tolist()
+    c = _case(gpu, lens, hq, hkv, bs, dtype, n)
+    _check(_attend(c), c["q"], c["cache"], bs, c["tables"], lens, SCALE)
+    part = _attend(c, partition_tokens=256)
+    _check(part, c["q"], c["cache"], bs, c["tables"], lens, SCALE)
+    out = torch.full((n, 3, hq, 128), 5.0, dtype=c["q"].dtype, device=gpu)
+    got = _attend(c, out=out[:, 1])
+    assert torch.equal(got, _attend(c)) and (out[:, ::2] == 5.0).all()
