@@ -36,7 +36,7 @@
 // bounds stand for the branch at a partition's end, 1 KiB of codes in one piece each.
 // Measured on MI355X (GPU time): bf16, 256 sequences of 1,024 to 2,048 tokens, 16/8 heads
 // 72.5 us (the bytes alone, at the 7.0 TB/s of a large copy: 60); 64 of 16,384 to 32,768
-// 278 (245); fp16, one of 115,000 31 (19), of which the second launch is 3; fp32, 4 of up
+// 282 (245); fp16, one of 115,000 31 (19), of which the second launch is 3; fp32, 4 of up
 // to 400 tokens 7.6, where latency alone counts.
 #include <algorithm>
 #include <climits>
@@ -467,8 +467,8 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
     // 8.4, 768 10.6).  Beyond, contexts of different lengths leave a round's end to a
     // few workgroups: the power of two from a quarter of it on, 1024 to 4096 (200 x 1-6k
     // at one head: 1024 32.9, 2048 36; 16 x 10-30k at 8: 1024 66.9, 2048 67.7, 6144 80;
-    // 100 x 2-6k at 4: 1024 45.0, 512 48.6, 4096 63; 64 x 16-32k at 8: 8192 272, 4096 276,
-    // 5632 282, 1024 302; 200 x 4-12k at 8: 4096 286, 8192 336).  No more than 64 parts to
+    // 100 x 2-6k at 4: 1024 45.0, 512 48.6, 4096 63; 64 x 16-32k at 8: 4096 282, 8192 288,
+    // 2048 293, 1024 308; 200 x 4-12k at 8: 4096 285, 8192 297, 2048 288).  No more than 64 parts to
     // combine (2 x 60k at 4: 1024 18.3, 768 20.3; one of 115k in fp16: 2048 30.5, 1024
     // 34.8, 4096 34.1).
     const int64_t items = (int64_t)n_seqs * hkv, round = cdiv(cap * items, fp32 ? 512 : 768);
@@ -484,7 +484,13 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
 }
 
 template <Dt DT> static void launch(const DecArgs& a, hipStream_t s) {
-  const dim3 grid(a.c.hkv, a.n_parts, a.n_seqs);
+  // An odd number of partitions: workgroups go round the XCDs and the shader engines of
+  // each in turn, so with 4 or 8, of which a captured step sized for the longest context has
+  // one or two that hold tokens, those would all fall on one or two engines of four (us,
+  // 256 x 300-1,500 in tables of 16,384 tokens at 8 heads 130 and 50, of 8,192 73 and 48,
+  // 64 x 500-2,000 in 32,768 48 and 26).  Where every partition holds tokens, the one that
+  // is empty costs up to 2% (64 x 16-32k 276 and 282), or nothing (200 x 4-12k).
+  const dim3 grid(a.c.hkv, a.n_parts | 1, a.n_seqs);
   if (a.c.block_size % kStep == 0)
     hipLaunchKernelGGL((kv4_decode_kernel<DT, true>), grid, dim3(256), 0, s, a);
   else

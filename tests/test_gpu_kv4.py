@@ -480,3 +480,14 @@ def test_attention_of_many_short_contexts(gpu, dtype, n, hq, hkv, bs):
     out = torch.full((n, 3, hq, 128), 5.0, dtype=c["q"].dtype, device=gpu)
     got = _attend(c, out=out[:, 1])
     assert torch.equal(got, _attend(c)) and (out[:, ::2] == 5.0).all()
+
+
+@pytest.mark.parametrize("width", [16, 40, 80])
+def test_attention_in_tables_far_wider_than_the_contexts(gpu, width):
+    """As a captured step has them: partitions for a capacity that no context reaches."""
+    c = _case(gpu, [1, 300, 0, 255, 700, 64], 8, 2, 64, "bf16", width)
+    tables = torch.full((6, width), -1, dtype=torch.int32, device=gpu)
+    tables[:, :c["tables"].shape[1]] = c["gtables"]
+    for part in (0, 256):
+        out = kv4.decode_paged_kv4(c["q"], c["gcache"], tables, c["ctx"], partition_tokens=part)
+        _check(out, c["q"], c["cache"], 64, c["tables"], c["lens"], SCALE, f"{width} blocks in {part}")
