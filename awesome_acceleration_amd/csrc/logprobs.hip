@@ -288,6 +288,7 @@ __device__ __forceinline__ uint2 wave_range(u32 key) {
 // two bits).
 __device__ __forceinline__ uint2 kth_of_wave(u32 key, int k, int j, bool near) {
   const uint2 range = wave_range(key);
+  if (k == 1) return make_uint2(range.y, range.y);
   const int top = 32 - __builtin_clz(range.x ^ range.y | 1u);  // bits from here up are alike
   u32 tk = top < 32 ? range.y >> top << top : 0, tj = tk;
 #pragma unroll 1
