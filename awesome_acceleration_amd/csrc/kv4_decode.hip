@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   __shared__ float sm_m[4][16], sm_l[4][16];
   const int part = blockIdx.y, b = blockIdx.z;
   int h = blockIdx.x;
+  if (part >= a.n_parts) return;  // (the one that makes them odd: its tokens may pass 31 bits)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // The waves take steps in turn.  A wave's first table entry does not depend on the
