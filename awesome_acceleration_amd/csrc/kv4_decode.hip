@@ -68,6 +68,11 @@ struct DecArgs {
   void* out;
   int64_t out_stride;
   int32_t n_parts, part_tokens;
+  // The plan's rule by a context's own length, for those far below the capacity (part_of):
+  int32_t tight;       // from here on partitions of part_tokens
+  int32_t whole;       // up to here no split
+  uint64_t per_round;  // items / those of a round of workgroups, 16 bits of fraction
+  u32 inv_parts;       // 2^32 / n_parts, rounded up
   float* ws_o;    // [n_seqs, hq, n_parts, 128]
   float* ws_lse;  // [n_seqs, hq, n_parts]
   // tile number -> block: (tile * magic) >> shift
@@ -77,13 +82,38 @@ struct DecArgs {
   int32_t alone;      // the longest context that one wave takes
 };
 
+constexpr int kStep = 64;         // tokens of a step
+constexpr int kTurn = 4 * kStep;  // of one turn of the workgroup's waves
+
+__host__ __device__ __forceinline__ int cdiv_turn(int tokens) { return (tokens + kTurn - 1) / kTurn * kTurn; }
+// A partition, from what one round of workgroups makes of all tokens (plan)
+__host__ __device__ __forceinline__ u32 rounds_part(u32 round) {
+  return round <= 1024 ? round : round <= 4096 ? 1024 : round <= 8192 ? 2048 : 4096;
+}
+
 __device__ __forceinline__ int context_len(const DecArgs& a, int len) {
   const int64_t ctx = (int64_t)len + a.lens_add;
   const int64_t cap = min((int64_t)a.max_blocks * a.c.block_size, kMaxContext);
   return (int)(ctx < 0 ? 0 : ctx > cap ? cap : ctx);
 }
-__device__ __forceinline__ int parts_of(const DecArgs& a, int ctx) {
-  return min(a.n_parts, (int)(((u32)ctx + (u32)a.part_tokens - 1) / (u32)a.part_tokens));
+// Tokens of a partition of a context.  The plan sizes them for the largest context that
+// there may be; one that would fill less than a quarter of its partitions (of a captured
+// step, mostly) is split by the same rule for its own length, never coarser and into
+// no more than n_parts (us, with its own length and with the plan's partitions, at 8
+// heads: 16 x 500-2,000 in tables of 32,768 14.9 and 19.9, 32 of them 17.6 and 22.1, 8 x 3-30k
+// in 131,072 20.4 and 48.2; without the quarter 100 x 2-6k in 6,000 took 93, not 83).
+__device__ __forceinline__ int part_of(const DecArgs& a, int ctx) {
+  if (ctx >= a.tight) return a.part_tokens;
+  int part = ctx;
+  if (ctx > a.whole) {
+    const u32 round = (u32)min((u64)(u32)ctx * a.per_round >> 16, (u64)(1u << 30));
+    const u32 least = (u32)(((u64)(u32)(ctx - 1) * a.inv_parts) >> 32) + 1;
+    part = (int)max(max(rounds_part(round), (u32)ctx >> 6), least);
+  }
+  return min(cdiv_turn(max(part, 1)), a.part_tokens);
+}
+__device__ __forceinline__ int parts_of(const DecArgs& a, int ctx, int part_tokens) {
+  return min(a.n_parts, (int)(((u32)ctx + (u32)part_tokens - 1) / (u32)part_tokens));
 }
 
 // The high halves of two floats as a bf16 pair, and what is left of each
@@ -113,7 +143,6 @@ struct Raw {
   u32 ks, vs;
 };
 
-constexpr int kStep = 64;      // tokens of a step
 constexpr int kLoadAux = 2;  // non-temporal: nothing reads the rows again
 
 // WIDE: block sizes are a multiple of a step, so that a step lies in one block.
@@ -133,8 +162,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   // context's length, so both are on their way together.
   typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
   const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
-  const int beg = part * a.part_tokens;
-  int t_first = beg + kStep * wave, stride = 4 * kStep;
+  int t_first = part * a.part_tokens + kStep * wave, stride = kTurn;  // (a guess: see below)
   const int tpb = a.c.block_size / kTile;
   constexpr int kLooks = WIDE ? 1 : 4;
   struct Where {
@@ -154,7 +182,8 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   Where w;
   look(t_first, a.cap_tiles, w);
   const int ctx = context_len(a, ((const cint*)(uintptr_t)a.lens)[b]);
-  const int np = parts_of(a, ctx);
+  const int part_tokens = part_of(a, ctx);
+  const int np = parts_of(a, ctx, part_tokens);
   if (part >= np) {  // workgroup-uniform
     if (part == 0) {  // an empty context
       for (int i = tid; i < a.g * (kDim / 2); i += 256)
@@ -173,7 +202,9 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     t_first = 0;
     stride = kStep;
   }
-  const int end = beg + min(ctx - beg, a.part_tokens), n_tiles = (end + kTile - 1) / kTile;
+  const int beg = part * part_tokens;
+  if (!alone) t_first = beg + kStep * wave;
+  const int end = beg + min(ctx - beg, part_tokens), n_tiles = (end + kTile - 1) / kTile;
 
   // A buffer of each tile's pages (K, then V) from the block number, and offsets that each
   // lane keeps.  Past the end the buffer is empty: the loads are issued all the same, so
@@ -430,11 +461,17 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
 
 template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArgs a) {
   const int hq = blockIdx.x, b = blockIdx.y;
-  const int np = parts_of(a, context_len(a, a.lens[b]));
+  const int ctx = context_len(a, a.lens[b]);
+  const int np = parts_of(a, ctx, part_of(a, ctx));
   if (np <= 1) return;
   combine_partitions<DT>(a.ws_o, a.ws_lse, ((int64_t)b * a.hq + hq) * a.n_parts, np, a.out,
                          (int64_t)b * a.out_stride + (int64_t)hq * kDim);
 }
+
+// Workgroups that the GPU holds at once: three per CU, fp32 two.
+static int round_of(bool fp32) { return fp32 ? 512 : 768; }
+// The longest context that is not split.
+static int32_t whole_context(int64_t items) { return items >= 512 ? 4096 : 768; }
 
 // The longest context that one wave takes, from four rounds of workgroups on (three per
 // CU, fp32 two; us, one wave / four: 512 x 1-64 at 8 heads 17.6 / 26.1, 129-256 31.0 /
@@ -442,7 +479,7 @@ template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArg
 // / 25.3).  Below that four waves a head are done sooner: bf16, 256 x 1-256 18.4 / 17.4, 128
 // x 1-200 15.4 / 10.6.
 static int32_t one_wave_context(int32_t n_seqs, int32_t hkv, bool fp32) {
-  return hkv % 4 == 0 && (int64_t)n_seqs * hkv >= 4 * (fp32 ? 512 : 768) ? 4 * kStep : 0;
+  return hkv % 4 == 0 && (int64_t)n_seqs * hkv >= 4 * round_of(fp32) ? 4 * kStep : 0;
 }
 
 struct Plan {
@@ -452,7 +489,6 @@ struct Plan {
 
 static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, int32_t max_blocks,
                  int32_t max_context_len, int32_t part_tokens, bool fp32) {
-  constexpr int kTurn = 4 * kStep;  // tokens of one turn of the workgroup's waves
   Plan p;
   int64_t cap = std::min<int64_t>((int64_t)max_blocks * block_size, kMaxContext);
   if (max_context_len > 0 && max_context_len < cap) cap = max_context_len;
@@ -472,10 +508,10 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
     // 2048 293, 1024 308; 200 x 4-12k at 8: 4096 285, 8192 297, 2048 288).  No more than 64 parts to
     // combine (2 x 60k at 4: 1024 18.3, 768 20.3; one of 115k in fp16: 2048 30.5, 1024
     // 34.8, 4096 34.1).
-    const int64_t items = (int64_t)n_seqs * hkv, round = cdiv(cap * items, fp32 ? 512 : 768);
-    part = round <= 1024 ? round : round <= 4096 ? 1024 : round <= 8192 ? 2048 : 4096;
+    const int64_t items = (int64_t)n_seqs * hkv, round = cdiv(cap * items, round_of(fp32));
+    part = rounds_part((u32)std::min<int64_t>(round, 1 << 30));
     part = std::max(part, cdiv(cap, 64));
-    if (cap <= 768 || (items >= 512 && cap <= 4096)) part = cap;
+    if (cap <= whole_context(items)) part = cap;
   }
   part = cdiv(std::min(part, cap), kTurn) * kTurn;
   p.part_tokens = (int32_t)part;
@@ -578,6 +614,13 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k
   a.shift = 27 + l;
   a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, kv4::kMaxContext / kv4::kTile);
   a.alone = kv4::one_wave_context(n_seqs, n_kv_heads, dtype == AAC_DTYPE_FP32);
+  if (partition_tokens <= 0 && p.n_parts > 1) {
+    const int64_t items = (int64_t)n_seqs * n_kv_heads;
+    a.tight = (int32_t)((int64_t)p.n_parts * p.part_tokens / 4);
+    a.whole = kv4::whole_context(items);
+    a.per_round = (uint64_t)std::min<int64_t>(items, 1 << 15) * 65536 / kv4::round_of(dtype == AAC_DTYPE_FP32);
+    a.inv_parts = (u32)(((uint64_t(1) << 32) + p.n_parts - 1) / p.n_parts);
+  }
   if (p.ws_bytes) {
     a.ws_o = reinterpret_cast<float*>(workspace);
     a.ws_lse = a.ws_o + (size_t)n_seqs * n_q_heads * p.n_parts * kv4::kDim;

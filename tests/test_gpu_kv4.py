@@ -491,3 +491,19 @@ def test_attention_in_tables_far_wider_than_the_contexts(gpu, width):
     for part in (0, 256):
         out = kv4.decode_paged_kv4(c["q"], c["gcache"], tables, c["ctx"], partition_tokens=part)
         _check(out, c["q"], c["cache"], 64, c["tables"], c["lens"], SCALE, f"{width} blocks in {part}")
+
+
+@pytest.mark.parametrize("dtype, n, hq, hkv, width", [
+    ("bf16", 6, 8, 2, 2048), ("fp16", 12, 16, 8, 700), ("fp32", 6, 4, 4, 2048), ("bf16", 70, 16, 8, 1024)])
+def test_attention_of_contexts_split_by_their_own_length(gpu, dtype, n, hq, hkv, width):
+    """Capacities far above the contexts, which lie about every bound of the rule."""
+    _say("own length", dtype, n, hq, hkv, width)
+    lens = ([0, 768, 769, 1500, 4096, 4097] if n > 60 else [1, 769, 1500, 5000, 12000, 0]) * (n // 6)
+    lens += [2500] * (n - len(lens))
+    c = _case(gpu, lens, hq, hkv, 64, dtype, n)
+    tables = torch.full((n, width), -1, dtype=torch.int32, device=gpu)
+    tables[:, :c["tables"].shape[1]] = c["gtables"]
+    out = kv4.decode_paged_kv4(c["q"], c["gcache"], tables, c["ctx"])
+    _check(out, c["q"], c["cache"], 64, c["tables"], lens, SCALE)
+    limit = kv4.decode_paged_kv4(c["q"], c["gcache"], tables, c["ctx"], max_context_len=64 * width)
+    assert torch.equal(out, limit)
