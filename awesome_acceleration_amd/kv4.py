@@ -206,11 +206,13 @@ def _decode(q, q_stride, n, hq, kv_cache, cache, tables, lens, k, v, ks, vs, sca
     nb, bs, hkv = cache
     mb = tables.shape[1]
     nbytes = _ws_bytes(n, hq, hkv, HEAD_DIM, bs, mb, mcl, part)
-    # from the allocator, in stream order: a captured call's belongs to its graph
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    # From the allocator, in stream order: a captured call's belongs to its graph.  Held until
+    # the library has returned, since other threads run while it enqueues its launches.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.launch("aac_kv4_decode", q.get_device(), q.data_ptr(), q_stride, k, v, ks, vs,
                 kv_cache.data_ptr(), nb, bs, tables.data_ptr(), mb, lens.data_ptr(), n, mcl, hq, hkv,
-                HEAD_DIM, scale, out.data_ptr(), out_stride, ws, nbytes, part, _code(q.dtype))
+                HEAD_DIM, scale, out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(), nbytes,
+                part, _code(q.dtype))
 
 
 def _heads(hq: int, hkv: int, d: int) -> None:

@@ -250,3 +250,39 @@ def test_limits_are_the_headers():
     assert limit("AAC_STEP_MAPS_MAX_SEQS") == paged.MAX_MAP_SEQS
     assert limit("AAC_LOGPROBS_MAX_TOP") == fused.MAX_TOP_LOGPROBS
     assert limit("AAC_LOGPROBS_MAX_COLS") == fused.MAX_LOGPROB_COLS
+
+
+@pytest.mark.parametrize("call", ["decode", "append", "logprobs"])
+def test_workspaces_live_until_the_library_has_returned(call, monkeypatch):
+    """Other threads get the interpreter and the allocator while the library enqueues its
+    launches: every buffer that a call allocates for it is held until then."""
+    import weakref
+    made, entered = [], []
+    empty = torch.empty
+
+    def recorded(*a, **o):
+        t = empty(*a, **o)
+        made.append((t.data_ptr(), weakref.ref(t)))
+        return t
+
+    def launch(name, device, *args):
+        held = {at: ref() is not None for at, ref in made if at}
+        entered.append([held[a] for a in args if a in held])
+
+    monkeypatch.setattr(torch, "empty", recorded)
+    monkeypatch.setattr(_lib, "launch", launch)
+    for module in (kv4, fused):
+        monkeypatch.setattr(module, "_on_gpu", lambda *ts: None)
+    cache = kv4.alloc_kv4_cache(70, 32, 2, device="cpu")
+    q, t = torch.zeros(4, 2, 128), torch.zeros(4, 64, dtype=torch.int32)
+    lens = torch.full((4,), 2000, dtype=torch.int32)
+    if call == "decode":
+        kv4.decode_paged_kv4(q, cache, t, lens, partition_tokens=256)
+    elif call == "append":
+        kv4.flash_attn_with_kv4cache(q[:, None], cache, k=q[:, None], v=q[:, None], cache_seqlens=lens,
+                                     block_table=t)
+    else:
+        fused.token_logprobs(torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64), 3)
+    (held,) = entered
+    # the workspace and the outputs of torch.empty (one; log probabilities two)
+    assert held == [True] * (3 if call == "logprobs" else 2)
