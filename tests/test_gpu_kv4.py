@@ -507,3 +507,15 @@ def test_attention_of_contexts_split_by_their_own_length(gpu, dtype, n, hq, hkv,
     _check(out, c["q"], c["cache"], 64, c["tables"], lens, SCALE)
     limit = kv4.decode_paged_kv4(c["q"], c["gcache"], tables, c["ctx"], max_context_len=64 * width)
     assert torch.equal(out, limit)
+
+
+@pytest.mark.parametrize("lens, bs", [([3000, 1, 900, 4500], 64), ([257, 100, 2047], 16)])
+def test_probabilities_of_bf16_calls_keep_more_than_bf16(gpu, lens, bs):
+    """Two truncated bfloat16 terms leave less than 2^-14 of a probability, and the sum below
+    the fraction line has all of it; one rounded term would leave 2^-8 of each."""
+    c = _case(gpu, lens, 8, 2, bs, "bf16", 50)
+    out = _attend(c)
+    ref, absv, z = oracle4.decode(f64(c["q"]), c["cache"], bs, c["tables"], lens, SCALE)
+    half = torch.finfo(torch.bfloat16).eps / 2
+    lim = half * np.abs(ref) + (2.0 ** -14 + 2.0 ** -16 * (1 + z)) * absv * (1 + half) + 2.0 ** -25
+    assert (np.abs(f64(out).reshape(ref.shape) - ref) <= lim).all()
