@@ -456,7 +456,7 @@ extern "C" int aac_qk_norm_rope_store_kv4(
   if (!fz_dtype(dtype, &dt)) return AAC_ERR_UNSUPPORTED;
   if (n_tokens < 0 || n_q_heads <= 0 || max_position <= 0) return AAC_ERR_INVALID_ARGUMENT;
   if (n_tokens == 0) return AAC_OK;
-  if (n_tokens >= (1 << 26)) return AAC_ERR_UNSUPPORTED;  // (a launch numbers its threads in 32 bits)
+  if (cdiv(n_tokens, 4) >= (1 << 24)) return AAC_ERR_UNSUPPORTED;  // (a launch numbers its threads in 32 bits)
   const int rc = kv4::check_cache(cache, num_blocks, block_size, n_kv_heads, head_dim);
   if (rc != AAC_OK) return rc;
   if (qkv_tok_stride < (int64_t)(n_q_heads + 2 * n_kv_heads) * head_dim) return AAC_ERR_SHAPE;

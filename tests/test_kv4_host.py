@@ -286,3 +286,13 @@ def test_workspaces_live_until_the_library_has_returned(call, monkeypatch):
     (held,) = entered
     # the workspace and the outputs of torch.empty (one; log probabilities two)
     assert held == [True] * (3 if call == "logprobs" else 2)
+
+
+def test_fused_store_refuses_2_32_threads():
+    """A wave a token, four a workgroup: 2^24 workgroups of 256 threads from 2^26 - 3 tokens on."""
+    L = _lib.lib()
+    call = lambda n, nb: L.aac_qk_norm_rope_store_kv4(  # noqa: E731
+        P, 4096, n, 16, 8, 128, P, P, 1e-6, P, P, 100, P, P, None, P, nb, 16, P, None, 0, None, 0, None)
+    for n in ((1 << 26) - 3, (1 << 26) - 1, 1 << 26):
+        assert call(n, 0) == -2, n
+    assert call((1 << 26) - 4, 0) == -1  # (of the cache: one token fewer is not refused for its number)
