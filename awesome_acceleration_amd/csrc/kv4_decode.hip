@@ -449,8 +449,10 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
     if (np == 1) {
       store_out2<DT>(a.out, (int64_t)b * a.out_stride + (int64_t)hq * kDim + d, o0 * inv, o1 * inv);
     } else {
+      // (scores of -inf alone: a weight of 0 to be, which NaN would not stand)
+      const float f = L == 0.f ? 0.f : inv;
       const int64_t slot = ((int64_t)b * a.hq + hq) * a.n_parts + part;
-      *reinterpret_cast<float2*>(a.ws_o + slot * kDim + d) = make_float2(o0 * inv, o1 * inv);
+      *reinterpret_cast<float2*>(a.ws_o + slot * kDim + d) = make_float2(o0 * f, o1 * f);
       if (d == 0) a.ws_lse[slot] = mx + __log2f(L);
     }
   }

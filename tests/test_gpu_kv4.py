@@ -519,3 +519,29 @@ def test_probabilities_of_bf16_calls_keep_more_than_bf16(gpu, lens, bs):
     half = torch.finfo(torch.bfloat16).eps / 2
     lim = half * np.abs(ref) + (2.0 ** -14 + 2.0 ** -16 * (1 + z)) * absv * (1 + half) + 2.0 ** -25
     assert (np.abs(f64(out).reshape(ref.shape) - ref) <= lim).all()
+
+
+@pytest.mark.parametrize("n, low", [(1024, 256), (1024, 0), (1024, 1024), (200, 64), (200, 200)])
+def test_scores_that_overflow_to_minus_infinity_weigh_nothing(gpu, n, low):
+    """q . k of -6e38 in the first ``low`` tokens is -inf in float: those have probability 0,
+    a whole partition of them too, and a context of nothing else has none, as softmax."""
+    _say("-inf scores", n, low)
+    k = torch.zeros((n, 1, 128), device=gpu)
+    k[:low, 0, 0] = -6.0
+    v = torch.ones((n, 1, 128), device=gpu)
+    v[:low] = 4.0
+    cache = kv4.alloc_kv4_cache(n // 16 + 1, 16, 1, device=gpu)
+    kv4.kv4_store(k, v, cache, torch.arange(n, device=gpu))
+    tables = torch.arange(n // 16 + 1, dtype=torch.int32, device=gpu)[None]
+    ctx = torch.tensor([n], dtype=torch.int32, device=gpu)
+    q = torch.zeros((1, 2, 128), device=gpu)
+    q[0, 0, 0] = 1e38
+    for part in (0, 256):
+        out = kv4.decode_paged_kv4(q, cache, tables, ctx, partition_tokens=part)
+        if low == n:
+            assert out[0, 0].isnan().all()
+        else:  # equal scores of equal values
+            assert (out[0, 0] == 1).all()
+        # the other head's scores are 0: the mean, whose sums of small whole numbers are exact
+        mean = (4.0 * low + n - low) / n
+        assert ((out[0, 1] - mean).abs() <= 2.0 ** -21 * mean).all()
