@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
 
   // Q operand: query n's dims 32 j + 8 i .. + 7 for product i, in NT terms
   // (a negative scale: -q and -scale, so that the largest product has the largest score)
-  const float cs = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: equal scores)
+  const float cs = vmax(fabsf(a.scale_log2), 1e-30f);  // (a scale of 0: equal scores; NaN stays)
   u32x4 qf[NT][4];
   {
     const bool row = n < a.g;

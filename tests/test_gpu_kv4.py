@@ -545,3 +545,13 @@ def test_scores_that_overflow_to_minus_infinity_weigh_nothing(gpu, n, low):
         # the other head's scores are 0: the mean, whose sums of small whole numbers are exact
         mean = (4.0 * low + n - low) / n
         assert ((out[0, 1] - mean).abs() <= 2.0 ** -21 * mean).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_scale_of_nan_gives_nan(gpu, dtype):
+    for lens, part in (([40, 3], 0), ([700, 300], 256)):
+        c = _case(gpu, lens, 4, 2, 16, dtype, 51)
+        assert _attend(c, softmax_scale=float("nan"), partition_tokens=part).isnan().all()
+    # (a wave a head)
+    c = _case(gpu, [20] * 400, 16, 8, 16, dtype, 52)
+    assert _attend(c, softmax_scale=float("nan")).isnan().all()
