@@ -79,7 +79,6 @@ struct DecArgs {
   // tile number -> block: (tile * magic) >> shift
   uint64_t magic;
   int32_t shift;
-  int32_t cap_tiles;  // of the tables
   int32_t alone;      // the longest context that one wave takes
 };
 
@@ -157,14 +156,11 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   __shared__ float sm_m[4][16], sm_l[4][16];
   const int part = blockIdx.y, b = blockIdx.z;
   int h = blockIdx.x;
-  if (part >= a.n_parts) return;  // (the one that makes them odd: its tokens may pass 31 bits)
+  if (part >= a.n_parts) return;  // (the one that makes their number odd)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // The waves take steps in turn.  A wave's first table entry does not depend on the
-  // context's length, so both are on their way together.
   typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
   const cint* table = (const cint*)(uintptr_t)(a.block_tables + (int64_t)b * a.max_blocks);
-  int t_first = part * a.part_tokens + kStep * wave, stride = kTurn;  // (a guess: see below)
   const int tpb = a.c.block_size / kTile;
   constexpr int kLooks = WIDE ? 1 : 4;
   struct Where {
@@ -181,8 +177,6 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
       w.row[k] = (tile - bi * tpb) * kTile;
     }
   };
-  Where w;
-  look(t_first, a.cap_tiles, w);
   const int ctx = context_len(a, ((const cint*)(uintptr_t)a.lens)[b]);
   const int part_tokens = part_of(a, ctx);
   const int np = parts_of(a, ctx, part_tokens);
@@ -201,11 +195,9 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   if (alone) {
     if ((h ^ (b + (b >> 2))) & 3) return;
     h = (h & ~3) + wave;
-    t_first = 0;
-    stride = kStep;
   }
-  const int beg = part * part_tokens;
-  if (!alone) t_first = beg + kStep * wave;
+  // The waves take steps in turn.
+  const int beg = part * part_tokens, t_first = alone ? 0 : beg + kStep * wave, stride = alone ? kStep : kTurn;
   const int end = beg + min(ctx - beg, part_tokens), n_tiles = (end + kTile - 1) / kTile;
 
   // A buffer of each tile's pages (K, then V) from the block number, and offsets that each
@@ -238,6 +230,7 @@ __global__ __launch_bounds__(256, DT == Dt::FP32 ? 2 : 3) void kv4_decode_kernel
   // One buffer of rows: those of the next step are asked for where this step's have been
   // taken.
   Raw r;
+  Where w;
   look(t_first, n_tiles, w);
   load_scales(w, r);
 #pragma unroll
@@ -611,7 +604,6 @@ extern "C" int aac_kv4_decode(const void* q, int64_t q_seq_stride, const void* k
   const int l = d == 1 ? 0 : 32 - __builtin_clz(d - 1);
   a.magic = (uint64_t(1) << (27 + l)) / d + 1;
   a.shift = 27 + l;
-  a.cap_tiles = (int32_t)std::min<int64_t>((int64_t)max_blocks_per_seq * d, kv4::kMaxContext / kv4::kTile);
   a.alone = kv4::one_wave_context(n_seqs, n_kv_heads, dtype == AAC_DTYPE_FP32);
   if (partition_tokens <= 0 && p.n_parts > 1) {
     const int64_t items = (int64_t)n_seqs * n_kv_heads;
