@@ -12,6 +12,7 @@ of the 16-bit paged cache; ``block_size`` is a multiple of 16 and ``head_dim`` 1
 ``decode_paged_kv4`` and ``flash_attn_with_kv4cache`` beside ``decode_paged`` and
 ``flash_attn_with_kvcache``, with their conventions: ``RuntimeError`` for a rejected
 argument, the current stream, no synchronisation, new outputs, caches updated in place.
+Lengths are int32 throughout.
 """
 from __future__ import annotations
 
@@ -264,14 +265,18 @@ def decode_paged_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torc
 
 def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
                              k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None, *,
-                             cache_seqlens: torch.Tensor, block_table: torch.Tensor,
-                             softmax_scale: Optional[float] = None,
+                             cache_seqlens: torch.Tensor | int, block_table: torch.Tensor,
+                             softmax_scale: Optional[float] = None, causal: bool = False,
+                             num_splits: int = 0,
                              max_context_len: Optional[int] = None) -> torch.Tensor:
     """``flash_attn_with_kvcache`` over the 4-bit cache: ``q [B, 1, Hq, 128]``; ``k``/``v``
     (``[B, 1, Hkv, 128]``), where given, are quantised into the cache at position
     ``cache_seqlens[b]`` and the call attends over ``cache_seqlens[b] + 1`` tokens,
-    otherwise over ``cache_seqlens[b]``.  The new token is attended to as the cache holds
-    it.  All rows are written before any is read; ``cache_seqlens`` is not modified."""
+    otherwise over ``cache_seqlens[b]`` (int32 ``[B]``, or an int for all).  The new token
+    is attended to as the cache holds it.  All rows are written before any is read;
+    ``cache_seqlens`` is not modified.  ``causal`` changes nothing for one query token;
+    ``num_splits``, where positive, is how many partitions the longest context is split into
+    at most (of a multiple of 256 tokens)."""
     if q.dim() != 4:
         raise RuntimeError("q must be [B, S, Hq, 128]")
     n, s, hq, d = q.shape
@@ -279,14 +284,19 @@ def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
         raise NotImplementedError("only one query token per sequence (decode) is supported")
     if (k is None) != (v is None):
         raise RuntimeError("k and v must be given together")
-    _on_gpu(q, kv_cache, k, v, cache_seqlens, block_table)
+    if isinstance(cache_seqlens, int):
+        _on_gpu(q, kv_cache, k, v, block_table)
+        cache_seqlens = torch.full((n,), cache_seqlens, dtype=torch.int32, device=q.device)
+    else:
+        _on_gpu(q, kv_cache, k, v, cache_seqlens, block_table)
+        cache_seqlens = cache_seqlens.contiguous()
     cache = _cache(kv_cache)
     hkv = cache[2]
     _heads(hq, hkv, d)
+    block_table = block_table.contiguous()
     _table(block_table, n)
-    if (cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (n,)
-            or not cache_seqlens.is_contiguous()):
-        raise RuntimeError("cache_seqlens must be contiguous int32 [B]")
+    if cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (n,):
+        raise RuntimeError("cache_seqlens must be int32 [B]")
     qst = q.stride()
     if qst[3] != 1 or qst[2] != d:
         q = q.contiguous()
@@ -310,6 +320,11 @@ def flash_attn_with_kv4cache(q: torch.Tensor, kv_cache: torch.Tensor,
         kp, vp = k.data_ptr(), v.data_ptr()
         ks, vs = (kst[0], vst[0]) if n > 1 else (row, row)
     row = hq * d
+    most = min(int(max_context_len or 0), 0x7fffffff)
+    part = 0
+    if num_splits and num_splits > 0:
+        cap = min(block_table.shape[1] * cache[1], 0x7fffffff)
+        part = -(-(min(most, cap) if most > 0 else cap) // int(num_splits))
     _decode(q, qst[0] if n > 1 else row, n, hq, kv_cache, cache, block_table, cache_seqlens, kp, vp, ks, vs,
-            _scale(softmax_scale, d), min(int(max_context_len or 0), 0x7fffffff), 0, out, row)
+            _scale(softmax_scale, d), most, part, out, row)
     return out

@@ -555,3 +555,31 @@ def test_a_scale_of_nan_gives_nan(gpu, dtype):
     # (a wave a head)
     c = _case(gpu, [20] * 400, 16, 8, 16, dtype, 52)
     assert _attend(c, softmax_scale=float("nan")).isnan().all()
+
+
+def test_append_takes_what_the_16_bit_call_takes(gpu):
+    """An int length, strided lengths and tables, causal, num_splits, as flash_attn_with_kvcache."""
+    rs = np.random.RandomState(53)
+    c = _case(gpu, [700, 700], 8, 2, 16, "bf16", 53)
+    q = c["q"][:, None]
+    k, v = (_rand(rs, 2, 1, 2, 128, dtype=torch.bfloat16).to(gpu) for _ in "kv")
+    wide = torch.full((2, 2 * c["gtables"].shape[1]), -7, dtype=torch.int32, device=gpu)
+    wide[:, ::2] = c["gtables"]
+    caches = [c["gcache"].clone() for _ in range(2)]
+    ref = kv4.flash_attn_with_kv4cache(q, caches[0], k=k, v=v, cache_seqlens=c["ctx"] - 1,
+                                       block_table=c["gtables"])
+    out = kv4.flash_attn_with_kv4cache(q, caches[1], k=k, v=v, cache_seqlens=699, block_table=wide[:, ::2],
+                                       causal=True)
+    assert torch.equal(out, ref) and torch.equal(*caches)
+    lens = torch.full((2, 3), 699, dtype=torch.int32, device=gpu)
+    out = kv4.flash_attn_with_kv4cache(q, caches[1], k=k, v=v, cache_seqlens=lens[:, 1], block_table=wide[:, ::2])
+    assert torch.equal(out, ref) and torch.equal(*caches)
+    want = _cache_np(caches[0])
+    for splits in (1, 2, 3, 100):
+        for most in (None, 700):
+            out = kv4.flash_attn_with_kv4cache(q, caches[0], cache_seqlens=700, block_table=c["gtables"],
+                                               num_splits=splits, max_context_len=most)
+            _check(out, c["q"], want, 16, c["tables"], c["lens"], SCALE)
+            if splits == 1:
+                whole = kv4.decode_paged_kv4(c["q"], caches[0], c["gtables"], c["ctx"], partition_tokens=1024)
+                assert torch.equal(out[:, 0], whole)

@@ -296,3 +296,19 @@ def test_fused_store_refuses_2_32_threads():
     for n in ((1 << 26) - 3, (1 << 26) - 1, 1 << 26):
         assert call(n, 0) == -2, n
     assert call((1 << 26) - 4, 0) == -1  # (of the cache: one token fewer is not refused for its number)
+
+
+@pytest.mark.parametrize("splits, most, part", [(0, None, 0), (1, None, 64 * 32), (3, None, 683), (4, 1000, 250),
+                                                (5000, None, 1), (2, 1 << 40, 1024)])
+def test_num_splits_and_lengths_as_the_16_bit_call_takes_them(splits, most, part, monkeypatch):
+    calls = []
+    monkeypatch.setattr(_lib, "launch", lambda name, device, *args: calls.append(args))
+    monkeypatch.setattr(kv4, "_on_gpu", lambda *ts: None)
+    cache, q = kv4.alloc_kv4_cache(70, 32, 2, device="cpu"), torch.zeros(4, 1, 2, 128)
+    table = torch.zeros(64, 4, dtype=torch.int32).t()
+    a = dict(block_table=table, num_splits=splits, max_context_len=most, causal=True)
+    kv4.flash_attn_with_kv4cache(q, cache, cache_seqlens=9, **a)
+    kv4.flash_attn_with_kv4cache(q, cache, cache_seqlens=torch.full((4,), 9, dtype=torch.int32), **a)
+    assert calls[0][-2] == calls[1][-2] == part
+    with pytest.raises(RuntimeError, match="cache_seqlens"):
+        kv4.flash_attn_with_kv4cache(q, cache, cache_seqlens=torch.full((4,), 9), **a)
