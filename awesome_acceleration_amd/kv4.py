@@ -219,7 +219,7 @@ def _decode(q, q_stride, n, hq, kv_cache, cache, tables, lens, k, v, ks, vs, sca
 def _heads(hq: int, hkv: int, d: int) -> None:
     if d != HEAD_DIM:
         raise RuntimeError(f"head_dim must be {HEAD_DIM}")
-    if hq % hkv or hq // hkv > 16:
+    if hkv == 0 or hq % hkv or hq // hkv > 16:
         raise RuntimeError("query heads must be 1 to 16 times the KV heads")
 
 

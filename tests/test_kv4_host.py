@@ -312,3 +312,13 @@ def test_num_splits_and_lengths_as_the_16_bit_call_takes_them(splits, most, part
     assert calls[0][-2] == calls[1][-2] == part
     with pytest.raises(RuntimeError, match="cache_seqlens"):
         kv4.flash_attn_with_kv4cache(q, cache, cache_seqlens=torch.full((4,), 9), **a)
+
+
+def test_a_cache_of_no_heads_is_refused(monkeypatch):
+    monkeypatch.setattr(kv4, "_on_gpu", lambda *ts: None)
+    cache, q = torch.zeros(3, 0, 2, 32 * 68, dtype=torch.uint8), torch.zeros(4, 2, 128)
+    t, lens = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        kv4.decode_paged_kv4(q, cache, t, lens)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        kv4.flash_attn_with_kv4cache(q[:, None], cache, cache_seqlens=lens, block_table=t)
