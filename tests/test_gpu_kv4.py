@@ -583,3 +583,30 @@ def test_append_takes_what_the_16_bit_call_takes(gpu):
             if splits == 1:
                 whole = kv4.decode_paged_kv4(c["q"], caches[0], c["gtables"], c["ctx"], partition_tokens=1024)
                 assert torch.equal(out[:, 0], whole)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [0, 1, 3, 40])
+def test_store_of_padding_alone_writes_nothing(gpu, dtype, n):
+    cache = torch.from_numpy(np.random.RandomState(54).randint(0, 256, (2, 3, 2, 16 * 68)).astype(np.uint8)).to(gpu)
+    before = cache.clone()
+    k = torch.ones((n, 3, 128), dtype=DTYPES[dtype], device=gpu)
+    slots = torch.full((n,), -1, dtype=torch.int64, device=gpu)
+    kv4.kv4_store(k, k, cache, slots)
+    assert torch.equal(cache, before)
+    for x in kv4.kv4_load(cache, slots, dtype=DTYPES[dtype]):
+        assert x.shape == (n, 3, 128) and (x == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_load_of_every_code_under_every_scale_byte(gpu, dtype):
+    """Scale bytes that no store writes (below 2, 253, 254) too, as the format has them."""
+    cache = np.zeros((1, 1, 2, 256 * 68), np.uint8)
+    codes = np.tile(oracle4.pack(np.arange(16)[None])[0], 8)
+    for r in range(256):
+        cache[0, 0, :, r * 64:r * 64 + 64] = codes
+        cache[0, 0, :, 256 * 64 + 4 * r:256 * 64 + 4 * r + 4] = r
+    slots = torch.arange(256, device=gpu)
+    for got, ref in zip(kv4.kv4_load(torch.from_numpy(cache).to(gpu), slots, dtype=DTYPES[dtype]),
+                        oracle4.load(cache, 256, range(256))):
+        assert np.array_equal(f64(got), f64(torch.from_numpy(ref).to(DTYPES[dtype])), equal_nan=True)
