@@ -610,3 +610,30 @@ def test_load_of_every_code_under_every_scale_byte(gpu, dtype):
     for got, ref in zip(kv4.kv4_load(torch.from_numpy(cache).to(gpu), slots, dtype=DTYPES[dtype]),
                         oracle4.load(cache, 256, range(256))):
         assert np.array_equal(f64(got), f64(torch.from_numpy(ref).to(DTYPES[dtype])), equal_nan=True)
+
+
+def test_two_threads_on_one_stream(gpu):
+    """Split calls from two threads on the default stream, each with tensors of its own made
+    and dropped between: every result is the eager one."""
+    import threading
+    cs = [_case(gpu, lens, 8, 2, 16, "bf16", 60 + i) for i, lens in enumerate(([900, 40, 1500], [700, 1200, 3]))]
+    refs = [_attend(c, partition_tokens=256) for c in cs]
+    torch.cuda.synchronize()
+    wrong, errors = [], []
+
+    def run(c, ref):
+        try:
+            for _ in range(200):
+                out = _attend(c, partition_tokens=256)
+                junk = torch.full((3 * 8 * 6 * 129,), float("nan"), device=gpu)
+                wrong.append((out != ref).any())
+                del junk
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(c, r)) for c, r in zip(cs, refs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(wrong) == 400 and not torch.stack(wrong).any()
