@@ -96,8 +96,10 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const u16* x, int64_t x_st
 // hold its row as the quantiser takes it.  The rounding of k to the activation type
 // stays, so the cache holds what a store of the returned k would write.  Bound by memory
 // from some thousand tokens on; us in bf16, 16/8 heads, here / the 16-bit store above /
-// norm and aac_kv4_store one after the other: 1 token 2.7 / 2.5 / 4.7, 256: 3.4 / 3.3 /
-// 5.3, 16,000: 42.8 (5.8 TB/s) / 50.2 / 52.2, 40,000: 112 / 123 / 126.
+// norm and aac_kv4_store one after the other: 1 token 2.4 / 2.2 / 4.4, 256: 3.2 / 3.0 /
+// 5.0, 16,000: 42.4 (5.8 TB/s) / 48.9 / 52.1 with rows just made, partly in the last-level
+// cache, 46.8 (5.3) / 50.7 / 53.5 with rows from memory, 40,000: 112 / 126 / 128, 262,144:
+// 712 (5.7 TB/s) / 893 / 855.
 struct Qk4Args : QkArgs {
   kv4::Cache c;
 };

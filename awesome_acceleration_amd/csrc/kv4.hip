@@ -15,10 +15,10 @@
 // A group of 256 threads takes 16 consecutive tokens of two heads, so that where they
 // fall into one tile of the cache (the usual case) the codes go out as 1 KiB in one
 // piece.  Bound by memory: 512 bytes in (16-bit types) and 136 out a token and head.
-// Measured: 32,768 tokens of 8 heads in bf16 27 us each way, 6.3 TB/s (rows that a
-// prefill has just made are in the last-level cache); 262,144 tokens 258 us stored, 5.3
-// TB/s, and 238 loaded, 5.7; fp32 5.9 and 7.0.  The load's results go out with
-// non-temporal stores (261 us without).
+// Measured: 32,768 tokens of 8 heads in bf16 26 us each way, 6.4 TB/s (rows that a
+// prefill has just made are in the last-level cache); 262,144 tokens, stored and then loaded,
+// 250 us, 5.4 TB/s, and 246, 5.5; 131,072 of fp32 6.2 and 7.1 TB/s.  The load's results go out
+// with non-temporal stores (10% slower without).
 #include "kv4_quant.h"
 
 namespace aac {
@@ -68,8 +68,9 @@ template <Dt DT, Read R> __device__ __forceinline__ Piece<DT> load_piece(const c
   return x;
 }
 
-// Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16,
-// store and load in us: one head 277 and 273, two 271 and 238, four and eight as two).
+// Heads of a workgroup, whose rows are asked for together (262,144 tokens of 8 heads, bf16, the
+// store through the caches, store and load in us, each alone: one head 277 and 273, two 271
+// and 238, four and eight as two).
 constexpr int kHeads = 2;
 constexpr int64_t kMaxGroups = 1 << 24;  // a launch's threads are numbered in 32 bits
 

@@ -14,7 +14,7 @@
 //   queries are split in 1, 2 or 3 bfloat16 terms (bf16, fp16, fp32), probabilities in 2,
 //   2 or 3, one product for each: queries are exact, and what is cut off a probability is
 //   below 2^-14 of it, in fp32 2^-21.  (A bf16 call's probabilities rounded to one term take 1 to 3%
-//   less time - the first case below 74.9 us against 75.5, the second 282 against 287 -
+//   less time - the first case below 73 us against 75, the second 281 against 285 -
 //   and leave an output 0.0020 off where its own rounding alone is 0.0017.)
 // Sums, the running maximum and the partial results are float.
 //
@@ -31,14 +31,15 @@
 // instead of a byte a lane for each tile.
 //
 // Bound by the way the rows arrive: with the arithmetic left out, the loads alone take
-// 69.7, 276 and 28 us of the cases below, and the arithmetic alone (rows held) 50, 198.
+// 69.7, 276 and 28 us of the cases below, and the arithmetic alone (rows held, one term of the
+// probabilities) 50, 198.
 // So rows are asked for where the last ones have been taken, a step ahead of their use
 // (deeper rings spill or lose a workgroup a CU, and gained nothing), as non-temporal buffer loads, whose
 // bounds stand for the branch at a partition's end, 1 KiB of codes in one piece each.
 // Measured on MI355X (GPU time): bf16, 256 sequences of 1,024 to 2,048 tokens, 16/8 heads
-// 72.5 us (the bytes alone, at the 7.0 TB/s of a large copy: 60); 64 of 16,384 to 32,768
-// 282 (245); fp16, one of 115,000 31 (19), of which the second launch is 3; fp32, 4 of up
-// to 400 tokens 7.6, where latency alone counts.
+// 75 us (the bytes alone, at the 7.0 TB/s of a large copy: 61); 64 of 16,384 to 32,768
+// 285 (244); fp16, one of 115,000 32 (19), of which the second launch is 4; fp32, 4 of up
+// to 400 tokens 7.7, where latency alone counts.
 #include <algorithm>
 #include <climits>
 
@@ -100,8 +101,8 @@ __device__ __forceinline__ int context_len(const DecArgs& a, int len) {
 // there may be; one that would fill less than a quarter of its partitions (of a captured
 // step, mostly) is split by the same rule for its own length, never coarser and into
 // no more than n_parts (us, with its own length and with the plan's partitions, at 8
-// heads: 16 x 500-2,000 in tables of 32,768 14.9 and 19.9, 32 of them 17.6 and 22.1, 8 x 3-30k
-// in 131,072 20.4 and 48.2; without the quarter 100 x 2-6k in 6,000 took 93, not 83).
+// heads: 16 x 500-2,000 in tables of 32,768 16.0 and 20.9, 32 of them 18.4 and 25.3, 8 x 3-30k
+// in 131,072 29.6 and 53.6; without the quarter 100 x 2-6k in 6,000 took 93, not 83).
 __device__ __forceinline__ int part_of(const DecArgs& a, int ctx) {
   if (ctx >= a.tight) return a.part_tokens;
   int part = ctx;
@@ -462,7 +463,12 @@ template <Dt DT> __global__ __launch_bounds__(256) void kv4_reduce_kernel(DecArg
 
 // Workgroups that the GPU holds at once: three per CU, fp32 two.
 static int round_of(bool fp32) { return fp32 ? 512 : 768; }
-// The longest context that is not split.
+// The longest context that is not split.  From 512 (sequence, head) items on whole contexts are
+// faster or as fast (us at 8 heads, whole / in 1024, of 1-2k and of 2-4k tokens: 64 sequences
+// 24.0 / 29.1 and 43.5 / 44.3, 96 33.3 / 38.9 and 61.0 / 62.2, 128 44.1 / 45.8 and 80.8 / 79.6,
+// 192 58.1 / 62.5 and 108 / 114, 256 75.0 / 81.7 and 143 / 150).  The two sides cross below
+// that: 32 16.4 / 17.5 and 28.5 / 28.2, 16 16.6 / 16.5 and 28.8 / 20.8, so that up to 63 sequences
+// of equal lengths (24.2 / 29.1 and 43.3 / 45.0) are split where whole ones would be faster.
 static int32_t whole_context(int64_t items) { return items >= 512 ? 4096 : 768; }
 
 // The longest context that one wave takes, from four rounds of workgroups on (three per
@@ -490,7 +496,7 @@ static Plan plan(int32_t n_seqs, int32_t hq, int32_t hkv, int32_t block_size, in
     // Measured on MI355X (us, graph replay).  A workgroup starts and ends in some 4 us, a
     // turn of 256 tokens takes 1.2 of latency, and the second launch 2.5.  So no split
     // up to 768 tokens (32 x 100-600 at 4 heads: 7.8 against 9.5 in 256), nor from 512
-    // (sequence, head) items up to 4096 (256 x 1-2k: 72.5 against 81 in 768 or 1024).  Else
+    // (sequence, head) items up to 4096 (whole_context).  Else
     // what one round of workgroups (three per CU, fp32 two) makes of the tables, up to
     // 1024 tokens (24 x 100-2063: 768 15.4, 256 17.4, unsplit 17.3; one of 8000: 256
     // 8.4, 768 10.6).  Beyond, contexts of different lengths leave a round's end to a
@@ -516,9 +522,9 @@ template <Dt DT> static void launch(const DecArgs& a, hipStream_t s) {
   // An odd number of partitions: workgroups go round the XCDs and the shader engines of
   // each in turn, so with 4 or 8, of which a captured step sized for the longest context has
   // one or two that hold tokens, those would all fall on one or two engines of four (us,
-  // 256 x 300-1,500 in tables of 16,384 tokens at 8 heads 130 and 50, of 8,192 73 and 48,
-  // 64 x 500-2,000 in 32,768 48 and 26).  Where every partition holds tokens, the one that
-  // is empty costs up to 2% (64 x 16-32k 276 and 282), or nothing (200 x 4-12k).
+  // 256 x 300-1,500 in tables of 16,384 tokens at 8 heads 138 and 54, of 8,192 82 and 53,
+  // 64 x 500-2,000 in 32,768 53 and 28).  Where every partition holds tokens, the one that
+  // is empty costs up to 1% (64 x 16-32k 283 and 285), or nothing (200 x 4-12k 286).
   const dim3 grid(a.c.hkv, a.n_parts | 1, a.n_seqs);
   if (a.c.block_size % kStep == 0)
     hipLaunchKernelGGL((kv4_decode_kernel<DT, true>), grid, dim3(256), 0, s, a);

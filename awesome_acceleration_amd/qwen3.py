@@ -148,8 +148,8 @@ class PagedKV4Cache:
     num_blocks, Hkv, 2, block_size * 68]``: 136 bytes a token, layer and KV head against
     512 in 16 bits.  A prefill attends to its own K and V as they are; decode steps read
     what the cache holds of them.  A decode step of Qwen3-0.6B on MI355X, us, 16 bits /
-    4 bits: 1 sequence of 4,096 tokens 861 / 859, 32 of 2,048 2479 / 1549, 256 of 1,024
-    6264 / 2811, 256 of 4,096 19830 / 6393."""
+    4 bits: 1 sequence of 4,096 tokens 865 / 875, 32 of 2,048 2371 / 1571, 256 of 1,024
+    6274 / 2869, 256 of 4,096 19905 / 6495."""
 
     def __init__(self, cfg: Qwen3Config, num_blocks: int, block_size: int, device):
         self.num_blocks = num_blocks
