@@ -10,6 +10,7 @@ from .flash_attn_interface import (  # noqa: F401
     flash_attn_varlen_func,
     flash_attn_with_kvcache,
     kv_store,
+    prefill_paged,
     varlen_prefill_with_kvcache,
 )
 from .kv4 import (  # noqa: F401
@@ -23,5 +24,6 @@ from .kv4 import (  # noqa: F401
     qk_norm_rope_store_kv4,
 )
 from .paged import BlockAllocator, SlotCacheManager  # noqa: F401
+from .rotary import RotaryEmbedding, apply_rotary_emb, rotary_append_paged  # noqa: F401
 
 __version__ = "0.1.0"

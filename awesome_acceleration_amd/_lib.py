@@ -110,6 +110,21 @@ SIGNATURES: dict[str, tuple] = {
     "aac_logprobs_workspace_bytes": (_size, [_i64, _i64, _i32]),
     "aac_token_logprobs": (
         _c_int, [_p, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _p, _p, _size, _i32, _p]),
+    "aac_prefill_paged_workspace_bytes": (_size, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "aac_prefill_paged": (
+        _c_int,
+        [_p, _i64, _i64, _p, _p, _i64, _i32, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
+         _i32, _f32, _i32, _p, _i64, _p, _size, _i32, _p]),
+    "aac_rotary": (
+        _c_int,
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i32, _i64, _p, _p, _i32, _i32, _i32, _p,
+         _p, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
+    "aac_rotary_append_paged": (
+        _c_int,
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _i32, _i32,
+         _i64, _p, _p, _p, _i32, _i32, _i32, _p, _p, _i32, _i32, _i32, _i32, _p, _p, _i64, _i32, _p,
+         _i32, _i32, _i32, _p]),
+    "aac_rotary_tables": (_c_int, [_p, _i32, _p, _i64, _i64, _f32, _p, _p, _i32, _p]),
 }
 
 ABI_VERSION = 2

@@ -1,0 +1,700 @@
+// Attention of a chunk of new tokens over the paged KV cache (gfx950, bf16/fp16 MFMA):
+// sequence b's n_b queries see its L_b cached tokens (the new ones among them) through
+// its block table, causal ones the first i + 1 + L_b - n_b of them.  The calls between a
+// prefill (llm.py:178-184) and a decode step (model/model.py:233-240): chunked prefill,
+// the next turn of a conversation, draft tokens to verify.
+//
+// A KV head's queries are rows: row r is query r / G of head r % G of its group, so any
+// group size fills the matrix tiles and every key read serves all of them.  A wave holds
+// 32 rows; S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16, the layouts, lazy
+// rescaling and rounding of the probabilities as in prefill_split.hip.  A workgroup is R
+// row blocks times SL key slices: the slices of a row block take 32-key sub-tiles s, s +
+// SL, ... and are merged through LDS at the end.
+//
+// Pages.  16 keys of a tile lie in one page (block sizes are multiples of 16, or one
+// block holds the sequence), so a wave finds their address with scalar loads and
+// arithmetic, one iteration ahead, and brings them with direct loads into LDS through a
+// buffer resource that ends at the context: rows behind it, whatever the page holds,
+// arrive as zeros.  Other block sizes look every row up in its lane (PAGE16 false).
+//
+// Too few workgroups for the GPU: the keys are split into pieces too, whose partial
+// results (fp32) a second kernel joins in piece order.
+
+#include <algorithm>
+
+#include "prefill_common.h"
+
+namespace aac {
+namespace pp {
+
+using pf::D;
+using pf::kRescale;
+
+constexpr int kSubBytes = 32 * D * 2;  // 8 KiB: 32 keys of K or V
+constexpr int kOutPitch = D * 2 + 16;
+
+struct Args {
+  const u16* q;
+  const u16* kc;
+  const u16* vc;
+  u16* out;
+  int64_t q_stride, o_stride;
+  const int32_t* cu_q;
+  const int32_t* ctx;   // context lengths, or null:
+  const int32_t* cu_k;  // their prefix sums
+  const int32_t* tables;
+  int64_t n_tokens;
+  u32 num_blocks;       // those an int32 table can name
+  int32_t n_seqs, hq, hkv, group;
+  int32_t max_q;        // queries of every sequence where cu_q is null
+  int32_t block_size, max_blocks;
+  int32_t capacity;     // keys a table can name
+  u32 magic, shift;     // 16-key group -> page (PAGE16), key -> page otherwise
+  int32_t row_bytes;    // of a cache row, all heads
+  float scale_log2;
+  int32_t n_rb;         // row blocks of the longest sequence
+  int32_t n_split;      // pieces of the keys at most
+  int32_t min_sub;      // sub-tiles of a piece at least
+  float* ws_o;          // [n_tokens][hq][n_split][128]
+  float2* ws_ml;        // [n_tokens][hq][n_split]
+};
+
+// x / d for x < 2^27: x * ceil(2^(27 + s) / d) >> (27 + s), s = ceil(log2 d).
+__device__ __forceinline__ int divide(const Args& a, int x) { return (int)(((uint64_t)(u32)x * a.magic) >> a.shift); }
+
+struct Seq {
+  int q_beg, Lq, Lk;
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int s) {
+  typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
+  const cint* cu = (const cint*)(uintptr_t)a.cu_q;
+  Seq r;
+  if (a.cu_q) {
+    r.q_beg = max(cu[s], 0);
+    r.Lq = (int)min((int64_t)cu[s + 1], a.n_tokens) - r.q_beg;
+  } else {
+    r.q_beg = s * a.max_q;
+    r.Lq = a.max_q;
+  }
+  int lk;
+  if (a.ctx) {
+    lk = ((const cint*)(uintptr_t)a.ctx)[s];
+  } else {
+    const cint* ck = (const cint*)(uintptr_t)a.cu_k;
+    lk = ck[s + 1] - ck[s];
+  }
+  r.Lk = min(max(lk, 0), a.capacity);
+  return r;
+}
+
+// The keys [0, end) that rows up to `row` see, and the pieces they are cut into.
+template <bool CAUSAL> __device__ __forceinline__ int end_of(const Args& a, const Seq& s, int row) {
+  return CAUSAL ? max(row / a.group + 1 + (s.Lk - s.Lq), 0) : s.Lk;
+}
+__device__ __forceinline__ int pieces_of(const Args& a, int end) {
+  const int nsub = (end + 31) / 32;
+  return max(1, min(a.n_split, nsub / a.min_sub));
+}
+
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// 1 KiB straight into LDS (dst + 16 lane); inline assembly, so that the compiler neither
+// counts it nor guards LDS reads with waits for it: the waits are explicit.  M0 is used
+// by nothing else here.
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, int voff, u32 dst) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(r), "s"(dst)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+__device__ __forceinline__ void load_lds16(const u16* p, u32 dst) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(p), "s"(dst)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// At most N of this wave's loads are in flight and its LDS reads are done, then the
+// workgroup's.
+template <int N> __device__ __forceinline__ void landed_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// R row blocks of 32 rows, SL key slices of KT sub-tiles an iteration, STAGES of LDS.
+template <int R_, int SL_, int KT_, int STAGES_> struct Shape {
+  static constexpr int R = R_, SL = SL_, KT = KT_, STAGES = STAGES_;
+  static constexpr int kWaves = R * SL, kThreads = 64 * kWaves;
+  static constexpr int kKeys = 32 * SL * KT;             // of an iteration
+  static constexpr int kTile = SL * KT * kSubBytes;      // bytes of K (or V) of a stage
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kGroups = 2 * kKeys / 16 / kWaves;  // 16-row loads a wave brings
+  static constexpr int kLoads = 4 * kGroups;             // instructions a wave and stage
+  static constexpr int kPart = SL > 1 ? kWaves * 4 * 4096 : 0;  // partial O of the merge
+  static constexpr int kOut = kWaves * 32 * kOutPitch;
+  static constexpr int kMl = kWaves * 32 * 8;
+  static constexpr int kRing = STAGES * kStage;
+  static constexpr int kBody = kRing > kPart + kMl ? kRing : kPart + kMl;
+  static constexpr int kLds = kBody > kOut ? kBody : kOut;
+  static_assert(2 * kKeys % (16 * kWaves) == 0, "whole groups a wave");
+};
+
+template <class S, bool CAUSAL, bool F16, bool PAGE16>
+__global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_paged_kernel(Args a) {
+  typedef pf::Mfma<F16> M;
+  constexpr int SL = S::SL, KT = S::KT, STAGES = S::STAGES;
+  constexpr u32 kExp = F16 ? 0x7c00u : 0x7f80u;  // exponent bits of infinities and NaN
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
+  const u32 lds0 = (u32)(uintptr_t)(lds_u8*)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rb_w = wave % S::R, sl = wave / S::R;  // row block of the workgroup, key slice
+  const int hl = lane >> 5, col = lane & 31;
+
+  // items: KV head fastest (one XCD per head when there are eight), the pieces and row
+  // blocks of a sequence together, the causal ones with the most keys first
+  int it = blockIdx.x;
+  const int h = it % a.hkv;
+  it /= a.hkv;
+  const int piece = it % a.n_split;
+  it /= a.n_split;
+  const int z = it % a.n_rb, sg = it / a.n_rb;
+  const Seq sq = seq_of(a, sg);
+  const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
+  constexpr int kRows = 32 * S::R;
+  const int nrb = (rows + kRows - 1) / kRows;
+  if (z >= nrb) return;  // workgroup-uniform
+  const int row0 = (min(nrb, a.n_rb) - 1 - z) * kRows;  // the workgroup's first row
+  const int kv_end = __builtin_amdgcn_readfirstlane(end_of<CAUSAL>(a, sq, min(row0 + kRows, rows) - 1));
+  const int np = pieces_of(a, kv_end);
+  if (piece >= np) return;
+  const int nsub_all = (kv_end + 31) / 32;
+  // the piece's sub-tiles [j0, j1)
+  const int per = nsub_all / np, more = nsub_all - per * np;
+  const int j0 = piece * per + min(piece, more), j1 = j0 + per + (piece < more ? 1 : 0);
+  const int n_it = (j1 - j0 + SL * KT - 1) / (SL * KT);
+
+  // this wave's and lane's rows
+  const int wrow = row0 + 32 * rb_w;
+  const int my_row = min(wrow + col, rows - 1);
+  const int my_q = my_row / a.group, my_head = h * a.group + (my_row - my_q * a.group);
+  const int w_end = wrow < rows ? end_of<CAUSAL>(a, sq, min(wrow + 31, rows - 1)) : 0;
+  const int full = CAUSAL ? end_of<CAUSAL>(a, sq, wrow) : sq.Lk;  // keys below need no mask
+  const int my_lim = end_of<CAUSAL>(a, sq, my_row);
+  const int w_sub = min(j1, (w_end + 31) / 32);
+
+  // ---- staging: 16-row group g of a stage is rows 16 g of K, then of V; this wave's
+  // are wave * kGroups and up.  16-byte chunk ch of row r sits at ch ^ (r & 15) (K) or
+  // ch ^ 4 (r & 3) (V).
+  typedef const int32_t __attribute__((address_space(4))) cint;
+  const cint* tab = (const cint*)(uintptr_t)(a.tables + (int64_t)sg * a.max_blocks);
+  constexpr int kKGroups = S::kKeys / 16;
+  const int r4 = lane >> 4;
+  int voff_k[4], voff_v;  // (rows of i = 1..3 of V: 4 i rows further)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) voff_k[i] = (4 * i + r4) * a.row_bytes + 16 * ((lane & 15) ^ (4 * i + r4));
+  voff_v = r4 * a.row_bytes + 16 * ((lane & 15) ^ (4 * r4));
+  const int key_base = 32 * j0;
+  int ent[S::kGroups];  // block numbers of the next stage's groups
+  auto first_key = [&](int n, int gi) { return key_base + n * S::kKeys + 16 * ((wave * S::kGroups + gi) % kKGroups); };
+  auto look_up = [&](int n) {
+    if constexpr (PAGE16) {
+#pragma unroll
+      for (int gi = 0; gi < S::kGroups; ++gi)
+        ent[gi] = tab[min(divide(a, first_key(n, gi) >> 4), a.max_blocks - 1)];
+    }
+  };
+  auto issue = [&](int n) {
+    const u32 st = lds0 + (u32)(n % STAGES * S::kStage);
+#pragma unroll
+    for (int gi = 0; gi < S::kGroups; ++gi) {
+      const int g = wave * S::kGroups + gi;
+      const bool is_k = g < kKGroups;
+      const int key = first_key(n, gi);
+      const u16* cache = (is_k ? a.kc : a.vc) + h * D;
+      const u32 dst = st + (u32)(g * 4096);
+      if constexpr (PAGE16) {
+        const int page = divide(a, key >> 4);
+        const int64_t blk = (u32)ent[gi] < a.num_blocks ? ent[gi] : 0;
+        const int64_t row = blk * a.block_size + (key - page * a.block_size);
+        // (the head's 256 bytes of a row lie before the next row's)
+        const int n_rows = min(16, kv_end - min(key, kv_end));
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<u16*>(cache + row * (u32)(a.row_bytes >> 1)), 0, n_rows * a.row_bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          load_lds16(rs, is_k ? voff_k[i] : voff_v + 4 * i * a.row_bytes, dst + i * 1024);
+      } else {
+        // every lane's own row; rows behind the context repeat its last one (masked)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * i + r4;
+          const int k = min(key + r, kv_end - 1);
+          const int page = divide(a, k);
+          const int e = a.tables[(int64_t)sg * a.max_blocks + page];
+          const int64_t blk = (u32)e < a.num_blocks ? e : 0;
+          const int64_t row = blk * a.block_size + (k - page * a.block_size);
+          const int ch = (lane & 15) ^ (is_k ? r : 4 * r4);
+          load_lds16(cache + row * (a.row_bytes >> 1) + 8 * ch, dst + i * 1024);
+        }
+      }
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < STAGES - 1; ++n)
+    if (n < n_it) {
+      look_up(n);
+      issue(n);
+    }
+  look_up(STAGES - 1);
+
+  // Q fragments (B operand of S^T = K Q^T: lane = row)
+  u32x4 qf[8];
+  {
+    const u16* qp = a.q + (int64_t)(sq.q_beg + my_q) * a.q_stride + my_head * D + hl * 8;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
+  }
+  // fragment addresses within a sub-tile (see prefill_wide.hip)
+  int koff[8], vo[4];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) koff[t] = col * 256 + 16 * ((2 * t + hl) ^ (col & 15));
+  {
+    const int g = lane >> 4, i = lane & 15;
+    const int l0 = (4 * (g >> 1) + (i >> 2)) * 256 + 32 * (g & 1) + 8 * (i & 3);
+#pragma unroll
+    for (int db = 0; db < 4; ++db) vo[db] = l0 + 64 * (db ^ (i >> 2));
+  }
+
+  const float cs = a.scale_log2, kthr = kRescale / cs;
+  f32x16 o[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+  float m = -1e30f, l = 0.f;  // reference max (raw scores), lane-partial row sum
+  // Q has arrived: left pending into the loop it would make every iteration wait for
+  // all loads (vmcnt 0, the others unconstrained)
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+
+  for (int n = 0; n < n_it; ++n) {
+    if (STAGES > 2 && n + STAGES - 2 < n_it) landed_barrier<(STAGES - 2) * S::kLoads>();
+    else landed_barrier<0>();
+    if (n + STAGES - 1 < n_it) {
+      issue(n + STAGES - 1);
+      look_up(n + STAGES);
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int sub = sl * KT + kt, j = j0 + n * SL * KT + sub;
+      if (j >= w_sub) break;  // wave-uniform
+      const lds_u8* kb = (const lds_u8*)lds + n % STAGES * S::kStage + sub * kSubBytes;
+      const lds_u8* vb = kb + S::kTile;
+      f32x16 s;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const u32x4 kf = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(kb + koff[t]);
+        s = M::run(kf, qf[t], s);
+      }
+      const bool masked = 32 * j + 32 > full;
+      if (masked) {
+        const int lim = my_lim - 32 * j - 4 * hl;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < lim ? s[i] : -INFINITY;
+      }
+      float mx = vmax3(s[0], s[1], s[2]);
+#pragma unroll
+      for (int i = 3; i < 15; i += 2) mx = vmax3(mx, s[i], s[i + 1]);
+      mx = vmax(mx, s[15]);
+      if (__ballot(!(mx <= m + kthr))) {  // any lane (or a NaN): rescale (rare after the first sub-tile)
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = vmax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        // (only the rows that need it: a row's result does not hang on its neighbours)
+        const float mn = mx <= m + kthr ? m : vmax(m, mx), alpha = fast_exp2((m - mn) * cs);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+      }
+      const float nb = -m * cs;
+      u32 pw[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        pw[w] = M::pack(fast_exp2(fmaf(s[2 * w], cs, nb)), fast_exp2(fmaf(s[2 * w + 1], cs, nb)));
+        l = M::dot2_ones(pw[w], l);
+      }
+      auto v_frag = [&](int db, int tt) {
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + vo[db] + 4096 * tt));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + vo[db] + 4096 * tt + 2048));
+        const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a0[0], a0[1], a1[0], a1[1]};
+      };
+      if (masked) {
+        // A value that a row does not see must not reach it, whatever it is: with an
+        // infinity or a NaN among these 32 keys' values, the product takes 0 in its
+        // place and the rows that see its key add it
+        u32 bad = 0;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int db = 0; db < 4; ++db) {
+            const u32x4 x = v_frag(db, tt);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              bad |= (u32)((x[e] & kExp) == kExp) | (u32)((x[e] & (kExp << 16)) == (kExp << 16));
+          }
+        if (__ballot(bad != 0)) {
+#pragma unroll 1
+          for (int tt = 0; tt < 2; ++tt) {
+            const u32x4 p = tt ? u32x4{pw[4], pw[5], pw[6], pw[7]} : u32x4{pw[0], pw[1], pw[2], pw[3]};
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+              u32x4 x = v_frag(db, tt);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((x[e] & kExp) == kExp) x[e] &= 0xffff0000u;
+                if ((x[e] & (kExp << 16)) == (kExp << 16)) x[e] &= 0xffffu;
+              }
+              o[db] = M::run(x, p, o[db]);
+            }
+          }
+          const int seen = my_lim - 32 * j;
+#pragma unroll 1
+          for (int k = 0; k < 32; ++k) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                // dims 32 db + 8 r + 4 hl .. + 3 of key k
+                const u32x2 x = *reinterpret_cast<const __attribute__((address_space(3))) u32x2*>(
+                    vb + k * 256 + 16 * ((4 * db + r) ^ (4 * (k & 3))) + 8 * hl);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const u32 b = e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xffffu;
+                  const float f = F16 ? f16lo(b) : bf16lo(b);
+                  if ((b & kExp) == kExp && k < seen) o[db][4 * r + e] += f;
+                }
+              }
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const u32x4 p = {pw[4 * tt], pw[4 * tt + 1], pw[4 * tt + 2], pw[4 * tt + 3]};
+#pragma unroll
+        for (int db = 0; db < 4; ++db) o[db] = M::run(v_frag(db, tt), p, o[db]);
+      }
+    }
+  }
+
+  // ---- merge the slices of each row block: slice s takes dims 128 s / SL and up, its own
+  // part from registers, the others' through LDS (over the dead stages)
+  {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  __syncthreads();
+  float mt = m, lt = l;
+  if constexpr (SL > 1) {
+    auto part = [&](int w, int db) { return reinterpret_cast<f32x4*>(lds + (4 * w + db) * 4096); };
+    float2* ml = reinterpret_cast<float2*>(lds + S::kPart);
+    if (lane < 32) ml[wave * 32 + col] = make_float2(m, l);
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      if (db * SL / 4 != sl) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          part(wave, db)[r * 64 + lane] = f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
+      }
+    __syncthreads();
+    float2 mls[SL];
+    mt = -1e30f;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      mls[k] = ml[(k * S::R + rb_w) * 32 + col];
+      mt = vmax(mt, mls[k].x);
+    }
+    float wt[SL];
+    lt = 0.f;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      wt[k] = fast_exp2((mls[k].x - mt) * cs);
+      lt = fmaf(mls[k].y, wt[k], lt);
+    }
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      if (db * SL / 4 == sl) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < SL; ++k) {  // in slice order
+            if (k == db * SL / 4) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = fmaf(o[db][4 * r + e], wt[k], v[e]);
+            } else {
+              const f32x4 x = part(k * S::R + rb_w, db)[r * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], wt[k], v[e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[db][4 * r + e] = v[e];
+        }
+      }
+  }
+
+  const int64_t orow = (int64_t)(sq.q_beg + my_q);
+  const bool real = wrow + col < rows;
+  if (np > 1) {  // a piece: unnormalised, in fp32
+    if (!real) return;
+    const int64_t slot = (orow * a.hq + my_head) * a.n_split + piece;
+    if (sl == 0 && hl == 0) a.ws_ml[slot] = make_float2(mt * cs, lt);
+    float* dst = a.ws_o + slot * D;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      if (SL == 1 || db * SL / 4 == sl) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * r + 4 * hl) =
+              f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
+      }
+    return;
+  }
+  const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : (lt == 0.f ? 0.f : lt);  // (a NaN stays one)
+  if constexpr (SL > 1) __syncthreads();  // the partial results have been read
+  unsigned char* stg = lds + rb_w * (32 * kOutPitch);
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+    if (SL == 1 || db * SL / 4 == sl) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        u32x2 w;
+        w[0] = M::pack(o[db][4 * r] * inv, o[db][4 * r + 1] * inv);
+        w[1] = M::pack(o[db][4 * r + 2] * inv, o[db][4 * r + 3] * inv);
+        *reinterpret_cast<u32x2*>(stg + col * kOutPitch + (32 * db + 8 * r + 4 * hl) * 2) = w;
+      }
+    }
+  __syncthreads();
+  // whole rows: 16 lanes a row
+  for (int r = tid >> 4; r < kRows; r += S::kThreads / 16) {
+    const int row = row0 + r;
+    if (row >= rows) break;
+    const int qi = row / a.group;
+    *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.q_beg + qi) * a.o_stride +
+                              (h * a.group + row - qi * a.group) * D + (lane & 15) * 8) =
+        *reinterpret_cast<const u32x4*>(lds + (r >> 5) * (32 * kOutPitch) + (r & 31) * kOutPitch + (lane & 15) * 16);
+  }
+}
+
+// Joins the pieces of a row, in piece order: a wave a row, two dims a lane.
+template <bool CAUSAL, bool F16, int ROWS>
+__global__ __launch_bounds__(256) void prefill_paged_join_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y;
+  for (int sg = blockIdx.z; sg < a.n_seqs; sg += gridDim.z) {
+    const Seq sq = seq_of(a, sg);
+    const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
+    if (row >= rows) continue;
+    const int last = min((row / ROWS + 1) * ROWS, rows) - 1;
+    const int np = pieces_of(a, end_of<CAUSAL>(a, sq, last));
+    if (np == 1) continue;  // written by its workgroup
+    const int qi = row / a.group, head = h * a.group + row - qi * a.group;
+    const int64_t slot = ((int64_t)(sq.q_beg + qi) * a.hq + head) * a.n_split;
+    float mx = -3e38f;
+    for (int p = 0; p < np; ++p) mx = vmax(mx, a.ws_ml[slot + p].x);
+    float o0 = 0.f, o1 = 0.f, lt = 0.f;
+    for (int p = 0; p < np; ++p) {
+      const float2 ml = a.ws_ml[slot + p];
+      const float2 v = *reinterpret_cast<const float2*>(a.ws_o + (slot + p) * D + 2 * lane);
+      const float w = fast_exp2(ml.x - mx);
+      lt = fmaf(ml.y, w, lt);
+      o0 = fmaf(v.x, w, o0);
+      o1 = fmaf(v.y, w, o1);
+    }
+    const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : (lt == 0.f ? 0.f : lt);
+    *reinterpret_cast<u32*>(a.out + (int64_t)(sq.q_beg + qi) * a.o_stride + head * D + 2 * lane) =
+        pf::Mfma<F16>::pack(o0 * inv, o1 * inv);
+  }
+}
+
+// ------------------------------------------------------------------ host
+typedef Shape<1, 4, 1, 2> Rows32;
+typedef Shape<2, 4, 1, 2> Rows64;
+typedef Shape<4, 2, 1, 4> Rows128;
+typedef Shape<8, 1, 2, 4> Rows256;
+
+struct Plan {
+  int rows;  // of a workgroup: 32, 64, 128 or 256
+  int n_split, min_sub;
+  size_t bytes;
+};
+
+static Plan plan(int64_t n_tokens, int32_t n_seqs, int32_t max_q, int32_t max_k, int32_t hq, int32_t hkv, int n_cu) {
+  Plan p = {};
+  const int64_t rows = (int64_t)max_q * (hq / hkv);
+  p.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  const int64_t items = (int64_t)n_seqs * hkv * cdiv(rows, p.rows);
+  // as many pieces as fill the GPU once, of eight sub-tiles (256 keys) at least
+  p.min_sub = 8;
+  const int64_t nsub = cdiv(max_k, 32);
+  p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / std::max<int64_t>(items, 1), nsub / p.min_sub));
+  if (p.n_split > 1) p.bytes = (size_t)n_tokens * hq * p.n_split * (D * 4 + 8);
+  return p;
+}
+
+template <class S, bool CAUSAL, bool F16>
+static int launch_s(Args a, bool page16, int32_t max_q, int32_t, hipStream_t st) {
+  const int64_t rows = (int64_t)max_q * a.group;
+  a.n_rb = (int)cdiv(rows, 32 * S::R);
+  const int64_t grid = (int64_t)a.n_seqs * a.n_rb * a.n_split * a.hkv;
+  if (grid >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
+  if (page16)
+    hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true>), dim3((unsigned)grid), dim3(S::kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false>), dim3((unsigned)grid), dim3(S::kThreads), 0, st, a);
+  if (a.n_split > 1)
+    hipLaunchKernelGGL((prefill_paged_join_kernel<CAUSAL, F16, 32 * S::R>),
+                       dim3((unsigned)cdiv(rows, 4), (unsigned)a.hkv, (unsigned)std::min(a.n_seqs, 65535)), dim3(256), 0,
+                       st, a);
+  return AAC_OK;
+}
+
+template <bool CAUSAL, bool F16>
+static int launch_r(const Args& a, const Plan& p, bool page16, int32_t max_q, int32_t max_k, hipStream_t st) {
+  switch (p.rows) {
+    case 32: return launch_s<Rows32, CAUSAL, F16>(a, page16, max_q, max_k, st);
+    case 64: return launch_s<Rows64, CAUSAL, F16>(a, page16, max_q, max_k, st);
+    case 128: return launch_s<Rows128, CAUSAL, F16>(a, page16, max_q, max_k, st);
+    default: return launch_s<Rows256, CAUSAL, F16>(a, page16, max_q, max_k, st);
+  }
+}
+
+}  // namespace pp
+}  // namespace aac
+
+using namespace aac;
+
+// The longest context the work is split for: the caller's estimate within what a table
+// can name.
+static int64_t capacity_of(int32_t block_size, int32_t max_blocks) {
+  return std::min<int64_t>((int64_t)max_blocks * block_size, (int64_t(1) << 31) - 4096);
+}
+static int32_t longest_of(int32_t max_context_len, int64_t cap) {
+  return max_context_len > 0 ? (int32_t)std::min<int64_t>(max_context_len, cap) : (int32_t)cap;
+}
+
+extern "C" size_t aac_prefill_paged_workspace_bytes(int64_t n_tokens, int32_t n_seqs, int32_t max_seqlen_q,
+                                                    int32_t max_context_len, int32_t block_size,
+                                                    int32_t max_blocks_per_seq, int32_t n_q_heads,
+                                                    int32_t n_kv_heads) {
+  int n_cu = 0;
+  if (n_tokens <= 0 || n_seqs <= 0 || max_seqlen_q <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
+      n_q_heads % n_kv_heads || block_size <= 0 || max_blocks_per_seq <= 0 || device_cu_count(&n_cu) != AAC_OK)
+    return 0;
+  const int32_t max_k = longest_of(max_context_len, capacity_of(block_size, max_blocks_per_seq));
+  return pp::plan(n_tokens, n_seqs, max_seqlen_q, max_k, n_q_heads, n_kv_heads, n_cu).bytes;
+}
+
+extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, const void* k_cache,
+                                 const void* v_cache, int64_t num_blocks, int32_t block_size,
+                                 const int32_t* block_tables, int32_t max_blocks_per_seq,
+                                 const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                                 const int32_t* cu_seqlens_k, int32_t n_seqs, int32_t max_seqlen_q,
+                                 int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                 float scale, int32_t causal, void* out, int64_t out_tok_stride, void* workspace,
+                                 size_t workspace_bytes, int32_t dtype, void* stream) {
+  if (dtype != AAC_DTYPE_BF16 && dtype != AAC_DTYPE_FP16) return AAC_ERR_UNSUPPORTED;
+  if (head_dim != pp::D) return AAC_ERR_UNSUPPORTED;
+  if (n_tokens < 0 || n_seqs < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || max_seqlen_q < 0 || num_blocks < 0 ||
+      block_size <= 0 || max_blocks_per_seq <= 0 || q_tok_stride < 0 || out_tok_stride < 0 || !(scale > 0.f) ||
+      scale > 3e38f)
+    return AAC_ERR_INVALID_ARGUMENT;
+  if (n_q_heads % n_kv_heads || n_tokens >= (int64_t(1) << 31) ||
+      (!cu_seqlens_q && n_tokens != (int64_t)n_seqs * max_seqlen_q))
+    return AAC_ERR_SHAPE;
+  if (n_tokens == 0 || n_seqs == 0 || max_seqlen_q == 0) return AAC_OK;
+  if (!q || !out || !block_tables || (!context_lens && !cu_seqlens_k))
+    return AAC_ERR_INVALID_ARGUMENT;
+  if (num_blocks == 0 || !k_cache || !v_cache) return AAC_ERR_INVALID_ARGUMENT;
+  if (q_tok_stride < (int64_t)n_q_heads * head_dim || out_tok_stride < (int64_t)n_q_heads * head_dim)
+    return AAC_ERR_SHAPE;
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16 || q_tok_stride % 8 ||
+      out_tok_stride % 8)
+    return AAC_ERR_MISALIGNED;
+  // 16 rows of the cache, all heads, within a buffer resource's 32-bit offsets; rows of a
+  // sequence numbered in int32; positions in 27 bits of groups or rows
+  const int64_t cap = capacity_of(block_size, max_blocks_per_seq);
+  if ((int64_t)n_kv_heads * head_dim * 2 * 16 >= (int64_t(1) << 31) ||
+      (int64_t)max_seqlen_q * (n_q_heads / n_kv_heads) >= (int64_t(1) << 30))
+    return AAC_ERR_UNSUPPORTED;
+  const bool one = max_blocks_per_seq == 1, page16 = one || block_size % 16 == 0;
+  if (!page16 && cap > (int64_t(1) << 27)) return AAC_ERR_UNSUPPORTED;
+  pp::Args a = {};
+  a.q = (const u16*)q;
+  a.kc = (const u16*)k_cache;
+  a.vc = (const u16*)v_cache;
+  a.out = (u16*)out;
+  a.q_stride = q_tok_stride;
+  a.o_stride = out_tok_stride;
+  a.cu_q = cu_seqlens_q;
+  a.ctx = context_lens;
+  a.cu_k = cu_seqlens_k;
+  a.tables = block_tables;
+  a.num_blocks = (u32)std::min<int64_t>(num_blocks, INT32_MAX);
+  a.n_tokens = n_tokens;
+  a.n_seqs = n_seqs;
+  a.hq = n_q_heads;
+  a.hkv = n_kv_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.max_q = max_seqlen_q;
+  a.block_size = block_size;
+  a.max_blocks = max_blocks_per_seq;
+  a.capacity = (int)cap;
+  a.row_bytes = n_kv_heads * head_dim * 2;
+  a.scale_log2 = scale * kLog2e;
+  {
+    // a single block: every key is on page 0
+    const int64_t d = one ? int64_t(1) << 27 : page16 ? block_size / 16 : block_size;
+    u32 s = 0;
+    while ((int64_t(1) << s) < d) ++s;
+    a.magic = (u32)cdiv(int64_t(1) << (27 + s), d);
+    a.shift = 27 + s;
+  }
+  int n_cu = 0;
+  int rc = device_cu_count(&n_cu);
+  if (rc != AAC_OK) return rc;
+  const int32_t max_k = longest_of(max_context_len, cap);
+  const pp::Plan p = pp::plan(n_tokens, n_seqs, max_seqlen_q, max_k, n_q_heads, n_kv_heads, n_cu);
+  a.n_split = p.n_split;
+  a.min_sub = p.min_sub;
+  if (p.bytes) {
+    if (!workspace || workspace_bytes < p.bytes) return AAC_ERR_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return AAC_ERR_MISALIGNED;
+    a.ws_o = (float*)workspace;
+    a.ws_ml = (float2*)(a.ws_o + (size_t)n_tokens * n_q_heads * p.n_split * pp::D);
+  }
+  hipStream_t st = (hipStream_t)stream;
+  const bool f16 = dtype == AAC_DTYPE_FP16;
+  if (causal) rc = f16 ? pp::launch_r<true, true>(a, p, page16, max_seqlen_q, max_k, st)
+                       : pp::launch_r<true, false>(a, p, page16, max_seqlen_q, max_k, st);
+  else rc = f16 ? pp::launch_r<false, true>(a, p, page16, max_seqlen_q, max_k, st)
+                : pp::launch_r<false, false>(a, p, page16, max_seqlen_q, max_k, st);
+  if (rc != AAC_OK) return rc;
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? AAC_OK : (int)e;
+}

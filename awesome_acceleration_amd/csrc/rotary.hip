@@ -1,0 +1,532 @@
+// Rotary positions (gfx950): the rotation of query and key heads by their tokens'
+// angles, alone or on the way into the paged KV cache, and the cos / sin tables.
+//
+// A head's first R dims are R / 2 pairs, (d, d + R/2) or, interleaved, (2 d, 2 d + 1);
+// pair d of a token at position p turns by the angle of row p, column d of the tables:
+//   (x1, x2) -> (x1 c - x2 s, x1 s + x2 c), in fp32, rounded once to the head's type;
+// dims from R on pass unchanged.  With caches, the rotated key and the value of new
+// token i of sequence b go to the row that b's block table has for position
+// cache_seqlens[b] + i (the k= / v= half of flash_attn_with_kvcache,
+// model/model.py:233-240, for any number of new tokens).
+//
+// Bound by memory: every row is read and written once.  A wave takes one token's rows
+// (query, key and value heads): CPR lanes a row, each with 8 pairs (two 16-byte vectors
+// of 16-bit values), so the angles are loaded once for all the rows a lane takes and a
+// pass over 64 / CPR rows needs no exchange between lanes.  kRows passes go out before
+// the first is used.
+
+#include <algorithm>
+
+#include "aac_common.h"
+
+namespace aac {
+namespace rot {
+
+constexpr int kWaves = 4;
+
+struct Rows {  // heads of one kind: element strides of a sequence, a token, a head
+  const char* in;
+  char* out;  // q: the rotated rows; k, v: the cache
+  int64_t seq, tok, head;
+  int64_t out_seq, out_tok, out_head;
+  int32_t heads;
+  int32_t len;  // tokens of a sequence that have such heads (without cu_seqlens)
+};
+
+struct Args {
+  Rows q, k, v;
+  const void* cos;
+  const void* sin;
+  int32_t table_rows, half;  // tables [table_rows, half]
+  const int32_t* offsets;    // first position of a sequence, or null: offset0
+  int32_t offset0;
+  int32_t q_step;            // 0: every query of a sequence stands at its first position
+  const int32_t* cu;         // packed tokens: their sequences' bounds, or null
+  int32_t n_seqs;
+  int32_t seqlen;            // tokens of a sequence (without cu)
+  int64_t n_tokens;
+  const int32_t* block_tables;
+  int32_t max_blocks, block_size;
+  int64_t num_blocks;
+  int32_t dim;
+  int32_t slots;  // waves a token
+  int32_t sign;   // -1: turned back
+  int32_t* context_lens;  // out, or null: first position + new keys
+};
+
+// Elements in their own type <-> fp32, N of them side by side.
+template <Dt DT> struct Io;
+template <> struct Io<Dt::FP32> {
+  typedef float T;
+  __device__ static inline float get(T x) { return x; }
+  __device__ static inline T put(float x) { return x; }
+};
+template <> struct Io<Dt::BF16> {
+  typedef u16 T;
+  __device__ static inline float get(T x) { return __uint_as_float((u32)x << 16); }
+  __device__ static inline T put(float x) { return (u16)Elem<Dt::BF16>::pack2_hw(x, x); }
+};
+template <> struct Io<Dt::FP16> {
+  typedef u16 T;
+  __device__ static inline float get(T x) { return (float)__builtin_bit_cast(_Float16, x); }
+  __device__ static inline T put(float x) { return __builtin_bit_cast(u16, (_Float16)x); }
+};
+
+template <Dt DT> struct Vec8 {  // 8 elements as loaded
+  u32x4 a;
+  __device__ inline void load(const void* p) { a = *reinterpret_cast<const u32x4*>(p); }
+  __device__ inline void store(void* p) const { *reinterpret_cast<u32x4*>(p) = a; }
+  __device__ inline void get(float* f) const { Elem<DT>::unpack8(a, f); }
+  __device__ inline void put(const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = Elem<DT>::pack2_hw(f[2 * i], f[2 * i + 1]);
+  }
+};
+template <> struct Vec8<Dt::FP32> {
+  u32x4 a, b;
+  __device__ inline void load(const void* p) {
+    a = reinterpret_cast<const u32x4*>(p)[0];
+    b = reinterpret_cast<const u32x4*>(p)[1];
+  }
+  __device__ inline void store(void* p) const {
+    reinterpret_cast<u32x4*>(p)[0] = a;
+    reinterpret_cast<u32x4*>(p)[1] = b;
+  }
+  __device__ inline void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __uint_as_float(a[i]);
+      f[4 + i] = __uint_as_float(b[i]);
+    }
+  }
+  __device__ inline void put(const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __float_as_uint(f[i]);
+      b[i] = __float_as_uint(f[4 + i]);
+    }
+  }
+};
+
+// The sequence of packed token t: the last b with cu[b] <= t (64 bounds a load).
+__device__ __forceinline__ int seq_of(const int32_t* cu, int n_seqs, int64_t t, int lane) {
+  int lo = 0, n = n_seqs;
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int at = lane * step;
+    const bool in = at < n && cu[lo + min(at, n - 1)] <= t;
+    const int hits = __popcll(__ballot(in));
+    const int skip = max(hits - 1, 0) * step;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  return lo;
+}
+
+struct Place {
+  int64_t q_at, in_at[3];  // element offsets of the token's rows: q out, q / k / v in
+  int64_t crow;            // cache row of k and v, or -1
+  int q_pos, k_pos;        // rows of the tables
+  bool has_q, has_kv;
+};
+
+__device__ __forceinline__ bool place_of(const Args& a, int64_t t, int lane, Place& p) {
+  int b;
+  int64_t s;
+  if (a.cu) {
+    b = seq_of(a.cu, a.n_seqs, t, lane);
+    s = t - a.cu[b];
+    if (s < 0 || t >= a.cu[b + 1]) return false;  // a row of no sequence
+    p.q_at = t * a.q.out_tok;
+    p.in_at[0] = t * a.q.tok;
+    p.in_at[1] = t * a.k.tok;
+    p.in_at[2] = t * a.v.tok;
+    p.has_q = p.has_kv = true;
+  } else {
+    b = (int)(t / a.seqlen);
+    s = t - (int64_t)b * a.seqlen;
+    p.q_at = b * a.q.out_seq + s * a.q.out_tok;
+    p.in_at[0] = b * a.q.seq + s * a.q.tok;
+    p.in_at[1] = b * a.k.seq + s * a.k.tok;
+    p.in_at[2] = b * a.v.seq + s * a.v.tok;
+    p.has_q = s < a.q.len;
+    p.has_kv = s < a.k.len;
+  }
+  const int64_t first = a.offsets ? a.offsets[b] : a.offset0;
+  if (a.context_lens && s == 0 && lane == 0) a.context_lens[b] = (int)first + a.k.len;
+  const int64_t last = max(a.table_rows - 1, 0);
+  p.k_pos = (int)min(max(first + s, (int64_t)0), last);
+  p.q_pos = (int)min(max(first + s * a.q_step, (int64_t)0), last);
+  p.crow = -1;
+  if (a.block_tables && p.has_kv) {
+    const int64_t at = first + s;
+    if (first >= 0 && at <= INT32_MAX && at < (int64_t)a.max_blocks * a.block_size) {
+      const int blk = a.block_tables[(int64_t)b * a.max_blocks + (int)at / a.block_size];
+      if (blk >= 0 && blk < a.num_blocks) p.crow = (int64_t)blk * a.block_size + (int)at % a.block_size;
+    }
+  }
+  return true;
+}
+
+// Where row r of a token's heads (query, key, value heads in this order) comes from and
+// goes; false for a row that is not written.
+__device__ __forceinline__ bool row_of(const Args& a, const Place& p, int r, int64_t& in, int64_t& out, int& kind) {
+  if (r < a.q.heads) {
+    kind = 0;
+    in = p.in_at[0] + r * a.q.head;
+    out = p.q_at + r * a.q.out_head;
+    return p.has_q;
+  }
+  r -= a.q.heads;
+  kind = r < a.k.heads ? 1 : 2;
+  const Rows& w = kind == 1 ? a.k : a.v;
+  r -= kind == 1 ? 0 : a.k.heads;
+  in = p.in_at[kind] + r * w.head;
+  out = (p.crow * w.heads + r) * a.dim;
+  return p.crow >= 0;
+}
+
+// 16 elements a lane: 8 pairs, rotated, or 16 dims past them, copied.  Head sizes of
+// 16 times a power of two up to 1024, rotated dims a multiple of 16, everything
+// 16-byte aligned.
+template <Dt DT, bool T32, bool INTER, int PASSES>
+__global__ __launch_bounds__(64 * kWaves) void rotary_kernel(Args a) {
+  constexpr int ES = Elem<DT>::kBytes;
+  constexpr Dt TT = T32 ? Dt::FP32 : DT;
+  const int lane = threadIdx.x & 63;
+  const int64_t w = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = w / a.slots;
+  if (t >= a.n_tokens) return;
+  Place p;
+  if (!place_of(a, t, lane, p)) return;
+  const int cpr = a.dim >> 4, c = lane & (cpr - 1), per = 64 / cpr;
+  const int total = a.q.heads + a.k.heads + a.v.heads;
+  const bool turn = 8 * c < a.half;  // this lane's dims are pairs
+  // element offsets of the lane's two vectors in a row
+  const int d0 = INTER || !turn ? 16 * c : 8 * c, d1 = INTER || !turn ? 16 * c + 8 : 8 * c + a.half;
+  const int r0 = (int)(w - t * a.slots) * (PASSES * per) + lane / cpr;
+
+  Vec8<DT> x[PASSES][2];
+  int64_t out[PASSES];
+  int kind[PASSES];
+  bool live[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = r0 + i * per;
+    int64_t in = 0;
+    live[i] = r < total && row_of(a, p, min(r, total - 1), in, out[i], kind[i]);
+    if (live[i]) {
+      const char* src = (kind[i] == 0 ? a.q.in : kind[i] == 1 ? a.k.in : a.v.in) + in * ES;
+      x[i][0].load(src + d0 * ES);
+      x[i][1].load(src + d1 * ES);
+    }
+  }
+  // queries' and keys' angles: one row of the tables unless the queries all stand at
+  // their sequence's first position
+  float cf[8], sf[8];
+  auto angles = [&](int pos) {
+    constexpr int TS = Elem<TT>::kBytes;
+    const int64_t at = ((int64_t)pos * a.half + 8 * c) * TS;
+    Vec8<TT> u;
+    u.load(reinterpret_cast<const char*>(a.cos) + at);
+    u.get(cf);
+    u.load(reinterpret_cast<const char*>(a.sin) + at);
+    u.get(sf);
+    if (a.sign < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sf[i] = -sf[i];
+    }
+  };
+  int have = -1;
+  if (turn && a.half > 0) angles(have = p.k_pos);
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    if (!live[i]) continue;
+    if (turn && kind[i] != 2) {
+      const int pos = kind[i] == 0 ? p.q_pos : p.k_pos;
+      if (pos != have) angles(have = pos);
+      float f[16];
+      x[i][0].get(f);
+      x[i][1].get(f + 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int e0 = INTER ? 2 * e : e, e1 = INTER ? 2 * e + 1 : e + 8;
+        const float a0 = f[e0], a1 = f[e1];
+        f[e0] = fmaf(a0, cf[e], -(a1 * sf[e]));
+        f[e1] = fmaf(a0, sf[e], a1 * cf[e]);
+      }
+      x[i][0].put(f);
+      x[i][1].put(f + 8);
+    }
+    char* dst = (kind[i] == 0 ? a.q.out : kind[i] == 1 ? a.k.out : a.v.out) + out[i] * ES;
+    // a value row's vectors where its lane reads them
+    x[i][0].store(dst + d0 * ES);
+    x[i][1].store(dst + d1 * ES);
+  }
+}
+
+// The same for any even head size, rotated dims and alignment, an element pair a lane.
+template <Dt DT, bool T32, bool INTER>
+__global__ __launch_bounds__(64 * kWaves) void rotary_any_kernel(Args a) {
+  typedef typename Io<DT>::T E;
+  constexpr Dt TT = T32 ? Dt::FP32 : DT;
+  typedef typename Io<TT>::T TE;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= a.n_tokens) return;
+  Place p;
+  if (!place_of(a, t, lane, p)) return;
+  const int total = a.q.heads + a.k.heads + a.v.heads, pairs = a.dim / 2;
+  for (int64_t i = lane; i < (int64_t)total * pairs; i += 64) {
+    const int r = (int)(i / pairs), c = (int)(i - (int64_t)r * pairs);
+    int64_t in, out;
+    int kind;
+    if (!row_of(a, p, r, in, out, kind)) continue;
+    const bool pair = c < a.half;
+    const int d0 = INTER || !pair ? 2 * c : c, d1 = INTER || !pair ? 2 * c + 1 : c + a.half;
+    const E* src = reinterpret_cast<const E*>(kind == 0 ? a.q.in : kind == 1 ? a.k.in : a.v.in) + in;
+    E* dst = reinterpret_cast<E*>(kind == 0 ? a.q.out : kind == 1 ? a.k.out : a.v.out) + out;
+    E x0 = src[d0], x1 = src[d1];
+    if (pair && kind != 2) {
+      const int64_t at = (int64_t)(kind == 0 ? p.q_pos : p.k_pos) * a.half + c;
+      const float cf = Io<TT>::get(reinterpret_cast<const TE*>(a.cos)[at]);
+      const float sf = Io<TT>::get(reinterpret_cast<const TE*>(a.sin)[at]) * (float)a.sign;
+      const float a0 = Io<DT>::get(x0), a1 = Io<DT>::get(x1);
+      x0 = Io<DT>::put(fmaf(a0, cf, -(a1 * sf)));
+      x1 = Io<DT>::put(fmaf(a0, sf, a1 * cf));
+    }
+    dst[d0] = x0;
+    dst[d1] = x1;
+  }
+}
+
+template <Dt DT, bool T32, bool INTER>
+static int launch_i(Args a, bool fast, int n_cu, hipStream_t st) {
+  if (!fast) {
+    const int64_t blocks = cdiv(a.n_tokens, kWaves);
+    if (blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((rotary_any_kernel<DT, T32, INTER>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
+    return AAC_OK;
+  }
+  const int per = 64 / (a.dim / 16), total = a.q.heads + a.k.heads + a.v.heads;
+  auto blocks_at = [&](int passes) {
+    a.slots = (int)cdiv(total, (int64_t)per * passes);
+    return cdiv(a.n_tokens * a.slots, kWaves);
+  };
+  const bool many = total > 2 * per && a.n_tokens * cdiv(total, 4 * (int64_t)per) >= 8 * (int64_t)n_cu;
+  const int64_t blocks = blocks_at(many ? 4 : 1);
+  if (blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
+  if (many)
+    hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 4>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
+  else
+    hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 1>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
+  return AAC_OK;
+}
+
+template <Dt DT>
+static int launch_t(const Args& a, bool t32, bool inter, bool fast, int n_cu, hipStream_t st) {
+  if constexpr (DT != Dt::FP32) {
+    if (!t32)
+      return inter ? launch_i<DT, false, true>(a, fast, n_cu, st) : launch_i<DT, false, false>(a, fast, n_cu, st);
+  }
+  return inter ? launch_i<DT, true, true>(a, fast, n_cu, st) : launch_i<DT, true, false>(a, fast, n_cu, st);
+}
+
+static int launch(const Args& a, int32_t table_dtype, bool inter, int32_t dtype, hipStream_t st) {
+  const int es = dtype == AAC_DTYPE_FP32 ? 4 : 2, ts = table_dtype == AAC_DTYPE_FP32 ? 4 : 2;
+  const int cpr = a.dim / 16;
+  // every vector the fast kernel touches: rows, heads and tables at multiples of 16 bytes
+  bool fast = a.dim % 16 == 0 && (cpr & (cpr - 1)) == 0 && cpr <= 64 && a.half % 8 == 0 &&
+              (((uintptr_t)a.cos | (uintptr_t)a.sin) % 16) == 0 && (a.half * ts) % 16 == 0;
+  for (const Rows* r : {&a.q, &a.k, &a.v})
+    if (r->heads) {
+      fast = fast && (((uintptr_t)r->in | (uintptr_t)r->out) % 16) == 0;
+      for (int64_t s : {r->seq, r->tok, r->head, r->out_seq, r->out_tok, r->out_head}) fast = fast && s * es % 16 == 0;
+    }
+  int n_cu = 0;
+  int rc = device_cu_count(&n_cu);
+  if (rc != AAC_OK) return rc;
+  const bool t32 = table_dtype == AAC_DTYPE_FP32;
+  switch (dtype) {
+    case AAC_DTYPE_BF16: rc = launch_t<Dt::BF16>(a, t32, inter, fast, n_cu, st); break;
+    case AAC_DTYPE_FP16: rc = launch_t<Dt::FP16>(a, t32, inter, fast, n_cu, st); break;
+    default: rc = launch_t<Dt::FP32>(a, t32, inter, fast, n_cu, st); break;
+  }
+  if (rc != AAC_OK) return rc;
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? AAC_OK : (int)e;
+}
+
+// Arguments both entry points check alike.
+static int check_tables(const void* cos, const void* sin, int32_t rows, int32_t rotary_dim, int32_t table_dtype,
+                        int32_t head_dim, int32_t dtype) {
+  if (dtype != AAC_DTYPE_BF16 && dtype != AAC_DTYPE_FP16 && dtype != AAC_DTYPE_FP32) return AAC_ERR_UNSUPPORTED;
+  if (head_dim <= 0 || rotary_dim < 0 || rows < 0) return AAC_ERR_INVALID_ARGUMENT;
+  if (head_dim % 2 || rotary_dim % 2 || rotary_dim > head_dim) return AAC_ERR_SHAPE;
+  if (rotary_dim == 0) return AAC_OK;
+  if (table_dtype != AAC_DTYPE_FP32 && table_dtype != dtype) return AAC_ERR_UNSUPPORTED;
+  if (!cos || !sin || rows == 0) return AAC_ERR_INVALID_ARGUMENT;
+  return AAC_OK;
+}
+
+// ------------------------------------------------------------------ tables
+// cos and sin of position p, frequency i: the angle in quarter turns, 4 p turns[i], and
+// its distance from a whole number of them in fp64 (at position 2^20 a radian has 2^-33
+// of its error left, where fp32 has 2^-4); what remains is within an eighth of a turn
+// and is exact to fp32's own precision.  Bound by the stores: 8 values of each a thread.
+template <Dt DT>
+__global__ __launch_bounds__(256) void tables_kernel(const double* turns, int32_t half, const int32_t* positions,
+                                                     int64_t start, int64_t n, float factor, void* cos_out,
+                                                     void* sin_out) {
+  typedef typename Io<DT>::T E;
+  const int groups = (half + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * groups) return;
+  const int64_t r = i / groups;
+  const int f0 = (int)(i - r * groups) * 8;
+  const double pos = (double)(positions ? (int64_t)positions[r] : start + r);
+  float c[8], s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double x = 4.0 * pos * turns[min(f0 + e, half - 1)];
+    const double k = rint(x);
+    float sn, cs;
+    sincospif((float)(x - k) * 0.5f, &sn, &cs);
+    const int quad = (int)((int64_t)k & 3);
+    const float u = quad & 1 ? sn : cs, v = quad & 1 ? cs : sn;
+    c[e] = (quad == 1 || quad == 2 ? -u : u) * factor;
+    s[e] = (quad >= 2 ? -v : v) * factor;
+  }
+  E* co = reinterpret_cast<E*>(cos_out) + r * half + f0;
+  E* so = reinterpret_cast<E*>(sin_out) + r * half + f0;
+  if (half % 8 == 0) {
+    Vec8<DT> o;
+    o.put(c);
+    o.store(co);
+    o.put(s);
+    o.store(so);
+  } else {
+    for (int e = 0; e < min(8, half - f0); ++e) {
+      co[e] = Io<DT>::put(c[e]);
+      so[e] = Io<DT>::put(s[e]);
+    }
+  }
+}
+
+}  // namespace rot
+}  // namespace aac
+
+using namespace aac;
+
+extern "C" int aac_rotary(const void* x, int64_t x_seq_stride, int64_t x_tok_stride, int64_t x_head_stride,
+                          void* out, int64_t out_seq_stride, int64_t out_tok_stride, int64_t out_head_stride,
+                          int32_t n_seqs, int32_t seqlen, int64_t n_tokens, const int32_t* cu_seqlens,
+                          const int32_t* offsets, int32_t offset, int32_t n_heads, int32_t head_dim,
+                          const void* cos_table, const void* sin_table, int32_t table_rows, int32_t rotary_dim,
+                          int32_t interleaved, int32_t conjugate, int32_t table_dtype, int32_t dtype,
+                          void* stream) {
+  int rc = rot::check_tables(cos_table, sin_table, table_rows, rotary_dim, table_dtype, head_dim, dtype);
+  if (rc != AAC_OK) return rc;
+  if (n_seqs < 0 || seqlen < 0 || n_tokens < 0 || n_heads < 0) return AAC_ERR_INVALID_ARGUMENT;
+  if (!cu_seqlens) n_tokens = (int64_t)n_seqs * seqlen;
+  if (n_tokens == 0 || n_seqs == 0 || n_heads == 0) return AAC_OK;
+  if (!x || !out) return AAC_ERR_INVALID_ARGUMENT;
+  rot::Args a = {};
+  a.q = {(const char*)x, (char*)out, x_seq_stride, x_tok_stride, x_head_stride, out_seq_stride, out_tok_stride,
+         out_head_stride, n_heads, seqlen};
+  a.cos = cos_table;
+  a.sin = sin_table;
+  a.table_rows = table_rows;
+  a.half = rotary_dim / 2;
+  a.offsets = offsets;
+  a.offset0 = offset;
+  a.q_step = 1;
+  a.cu = cu_seqlens;
+  a.n_seqs = n_seqs;
+  a.seqlen = std::max(seqlen, 1);
+  a.n_tokens = n_tokens;
+  a.dim = head_dim;
+  a.sign = conjugate ? -1 : 1;
+  return rot::launch(a, rotary_dim ? table_dtype : (int32_t)AAC_DTYPE_FP32, interleaved != 0, dtype,
+                     (hipStream_t)stream);
+}
+
+extern "C" int aac_rotary_append_paged(
+    const void* q, int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+    int64_t k_seq_stride, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_seq_stride,
+    int64_t v_tok_stride, int64_t v_head_stride, void* q_out, int32_t n_seqs, int32_t seqlen_q, int32_t seqlen_k,
+    int64_t n_tokens, const int32_t* cu_seqlens, const int32_t* cache_seqlens, int32_t* context_lens, int32_t n_q_heads,
+    int32_t n_kv_heads, int32_t head_dim, const void* cos_table, const void* sin_table, int32_t table_rows,
+    int32_t rotary_dim, int32_t interleaved, int32_t queries_at_first, void* k_cache, void* v_cache,
+    int64_t num_blocks, int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq,
+    int32_t table_dtype, int32_t dtype, void* stream) {
+  int rc = rot::check_tables(cos_table, sin_table, table_rows, rotary_dim, table_dtype, head_dim, dtype);
+  if (rc != AAC_OK) return rc;
+  if (n_seqs < 0 || seqlen_q < 0 || seqlen_k < 0 || n_tokens < 0 || n_q_heads < 0 || n_kv_heads <= 0 ||
+      num_blocks < 0 || block_size <= 0 || max_blocks_per_seq <= 0)
+    return AAC_ERR_INVALID_ARGUMENT;
+  const int32_t seqlen = std::max(q ? seqlen_q : 0, seqlen_k);
+  if (!cu_seqlens) n_tokens = (int64_t)n_seqs * seqlen;
+  if (n_tokens == 0 || n_seqs == 0) return AAC_OK;
+  if (!k || !v || !k_cache || !v_cache || !block_tables || !cache_seqlens || (q && !q_out))
+    return AAC_ERR_INVALID_ARGUMENT;
+  rot::Args a = {};
+  if (q && n_q_heads)
+    a.q = {(const char*)q, (char*)q_out, q_seq_stride, q_tok_stride, q_head_stride,
+           (int64_t)seqlen_q * n_q_heads * head_dim, (int64_t)n_q_heads * head_dim, head_dim, n_q_heads, seqlen_q};
+  a.k = {(const char*)k, (char*)k_cache, k_seq_stride, k_tok_stride, k_head_stride, 0, 0, head_dim, n_kv_heads,
+         seqlen_k};
+  a.v = {(const char*)v, (char*)v_cache, v_seq_stride, v_tok_stride, v_head_stride, 0, 0, head_dim, n_kv_heads,
+         seqlen_k};
+  a.cos = cos_table;
+  a.sin = sin_table;
+  a.table_rows = table_rows;
+  a.half = rotary_dim / 2;
+  a.offsets = cache_seqlens;
+  a.q_step = queries_at_first ? 0 : 1;
+  a.cu = cu_seqlens;
+  a.n_seqs = n_seqs;
+  a.seqlen = std::max(seqlen, 1);
+  a.n_tokens = n_tokens;
+  a.context_lens = cu_seqlens ? nullptr : context_lens;
+  a.block_tables = block_tables;
+  a.max_blocks = max_blocks_per_seq;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.dim = head_dim;
+  a.sign = 1;
+  return rot::launch(a, rotary_dim ? table_dtype : (int32_t)AAC_DTYPE_FP32, interleaved != 0, dtype,
+                     (hipStream_t)stream);
+}
+
+extern "C" int aac_rotary_tables(const void* turns, int32_t n_freqs, const int32_t* positions, int64_t start,
+                                 int64_t n_positions, float factor, void* cos_out, void* sin_out, int32_t dtype,
+                                 void* stream) {
+  if (dtype != AAC_DTYPE_BF16 && dtype != AAC_DTYPE_FP16 && dtype != AAC_DTYPE_FP32) return AAC_ERR_UNSUPPORTED;
+  if (n_freqs <= 0 || n_positions < 0) return AAC_ERR_INVALID_ARGUMENT;
+  if (n_positions == 0) return AAC_OK;
+  if (!turns || !cos_out || !sin_out) return AAC_ERR_INVALID_ARGUMENT;
+  if (n_freqs % 8 == 0 && ((uintptr_t)cos_out | (uintptr_t)sin_out) % 16) return AAC_ERR_MISALIGNED;
+  // (positions are whole numbers in fp64, and their product with 4 turns has a quadrant)
+  if (start < -(int64_t(1) << 40) || start > (int64_t(1) << 40)) return AAC_ERR_SHAPE;
+  const int64_t blocks = cdiv(n_positions * cdiv(n_freqs, 8), 256);
+  if (n_positions >= (int64_t(1) << 40) / n_freqs || blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)blocks), block(256);
+  const double* f = (const double*)turns;
+  hipStream_t st = (hipStream_t)stream;
+  switch (dtype) {
+    case AAC_DTYPE_BF16:
+      hipLaunchKernelGGL((rot::tables_kernel<Dt::BF16>), grid, block, 0, st, f, n_freqs, positions, start, n_positions,
+                         factor, cos_out, sin_out);
+      break;
+    case AAC_DTYPE_FP16:
+      hipLaunchKernelGGL((rot::tables_kernel<Dt::FP16>), grid, block, 0, st, f, n_freqs, positions, start, n_positions,
+                         factor, cos_out, sin_out);
+      break;
+    default:
+      hipLaunchKernelGGL((rot::tables_kernel<Dt::FP32>), grid, block, 0, st, f, n_freqs, positions, start, n_positions,
+                         factor, cos_out, sin_out);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? AAC_OK : (int)e;
+}

@@ -14,9 +14,14 @@ plus the KV store the reference does with ``index_copy_`` (llm.py:171-174):
 * ``kv_store``                -- slot_mapping row scatter
 * ``varlen_prefill_with_kvcache`` -- store + varlen attention in one call
 
-Only the features the reference uses are accepted (no dropout, no sliding
-window, no ALiBi, no softcap, no rotary inside the call); anything else
-raises ``NotImplementedError`` instead of silently computing something else.
+and what lies between a prefill and a decode step, chunks of new tokens over the
+paged cache: ``prefill_paged``, ``flash_attn_varlen_func(block_table=...)`` and
+``flash_attn_with_kvcache`` with several tokens a sequence, with the rotary positions
+(``rotary``) applied in the call where tables are given.
+
+Dropout, sliding windows, ALiBi, softcap and return_softmax_lse, which the reference
+does not use, are not accepted; they
+raise ``NotImplementedError`` instead of silently computing something else.
 Every op runs on ``torch.cuda.current_stream()`` and never synchronises.
 Outputs are allocated here (FA2 returns a new tensor); caches are updated in
 place; ``cache_seqlens`` is never modified (the reference increments it
@@ -42,6 +47,7 @@ __all__ = [
     "flash_attn_func",
     "decode_paged",
     "decode_qkv_paged",
+    "prefill_paged",
 ]
 
 _CHECK = os.environ.get("AAC_CHECK", "0") not in ("", "0")
@@ -256,11 +262,14 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
 
     q ``[Nq, Hq, D]``, k/v ``[Nk, Hkv, D]``, ``cu_seqlens_*`` int32
     ``[batch+1]``.  Returns a new ``[Nq, Hq, D]`` tensor.  ``causal`` masks
-    bottom-right aligned, as FA2 >= 2.1 does.
+    bottom-right aligned, as FA2 >= 2.1 does.  With ``block_table`` (int32 ``[batch,
+    max_blocks]``) k and v are paged caches ``[num_blocks, block_size, Hkv, D]`` and
+    ``cu_seqlens_k`` the prefix sums of the context lengths (``prefill_paged``).
     """
     _unsupported(dropout_p, window_size, softcap, alibi_slopes, return_attn_probs)
     if block_table is not None:
-        raise NotImplementedError("paged K/V for varlen prefill is not supported")
+        return _prefill_paged(q, k, v, cu_seqlens_q, block_table, None, cu_seqlens_k, max_seqlen_q,
+                              max_seqlen_k, softmax_scale, causal, None)
     qs, ks, vs = _prefill_checks(q, k, v, cu_seqlens_q, cu_seqlens_k)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -336,6 +345,84 @@ def flash_attn_func(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False,
     out = flash_attn_varlen_func(qf, kf, vf, cu_q, cu_k, Tq, Tk, softmax_scale=softmax_scale,
                                  causal=causal)
     return out.view(B, Tq, Hq, D)
+
+
+# ---------------------------------------------------------------- chunks over the paged cache
+@functools.lru_cache(maxsize=4096)
+def _chunk_ws_bytes(device_index: int, *args: int) -> int:
+    """aac_prefill_paged_workspace_bytes on that device (its plan counts the CUs)."""
+    with torch.cuda.device(device_index):
+        return _lib.lib().aac_prefill_paged_workspace_bytes(*args)
+
+
+def _launch_chunk(q, q_stride, n_tokens, k_cache, v_cache, tables, cu_q, ctx, cu_k, n_seqs, max_q,
+                  max_k, scale, causal, out, out_stride):
+    """aac_prefill_paged on checked arguments.  The workspace comes from the allocator call by
+    call: two streams, threads or captured graphs never share one."""
+    nblk, bs, hkv, D = k_cache.shape
+    mb, hq, dev = tables.shape[1], q.shape[-2], q.get_device()
+    ws_bytes = _chunk_ws_bytes(dev, n_tokens, n_seqs, max_q, max_k, bs, mb, hq, hkv)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _lib.launch("aac_prefill_paged", dev, q.data_ptr(), q_stride, n_tokens, k_cache.data_ptr(),
+                v_cache.data_ptr(), nblk, bs, tables.data_ptr(), mb,
+                None if cu_q is None else cu_q.data_ptr(), None if ctx is None else ctx.data_ptr(),
+                None if cu_k is None else cu_k.data_ptr(), n_seqs, max_q, max_k, hq, hkv, D, scale,
+                int(bool(causal)), out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(),
+                ws_bytes, _dtype_code(q))
+
+
+def _prefill_paged(q, k_cache, v_cache, cu_q, tables, ctx, cu_k, max_q, max_k, softmax_scale, causal, out):
+    _on_gpu(q, k_cache, v_cache, cu_q, tables, ctx, cu_k, out)
+    qs = _token_rows(q, "q")
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
+        raise RuntimeError("prefill supports fp16 and bf16 only")
+    _check_cache(q, k_cache, v_cache)
+    if cu_q.dtype is not torch.int32 or cu_q.dim() != 1 or not cu_q.is_contiguous() or cu_q.shape[0] == 0:
+        raise RuntimeError("cu_seqlens must be contiguous int32 [batch+1]")
+    B = cu_q.shape[0] - 1
+    if cu_k is not None and (cu_k.dtype is not torch.int32 or cu_k.shape != cu_q.shape
+                             or not cu_k.is_contiguous()):
+        raise RuntimeError("cu_seqlens must be contiguous int32 [batch+1]")
+    if ctx is not None and (ctx.dtype is not torch.int32 or ctx.shape != (B,) or not ctx.is_contiguous()):
+        raise RuntimeError("context_lens must be contiguous int32 [B]")
+    if (tables.dtype is not torch.int32 or tables.dim() != 2 or tables.shape[0] != B
+            or not tables.is_contiguous()):
+        raise RuntimeError("block_tables must be contiguous int32 [B, max_blocks]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        os = q.shape[1] * q.shape[2]
+    else:
+        os = _token_rows(out, "out")
+        if out.dtype is not q.dtype or out.shape != q.shape:
+            raise RuntimeError("out must be as q")
+    scale = _scale(softmax_scale, q.shape[-1])
+    if not 0 < scale < math.inf:
+        raise RuntimeError("softmax_scale must be positive")
+    if q.shape[0] == 0 or B == 0:
+        return out
+    if k_cache.numel() == 0 or tables.shape[1] == 0:  # no key anywhere: every row sees none
+        return out.zero_()
+    _launch_chunk(q, qs, q.shape[0], k_cache, v_cache, tables, cu_q, ctx, cu_k, B, int(max_q),
+                  int(max_k or 0), scale, causal, out, os)
+    return out
+
+
+def prefill_paged(q, k_cache, v_cache, cu_seqlens_q, block_tables, context_lens, max_seqlen_q, *,
+                  max_context_len=None, softmax_scale=None, causal=True, out=None):
+    """Chunks of new tokens over the paged cache: sequence ``b``'s queries, rows
+    ``cu_seqlens_q[b]`` to ``cu_seqlens_q[b + 1]`` of q ``[N, Hq, D]`` (any token stride),
+    attend to the first ``context_lens[b]`` tokens (int32 ``[B]``) of its blocks, the new
+    ones, stored before, among them (``rotary.rotary_append_paged``, ``kv_store``).
+
+    block_tables int32 ``[B, max_blocks]``, caches ``[num_blocks, block_size, Hkv, D]``.
+    ``causal``: query ``i`` of ``n`` sees keys ``j <= i + context_lens[b] - n``.  A query that
+    sees no key gets zeros; the value of a key it does not see, infinite or NaN though it
+    may be, does not reach it.  Rows of q of no sequence are left as they are in ``out`` (undefined
+    in a new one).  ``max_seqlen_q`` bounds the new tokens of a sequence, ``max_context_len``
+    (default: the tables' capacity) is an estimate that sizes the split of the keys.  bf16
+    and fp16, head_dim 128, any number of query heads a KV head."""
+    return _prefill_paged(q, k_cache, v_cache, cu_seqlens_q, block_tables, context_lens, None,
+                          max_seqlen_q, max_context_len, softmax_scale, causal, out)
 
 
 # ---------------------------------------------------------------- decode
@@ -443,7 +530,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
                             *, max_context_len=None):
     """Decode with KV cache (model/model.py:233-240).
 
-    q ``[B, 1, Hq, D]``.  Without ``block_table`` the caches are the
+    q ``[B, S, Hq, D]``, one token a sequence (S = 1) or a chunk of them (bf16 and fp16).  Without ``block_table`` the caches are the
     reference's slot caches ``[num_slots, max_seq_len, Hkv, D]`` and batch
     row ``b`` uses slot ``cache_batch_idx[b]`` (default ``b``); with
     ``block_table`` (int32 ``[B, max_blocks]``) they are paged caches
@@ -453,12 +540,20 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     ``cache_seqlens[b]``.  All rows are written before any is read: one
     sequence may be given as several rows (the same table, positions ``n``,
     ``n + 1``, ...).  ``cache_seqlens`` is not modified.  Returns a new
-    ``[B, 1, Hq, D]`` tensor.
+    ``[B, S, Hq, D]`` tensor.
+
+    With S > 1, k and v ``[B, S_new, Hkv, D]`` (S_new need not be S) go to positions
+    ``cache_seqlens[b]`` and up, and ``causal`` masks as in ``prefill_paged``; ``num_splits`` is
+    then the library's choice.  ``rotary_cos`` and ``rotary_sin`` (``[positions, R / 2]``, q's
+    type or float32; with k and v) turn the first R dims of the new keys by their positions
+    and of the queries by ``cache_seqlens[b] + i`` if ``causal``, else all by
+    ``cache_seqlens[b]``, as ``rotary.apply_rotary_emb`` does (interleaved pairs unless
+    ``rotary_interleaved`` is false): rounded to their type, then stored and attended.
     """
     if softcap or alibi_slopes is not None or window_size != (-1, -1):
         _unsupported(0.0, window_size, softcap, alibi_slopes, False)
-    if rotary_cos is not None or rotary_sin is not None:
-        raise NotImplementedError("rotary inside the kernel is not supported; apply RoPE first")
+    if (rotary_cos is None) != (rotary_sin is None):
+        raise NotImplementedError("rotary_cos without rotary_sin, or the reverse, is not supported")
     if cache_leftpad is not None:
         raise NotImplementedError("cache_leftpad is not supported")
     if return_softmax_lse:
@@ -466,8 +561,6 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     if q.dim() != 4:
         raise RuntimeError("q must be [B, S, Hq, D]")
     B, S, Hq, D = q.shape
-    if S != 1:
-        raise NotImplementedError("only one query token per sequence (decode) is supported")
     if (k is None) != (v is None):
         raise RuntimeError("k and v must be given together")
     _on_gpu(q, k_cache, v_cache, k, v, cache_batch_idx, block_table)
@@ -495,6 +588,9 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         seqlens = cache_seqlens.to(torch.int32).contiguous()
         if seqlens.shape != (B,):
             raise RuntimeError("cache_seqlens must be [B]")
+    if S != 1 or rotary_cos is not None or (k is not None and k.dim() == 4 and k.shape[1] != 1):
+        return _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqlens, tables,
+                                   softmax_scale, causal, rotary_interleaved, max_context_len)
     q3 = q if q.is_contiguous() else q.reshape(B, Hq, D)
     if q3 is q:
         q_stride = Hq * D
@@ -547,4 +643,56 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         D, _scale(softmax_scale, D), out.data_ptr(), Hq * D, wsp, ws_bytes, counters, part,
         _dtype_code(q), _stream(q))
     _lib.check(rc, "aac_decode_append_merge_paged")
+    return out
+
+
+def _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqlens, tables, softmax_scale,
+                        causal, interleaved, max_context_len):
+    """``flash_attn_with_kvcache`` of several tokens a sequence, or with rotary tables: the
+    (turned) append, then the attention."""
+    from . import rotary
+    B, S, Hq, D = q.shape
+    nblk, bs, hkv, _ = k_cache.shape
+    if rotary_cos is not None and k is None:
+        raise RuntimeError("rotary_cos needs the new keys and values")
+    # (the decode kernels take groups of 1, 2, 4 and 8)
+    one = S == 1 and (k is None or k.shape[1] == 1) and Hq // hkv in (1, 2, 4, 8)
+    if not one and q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
+        raise RuntimeError("more than one token a sequence, or a group that is not 1, 2, 4 or 8: fp16 "
+                           "and bf16 only")
+    scale = _scale(softmax_scale, D)
+    if not one and not 0 < scale < math.inf:
+        raise RuntimeError("softmax_scale must be positive")
+    ctx = seqlens
+    if k is not None:
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[2:] != (hkv, D):
+            raise RuntimeError("k/v must be [B, S, Hkv, D], their heads as the cache's")
+        if k.dtype is not q.dtype or v.dtype is not q.dtype:
+            raise RuntimeError("k/v dtype mismatch")
+        _on_gpu(q, rotary_cos, rotary_sin)
+        k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (k, v))
+        if k.shape[1] and B and nblk:
+            ctx = torch.empty_like(seqlens)
+            turned = q if q.stride(3) == 1 else q.contiguous()
+            # without tables the queries stay where they are
+            turned = rotary._append(None if rotary_cos is None else turned, k, v, k_cache, v_cache, tables,
+                                    seqlens, rotary_cos, rotary_sin, interleaved, None, not causal, ctx)
+            q = q if turned is None else turned
+        elif rotary_cos is not None:  # no new key: the queries alone
+            q = rotary.apply_rotary_emb(
+                q if causal else q.reshape(B, 1, S * Hq, D), rotary_cos, rotary_sin,
+                interleaved=interleaved, seqlen_offsets=seqlens).view(B, S, Hq, D)
+    if one:
+        return decode_paged(q.reshape(B, Hq, D), k_cache, v_cache, tables, ctx, softmax_scale=softmax_scale,
+                            max_context_len=max_context_len).view(B, 1, Hq, D)
+    out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    if k_cache.numel() == 0 or tables.shape[1] == 0:
+        return out.zero_()
+    q = q.reshape(B * S, Hq, D)
+    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    _launch_chunk(q, q.stride(0) if B * S > 1 else Hq * D, B * S, k_cache, v_cache, tables, None, ctx, None,
+                  B, S, int(max_context_len or 0), scale, causal, out, Hq * D)
     return out

@@ -550,6 +550,90 @@ int aac_token_logprobs(const void* logits, int64_t row_stride, int64_t n_rows, i
                        float* top_logprobs, int64_t* top_ids, void* workspace,
                        size_t workspace_bytes, int32_t dtype, void* stream);
 
+/*
+ * Attention of a chunk of new tokens over the paged cache.  Sequence b's queries are rows
+ * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q [n_tokens, n_q_heads, head_dim] (token stride
+ * q_tok_stride), or, where cu_seqlens_q is null, max_seqlen_q rows each; its keys are the first L_b tokens of its blocks, L_b = context_lens[b]
+ * or, where that is null, cu_seqlens_k[b+1] - cu_seqlens_k[b] (the new tokens' rows among
+ * them: they are stored first).  With causal != 0 the mask is bottom-right aligned: query i
+ * of n sees keys j <= i + L_b - n.  A query that sees no key gets zeros; what a masked key's
+ * value or a row behind the context holds, infinities and NaN too, reaches no query that
+ * does not see it.  Rows of q behind the last sequence are left as they are in out.
+ * Tables as in aac_decode_paged: a context longer than the table is cut to it, block ids
+ * outside [0, num_blocks) are read as block 0.  max_seqlen_q: an upper bound on the
+ * sequences' queries (of a longer one, rows past it may be left unwritten);
+ * max_context_len (<= 0: the table's capacity): an estimate of the longest context, which
+ * only chooses how the work is split.
+ * BF16 or FP16, head_dim 128, n_q_heads any multiple of n_kv_heads, scale > 0.  A
+ * table of more than one block whose size is not a multiple of 16 names 2^27 tokens at most.
+ * workspace: aac_prefill_paged_workspace_bytes(...) bytes (the same arguments) where
+ * that is not 0, 16-byte aligned, any contents, not shared with a call that may overlap.
+ */
+size_t aac_prefill_paged_workspace_bytes(int64_t n_tokens, int32_t n_seqs, int32_t max_seqlen_q,
+                                         int32_t max_context_len, int32_t block_size,
+                                         int32_t max_blocks_per_seq, int32_t n_q_heads,
+                                         int32_t n_kv_heads);
+int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, const void* k_cache,
+                      const void* v_cache, int64_t num_blocks, int32_t block_size,
+                      const int32_t* block_tables, int32_t max_blocks_per_seq,
+                      const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                      const int32_t* cu_seqlens_k, int32_t n_seqs, int32_t max_seqlen_q,
+                      int32_t max_context_len, int32_t n_q_heads, int32_t n_kv_heads,
+                      int32_t head_dim, float scale, int32_t causal, void* out,
+                      int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
+                      int32_t dtype, void* stream);
+
+/*
+ * Rotary positions.  The first rotary_dim dims of a head are rotary_dim / 2 pairs, (d, d +
+ * rotary_dim / 2) or, interleaved, (2 d, 2 d + 1); pair d of a token at position p becomes
+ * (x1 c - x2 s, x1 s + x2 c) with c, s = cos_table, sin_table [table_rows, rotary_dim / 2]
+ * at (p, d): in fp32, rounded once.  The other dims pass unchanged.  Positions outside the
+ * tables take their first or last row.  dtype BF16, FP16 or FP32; table_dtype dtype or
+ * FP32; head_dim even, rotary_dim even and at most head_dim.  Head strides are free.
+ *
+ * aac_rotary: x -> out (out may be x).  Without cu_seqlens: [n_seqs, seqlen, n_heads,
+ * head_dim] by its strides, token i of sequence b at position offsets[b] + i (offsets null:
+ * offset + i); n_tokens is not read.  With cu_seqlens [n_seqs + 1]: packed [n_tokens,
+ * n_heads, head_dim] (the sequence strides are not read), token cu_seqlens[b] + i at
+ * position offsets[b] + i; rows of no sequence are left as they are.  conjugate != 0 turns
+ * back.
+ *
+ * aac_rotary_append_paged: new token i of sequence b, at position cache_seqlens[b] + i: its
+ * key turned and its value as it is into the row its block table names for that position
+ * (none: skipped, as aac_kv_append_paged), its queries turned into q_out (contiguous, as q
+ * is shaped; q null: no queries).  Without cu_seqlens q is [n_seqs, seqlen_q, ...] and k,
+ * v [n_seqs, seqlen_k, ...]; with it all are packed [n_tokens, ...].  queries_at_first !=
+ * 0: every query of a sequence turns at cache_seqlens[b].  rotary_dim 0: the append alone
+ * (q is copied).  cache_seqlens is not modified; context_lens (or null; without
+ * cu_seqlens) gets cache_seqlens[b] + seqlen_k.
+ * The k= / v= / rotary_cos= half of flash_attn_with_kvcache (model/model.py:233-240).
+ *
+ * aac_rotary_tables: cos_out, sin_out [n_positions, n_freqs] = factor * cos, sin of
+ * 2 pi p turns[i] at positions p = positions[r] or, where that is null, start + r.  turns:
+ * double [n_freqs] on the device, turns a position; the angle is reduced in 64 bits.
+ * |start| up to 2^40; cos_out and sin_out 16-byte aligned where n_freqs is a multiple of 8.
+ */
+int aac_rotary(const void* x, int64_t x_seq_stride, int64_t x_tok_stride, int64_t x_head_stride,
+               void* out, int64_t out_seq_stride, int64_t out_tok_stride, int64_t out_head_stride,
+               int32_t n_seqs, int32_t seqlen, int64_t n_tokens, const int32_t* cu_seqlens,
+               const int32_t* offsets, int32_t offset, int32_t n_heads, int32_t head_dim,
+               const void* cos_table, const void* sin_table, int32_t table_rows,
+               int32_t rotary_dim, int32_t interleaved, int32_t conjugate, int32_t table_dtype,
+               int32_t dtype, void* stream);
+int aac_rotary_append_paged(
+    const void* q, int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+    int64_t k_seq_stride, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+    int64_t v_seq_stride, int64_t v_tok_stride, int64_t v_head_stride, void* q_out, int32_t n_seqs,
+    int32_t seqlen_q, int32_t seqlen_k, int64_t n_tokens, const int32_t* cu_seqlens,
+    const int32_t* cache_seqlens, int32_t* context_lens, int32_t n_q_heads, int32_t n_kv_heads,
+    int32_t head_dim, const void* cos_table, const void* sin_table, int32_t table_rows,
+    int32_t rotary_dim, int32_t interleaved, int32_t queries_at_first, void* k_cache, void* v_cache, int64_t num_blocks,
+    int32_t block_size, const int32_t* block_tables, int32_t max_blocks_per_seq, int32_t table_dtype,
+    int32_t dtype, void* stream);
+int aac_rotary_tables(const void* turns, int32_t n_freqs, const int32_t* positions, int64_t start,
+                      int64_t n_positions, float factor, void* cos_out, void* sin_out, int32_t dtype,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

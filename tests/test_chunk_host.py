@@ -1,0 +1,134 @@
+"""Chunks over the paged cache and rotary positions, on the host: the C entry points' refusals,
+the page arithmetic, the frequencies' scaling rules (against transformers' where it is
+installed)."""
+import math
+
+import pytest
+import torch
+
+from awesome_acceleration_amd import _lib, rotary
+
+
+def _chunk(q=64, qs=2048, n=5, kc=64, vc=64, nb=4, bs=16, tab=64, mb=3, cu=64, ctx=64, cuk=None, B=2, mq=3, mk=0,
+           hq=16, hkv=8, d=128, scale=0.1, causal=1, out=64, os=2048, ws=None, wb=0, dt=0):
+    return _lib.lib().aac_prefill_paged(q, qs, n, kc, vc, nb, bs, tab, mb, cu, ctx, cuk, B, mq, mk, hq, hkv, d,
+                                        scale, causal, out, os, ws, wb, dt, None)
+
+
+def test_chunk_refusals():
+    """Before any launch: every call here is refused on its arguments alone."""
+    for a in (dict(dt=2), dict(dt=7), dict(d=64), dict(bs=7, mb=1 << 25)):
+        assert _chunk(**a) == -2, a
+    for a in (dict(n=-1), dict(B=-1), dict(hq=0), dict(mq=-1), dict(bs=0), dict(mb=0), dict(scale=0.0),
+              dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(q=None), dict(out=None),
+              dict(tab=None), dict(ctx=None), dict(kc=None), dict(vc=None), dict(nb=0), dict(nb=-1)):
+        assert _chunk(**a) == -1, a
+    for a in (dict(hq=12), dict(qs=2047 // 2), dict(os=1024), dict(cu=None, n=5), dict(n=1 << 31)):
+        assert _chunk(**a) == -5, a
+    for a in (dict(q=72), dict(kc=72), dict(vc=68), dict(out=2), dict(qs=2052), dict(os=2052)):
+        assert _chunk(**a) == -3, a
+    for a in (dict(n=0), dict(B=0), dict(mq=0)):
+        assert _chunk(**a, q=None, kc=None) == 0, a
+
+
+def test_rotary_refusals():
+    def f(x=64, out=64, B=2, S=3, n=0, cu=None, h=4, d=128, cos=64, sin=64, rows=9, rot=64, td=2, dt=0):
+        return _lib.lib().aac_rotary(x, 1, 1, 128, out, 1, 1, 128, B, S, n, cu, None, 0, h, d, cos, sin, rows, rot,
+                                     0, 0, td, dt, None)
+
+    for a in (dict(dt=3), dict(td=1), dict(td=9)):
+        assert f(**a) == -2, a
+    for a in (dict(rot=3), dict(rot=130), dict(d=127)):
+        assert f(**a) == -5, a
+    for a in (dict(d=0), dict(rot=-2), dict(rows=0), dict(rows=-1), dict(cos=None), dict(sin=None), dict(B=-1),
+              dict(S=-1), dict(h=-1), dict(x=None), dict(out=None), dict(cu=64, n=-1)):
+        assert f(**a) == -1, a
+    for a in (dict(B=0), dict(S=0), dict(h=0), dict(cu=64, n=0)):
+        assert f(**a, x=None) == 0, a
+
+    def g(q=None, qo=None, k=64, v=64, kc=64, vc=64, tab=64, lens=64, B=2, sk=3, hkv=4, bs=16, mb=2, nb=5, rot=0):
+        return _lib.lib().aac_rotary_append_paged(q, 1, 1, 128, k, 1, 1, 128, v, 1, 1, 128, qo, B, 3, sk, 0, None,
+                                                  lens, None, 4, hkv, 128, None, None, 0, rot, 0, 0, kc, vc, nb, bs,
+                                                  tab, mb, 0, 0, None)
+
+    for a in (dict(k=None), dict(v=None), dict(kc=None), dict(vc=None), dict(tab=None), dict(lens=None), dict(q=64),
+              dict(hkv=0), dict(bs=0), dict(mb=0), dict(nb=-1), dict(B=-1), dict(sk=-1), dict(rot=64)):
+        assert g(**a) == -1, a
+    assert g(B=0, k=None) == 0 and g(sk=0, k=None) == 0
+
+    def t(f=64, n=8, start=0, rows=5, cos=64, sin=64, dt=0):
+        return _lib.lib().aac_rotary_tables(f, n, None, start, rows, 1.0, cos, sin, dt, None)
+
+    assert t(dt=3) == -2 and t(n=0) == -1 and t(rows=-1) == -1 and t(f=None) == -1 and t(cos=None) == -1
+    assert t(cos=68) == -3 and t(start=(1 << 40) + 1) == -5 and t(rows=0, f=None) == 0
+    assert t(rows=1 << 39) == -2
+
+
+def test_page_of_a_key_by_multiplication():
+    """x / d as x * ceil(2^(27 + s) / d) >> (27 + s) with s = ceil(log2 d), exact for x < 2^27."""
+    import random
+    r = random.Random(0)
+    for d in [*range(1, 70), 255, 256, 257, (1 << 27) - 1, 1 << 27, *(r.randrange(1, 1 << 27) for _ in range(200))]:
+        s = (d - 1).bit_length()
+        m = -(-(1 << (27 + s)) // d)
+        assert m < 1 << 32
+        for k in [0, 1, 2, ((1 << 27) - 1) // d, *(r.randrange((1 << 27) // d + 1) for _ in range(20))]:
+            for x in (k * d - 1, k * d, k * d + d - 1):
+                if 0 <= x < 1 << 27:
+                    assert x * m < 1 << 64 and (x * m) >> (27 + s) == x // d
+
+
+RULES = [
+    dict(rope_type="linear", factor=4.0),
+    dict(rope_type="dynamic", factor=4.0, original_max_position_embeddings=2048),
+    dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768),
+    dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096, mscale=1.0, mscale_all_dim=0.8,
+         beta_fast=16, beta_slow=2),
+    dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=4096, attention_factor=1.5, truncate=False),
+    dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+         original_max_position_embeddings=8192),
+]
+
+
+@pytest.mark.parametrize("rule", RULES, ids=lambda r: r["rope_type"])
+@pytest.mark.parametrize("dim", [128, 64])
+def test_scaled_frequencies_are_transformers(rule, dim):
+    """transformers computes them in float32: 2^-18 apart at most (powers and logarithms of
+    some tens of rounded steps, and its ramp's differences of near values)."""
+    rope = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import LlamaConfig
+    old = int(rule.get("original_max_position_embeddings", 4096))
+    cfg = LlamaConfig(hidden_size=8 * dim, num_attention_heads=8, head_dim=dim, max_position_embeddings=old,
+                      rope_parameters=dict(rule, rope_theta=1e6))
+    fn = rope.ROPE_INIT_FUNCTIONS[rule["rope_type"]]
+    n = 3 * old
+    try:
+        inv, factor = fn(cfg, torch.device("cpu"), seq_len=n)
+    except (KeyError, AttributeError, TypeError) as e:
+        pytest.skip(f"this transformers reads its configuration otherwise: {e!r}")
+    got, f = rotary.scaled_frequencies(dim, 1e6, rule, n)
+    assert got.dtype == torch.float64 and got.shape == (dim // 2,)
+    assert abs(f - factor) < 1e-6
+    assert ((got - inv.double()).abs() <= 2.0 ** -18 * got).all()
+
+
+def test_scaling_refusals():
+    f = rotary.scaled_frequencies
+    base, one = f(8, 100.0)
+    assert one == 1.0 and torch.allclose(base, 100.0 ** (-torch.arange(4, dtype=torch.float64) / 4))
+    assert torch.equal(f(8, 100.0, {})[0], base) and torch.equal(f(8, 100.0, dict(rope_type="default"))[0], base)
+    for match, a in (("unknown", dict(rope_type="longer", factor=2.0, original_max_position_embeddings=9)),
+                     ("factor", dict(rope_type="linear")), ("1 or more", dict(rope_type="linear", factor=0.5)),
+                     ("original_max", dict(rope_type="yarn", factor=2.0)),
+                     ("low_freq", dict(rope_type="llama3", factor=2.0, original_max_position_embeddings=9)),
+                     ("above", dict(rope_type="llama3", factor=2.0, original_max_position_embeddings=9,
+                                    low_freq_factor=4, high_freq_factor=4))):
+        with pytest.raises(RuntimeError, match=match):
+            f(8, 100.0, a)
+    for dim, theta in ((7, 1.0), (0, 1.0), (8, 0.0)):
+        with pytest.raises(RuntimeError):
+            f(dim, theta)
+    with pytest.raises(RuntimeError, match="GPU"):
+        rotary.RotaryEmbedding(8, device="cpu")
+    with pytest.raises(RuntimeError, match="GPU"):
+        rotary.apply_rotary_emb(torch.zeros(1, 1, 1, 8), torch.zeros(1, 4), torch.zeros(1, 4))
