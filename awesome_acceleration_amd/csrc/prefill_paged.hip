@@ -122,6 +122,15 @@ __device__ __forceinline__ void load_lds16(const u16* p, u32 dst) {
 #pragma clang diagnostic pop
 }
 
+// 0x8000 in each half of x that holds a finite value: with the exponent's bits turned over,
+// all of them set leaves 0, which alone stays below 0x8000 when 0x7fff is added.
+template <bool F16> __device__ __forceinline__ u32 finite16(u32 x) {
+  constexpr u32 kExp = F16 ? 0x7c007c00u : 0x7f807f80u;
+  return ((~x & kExp) + 0x7fff7fffu) & 0x80008000u;
+}
+// 0x8000 -> 0xffff, 0 -> 0 in each half
+__device__ __forceinline__ u32 spread16(u32 t) { return (t - (t >> 15)) | t; }
+
 // At most N of this wave's loads are in flight and its LDS reads are done, then the
 // workgroup's.
 template <int N> __device__ __forceinline__ void landed_barrier() {
@@ -150,7 +159,6 @@ template <class S, bool CAUSAL, bool F16, bool PAGE16>
 __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_paged_kernel(Args a) {
   typedef pf::Mfma<F16> M;
   constexpr int SL = S::SL, KT = S::KT, STAGES = S::STAGES;
-  constexpr u32 kExp = F16 ? 0x7c00u : 0x7f80u;  // exponent bits of infinities and NaN
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
   const u32 lds0 = (u32)(uintptr_t)(lds_u8*)lds;
 
@@ -254,7 +262,6 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
       look_up(n);
       issue(n);
     }
-  look_up(STAGES - 1);
 
   // Q fragments (B operand of S^T = K Q^T: lane = row)
   u32x4 qf[8];
@@ -281,10 +288,110 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float m = -1e30f, l = 0.f;  // reference max (raw scores), lane-partial row sum
+
+  f32x16 s;      // scores of a sub-tile, then:
+  u32x4 pb[2];   // its probabilities, two steps of 16 keys
+  u32x4 kf[8], vf[8];
+  typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
+  auto tile = [&](int n, int sub) { return (const lds_u8*)lds + n % STAGES * S::kStage + sub * kSubBytes; };
+  auto read_k = [&](const lds_u8* kb) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) kf[t] = *reinterpret_cast<lds_u32x4*>(kb + koff[t]);
+  };
+  auto v_frag = [&](const lds_u8* vb, int i) {  // step i / 4, dims 32 (i % 4) and up
+    const lds_u8* at = vb + vo[i & 3] + 4096 * (i >> 2);
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
+    const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a0[0], a0[1], a1[0], a1[1]};
+  };
+  auto read_v = [&](const lds_u8* vb) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i] = v_frag(vb, i);
+  };
+  auto scores = [&]() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) s = M::run(kf[t], qf[t], s);
+  };
+  auto product = [&]() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i & 3] = M::run(vf[i], pb[i >> 2], o[i & 3]);
+  };
+  // Probabilities of sub-tile j's scores; its values are at vb, their fragments in vf.
+  auto softmax = [&](int j, const lds_u8* vb) {
+    const bool masked = 32 * j + 32 > full;
+    if (masked) {
+      const int lim = my_lim - 32 * j - 4 * hl;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < lim ? s[i] : -INFINITY;
+    }
+    float mx = vmax3(s[0], s[1], s[2]);
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) mx = vmax3(mx, s[i], s[i + 1]);
+    mx = vmax(mx, s[15]);
+    if (__ballot(!(mx <= m + kthr))) {  // any lane (or a NaN): rescale (rare after the first sub-tile)
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = vmax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+      // (only the rows that need it: a row's result does not hang on its neighbours)
+      const float mn = mx <= m + kthr ? m : vmax(m, mx), alpha = fast_exp2((m - mn) * cs);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+    }
+    const float nb = -m * cs;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const u32 p = M::pack(fast_exp2(fmaf(s[2 * w], cs, nb)), fast_exp2(fmaf(s[2 * w + 1], cs, nb)));
+      pb[w >> 2][w & 3] = p;
+      l = M::dot2_ones(p, l);
+    }
+    if (masked) {
+      // A value that a row does not see must not reach it, whatever it is: with an
+      // infinity or a NaN among these 32 keys' values, the product takes 0 in its place
+      // and the rows that see its key add it
+      u32 fine = 0x80008000u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fine &= finite16<F16>(vf[i][e]);
+      if (__ballot(fine != 0x80008000u)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[i][e] &= spread16(finite16<F16>(vf[i][e]));
+        const int seen = my_lim - 32 * j;
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {
+          const u32 on = k < seen ? ~0u : 0u;
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // dims 32 db + 8 r + 4 hl .. + 3 of key k; the finite ones add 0
+              const u32x2 x = *reinterpret_cast<const __attribute__((address_space(3))) u32x2*>(
+                  vb + k * 256 + 16 * ((4 * db + r) ^ (4 * (k & 3))) + 8 * hl);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const u32 y = x[e] & ~spread16(finite16<F16>(x[e])) & on;
+                o[db][4 * r + 2 * e] += F16 ? f16lo(y) : bf16lo(y);
+                o[db][4 * r + 2 * e + 1] += F16 ? f16hi(y) : bf16hi(y);
+              }
+            }
+        }
+      }
+    }
+  };
+
   // Q has arrived: left pending into the loop it would make every iteration wait for
   // all loads (vmcnt 0, the others unconstrained)
   __builtin_amdgcn_s_waitcnt(0x0F70);
 
+  look_up(STAGES - 1);
   for (int n = 0; n < n_it; ++n) {
     if (STAGES > 2 && n + STAGES - 2 < n_it) landed_barrier<(STAGES - 2) * S::kLoads>();
     else landed_barrier<0>();
@@ -294,109 +401,14 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int sub = sl * KT + kt, j = j0 + n * SL * KT + sub;
+      const int j = j0 + (n * SL + sl) * KT + kt;
       if (j >= w_sub) break;  // wave-uniform
-      const lds_u8* kb = (const lds_u8*)lds + n % STAGES * S::kStage + sub * kSubBytes;
-      const lds_u8* vb = kb + S::kTile;
-      f32x16 s;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const u32x4 kf = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(kb + koff[t]);
-        s = M::run(kf, qf[t], s);
-      }
-      const bool masked = 32 * j + 32 > full;
-      if (masked) {
-        const int lim = my_lim - 32 * j - 4 * hl;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < lim ? s[i] : -INFINITY;
-      }
-      float mx = vmax3(s[0], s[1], s[2]);
-#pragma unroll
-      for (int i = 3; i < 15; i += 2) mx = vmax3(mx, s[i], s[i + 1]);
-      mx = vmax(mx, s[15]);
-      if (__ballot(!(mx <= m + kthr))) {  // any lane (or a NaN): rescale (rare after the first sub-tile)
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = vmax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        // (only the rows that need it: a row's result does not hang on its neighbours)
-        const float mn = mx <= m + kthr ? m : vmax(m, mx), alpha = fast_exp2((m - mn) * cs);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-      }
-      const float nb = -m * cs;
-      u32 pw[8];
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        pw[w] = M::pack(fast_exp2(fmaf(s[2 * w], cs, nb)), fast_exp2(fmaf(s[2 * w + 1], cs, nb)));
-        l = M::dot2_ones(pw[w], l);
-      }
-      auto v_frag = [&](int db, int tt) {
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + vo[db] + 4096 * tt));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vb + vo[db] + 4096 * tt + 2048));
-        const u32x2 a0 = __builtin_bit_cast(u32x2, lo), a1 = __builtin_bit_cast(u32x2, hi);
-        return u32x4{a0[0], a0[1], a1[0], a1[1]};
-      };
-      if (masked) {
-        // A value that a row does not see must not reach it, whatever it is: with an
-        // infinity or a NaN among these 32 keys' values, the product takes 0 in its
-        // place and the rows that see its key add it
-        u32 bad = 0;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int db = 0; db < 4; ++db) {
-            const u32x4 x = v_frag(db, tt);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              bad |= (u32)((x[e] & kExp) == kExp) | (u32)((x[e] & (kExp << 16)) == (kExp << 16));
-          }
-        if (__ballot(bad != 0)) {
-#pragma unroll 1
-          for (int tt = 0; tt < 2; ++tt) {
-            const u32x4 p = tt ? u32x4{pw[4], pw[5], pw[6], pw[7]} : u32x4{pw[0], pw[1], pw[2], pw[3]};
-#pragma unroll
-            for (int db = 0; db < 4; ++db) {
-              u32x4 x = v_frag(db, tt);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((x[e] & kExp) == kExp) x[e] &= 0xffff0000u;
-                if ((x[e] & (kExp << 16)) == (kExp << 16)) x[e] &= 0xffffu;
-              }
-              o[db] = M::run(x, p, o[db]);
-            }
-          }
-          const int seen = my_lim - 32 * j;
-#pragma unroll 1
-          for (int k = 0; k < 32; ++k) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                // dims 32 db + 8 r + 4 hl .. + 3 of key k
-                const u32x2 x = *reinterpret_cast<const __attribute__((address_space(3))) u32x2*>(
-                    vb + k * 256 + 16 * ((4 * db + r) ^ (4 * (k & 3))) + 8 * hl);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const u32 b = e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xffffu;
-                  const float f = F16 ? f16lo(b) : bf16lo(b);
-                  if ((b & kExp) == kExp && k < seen) o[db][4 * r + e] += f;
-                }
-              }
-          }
-          continue;
-        }
-      }
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const u32x4 p = {pw[4 * tt], pw[4 * tt + 1], pw[4 * tt + 2], pw[4 * tt + 3]};
-#pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] = M::run(v_frag(db, tt), p, o[db]);
-      }
+      const lds_u8* kb = tile(n, sl * KT + kt);
+      read_k(kb);
+      scores();
+      read_v(kb + S::kTile);
+      softmax(j, kb + S::kTile);
+      product();
     }
   }
 

@@ -72,41 +72,55 @@ template <> struct Io<Dt::FP16> {
   __device__ static inline T put(float x) { return __builtin_bit_cast(u16, (_Float16)x); }
 };
 
-template <Dt DT> struct Vec8 {  // 8 elements as loaded
-  u32x4 a;
-  __device__ inline void load(const void* p) { a = *reinterpret_cast<const u32x4*>(p); }
-  __device__ inline void store(void* p) const { *reinterpret_cast<u32x4*>(p) = a; }
-  __device__ inline void get(float* f) const { Elem<DT>::unpack8(a, f); }
-  __device__ inline void put(const float* f) {
+// 16 bytes; NT: non-temporal, past the caches.
+template <bool NT> __device__ __forceinline__ u32x4 get16(const void* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  else return *reinterpret_cast<const u32x4*>(p);
+}
+template <bool NT> __device__ __forceinline__ void put16(void* p, const u32x4& w) {
+  if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<u32x4*>(p) = w;
+}
+
+// 16 bytes of elements <-> fp32: kN of them.
+template <Dt DT> struct Vec {
+  static constexpr int kN = 16 / Elem<DT>::kBytes;
+  __device__ static inline void get(const u32x4& w, float* f) {
+    if constexpr (DT == Dt::FP32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = Elem<DT>::pack2_hw(f[2 * i], f[2 * i + 1]);
-  }
-};
-template <> struct Vec8<Dt::FP32> {
-  u32x4 a, b;
-  __device__ inline void load(const void* p) {
-    a = reinterpret_cast<const u32x4*>(p)[0];
-    b = reinterpret_cast<const u32x4*>(p)[1];
-  }
-  __device__ inline void store(void* p) const {
-    reinterpret_cast<u32x4*>(p)[0] = a;
-    reinterpret_cast<u32x4*>(p)[1] = b;
-  }
-  __device__ inline void get(float* f) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = __uint_as_float(a[i]);
-      f[4 + i] = __uint_as_float(b[i]);
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+      Elem<DT>::unpack8(w, f);
     }
   }
-  __device__ inline void put(const float* f) {
+  __device__ static inline u32x4 put(const float* f) {
+    u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      a[i] = __float_as_uint(f[i]);
-      b[i] = __float_as_uint(f[4 + i]);
+      if constexpr (DT == Dt::FP32) w[i] = __float_as_uint(f[i]);
+      else w[i] = Elem<DT>::pack2_hw(f[2 * i], f[2 * i + 1]);
     }
+    return w;
   }
 };
+
+// K table values side by side, 8-byte aligned at least.
+template <Dt DT, int K> __device__ __forceinline__ void table_values(const void* t, int64_t at, float* f) {
+  typedef typename Io<DT>::T E;
+  const E* p = reinterpret_cast<const E*>(t) + at;
+  if constexpr (K * sizeof(E) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < (int)(K * sizeof(E) / 16); ++i)
+      Vec<DT>::get(reinterpret_cast<const u32x4*>(p)[i], f + i * Vec<DT>::kN);
+  } else {
+    static_assert(K * sizeof(E) == 8, "half a vector");
+    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+    float g[Vec<DT>::kN];
+    Vec<DT>::get(u32x4{w[0], w[1], 0, 0}, g);
+#pragma unroll
+    for (int i = 0; i < K; ++i) f[i] = g[i];
+  }
+}
 
 // The sequence of packed token t: the last b with cu[b] <= t (64 bounds a load).
 __device__ __forceinline__ int seq_of(const int32_t* cu, int n_seqs, int64_t t, int lane) {
@@ -126,142 +140,184 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int n_seqs, int64_t t, 
 struct Place {
   int64_t q_at, in_at[3];  // element offsets of the token's rows: q out, q / k / v in
   int64_t crow;            // cache row of k and v, or -1
+  int64_t s;               // number in its sequence
+  int seq;
   int q_pos, k_pos;        // rows of the tables
   bool has_q, has_kv;
 };
 
-__device__ __forceinline__ bool place_of(const Args& a, int64_t t, int lane, Place& p) {
-  int b;
-  int64_t s;
+// Where a token's rows come from: known before its sequence and position are, so that
+// they are on their way while those are looked up.
+__device__ __forceinline__ void source_of(const Args& a, int64_t t, Place& p) {
   if (a.cu) {
-    b = seq_of(a.cu, a.n_seqs, t, lane);
-    s = t - a.cu[b];
-    if (s < 0 || t >= a.cu[b + 1]) return false;  // a row of no sequence
-    p.q_at = t * a.q.out_tok;
     p.in_at[0] = t * a.q.tok;
     p.in_at[1] = t * a.k.tok;
     p.in_at[2] = t * a.v.tok;
     p.has_q = p.has_kv = true;
   } else {
-    b = (int)(t / a.seqlen);
-    s = t - (int64_t)b * a.seqlen;
-    p.q_at = b * a.q.out_seq + s * a.q.out_tok;
-    p.in_at[0] = b * a.q.seq + s * a.q.tok;
-    p.in_at[1] = b * a.k.seq + s * a.k.tok;
-    p.in_at[2] = b * a.v.seq + s * a.v.tok;
-    p.has_q = s < a.q.len;
-    p.has_kv = s < a.k.len;
+    p.seq = (int)(t / a.seqlen);
+    p.s = t - (int64_t)p.seq * a.seqlen;
+    p.in_at[0] = p.seq * a.q.seq + p.s * a.q.tok;
+    p.in_at[1] = p.seq * a.k.seq + p.s * a.k.tok;
+    p.in_at[2] = p.seq * a.v.seq + p.s * a.v.tok;
+    p.has_q = p.s < a.q.len;
+    p.has_kv = p.s < a.k.len;
   }
-  const int64_t first = a.offsets ? a.offsets[b] : a.offset0;
-  if (a.context_lens && s == 0 && lane == 0) a.context_lens[b] = (int)first + a.k.len;
+}
+
+// The token's position and where its rows go; false for a row of no sequence.
+__device__ __forceinline__ bool target_of(const Args& a, int64_t t, int lane, Place& p) {
+  if (a.cu) {
+    p.seq = seq_of(a.cu, a.n_seqs, t, lane);
+    p.s = t - a.cu[p.seq];
+    if (p.s < 0 || t >= a.cu[p.seq + 1]) return false;
+    p.q_at = t * a.q.out_tok;
+  } else {
+    p.q_at = p.seq * a.q.out_seq + p.s * a.q.out_tok;
+  }
+  const int64_t first = a.offsets ? a.offsets[p.seq] : a.offset0;
+  if (a.context_lens && p.s == 0 && lane == 0) a.context_lens[p.seq] = (int)first + a.k.len;
   const int64_t last = max(a.table_rows - 1, 0);
-  p.k_pos = (int)min(max(first + s, (int64_t)0), last);
-  p.q_pos = (int)min(max(first + s * a.q_step, (int64_t)0), last);
+  p.k_pos = (int)min(max(first + p.s, (int64_t)0), last);
+  p.q_pos = (int)min(max(first + p.s * a.q_step, (int64_t)0), last);
   p.crow = -1;
   if (a.block_tables && p.has_kv) {
-    const int64_t at = first + s;
+    const int64_t at = first + p.s;
     if (first >= 0 && at <= INT32_MAX && at < (int64_t)a.max_blocks * a.block_size) {
-      const int blk = a.block_tables[(int64_t)b * a.max_blocks + (int)at / a.block_size];
+      const int blk = a.block_tables[(int64_t)p.seq * a.max_blocks + (int)at / a.block_size];
       if (blk >= 0 && blk < a.num_blocks) p.crow = (int64_t)blk * a.block_size + (int)at % a.block_size;
     }
   }
   return true;
 }
 
-// Where row r of a token's heads (query, key, value heads in this order) comes from and
-// goes; false for a row that is not written.
-__device__ __forceinline__ bool row_of(const Args& a, const Place& p, int r, int64_t& in, int64_t& out, int& kind) {
+// Row r of a token's heads (query, key, value heads in this order): its kind, its address
+// in its tensor; -1 for a row the token lacks.
+__device__ __forceinline__ int64_t row_in(const Args& a, const Place& p, int r, int& kind) {
   if (r < a.q.heads) {
     kind = 0;
-    in = p.in_at[0] + r * a.q.head;
-    out = p.q_at + r * a.q.out_head;
-    return p.has_q;
+    return p.has_q ? p.in_at[0] + r * a.q.head : -1;
   }
   r -= a.q.heads;
   kind = r < a.k.heads ? 1 : 2;
-  const Rows& w = kind == 1 ? a.k : a.v;
   r -= kind == 1 ? 0 : a.k.heads;
-  in = p.in_at[kind] + r * w.head;
-  out = (p.crow * w.heads + r) * a.dim;
-  return p.crow >= 0;
+  return p.has_kv ? p.in_at[kind] + r * (kind == 1 ? a.k.head : a.v.head) : -1;
+}
+// where it goes; -1: nowhere
+__device__ __forceinline__ int64_t row_out(const Args& a, const Place& p, int r, int kind) {
+  if (kind == 0) return p.q_at + r * a.q.out_head;
+  r -= a.q.heads + (kind == 1 ? 0 : a.k.heads);
+  return p.crow >= 0 ? (p.crow * a.k.heads + r) * a.dim : -1;
 }
 
-// 16 elements a lane: 8 pairs, rotated, or 16 dims past them, copied.  Head sizes of
-// 16 times a power of two up to 1024, rotated dims a multiple of 16, everything
+// Two vectors of N elements a lane, placed so that a row's lanes read and write side by
+// side: the two halves of N pairs, or N / 2 adjacent pairs each, or dims past them.  Head
+// sizes of 2 N times a power of two up to 64, whole vectors of rotated dims, everything
 // 16-byte aligned.
-template <Dt DT, bool T32, bool INTER, int PASSES>
+template <Dt DT, bool T32, bool INTER, int PASSES, bool NT>
 __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(Args a) {
-  constexpr int ES = Elem<DT>::kBytes;
+  constexpr int ES = Elem<DT>::kBytes, N = Vec<DT>::kN;
   constexpr Dt TT = T32 ? Dt::FP32 : DT;
   const int lane = threadIdx.x & 63;
   const int64_t w = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = w / a.slots;
   if (t >= a.n_tokens) return;
   Place p;
-  if (!place_of(a, t, lane, p)) return;
-  const int cpr = a.dim >> 4, c = lane & (cpr - 1), per = 64 / cpr;
+  source_of(a, t, p);
+  const int cpr = a.dim / (2 * N), c = lane & (cpr - 1), per = 64 / cpr;
   const int total = a.q.heads + a.k.heads + a.v.heads;
-  const bool turn = 8 * c < a.half;  // this lane's dims are pairs
-  // element offsets of the lane's two vectors in a row
-  const int d0 = INTER || !turn ? 16 * c : 8 * c, d1 = INTER || !turn ? 16 * c + 8 : 8 * c + a.half;
+  // the lane's vectors in a row, and which of them are pairs
+  const int rot = a.half / N;  // lanes whose vectors are halves of pairs (not INTER)
+  int d0, d1;
+  bool turn0, turn1;
+  if (INTER) {
+    d0 = N * c;
+    d1 = d0 + a.dim / 2;
+    turn0 = d0 < 2 * a.half;
+    turn1 = d1 < 2 * a.half;
+  } else {
+    turn0 = turn1 = c < rot;
+    d0 = N * c + (turn0 ? 0 : a.half);
+    d1 = d0 + (turn0 ? a.half : N * (cpr - rot));
+  }
   const int r0 = (int)(w - t * a.slots) * (PASSES * per) + lane / cpr;
 
-  Vec8<DT> x[PASSES][2];
-  int64_t out[PASSES];
+  u32x4 x[PASSES][2];
   int kind[PASSES];
   bool live[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int r = r0 + i * per;
-    int64_t in = 0;
-    live[i] = r < total && row_of(a, p, min(r, total - 1), in, out[i], kind[i]);
+    const int64_t in = row_in(a, p, min(r, total - 1), kind[i]);
+    live[i] = r < total && in >= 0;
     if (live[i]) {
       const char* src = (kind[i] == 0 ? a.q.in : kind[i] == 1 ? a.k.in : a.v.in) + in * ES;
-      x[i][0].load(src + d0 * ES);
-      x[i][1].load(src + d1 * ES);
+      x[i][0] = get16<NT>(src + d0 * ES);
+      x[i][1] = get16<NT>(src + d1 * ES);
     }
   }
+  if (!target_of(a, t, lane, p)) return;
   // queries' and keys' angles: one row of the tables unless the queries all stand at
   // their sequence's first position
-  float cf[8], sf[8];
+  float cf[N], sf[N];
   auto angles = [&](int pos) {
-    constexpr int TS = Elem<TT>::kBytes;
-    const int64_t at = ((int64_t)pos * a.half + 8 * c) * TS;
-    Vec8<TT> u;
-    u.load(reinterpret_cast<const char*>(a.cos) + at);
-    u.get(cf);
-    u.load(reinterpret_cast<const char*>(a.sin) + at);
-    u.get(sf);
+    const int64_t at = (int64_t)pos * a.half;
+    if constexpr (INTER) {
+      if (turn0) {
+        table_values<TT, N / 2>(a.cos, at + d0 / 2, cf);
+        table_values<TT, N / 2>(a.sin, at + d0 / 2, sf);
+      }
+      if (turn1) {
+        table_values<TT, N / 2>(a.cos, at + d1 / 2, cf + N / 2);
+        table_values<TT, N / 2>(a.sin, at + d1 / 2, sf + N / 2);
+      }
+    } else if (turn0) {
+      table_values<TT, N>(a.cos, at + d0, cf);
+      table_values<TT, N>(a.sin, at + d0, sf);
+    }
     if (a.sign < 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sf[i] = -sf[i];
+      for (int i = 0; i < N; ++i) sf[i] = -sf[i];
     }
   };
+  auto rotate = [](float& u, float& v, float cs, float sn) {
+    const float u0 = u;
+    u = fmaf(u0, cs, -(v * sn));
+    v = fmaf(u0, sn, v * cs);
+  };
   int have = -1;
-  if (turn && a.half > 0) angles(have = p.k_pos);
+  if (a.half > 0) angles(have = p.k_pos);
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    if (!live[i]) continue;
-    if (turn && kind[i] != 2) {
+    const int64_t out = row_out(a, p, r0 + i * per, kind[i]);
+    if (!live[i] || out < 0) continue;
+    if (kind[i] != 2 && a.half > 0) {
       const int pos = kind[i] == 0 ? p.q_pos : p.k_pos;
       if (pos != have) angles(have = pos);
-      float f[16];
-      x[i][0].get(f);
-      x[i][1].get(f + 8);
+      float f[N], g[N];
+      Vec<DT>::get(x[i][0], f);
+      Vec<DT>::get(x[i][1], g);
+      if constexpr (INTER) {
+        if (turn0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int e0 = INTER ? 2 * e : e, e1 = INTER ? 2 * e + 1 : e + 8;
-        const float a0 = f[e0], a1 = f[e1];
-        f[e0] = fmaf(a0, cf[e], -(a1 * sf[e]));
-        f[e1] = fmaf(a0, sf[e], a1 * cf[e]);
+          for (int e = 0; e < N / 2; ++e) rotate(f[2 * e], f[2 * e + 1], cf[e], sf[e]);
+          x[i][0] = Vec<DT>::put(f);
+        }
+        if (turn1) {
+#pragma unroll
+          for (int e = 0; e < N / 2; ++e) rotate(g[2 * e], g[2 * e + 1], cf[N / 2 + e], sf[N / 2 + e]);
+          x[i][1] = Vec<DT>::put(g);
+        }
+      } else if (turn0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) rotate(f[e], g[e], cf[e], sf[e]);
+        x[i][0] = Vec<DT>::put(f);
+        x[i][1] = Vec<DT>::put(g);
       }
-      x[i][0].put(f);
-      x[i][1].put(f + 8);
     }
-    char* dst = (kind[i] == 0 ? a.q.out : kind[i] == 1 ? a.k.out : a.v.out) + out[i] * ES;
-    // a value row's vectors where its lane reads them
-    x[i][0].store(dst + d0 * ES);
-    x[i][1].store(dst + d1 * ES);
+    char* dst = (kind[i] == 0 ? a.q.out : kind[i] == 1 ? a.k.out : a.v.out) + out * ES;
+    put16<NT>(dst + d0 * ES, x[i][0]);
+    put16<NT>(dst + d1 * ES, x[i][1]);
   }
 }
 
@@ -275,13 +331,14 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_any_kernel(Args a) {
   const int64_t t = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= a.n_tokens) return;
   Place p;
-  if (!place_of(a, t, lane, p)) return;
+  source_of(a, t, p);
+  if (!target_of(a, t, lane, p)) return;
   const int total = a.q.heads + a.k.heads + a.v.heads, pairs = a.dim / 2;
   for (int64_t i = lane; i < (int64_t)total * pairs; i += 64) {
     const int r = (int)(i / pairs), c = (int)(i - (int64_t)r * pairs);
-    int64_t in, out;
     int kind;
-    if (!row_of(a, p, r, in, out, kind)) continue;
+    const int64_t in = row_in(a, p, r, kind), out = row_out(a, p, r, kind);
+    if (in < 0 || out < 0) continue;
     const bool pair = c < a.half;
     const int d0 = INTER || !pair ? 2 * c : c, d1 = INTER || !pair ? 2 * c + 1 : c + a.half;
     const E* src = reinterpret_cast<const E*>(kind == 0 ? a.q.in : kind == 1 ? a.k.in : a.v.in) + in;
@@ -308,18 +365,22 @@ static int launch_i(Args a, bool fast, int n_cu, hipStream_t st) {
     hipLaunchKernelGGL((rotary_any_kernel<DT, T32, INTER>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
     return AAC_OK;
   }
-  const int per = 64 / (a.dim / 16), total = a.q.heads + a.k.heads + a.v.heads;
+  const int per = 64 / (a.dim / (2 * Vec<DT>::kN)), total = a.q.heads + a.k.heads + a.v.heads;
   auto blocks_at = [&](int passes) {
     a.slots = (int)cdiv(total, (int64_t)per * passes);
     return cdiv(a.n_tokens * a.slots, kWaves);
   };
-  const bool many = total > 2 * per && a.n_tokens * cdiv(total, 4 * (int64_t)per) >= 8 * (int64_t)n_cu;
-  const int64_t blocks = blocks_at(many ? 4 : 1);
+  // Many tokens: two passes a wave (260k tokens at 16/8 heads appended, us, 1 / 2 / 4 / 8
+  // passes: 852 / 765 / 822 / 798).  What passes the caches anyway goes round them: 765
+  // against 823, 16 x 4096 x 32 heads rotated 180 against 198.
+  const bool many = total > per && a.n_tokens * cdiv(total, 2 * (int64_t)per) >= 8 * (int64_t)n_cu;
+  const bool large = many && a.n_tokens * total * a.dim * Elem<DT>::kBytes >= (int64_t(64) << 20);
+  const int64_t blocks = blocks_at(many ? 2 : 1);
   if (blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
-  if (many)
-    hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 4>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
-  else
-    hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 1>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
+  const dim3 grid((unsigned)blocks), block(64 * kWaves);
+  if (large) hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 2, true>), grid, block, 0, st, a);
+  else if (many) hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 2, false>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 1, false>), grid, block, 0, st, a);
   return AAC_OK;
 }
 
@@ -334,10 +395,11 @@ static int launch_t(const Args& a, bool t32, bool inter, bool fast, int n_cu, hi
 
 static int launch(const Args& a, int32_t table_dtype, bool inter, int32_t dtype, hipStream_t st) {
   const int es = dtype == AAC_DTYPE_FP32 ? 4 : 2, ts = table_dtype == AAC_DTYPE_FP32 ? 4 : 2;
-  const int cpr = a.dim / 16;
+  const int n = 16 / es, cpr = a.dim / (2 * n), unit = inter ? n / 2 : n;
   // every vector the fast kernel touches: rows, heads and tables at multiples of 16 bytes
-  bool fast = a.dim % 16 == 0 && (cpr & (cpr - 1)) == 0 && cpr <= 64 && a.half % 8 == 0 &&
-              (((uintptr_t)a.cos | (uintptr_t)a.sin) % 16) == 0 && (a.half * ts) % 16 == 0;
+  // (interleaved pairs: tables of half vectors)
+  bool fast = a.dim % (2 * n) == 0 && (cpr & (cpr - 1)) == 0 && cpr <= 64 && a.half % unit == 0 &&
+              (((uintptr_t)a.cos | (uintptr_t)a.sin) % 16) == 0 && a.half * ts % std::min(16, unit * ts) == 0;
   for (const Rows* r : {&a.q, &a.k, &a.v})
     if (r->heads) {
       fast = fast && (((uintptr_t)r->in | (uintptr_t)r->out) % 16) == 0;
@@ -370,46 +432,52 @@ static int check_tables(const void* cos, const void* sin, int32_t rows, int32_t 
 }
 
 // ------------------------------------------------------------------ tables
-// cos and sin of position p, frequency i: the angle in quarter turns, 4 p turns[i], and
-// its distance from a whole number of them in fp64 (at position 2^20 a radian has 2^-33
-// of its error left, where fp32 has 2^-4); what remains is within an eighth of a turn
-// and is exact to fp32's own precision.  Bound by the stores: 8 values of each a thread.
+// cos and sin of position p, frequency i: the angle in quarter turns, 4 p turns[i], less the
+// nearest whole number of them, in fp64 (at position 2^20 a radian keeps 2^-33 of
+// precision there, 2^-4 in fp32); what remains is within an eighth of a turn, and its
+// sine and cosine are polynomials in fp32, near-minimax from interpolation at Chebyshev
+// nodes (truncation below 1e-10, with their rounding 8.5e-8).  The whole number's last
+// bits, the quadrant, are the low bits of its sum with 1.5 * 2^52.
+// A vector of each a thread.
+__device__ __forceinline__ void cos_sin_of(double x, float factor, float& c, float& s) {
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
+  const double y = x + kRound;
+  const float r = (float)(x - (y - kRound)), u = r * r;
+  const u32 quad = (u32)(uint64_t)__double_as_longlong(y);
+  const float sn = r * factor * fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0.00015820628f, -0.0046812664f), 0.07969258f), -0.6459641f), 1.5707964f);
+  const float cn = factor * fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0.00090362807f, -0.02086007f), 0.2536692f), -1.2337005f), 1.0f);
+  const float a = quad & 1 ? sn : cn, b = quad & 1 ? cn : sn;
+  c = __uint_as_float(__float_as_uint(a) ^ ((quad + 1) << 30 & 0x80000000u));
+  s = __uint_as_float(__float_as_uint(b) ^ (quad << 30 & 0x80000000u));
+}
+
 template <Dt DT>
 __global__ __launch_bounds__(256) void tables_kernel(const double* turns, int32_t half, const int32_t* positions,
                                                      int64_t start, int64_t n, float factor, void* cos_out,
                                                      void* sin_out) {
   typedef typename Io<DT>::T E;
-  const int groups = (half + 7) / 8;
+  constexpr int N = Vec<DT>::kN;
+  const u32 groups = (half + N - 1) / N;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n * groups) return;
-  const int64_t r = i / groups;
-  const int f0 = (int)(i - r * groups) * 8;
-  const double pos = (double)(positions ? (int64_t)positions[r] : start + r);
-  float c[8], s[8];
+  const int64_t r = i >> 32 ? i / groups : (int64_t)((u32)i / groups);
+  const int f0 = (int)(i - r * groups) * N;
+  const double pos = 4.0 * (double)(positions ? (int64_t)positions[r] : start + r);
+  float c[N], s[N];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double x = 4.0 * pos * turns[min(f0 + e, half - 1)];
-    const double k = rint(x);
-    float sn, cs;
-    sincospif((float)(x - k) * 0.5f, &sn, &cs);
-    const int quad = (int)((int64_t)k & 3);
-    const float u = quad & 1 ? sn : cs, v = quad & 1 ? cs : sn;
-    c[e] = (quad == 1 || quad == 2 ? -u : u) * factor;
-    s[e] = (quad >= 2 ? -v : v) * factor;
-  }
+  for (int e = 0; e < N; ++e) cos_sin_of(pos * turns[min(f0 + e, half - 1)], factor, c[e], s[e]);
   E* co = reinterpret_cast<E*>(cos_out) + r * half + f0;
   E* so = reinterpret_cast<E*>(sin_out) + r * half + f0;
-  if (half % 8 == 0) {
-    Vec8<DT> o;
-    o.put(c);
-    o.store(co);
-    o.put(s);
-    o.store(so);
+  if (half % N == 0) {
+    *reinterpret_cast<u32x4*>(co) = Vec<DT>::put(c);
+    *reinterpret_cast<u32x4*>(so) = Vec<DT>::put(s);
   } else {
-    for (int e = 0; e < min(8, half - f0); ++e) {
-      co[e] = Io<DT>::put(c[e]);
-      so[e] = Io<DT>::put(s[e]);
-    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (f0 + e < half) {
+        co[e] = Io<DT>::put(c[e]);
+        so[e] = Io<DT>::put(s[e]);
+      }
   }
 }
 
@@ -506,10 +574,11 @@ extern "C" int aac_rotary_tables(const void* turns, int32_t n_freqs, const int32
   if (n_freqs <= 0 || n_positions < 0) return AAC_ERR_INVALID_ARGUMENT;
   if (n_positions == 0) return AAC_OK;
   if (!turns || !cos_out || !sin_out) return AAC_ERR_INVALID_ARGUMENT;
-  if (n_freqs % 8 == 0 && ((uintptr_t)cos_out | (uintptr_t)sin_out) % 16) return AAC_ERR_MISALIGNED;
+  const int vec = dtype == AAC_DTYPE_FP32 ? 4 : 8;
+  if (n_freqs % vec == 0 && ((uintptr_t)cos_out | (uintptr_t)sin_out) % 16) return AAC_ERR_MISALIGNED;
   // (positions are whole numbers in fp64, and their product with 4 turns has a quadrant)
   if (start < -(int64_t(1) << 40) || start > (int64_t(1) << 40)) return AAC_ERR_SHAPE;
-  const int64_t blocks = cdiv(n_positions * cdiv(n_freqs, 8), 256);
+  const int64_t blocks = cdiv(n_positions * cdiv(n_freqs, vec), 256);
   if (n_positions >= (int64_t(1) << 40) / n_freqs || blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks), block(256);
   const double* f = (const double*)turns;

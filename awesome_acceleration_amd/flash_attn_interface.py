@@ -518,7 +518,7 @@ def _check_cache(q, k_cache, v_cache):
     qshape = q.shape
     if shape[3] != qshape[-1]:
         raise RuntimeError("head_dim mismatch")
-    if qshape[-2] % shape[2]:
+    if not shape[2] or qshape[-2] % shape[2]:
         raise RuntimeError("query heads must be a multiple of KV heads")
 
 
@@ -682,15 +682,21 @@ def _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqle
             q = rotary.apply_rotary_emb(
                 q if causal else q.reshape(B, 1, S * Hq, D), rotary_cos, rotary_sin,
                 interleaved=interleaved, seqlen_offsets=seqlens).view(B, S, Hq, D)
-    if one:
-        return decode_paged(q.reshape(B, Hq, D), k_cache, v_cache, tables, ctx, softmax_scale=softmax_scale,
-                            max_context_len=max_context_len).view(B, 1, Hq, D)
     out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
     if out.numel() == 0:
         return out
-    if k_cache.numel() == 0 or tables.shape[1] == 0:
+    mb = tables.shape[1]
+    if nblk == 0 or bs == 0 or mb == 0:
         return out.zero_()
     q = q.reshape(B * S, Hq, D)
+    if one and q.stride(2) == 1 and q.stride(1) == D:
+        mcl = int(max_context_len or 0)
+        ws_bytes = _decode_ws_bytes(B, Hq, hkv, D, bs, mb, mcl, 0)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        _lib.launch("aac_decode_paged", q.get_device(), q.data_ptr(), q.stride(0), k_cache.data_ptr(),
+                    v_cache.data_ptr(), nblk, bs, tables.data_ptr(), mb, ctx.data_ptr(), B, mcl, Hq, hkv, D,
+                    scale, out.data_ptr(), Hq * D, None if ws is None else ws.data_ptr(), ws_bytes, 0, _dtype_code(q))
+        return out
     if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
     _launch_chunk(q, q.stride(0) if B * S > 1 else Hq * D, B * S, k_cache, v_cache, tables, None, ctx, None,

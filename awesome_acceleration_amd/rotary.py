@@ -22,35 +22,44 @@ from .flash_attn_interface import _on_gpu, _require
 __all__ = ["apply_rotary_emb", "rotary_append_paged", "RotaryEmbedding", "scaled_frequencies"]
 
 
-def _code(t: torch.Tensor) -> int:
-    code = _lib.AAC_DTYPE.get(t.dtype)
-    _require(code is not None, f"unsupported dtype {t.dtype}")
-    return code
+_CODES = _lib.AAC_DTYPE
 
 
+def _bad_dtype(dtype):
+    raise RuntimeError(f"unsupported dtype {dtype}")
+
+
+# (A call's host time is its latency for a single token: one condition a line, messages
+# built where they are raised.)
 def _tables(cos: torch.Tensor, sin: torch.Tensor, dtype: torch.dtype, head_dim: int):
     """(cos, sin addresses, rows, rotary dims, type code) of the tables, checked."""
-    _require(cos.dim() == 2 and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous(),
-             "cos and sin must be contiguous [positions, rotary_dim / 2]")
-    _require(cos.dtype is sin.dtype and cos.dtype in (dtype, torch.float32),
-             "cos and sin must be float32 or of the heads' dtype")
-    rows, half = cos.shape
-    _require(rows > 0 and half > 0, "empty tables")
-    _require(2 * half <= head_dim, "rotary_dim is larger than head_dim")
-    return cos.data_ptr(), sin.data_ptr(), min(rows, (1 << 31) - 1), 2 * half, _code(cos)
+    shape = cos.shape
+    if len(shape) != 2 or sin.shape != shape or not cos.is_contiguous() or not sin.is_contiguous():
+        raise RuntimeError("cos and sin must be contiguous [positions, rotary_dim / 2]")
+    td = cos.dtype
+    if sin.dtype is not td or (td is not dtype and td is not torch.float32):
+        raise RuntimeError("cos and sin must be float32 or of the heads' dtype")
+    rows, half = shape
+    if rows == 0 or half == 0:
+        raise RuntimeError("empty tables")
+    if 2 * half > head_dim:
+        raise RuntimeError("rotary_dim is larger than head_dim")
+    return cos.data_ptr(), sin.data_ptr(), min(rows, (1 << 31) - 1), 2 * half, _CODES.get(td)
 
 
-def _ints(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    _require(t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous(),
-             f"{name} must be contiguous int32 [{n}]")
-    return t
+def _ints(t: torch.Tensor, n: int, name: str) -> int:
+    """The address of an int32 vector, checked."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous int32 [{n}]")
+    return t.data_ptr()
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+def _strides(t: torch.Tensor):
     """(sequence, token, head) strides of [B, S, H, D] or, with 0 first, [N, H, D]."""
     st = t.stride()
-    _require(st[-1] == 1 or t.shape[-1] == 1, "head_dim must be contiguous")
-    return (st[0], st[1], st[2]) if t.dim() == 4 else (0, st[0], st[1])
+    if st[-1] != 1 and t.shape[-1] != 1:
+        raise RuntimeError("head_dim must be contiguous")
+    return st[:3] if len(st) == 4 else (0, st[0], st[1])
 
 
 def apply_rotary_emb(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False,
@@ -66,62 +75,85 @@ def apply_rotary_emb(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, inte
     is not needed.  Any strides whose last is 1.  ``conjugate`` turns back (the inverse).
     Returns a new contiguous tensor, or ``x`` itself with ``inplace``.  bf16, fp16 and
     float32, any even head_dim."""
-    _on_gpu(x, cos, sin, cu_seqlens)
-    packed = cu_seqlens is not None
-    _require(x.dim() == (3 if packed else 4),
-             "x must be [tokens, heads, head_dim] with cu_seqlens, [B, S, heads, head_dim] without")
-    H, D = x.shape[-2:]
-    _require(D % 2 == 0, "head_dim must be even")
-    if packed:
-        _require(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be [B + 1]")
-        B, S, N = cu_seqlens.shape[0] - 1, 0, x.shape[0]
-        cu = _ints(cu_seqlens, B + 1, "cu_seqlens").data_ptr()
+    dev = x.get_device()
+    if dev < 0 or cos.get_device() != dev or sin.get_device() != dev:
+        _on_gpu(x, cos, sin)
+    shape = x.shape
+    if len(shape) != (4 if cu_seqlens is None else 3):
+        raise RuntimeError("x must be [tokens, heads, head_dim] with cu_seqlens, [B, S, heads, head_dim] without")
+    D = shape[-1]
+    if D % 2:
+        raise RuntimeError("head_dim must be even")
+    if cu_seqlens is not None:
+        _on_gpu(x, cu_seqlens)
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+            raise RuntimeError("cu_seqlens must be [B + 1]")
+        B, S, N = cu_seqlens.shape[0] - 1, 0, shape[0]
+        cu = _ints(cu_seqlens, B + 1, "cu_seqlens")
     else:
-        B, S = x.shape[:2]
-        N, cu = B * S, None
-    offset, offsets = 0, None
+        B, S = shape[0], shape[1]
+        N, cu = 0, None
     if isinstance(seqlen_offsets, torch.Tensor):
-        _on_gpu(x, seqlen_offsets)
-        offsets = _ints(seqlen_offsets, B, "seqlen_offsets").data_ptr()
+        if seqlen_offsets.get_device() != dev:
+            _on_gpu(x, seqlen_offsets)
+        offset, offsets = 0, _ints(seqlen_offsets, B, "seqlen_offsets")
     else:
-        offset = int(seqlen_offsets)
-        _require(-(1 << 31) <= offset < 1 << 31, "seqlen_offsets does not fit in 32 bits")
-    cp, sp, rows, rot, tcode = _tables(cos, sin, x.dtype, D)
-    code, st = _code(x), _strides(x)
+        offset, offsets = int(seqlen_offsets), None
+        if not -(1 << 31) <= offset < 1 << 31:
+            raise RuntimeError("seqlen_offsets does not fit in 32 bits")
+    dt = x.dtype
+    cp, sp, rows, rot, tcode = _tables(cos, sin, dt, D)
+    code = _CODES.get(dt)
+    if code is None:
+        _bad_dtype(dt)
+    s0, s1, s2 = _strides(x)
     if inplace:
-        out = x
-        for n, s in zip(x.shape, x.stride()):
-            _require(s != 0 or n < 2, "x is broadcast: it cannot be turned in place")
+        out, (o0, o1, o2) = x, (s0, s1, s2)
+        for n, s in zip(shape, x.stride()):
+            if s == 0 and n > 1:
+                raise RuntimeError("x is broadcast: it cannot be turned in place")
     else:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty(shape, dtype=dt, device=x.device)
+        o2 = D
+        o1 = shape[-2] * D
+        o0 = S * o1
     if x.numel() and B:
-        _lib.launch("aac_rotary", x.get_device(), x.data_ptr(), *st, out.data_ptr(), *_strides(out), B, S,
-                    N, cu, offsets, offset, H, D, cp, sp, rows, rot, int(bool(interleaved)),
-                    int(bool(conjugate)), tcode, code)
+        _lib.launch("aac_rotary", dev, x.data_ptr(), s0, s1, s2, out.data_ptr(), o0, o1, o2, B, S, N, cu,
+                    offsets, offset, shape[-2], D, cp, sp, rows, rot, 1 if interleaved else 0,
+                    1 if conjugate else 0, tcode, code)
     return out
 
 
 def _append(q, k, v, k_cache, v_cache, tables, seqlens, cos, sin, interleaved, cu, q_at_first, ctx=None):
     """The launch of ``rotary_append_paged``; shapes of q, k, v and tables checked there."""
-    hkv, D = k_cache.shape[2], k_cache.shape[3]
-    tab = (None, None, 0, 0, 0) if cos is None else _tables(cos, sin, k.dtype, D)
-    code = _code(k)
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    nblk, bs, hkv, D = k_cache.shape
+    dt = k.dtype
+    cp, sp, rows, rot, tcode = (None, None, 0, 0, 0) if cos is None else _tables(cos, sin, dt, D)
+    code = _CODES.get(dt)
+    if code is None:
+        _bad_dtype(dt)
     B = seqlens.shape[0]
     if cu is None:
-        sq, sk, n = (0 if q is None else q.shape[1]), k.shape[1], 0
+        sk, n = k.shape[1], 0
     else:
-        sq = sk = 0
-        n = k.shape[0]
-    if B and k_cache.shape[0] and (k.numel() or (q is not None and q.numel())):
-        _lib.launch(
-            "aac_rotary_append_paged", k.get_device(), None if q is None else q.data_ptr(),
-            *((0, 0, 0) if q is None else _strides(q)), k.data_ptr() or k_cache.data_ptr(), *_strides(k),
-            v.data_ptr() or k_cache.data_ptr(), *_strides(v), None if q is None else out.data_ptr(), B,
-            sq, sk, n, None if cu is None else cu.data_ptr(), seqlens.data_ptr(),
-            None if ctx is None else ctx.data_ptr(), 0 if q is None else q.shape[-2], hkv, D, *tab[:4], int(bool(interleaved)),
-            int(bool(q_at_first)), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
-            k_cache.shape[1], tables.data_ptr(), tables.shape[1], tab[4], code)
+        sk, n, cu = 0, k.shape[0], cu.data_ptr()
+    k0, k1, k2 = _strides(k)
+    v0, v1, v2 = _strides(v)
+    out = qp = qo = None
+    q0 = q1 = q2 = sq = hq = 0
+    if q is not None:
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        q0, q1, q2 = _strides(q)
+        qp, qo, hq = q.data_ptr(), out.data_ptr(), q.shape[-2]
+        if cu is None:
+            sq = q.shape[1]
+    if B and nblk and (k.numel() or (q is not None and q.numel())):
+        kc = k_cache.data_ptr()
+        _lib.launch("aac_rotary_append_paged", k.get_device(), qp, q0, q1, q2, k.data_ptr() or kc, k0, k1, k2,
+                    v.data_ptr() or kc, v0, v1, v2, qo, B, sq, sk, n, cu, seqlens.data_ptr(),
+                    None if ctx is None else ctx.data_ptr(), hq, hkv, D, cp, sp, rows, rot,
+                    1 if interleaved else 0, 1 if q_at_first else 0, kc, v_cache.data_ptr(), nblk, bs,
+                    tables.data_ptr(), tables.shape[1], tcode, code)
     return out
 
 
@@ -145,29 +177,34 @@ def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     distinct: of two tokens for one row an unspecified one stays.  bf16, fp16, float32, any
     even head_dim."""
     _on_gpu(q, k, v, k_cache, v_cache, block_tables, cache_seqlens, rotary_cos, rotary_sin, cu_seqlens)
-    _require((rotary_cos is None) == (rotary_sin is None), "rotary_cos and rotary_sin go together")
-    _require(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.is_contiguous()
-             and v_cache.is_contiguous(),
-             "caches must be contiguous [num_blocks, block_size, Hkv, D], alike")
+    if (rotary_cos is None) != (rotary_sin is None):
+        raise RuntimeError("rotary_cos and rotary_sin go together")
+    cshape, kshape = k_cache.shape, k.shape
+    if (len(cshape) != 4 or cshape != v_cache.shape or not k_cache.is_contiguous()
+            or not v_cache.is_contiguous()):
+        raise RuntimeError("caches must be contiguous [num_blocks, block_size, Hkv, D], alike")
     nd = 4 if cu_seqlens is None else 3
-    _require(k.dim() == nd and k.shape == v.shape and k.shape[-2:] == k_cache.shape[-2:],
-             "k and v must be [B, S, Hkv, D], or [N, Hkv, D] with cu_seqlens, as the caches' rows")
-    _require(k.dtype is v.dtype and k.dtype is k_cache.dtype and k.dtype is v_cache.dtype, "dtype mismatch")
-    D = k.shape[-1]
-    _require(D % 2 == 0 and k_cache.shape[1] > 0 and k_cache.shape[2] > 0, "head_dim must be even, blocks and heads not empty")
-    if q is not None:
-        _require(q.dim() == nd and q.dtype is k.dtype and q.shape[-1] == D
-                 and q.shape[:nd - 2] == k.shape[:nd - 2],
-                 "q must be [B, S, Hq, D], or [N, Hq, D], of k's tokens and dtype")
+    if len(kshape) != nd or kshape != v.shape or kshape[-2:] != cshape[2:]:
+        raise RuntimeError("k and v must be [B, S, Hkv, D], or [N, Hkv, D] with cu_seqlens, as the caches' rows")
+    dt = k.dtype
+    if v.dtype is not dt or k_cache.dtype is not dt or v_cache.dtype is not dt:
+        raise RuntimeError("dtype mismatch")
+    D = cshape[3]
+    if D % 2 or cshape[1] == 0 or cshape[2] == 0:
+        raise RuntimeError("head_dim must be even, blocks and heads not empty")
+    if q is not None and (q.dim() != nd or q.dtype is not dt or q.shape[-1] != D
+                          or q.shape[:nd - 2] != kshape[:nd - 2]):
+        raise RuntimeError("q must be [B, S, Hq, D], or [N, Hq, D], of k's tokens and dtype")
     B = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
     _ints(cache_seqlens, B, "cache_seqlens")
-    if cu_seqlens is None:
-        _require(k.shape[0] == B, "cache_seqlens must be [B]")
-    else:
+    if cu_seqlens is not None:
         _ints(cu_seqlens, B + 1, "cu_seqlens")
-    _require(block_tables.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == B
-             and block_tables.shape[1] > 0 and block_tables.is_contiguous(),
-             "block_tables must be contiguous int32 [B, max_blocks]")
+    elif kshape[0] != B:
+        raise RuntimeError("cache_seqlens must be [B]")
+    tshape = block_tables.shape
+    if (block_tables.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != B or tshape[1] == 0
+            or not block_tables.is_contiguous()):
+        raise RuntimeError("block_tables must be contiguous int32 [B, max_blocks]")
     return _append(q, k, v, k_cache, v_cache, block_tables, cache_seqlens, rotary_cos, rotary_sin,
                    interleaved, cu_seqlens, False)
 
@@ -255,6 +292,7 @@ class RotaryEmbedding:
         self.device = torch.device(device)
         _require(self.device.type == "cuda", "the tables are built on a GPU (no CPU path exists)")
         self._turns = (self.frequencies / (2 * math.pi)).to(self.device)
+        self.device = self._turns.device
 
     def cos_sin(self, n: Optional[int] = None, *, start: int = 0,
                 positions: Optional[torch.Tensor] = None,
@@ -262,19 +300,23 @@ class RotaryEmbedding:
         """cos and sin, times the scaling's factor, ``[n, rotary_dim / 2]`` of positions
         ``start`` to ``start + n - 1``, or of ``positions`` (int32 ``[n]`` on the GPU).
         Angles are reduced in 64 bits: far positions lose nothing."""
-        code = _lib.AAC_DTYPE.get(dtype)
-        _require(code is not None, f"unsupported dtype {dtype}")
-        at = None
+        code = _CODES.get(dtype)
+        if code is None:
+            _bad_dtype(dtype)
+        dev, at = self._turns.get_device(), None
         if positions is not None:
-            _require(n is None and start == 0, "positions, or n and start")
-            _require(positions.dim() == 1 and positions.get_device() == self._turns.get_device(),
-                     "positions must be one-dimensional, on the tables' GPU")
+            if n is not None or start:
+                raise RuntimeError("positions, or n and start")
+            if positions.dim() != 1 or positions.get_device() != dev:
+                raise RuntimeError("positions must be one-dimensional, on the tables' GPU")
             n = positions.shape[0]
-            at = _ints(positions, n, "positions").data_ptr()
-        _require(n is not None and n >= 0, "n must be given, 0 or more")
+            at = _ints(positions, n, "positions")
+        if n is None or n < 0:
+            raise RuntimeError("n must be given, 0 or more")
         half = self.rotary_dim // 2
-        cos, sin = (torch.empty((n, half), dtype=dtype, device=self._turns.device) for _ in range(2))
+        cos = torch.empty((n, half), dtype=dtype, device=self.device)
+        sin = torch.empty((n, half), dtype=dtype, device=self.device)
         if n:
-            _lib.launch("aac_rotary_tables", self._turns.get_device(), self._turns.data_ptr(), half, at,
-                        int(start), n, self.factor, cos.data_ptr(), sin.data_ptr(), code)
+            _lib.launch("aac_rotary_tables", dev, self._turns.data_ptr(), half, at, int(start), n, self.factor,
+                        cos.data_ptr(), sin.data_ptr(), code)
         return cos, sin
