@@ -25,6 +25,10 @@ Changes on the hot path:
   positions and cache lengths advanced in place) before the host reads the
   previous step's tokens, so the host's bookkeeping overlaps the GPU; the
   reference's loop syncs on every step's tokens (llm.py:404-405, :413-443).
+* With ``prefill_chunk`` a step takes at most that many prompt tokens: long prompts are
+  prefilled in chunks that attend to the cached part of their prompt
+  (``flash_attn_interface.prefill_paged``), between decode steps of the sequences that
+  generate, so that no prompt holds those up for longer than a chunk takes.
 * No tokenizer is available offline, so prompts are token-id lists and
   ``GenerationOutput.text`` is empty unless a ``decode_fn`` is supplied.
 """
@@ -86,6 +90,7 @@ class _Seq:
     pos: int                 # position of the next token to feed
     done: bool = False       # finished (a step launched ahead may still hold its row)
     scores: list = field(default_factory=list)  # (log probability, entropy, alternatives) of each token
+    filled: int = 0          # prompt tokens in the cache (while it is prefilled in chunks)
 
 
 class LLM:
@@ -95,16 +100,24 @@ class LLM:
     ``num_blocks`` defaults to enough blocks for ``max_num_seqs`` sequences
     of ``max_seq_len`` tokens.  ``kv_cache_dtype`` "mxfp4" keeps K and V in four bits
     (``PagedKV4Cache``; head_dim 128, blocks of a multiple of 16 tokens), in 27 % of the
-    memory; ``None`` in ``dtype``.
+    memory; ``None`` in ``dtype``.  ``prefill_chunk``: the most prompt tokens of a step
+    (``None``: admitted prompts are prefilled whole); not with the 4-bit cache.
     """
 
     def __init__(self, config: Optional[Qwen3Config] = None, max_num_seqs: int = 32,
                  max_seq_len: int = 4096, dtype=torch.bfloat16, block_size: int = 256,
                  num_blocks: Optional[int] = None, seed: int = 0, device="cuda",
                  decode_fn: Optional[Callable[[list[int]], str]] = None, use_graphs: bool = True,
-                 fused: bool = True, kv_cache_dtype: Optional[str] = None):
+                 fused: bool = True, kv_cache_dtype: Optional[str] = None,
+                 prefill_chunk: Optional[int] = None):
         if kv_cache_dtype not in (None, "mxfp4"):
             raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: None or \"mxfp4\"")
+        if prefill_chunk is not None:
+            if not isinstance(prefill_chunk, int) or prefill_chunk < 1:
+                raise ValueError("prefill_chunk must be a positive number of tokens")
+            if kv_cache_dtype is not None:
+                raise ValueError("prefill_chunk needs the cache in the model's dtype")
+        self.prefill_chunk = prefill_chunk
         self.device = torch.device(device)
         self.dtype = dtype
         self.config = config or Qwen3Config()
@@ -242,24 +255,31 @@ class LLM:
         return out
 
     def _prefill_maps(self, lens: list[int], seqs: list[_Seq]):
-        """(cu_seqlens, positions, slot_mapping) of a prefill of whole prompts.  Built on
-        the GPU from the lengths and block tables, which go there in one copy; a block
-        outside the cache raises IndexError here, before any launch, as the reference's
-        index_copy_ store does (llm.py:171-174)."""
+        """(cu_seqlens, positions, slot_mapping) of a prefill of whole prompts."""
+        if len(seqs) > MAX_MAP_SEQS:
+            return build_prefill_metadata(lens, pad_block_tables([s.blocks for s in seqs], self.blocks_per_seq),
+                                          self.block_size, self.device,
+                                          num_cache_rows=self.cache.num_blocks * self.block_size)
+        return self._chunk_maps(lens, seqs, None)[0][:3]
+
+    def _chunk_maps(self, lens: list[int], seqs: list[_Seq], cached: Optional[list[int]]):
+        """The maps (``paged.StepMaps``) and block tables of ``lens`` new tokens behind
+        ``cached`` ones (``None``: none).  Built on the GPU from the lengths and tables, which
+        go there in one copy; a block outside the cache raises IndexError here, before any
+        launch, as the reference's index_copy_ store does (llm.py:171-174)."""
         tables = pad_block_tables([s.blocks for s in seqs], self.blocks_per_seq)
-        n, rows = len(seqs), self.cache.num_blocks * self.block_size
-        if n > MAX_MAP_SEQS:
-            return build_prefill_metadata(lens, tables, self.block_size, self.device,
-                                          num_cache_rows=rows)
-        for L, s in zip(lens, seqs):
-            used = s.blocks[:blocks_needed(L, self.block_size)]
+        n = len(seqs)
+        for i, (L, s) in enumerate(zip(lens, seqs)):
+            used = s.blocks[:blocks_needed(L + (cached[i] if cached else 0), self.block_size)]
             if min(used) < 0 or max(used) >= self.cache.num_blocks:
                 raise IndexError(f"prefill store outside the KV cache ({self.cache.num_blocks} blocks "
                                  f"of {self.block_size})")
-        packed = torch.from_numpy(np.concatenate((np.asarray(lens, np.int32), tables.reshape(-1))))
+        packed = torch.from_numpy(np.concatenate((np.asarray(lens, np.int32),
+                                                  np.asarray(cached or (), np.int32), tables.reshape(-1))))
         d = packed.to(self.device)
-        maps = build_step_maps(d[:n], None, d[n:].view(n, -1), self.block_size, sum(lens))
-        return maps[:3]
+        held = d[n:2 * n] if cached else None
+        d_tables = d[2 * n if cached else n:].view(n, -1)
+        return build_step_maps(d[:n], held, d_tables, self.block_size, sum(lens)), d_tables
 
     def _prefill(self, seqs: list[_Seq]) -> torch.Tensor:
         """Packed varlen prefill of newly admitted sequences (llm.py:116-208)."""
@@ -274,6 +294,40 @@ class LLM:
         self.stats["prefill_calls"] += 1
         self.stats["prefill_tokens"] += sum(lens)
         return self.model.forward(ids, meta, self.cache, prefill=True)
+
+    def _prefill_chunk(self, filling: list[_Seq]) -> tuple[torch.Tensor, list[_Seq]]:
+        """One step's share of the prompts being prefilled: in their order, at most
+        ``prefill_chunk`` tokens (and MAX_MAP_SEQS prompts), the last of them in part.
+        Returns the logits of the prompts that it ends, and those."""
+        left, seqs, lens = self.prefill_chunk, [], []
+        for s in filling[:MAX_MAP_SEQS]:
+            if left == 0:
+                break
+            seqs.append(s)
+            lens.append(min(left, len(s.req.token_ids[s.prompt_idx]) - s.filled))
+            left -= lens[-1]
+        cached = [s.filled for s in seqs]
+        ended = [i for i, (s, n) in enumerate(zip(seqs, lens))
+                 if s.filled + n == len(s.req.token_ids[s.prompt_idx])]
+        if not any(cached) and len(ended) == len(seqs):
+            logits = self._prefill(seqs)  # whole prompts
+        else:
+            maps, tables = self._chunk_maps(lens, seqs, cached)
+            ids = torch.tensor([t for s, n in zip(seqs, lens)
+                                for t in s.req.token_ids[s.prompt_idx][s.filled:s.filled + n]],
+                               dtype=torch.int64).to(self.device)
+            ends = np.cumsum(lens)
+            last = torch.tensor([int(ends[i]) - 1 for i in ended], dtype=torch.int64).to(self.device)
+            meta = StepMeta(positions=maps.positions, cu_seqlens=maps.cu_seqlens,
+                            slot_mapping=maps.slot_mapping, max_seqlen=max(lens), last_idx=last,
+                            block_tables=tables, context_lens=maps.context_lens,
+                            max_context_len=max(a + b for a, b in zip(cached, lens)))
+            self.stats["prefill_calls"] += 1
+            self.stats["prefill_tokens"] += sum(lens)
+            logits = self.model.forward(ids, meta, self.cache, prefill=True)
+        for s, n in zip(seqs, lens):
+            s.filled += n
+        return logits, [seqs[i] for i in ended]
 
     def _decode_meta(self, B: int, max_context_len: int) -> StepMeta:
         d, W = self._dev, self.blocks_per_seq
@@ -414,15 +468,16 @@ class LLM:
         free_rows = list(range(self.max_num_seqs))
         active: dict[int, _Seq] = {}
         pending: list[_Request] = []
+        filling: list[_Seq] = []  # admitted, their prompts not all in the cache
         try:
-            while self._loop_running or pending or active:
+            while self._loop_running or pending or active or filling:
                 # Phase 1: drain the queue
                 while True:
                     try:
                         pending.append(self._request_queue.get_nowait())
                     except queue.Empty:
                         break
-                if not pending and not active:
+                if not pending and not active and not filling:
                     if not self._loop_running:
                         break
                     time.sleep(0.001)
@@ -444,9 +499,19 @@ class LLM:
                     elif not free_rows or self.allocator.num_free == 0:
                         break
                 # Phase 3: prefill the admitted prompts, sample their first token
-                if new:
-                    sampled = self._sample_step(new, self._prefill(new), new[0].req.temperature)
-                    for s, tok in zip(new, sampled):
+                # (with prefill_chunk: a chunk of those being prefilled, and the first
+                # tokens of the prompts that it ends)
+                filling += new
+                ended: list[_Seq] = []
+                if filling:
+                    if self.prefill_chunk is None:
+                        logits, ended, filling = self._prefill(filling), filling, []
+                    else:
+                        logits, ended = self._prefill_chunk(filling)
+                        filling = [s for s in filling if s.filled < len(s.req.token_ids[s.prompt_idx])]
+                if ended:
+                    sampled = self._sample_step(ended, logits, ended[0].req.temperature)
+                    for s, tok in zip(ended, sampled):
                         s.tokens.append(tok)
                         if 1 >= s.req.max_tokens or (not s.req.ignore_eos
                                                      and tok == self.config.eos_token_id):
@@ -475,7 +540,7 @@ class LLM:
                 h = self._sample_ahead(len(seqs), temp, top)
                 while True:
                     ahead = None
-                    if self._request_queue.empty() and (not pending or not free_rows):
+                    if self._request_queue.empty() and not filling and (not pending or not free_rows):
                         self._step_ahead(len(seqs))
                         ahead = self._sample_ahead(len(seqs), temp, top)
                     finished = self._retire(seqs, self._tokens(h, seqs), active, free_rows)
@@ -486,7 +551,7 @@ class LLM:
                         self._retire(seqs, self._tokens(h, seqs), active, free_rows)
                         break
         except BaseException as e:  # surface failures to every waiting caller
-            for s in active.values():
+            for s in (*active.values(), *filling):
                 if not s.req.future.done():
                     s.req.future.set_exception(e)
             for req in pending:

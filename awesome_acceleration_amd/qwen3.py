@@ -36,6 +36,7 @@ from . import fused as fz
 from . import kv4
 from . import kv_transfer
 from . import paged
+from . import rotary
 
 __all__ = ["Qwen3Config", "Qwen3ForCausalLM", "PagedKVCache", "PagedKV4Cache", "StepMeta"]
 
@@ -55,7 +56,10 @@ LM_HEAD_ROWS = 8
 
 @dataclass
 class Qwen3Config:
-    """Same fields and defaults as the reference's Qwen3Config (model/model.py:13-37)."""
+    """Same fields and defaults as the reference's Qwen3Config (model/model.py:13-37), and
+    ``rope_scaling``: the rule for long contexts as a configuration file holds it
+    (``rotary.scaled_frequencies``; ``original_max_position_embeddings`` defaults to
+    ``max_position_embeddings``)."""
     vocab_size: int = 151936
     hidden_size: int = 1024
     intermediate_size: int = 3072
@@ -70,6 +74,7 @@ class Qwen3Config:
     tie_word_embeddings: bool = True
     bos_token_id: int = 151643
     eos_token_id: int = 151645
+    rope_scaling: dict | None = None
 
     @classmethod
     def from_json(cls, path: str):
@@ -89,16 +94,25 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
 
 class Rope:
     """cos/sin tables in the activation dtype (model/model.py:64-78), indexed
-    by position on the device."""
+    by position on the device.  With ``scaling`` (a ``rope_scaling`` rule) they are
+    ``rotary.RotaryEmbedding``'s, of ``factor`` times the original context's positions."""
 
-    def __init__(self, head_dim: int, max_pos: int, theta: float, device, dtype):
+    def __init__(self, head_dim: int, max_pos: int, theta: float, device, dtype, scaling=None):
+        self.half = head_dim // 2
+        if scaling and scaling.get("rope_type", scaling.get("type", "default")) != "default":
+            rule = dict(scaling)
+            if rule.get("original_max_position_embeddings") is None:
+                rule["original_max_position_embeddings"] = max_pos
+            n = max(max_pos, int(float(rule.get("factor") or 1) * rule["original_max_position_embeddings"]))
+            scaled = rotary.RotaryEmbedding(head_dim, theta, rule, seq_len=n, device=device)
+            self.cos, self.sin = (torch.cat((t, t), -1) for t in scaled.cos_sin(n, dtype=dtype))
+            return
         inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))
         t = torch.arange(max_pos, dtype=torch.float32)
         freqs = torch.outer(t, inv)
         emb = torch.cat((freqs, freqs), dim=-1)
         self.cos = emb.cos().to(device=device, dtype=dtype)
         self.sin = emb.sin().to(device=device, dtype=dtype)
-        self.half = head_dim // 2
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """x [T, H, D], positions [T] -> x*cos + rotate_half(x)*sin (model/model.py:86-99)."""
@@ -197,7 +211,10 @@ class StepMeta:
     """Device-side metadata of one forward pass.
 
     prefill: ``cu_seqlens`` int32 [n+1], ``positions`` int64 [N],
-             ``slot_mapping`` int64 [N], ``max_seqlen``, ``last_idx`` int64 [n]
+             ``slot_mapping`` int64 [N], ``max_seqlen``, ``last_idx`` int64 (the
+             rows whose logits are wanted); for chunks of prompts, part of which is in
+             the cache, also ``block_tables``, ``context_lens`` (cached + new) and
+             ``max_context_len``
     decode:  ``positions`` int32 [B], ``block_tables`` int32 [B, W],
              ``cache_seqlens`` int32 [B] (length before this step's append),
              ``context_lens`` int32 [B] (= cache_seqlens + 1),
@@ -241,7 +258,8 @@ class Qwen3ForCausalLM:
         # up to this many sequences the residual add and RMSNorm before a
         # projection run in the projection's own launch
         self.norm_gemm_rows = NORM_GEMM_ROWS if self.small_gemm_rows and H in (512, 1024) else 0
-        self.rope = Rope(self.d, cfg.max_position_embeddings, cfg.rope_theta, self.device, dtype)
+        self.rope = Rope(self.d, cfg.max_position_embeddings, cfg.rope_theta, self.device, dtype,
+                         cfg.rope_scaling)
 
     @torch.no_grad()
     def init_weights(self, seed: int, std: float = 0.02):
@@ -297,6 +315,12 @@ class Qwen3ForCausalLM:
         q, k, v = self._qkv(L, x, meta.positions)
         if isinstance(cache, PagedKV4Cache):
             attn = self._attend_kv4(li, q, k, v, meta, cache, prefill)
+        elif prefill and meta.block_tables is not None:
+            # a chunk: store, then attend to the cached tokens and the new ones
+            fai.kv_store(k, v, cache.k(li), cache.v(li), meta.slot_mapping)
+            attn = fai.prefill_paged(
+                q, cache.k(li), cache.v(li), meta.cu_seqlens, meta.block_tables, meta.context_lens,
+                meta.max_seqlen, max_context_len=meta.max_context_len, softmax_scale=self.scale)
         elif prefill:
             # store K/V through slot_mapping and attend (llm.py:171-184)
             attn = fai.varlen_prefill_with_kvcache(
@@ -317,6 +341,8 @@ class Qwen3ForCausalLM:
 
     def _attend_kv4(self, li, q, k, v, meta: StepMeta, cache: PagedKV4Cache, prefill: bool):
         if prefill:
+            if meta.block_tables is not None:
+                raise RuntimeError("chunks of prompts need the 16-bit cache")
             kv4.kv4_store(k, v, cache.layer(li), meta.slot_mapping)
             return fai.flash_attn_varlen_func(q, k, v, meta.cu_seqlens, meta.cu_seqlens,
                                               meta.max_seqlen, meta.max_seqlen,
@@ -362,6 +388,8 @@ class Qwen3ForCausalLM:
                     qkv = lin(x, L["qkv"])
             if prefill:
                 if four:
+                    if meta.block_tables is not None:
+                        raise RuntimeError("chunks of prompts need the 16-bit cache")
                     q, k = kv4.qk_norm_rope_store_kv4(
                         qkv, self.hq, L["q_norm"], L["k_norm"], eps, self.rope.cos, self.rope.sin,
                         pos, cache.layer(li), slot_mapping=meta.slot_mapping)
@@ -369,10 +397,16 @@ class Qwen3ForCausalLM:
                     q, k = fz.qk_norm_rope_store(
                         qkv, self.hq, self.hkv, L["q_norm"], L["k_norm"], eps, self.rope.cos,
                         self.rope.sin, pos, cache.k(li), cache.v(li), slot_mapping=meta.slot_mapping)
-                v = qkv[:, self.q_size + self.kv_size:].view(T, self.hkv, self.d)
-                attn = fai.flash_attn_varlen_func(q, k, v, meta.cu_seqlens, meta.cu_seqlens,
-                                                  meta.max_seqlen, meta.max_seqlen,
-                                                  softmax_scale=self.scale, causal=True)
+                if meta.block_tables is not None:  # a chunk: its own keys are in the cache too
+                    attn = fai.prefill_paged(
+                        q, cache.k(li), cache.v(li), meta.cu_seqlens, meta.block_tables,
+                        meta.context_lens, meta.max_seqlen, max_context_len=meta.max_context_len,
+                        softmax_scale=self.scale)
+                else:
+                    v = qkv[:, self.q_size + self.kv_size:].view(T, self.hkv, self.d)
+                    attn = fai.flash_attn_varlen_func(q, k, v, meta.cu_seqlens, meta.cu_seqlens,
+                                                      meta.max_seqlen, meta.max_seqlen,
+                                                      softmax_scale=self.scale, causal=True)
             elif four:
                 q, _ = kv4.qk_norm_rope_store_kv4(
                     qkv, self.hq, L["q_norm"], L["k_norm"], eps, self.rope.cos, self.rope.sin, pos,
@@ -411,6 +445,8 @@ class Qwen3ForCausalLM:
             else:
                 delta = F.linear(fz.silu_mul(F.linear(x, L["gate_up"])), L["down"])
         if prefill:
+            if meta.last_idx.shape[0] == 0:  # chunks of which none ends its prompt
+                return self.embed.new_empty((0, self.embed.shape[0]))
             delta, res = delta[meta.last_idx], res[meta.last_idx]
         h, _ = fz.rmsnorm(delta, self.norm, eps, residual=res)
         # tied embeddings

@@ -132,3 +132,11 @@ def test_scaling_refusals():
         rotary.RotaryEmbedding(8, device="cpu")
     with pytest.raises(RuntimeError, match="GPU"):
         rotary.apply_rotary_emb(torch.zeros(1, 1, 1, 8), torch.zeros(1, 4), torch.zeros(1, 4))
+
+
+def test_engine_refuses_a_chunk_of_no_tokens_and_chunks_with_the_4_bit_cache():
+    from awesome_acceleration_amd.llm import LLM
+    for a in (dict(prefill_chunk=0), dict(prefill_chunk=-3), dict(prefill_chunk=2.5),
+              dict(prefill_chunk=64, kv_cache_dtype="mxfp4")):
+        with pytest.raises(ValueError, match="prefill_chunk"):
+            LLM(**a)
