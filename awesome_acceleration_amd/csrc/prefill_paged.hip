@@ -17,8 +17,7 @@
 // buffer resource that ends at the context: rows behind it, whatever the page holds,
 // arrive as zeros.  Other block sizes look every row up in its lane (PAGE16 false).
 //
-// Too few workgroups for the GPU: the keys are split into pieces too, whose partial
-// results (fp32) a second kernel joins in piece order.
+// Few or uneven sequences: the workgroups share the work out evenly (below).
 
 #include <algorithm>
 
@@ -53,10 +52,16 @@ struct Args {
   int32_t row_bytes;    // of a cache row, all heads
   float scale_log2;
   int32_t n_rb;         // row blocks of the longest sequence
-  int32_t n_split;      // pieces of the keys at most
-  int32_t min_sub;      // sub-tiles of a piece at least
-  float* ws_o;          // [n_tokens][hq][n_split][128]
-  float2* ws_ml;        // [n_tokens][hq][n_split]
+  float* ws_o;          // shared work: [workgroup][2][row blocks][4][4][64 lanes][4]
+  float2* ws_ml;        // [workgroup][2][row blocks][32]
+  struct Cut* ws_cut;   // [workgroup]
+};
+
+// The item at the start of a share, for the kernel that joins its parts: those of shares
+// first to last, where they are two or more and this is the item's first cut; share
+// `opens` holds its beginning.
+struct Cut {
+  int first, last, opens, row0, rows, q_beg, unused[2];
 };
 
 // x / d for x < 2^27: x * ceil(2^(27 + s) / d) >> (27 + s), s = ceil(log2 d).
@@ -87,13 +92,9 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int s) {
   return r;
 }
 
-// The keys [0, end) that rows up to `row` see, and the pieces they are cut into.
+// The keys [0, end) that rows up to `row` see.
 template <bool CAUSAL> __device__ __forceinline__ int end_of(const Args& a, const Seq& s, int row) {
   return CAUSAL ? max(row / a.group + 1 + (s.Lk - s.Lq), 0) : s.Lk;
-}
-__device__ __forceinline__ int pieces_of(const Args& a, int end) {
-  const int nsub = (end + 31) / 32;
-  return max(1, min(a.n_split, nsub / a.min_sub));
 }
 
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
@@ -102,11 +103,12 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 // 1 KiB straight into LDS (dst + 16 lane); inline assembly, so that the compiler neither
 // counts it nor guards LDS reads with waits for it: the waits are explicit.  M0 is used
-// by nothing else here.
+// by nothing else here.  (s_nop 4: should a vector instruction, such as the restoring of a
+// spilled register, have written the resource right before, the load may read it.)
 __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, int voff, u32 dst) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :
                : "v"(voff), "s"(r), "s"(dst)
                : "memory", "m0");
@@ -131,6 +133,14 @@ template <bool F16> __device__ __forceinline__ u32 finite16(u32 x) {
 // 0x8000 -> 0xffff, 0 -> 0 in each half
 __device__ __forceinline__ u32 spread16(u32 t) { return (t - (t >> 15)) | t; }
 
+// min(max(end - key, 0), 16) in scalar registers, where the compiler would take a vector
+// instruction for the clamp and the buffer resource could not be built.
+__device__ __forceinline__ int rows_left(int end, int key) {
+  int n;
+  asm("s_sub_i32 %0, %1, %2\n\ts_max_i32 %0, %0, 0\n\ts_min_i32 %0, %0, 16" : "=&s"(n) : "s"(end), "s"(key) : "scc");
+  return n;
+}
+
 // At most N of this wave's loads are in flight and its LDS reads are done, then the
 // workgroup's.
 template <int N> __device__ __forceinline__ void landed_barrier() {
@@ -153,13 +163,101 @@ template <int R_, int SL_, int KT_, int STAGES_> struct Shape {
   static constexpr int kBody = kRing > kPart + kMl ? kRing : kPart + kMl;
   static constexpr int kLds = kBody > kOut ? kBody : kOut;
   static_assert(2 * kKeys % (16 * kWaves) == 0, "whole groups a wave");
+  static constexpr int kRows = 32 * R;
+  // shared work, in iterations: what an item's start, merge and output cost, and the
+  // least a workgroup takes
+  static constexpr int kStart = R == 8 ? 2 : 3, kLeast = 6;
 };
 
-template <class S, bool CAUSAL, bool F16, bool PAGE16>
+// Shared work.  Where the items (row block, sequence, KV head) are few or uneven, the
+// workgroups of a head divide its iterations evenly instead: the items' iterations, with
+// kStart more for each, follow each other on a line, cut into equal shares.  A share is
+// the end of one item, whole items, and the start of another; an item that is cut leaves
+// partial results, which a second kernel joins in the order of the line.
+constexpr int kMaxSharedSeqs = 1024;
+
+struct Line {  // of one KV head: pre[s] is where sequence s begins
+  int total, share;
+};
+struct Item {
+  int sg, row0, end, n_it;  // sequence, first row, keys its rows see, iterations of them
+  int begin, units;         // its place on the line
+  Seq sq;
+  int rows;
+};
+
+template <class S, bool CAUSAL> __device__ __forceinline__ int units_of(const Args& a, const Seq& sq, int& per) {
+  const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
+  // (the row block with the most keys stands for all of its sequence)
+  per = (rows > 0 ? (end_of<CAUSAL>(a, sq, rows - 1) + S::kKeys - 1) / S::kKeys : 0) + S::kStart;
+  return min((rows + S::kRows - 1) / S::kRows, a.n_rb) * per;
+}
+
+// pre[0 .. n_seqs] in LDS, by NT threads; tmp: one value a wave.
+template <class S, bool CAUSAL, int NT>
+__device__ __forceinline__ Line line_of(const Args& a, int* pre, int* tmp, int n_shares) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (a.n_seqs + NT - 1) / NT, s0 = min(tid * each, a.n_seqs), s1 = min(s0 + each, a.n_seqs);
+  int sum = 0, per;
+  for (int s = s0; s < s1; ++s) sum += units_of<S, CAUSAL>(a, seq_of(a, s), per);
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o);
+    upto += lane >= o ? x : 0;
+  }
+  if (lane == 63) tmp[wave] = upto;
+  __syncthreads();
+  int at = upto - sum;
+  for (int w = 0; w < wave; ++w) at += tmp[w];
+  for (int s = s0; s < s1; ++s) {
+    pre[s] = at;
+    at += units_of<S, CAUSAL>(a, seq_of(a, s), per);
+  }
+  if (tid == NT - 1) pre[a.n_seqs] = at;
+  __syncthreads();
+  Line l;
+  l.total = __builtin_amdgcn_readfirstlane(pre[a.n_seqs]);
+  l.share = max((l.total + n_shares - 1) / n_shares, S::kLeast);
+  return l;
+}
+
+// The item at unit u of the line, u < total.
+template <class S, bool CAUSAL> __device__ __forceinline__ Item item_at(const Args& a, const int* pre, int u) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = a.n_seqs;
+  while (n > 1) {  // the last s with pre[s] <= u, 64 bounds a step
+    const int step = (n + 63) / 64, at = lane * step;
+    const int hits = __popcll(__ballot(at < n && pre[lo + min(at, n - 1)] <= u));
+    lo += (hits - 1) * step;
+    n = min(step, n - (hits - 1) * step);
+  }
+  Item it;
+  it.sg = __builtin_amdgcn_readfirstlane(lo);
+  const int begin = __builtin_amdgcn_readfirstlane(pre[lo]);
+  it.sq = seq_of(a, it.sg);
+  it.rows = it.sq.Lq * a.group;
+  const int nrb = min((it.rows + S::kRows - 1) / S::kRows, a.n_rb);
+  units_of<S, CAUSAL>(a, it.sq, it.units);
+  const int z = (u - begin) / it.units;
+  it.begin = begin + z * it.units;
+  // causal row blocks: the ones with most and least keys in turn
+  it.row0 = (z & 1 ? z >> 1 : nrb - 1 - (z >> 1)) * S::kRows;
+  it.end = __builtin_amdgcn_readfirstlane(end_of<CAUSAL>(a, it.sq, min(it.row0 + S::kRows, it.rows) - 1));
+  it.n_it = (it.end + S::kKeys - 1) / S::kKeys;
+  return it;
+}
+// Units [x0, x1) of an item as its iterations.
+template <class S> __device__ __forceinline__ int iteration_of(const Item& it, int x) {
+  return min(max(x - S::kStart, 0), it.n_it);
+}
+
+template <class S, bool CAUSAL, bool F16, bool PAGE16, bool SHARED>
 __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_paged_kernel(Args a) {
   typedef pf::Mfma<F16> M;
-  constexpr int SL = S::SL, KT = S::KT, STAGES = S::STAGES;
+  constexpr int SL = S::SL, KT = S::KT, STAGES = S::STAGES, kRows = S::kRows;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
+  __shared__ int pre[SHARED ? kMaxSharedSeqs + 1 + S::kWaves : 1];
   const u32 lds0 = (u32)(uintptr_t)(lds_u8*)lds;
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -167,28 +265,68 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
   const int rb_w = wave % S::R, sl = wave / S::R;  // row block of the workgroup, key slice
   const int hl = lane >> 5, col = lane & 31;
 
-  // items: KV head fastest (one XCD per head when there are eight), the pieces and row
-  // blocks of a sequence together, the causal ones with the most keys first
-  int it = blockIdx.x;
-  const int h = it % a.hkv;
-  it /= a.hkv;
-  const int piece = it % a.n_split;
-  it /= a.n_split;
-  const int z = it % a.n_rb, sg = it / a.n_rb;
-  const Seq sq = seq_of(a, sg);
-  const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
-  constexpr int kRows = 32 * S::R;
-  const int nrb = (rows + kRows - 1) / kRows;
-  if (z >= nrb) return;  // workgroup-uniform
-  const int row0 = (min(nrb, a.n_rb) - 1 - z) * kRows;  // the workgroup's first row
-  const int kv_end = __builtin_amdgcn_readfirstlane(end_of<CAUSAL>(a, sq, min(row0 + kRows, rows) - 1));
-  const int np = pieces_of(a, kv_end);
-  if (piece >= np) return;
-  const int nsub_all = (kv_end + 31) / 32;
-  // the piece's sub-tiles [j0, j1)
-  const int per = nsub_all / np, more = nsub_all - per * np;
-  const int j0 = piece * per + min(piece, more), j1 = j0 + per + (piece < more ? 1 : 0);
-  const int n_it = (j1 - j0 + SL * KT - 1) / (SL * KT);
+  // KV head fastest: one XCD per head when there are eight
+  const int h = blockIdx.x % a.hkv;
+  Item item;
+  int unit = 0, unit_end = 0;
+  if constexpr (SHARED) {
+    const Line l = line_of<S, CAUSAL, S::kThreads>(a, pre, pre + kMaxSharedSeqs + 1, gridDim.x / a.hkv);
+    unit = (int)(blockIdx.x / a.hkv) * l.share;
+    unit_end = min(unit + l.share, l.total);
+    // Whether the share starts inside an item, for the joining kernel
+    Cut cut = {0, -1};
+    if (unit < unit_end) {
+      const int w = (int)(blockIdx.x / a.hkv);
+      const Item it = item_at<S, CAUSAL>(a, pre, unit);
+      if (unit > it.begin && unit - l.share <= it.begin) {
+        // shares whose iterations of it are not none: all but perhaps its ends
+        const int head = min(l.share * w, it.begin + it.units) - it.begin, last = (it.begin + it.units - 1) / l.share;
+        cut.first = iteration_of<S>(it, head) > 0 ? w - 1 : w;
+        cut.last = w - 1;
+        for (int x = w; x <= last && iteration_of<S>(it, x * l.share - it.begin) < it.n_it; ++x)
+          if (iteration_of<S>(it, (x + 1) * l.share - it.begin) > 0) cut.last = x;
+        cut.opens = w - 1;
+        cut.row0 = it.row0;
+        cut.rows = it.rows;
+        cut.q_beg = it.sq.q_beg;
+      }
+    }
+    if (tid == 0) a.ws_cut[blockIdx.x] = cut;
+    if (unit >= unit_end) return;  // workgroup-uniform
+  } else {
+    // an item a workgroup: the row blocks of a sequence together, the causal ones with
+    // the most keys first
+    const int i = blockIdx.x / a.hkv, z = i % a.n_rb;
+    item.sg = i / a.n_rb;
+    item.sq = seq_of(a, item.sg);
+    item.rows = item.sq.Lq > 0 ? item.sq.Lq * a.group : 0;
+    const int nrb = min((item.rows + kRows - 1) / kRows, a.n_rb);
+    if (z >= nrb) return;  // workgroup-uniform
+    item.row0 = (nrb - 1 - z) * kRows;
+    item.end = __builtin_amdgcn_readfirstlane(end_of<CAUSAL>(a, item.sq, min(item.row0 + kRows, item.rows) - 1));
+    item.n_it = (item.end + S::kKeys - 1) / S::kKeys;
+  }
+  for (;;) {
+  int i0 = 0, i1, slot = -1;  // iterations, place of a partial result
+  if constexpr (SHARED) {
+    if (unit >= unit_end) break;
+    item = item_at<S, CAUSAL>(a, pre, unit);
+    const int x0 = unit - item.begin, x1 = min(item.units, unit_end - item.begin);
+    unit = item.begin + x1;
+    i0 = __builtin_amdgcn_readfirstlane(iteration_of<S>(item, x0));
+    i1 = __builtin_amdgcn_readfirstlane(iteration_of<S>(item, x1));
+    // no iteration here (an item of none at all: its zeros are the first share's)
+    if (item.n_it == 0 ? x0 > 0 : i0 == i1) continue;
+    // cut: only a share's first item can have begun before it, only its last go on
+    if (i1 - i0 < item.n_it) slot = 2 * (int)blockIdx.x + (x0 > 0 ? 0 : 1);
+  } else {
+    i1 = item.n_it;
+  }
+  const Seq& sq = item.sq;
+  const int sg = item.sg, rows = item.rows, row0 = item.row0, kv_end = item.end;
+  // sub-tiles [j0, j1) of 32 keys
+  const int j0 = i0 * SL * KT, j1 = min(i1 * SL * KT, (kv_end + 31) / 32);
+  const int n_it = i1 - i0;
 
   // this wave's and lane's rows
   const int wrow = row0 + 32 * rb_w;
@@ -234,7 +372,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
         const int64_t blk = (u32)ent[gi] < a.num_blocks ? ent[gi] : 0;
         const int64_t row = blk * a.block_size + (key - page * a.block_size);
         // (the head's 256 bytes of a row lie before the next row's)
-        const int n_rows = min(16, kv_end - min(key, kv_end));
+        const int n_rows = rows_left(kv_end, key);
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<u16*>(cache + row * (u32)(a.row_bytes >> 1)), 0, n_rows * a.row_bytes, 0x00020000);
 #pragma unroll
@@ -469,22 +607,19 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
       }
   }
 
-  const int64_t orow = (int64_t)(sq.q_beg + my_q);
-  const bool real = wrow + col < rows;
-  if (np > 1) {  // a piece: unnormalised, in fp32
-    if (!real) return;
-    const int64_t slot = (orow * a.hq + my_head) * a.n_split + piece;
-    if (sl == 0 && hl == 0) a.ws_ml[slot] = make_float2(mt * cs, lt);
-    float* dst = a.ws_o + slot * D;
+  if (slot >= 0) {  // a part of the item: unnormalised, in fp32, as the lanes hold it
+    const int at = slot * S::R + rb_w;
+    if (sl == 0 && hl == 0) a.ws_ml[(int64_t)at * 32 + col] = make_float2(mt * cs, lt);
+    f32x4* dst = reinterpret_cast<f32x4*>(a.ws_o) + (int64_t)at * 1024 + lane;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
       if (SL == 1 || db * SL / 4 == sl) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * r + 4 * hl) =
-              f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
+          dst[(4 * db + r) * 64] = f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
       }
-    return;
+    __syncthreads();  // the next item's loads overwrite what the merge read
+    continue;
   }
   const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : (lt == 0.f ? 0.f : lt);  // (a NaN stays one)
   if constexpr (SL > 1) __syncthreads();  // the partial results have been read
@@ -510,89 +645,122 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
                               (h * a.group + row - qi * a.group) * D + (lane & 15) * 8) =
         *reinterpret_cast<const u32x4*>(lds + (r >> 5) * (32 * kOutPitch) + (r & 31) * kOutPitch + (lane & 15) * 16);
   }
+  if constexpr (!SHARED) break;
+  __syncthreads();
+  }
 }
 
-// Joins the pieces of a row, in piece order: a wave a row, two dims a lane.
-template <bool CAUSAL, bool F16, int ROWS>
+// Joins the parts of a cut item, in the line's order: workgroup (x, y) those of cut x, row
+// block y of 32, a wave 32 dims, in the layout the parts' waves left them.
+template <class S, bool F16>
 __global__ __launch_bounds__(256) void prefill_paged_join_kernel(Args a) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y;
-  for (int sg = blockIdx.z; sg < a.n_seqs; sg += gridDim.z) {
-    const Seq sq = seq_of(a, sg);
-    const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
-    if (row >= rows) continue;
-    const int last = min((row / ROWS + 1) * ROWS, rows) - 1;
-    const int np = pieces_of(a, end_of<CAUSAL>(a, sq, last));
-    if (np == 1) continue;  // written by its workgroup
-    const int qi = row / a.group, head = h * a.group + row - qi * a.group;
-    const int64_t slot = ((int64_t)(sq.q_beg + qi) * a.hq + head) * a.n_split;
-    float mx = -3e38f;
-    for (int p = 0; p < np; ++p) mx = vmax(mx, a.ws_ml[slot + p].x);
-    float o0 = 0.f, o1 = 0.f, lt = 0.f;
-    for (int p = 0; p < np; ++p) {
-      const float2 ml = a.ws_ml[slot + p];
-      const float2 v = *reinterpret_cast<const float2*>(a.ws_o + (slot + p) * D + 2 * lane);
-      const float w = fast_exp2(ml.x - mx);
-      lt = fmaf(ml.y, w, lt);
-      o0 = fmaf(v.x, w, o0);
-      o1 = fmaf(v.y, w, o1);
+  const Cut c = a.ws_cut[blockIdx.x + a.hkv];  // (share 0 of a head begins no cut)
+  const int h = blockIdx.x % a.hkv, rb = blockIdx.y, lane = threadIdx.x & 63, hl = lane >> 5, col = lane & 31;
+  if (c.first >= c.last || c.row0 + 32 * rb >= c.rows) return;
+  const int db = threadIdx.x >> 6;
+  auto place_of = [&](int w) { return (int64_t)(2 * (w * a.hkv + h) + (w == c.opens ? 1 : 0)) * S::R + rb; };
+  float mx = -3e38f, lt = 0.f;
+#pragma unroll 4
+  for (int w = c.first; w <= c.last; ++w) mx = vmax(mx, a.ws_ml[place_of(w) * 32 + col].x);
+  f32x4 acc[4] = {};
+#pragma unroll 2
+  for (int w = c.first; w <= c.last; ++w) {
+    const int64_t at = place_of(w);
+    const float2 ml = a.ws_ml[at * 32 + col];
+    const f32x4* src = reinterpret_cast<const f32x4*>(a.ws_o) + at * 1024 + 256 * db + lane;
+    const float wt = fast_exp2(ml.x - mx);
+    lt = fmaf(ml.y, wt, lt);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 v = src[64 * r];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(v[e], wt, acc[r][e]);
     }
-    const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : (lt == 0.f ? 0.f : lt);
-    *reinterpret_cast<u32*>(a.out + (int64_t)(sq.q_beg + qi) * a.o_stride + head * D + 2 * lane) =
-        pf::Mfma<F16>::pack(o0 * inv, o1 * inv);
+  }
+  const int row = c.row0 + 32 * rb + col;
+  if (row >= c.rows) return;
+  const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : (lt == 0.f ? 0.f : lt);
+  const int qi = row / a.group, head = h * a.group + row - qi * a.group;
+  u16* out = a.out + (int64_t)(c.q_beg + qi) * a.o_stride + head * D + 32 * db + 4 * hl;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    u32x2 w;
+    w[0] = pf::Mfma<F16>::pack(acc[r][0] * inv, acc[r][1] * inv);
+    w[1] = pf::Mfma<F16>::pack(acc[r][2] * inv, acc[r][3] * inv);
+    *reinterpret_cast<u32x2*>(out + 8 * r) = w;
   }
 }
 
 // ------------------------------------------------------------------ host
-typedef Shape<1, 4, 1, 2> Rows32;
 typedef Shape<2, 4, 1, 2> Rows64;
 typedef Shape<4, 2, 1, 4> Rows128;
 typedef Shape<8, 1, 2, 4> Rows256;
 
 struct Plan {
-  int rows;  // of a workgroup: 32, 64, 128 or 256
-  int n_split, min_sub;
+  int rows;    // of a workgroup: 64, 128 or 256
+  int shares;  // of a KV head's work, or 0: an item a workgroup
   size_t bytes;
 };
 
-static Plan plan(int64_t n_tokens, int32_t n_seqs, int32_t max_q, int32_t max_k, int32_t hq, int32_t hkv, int n_cu) {
+static Plan plan(int32_t n_seqs, int32_t max_q, int32_t max_k, int64_t cap, int32_t hq, int32_t hkv, int n_cu) {
   Plan p = {};
   const int64_t rows = (int64_t)max_q * (hq / hkv);
-  p.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-  const int64_t items = (int64_t)n_seqs * hkv * cdiv(rows, p.rows);
-  // as many pieces as fill the GPU once, of eight sub-tiles (256 keys) at least
-  p.min_sub = 8;
-  const int64_t nsub = cdiv(max_k, 32);
-  p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / std::max<int64_t>(items, 1), nsub / p.min_sub));
-  if (p.n_split > 1) p.bytes = (size_t)n_tokens * hq * p.n_split * (D * 4 + 8);
+  auto items_of = [&](int r) { return (int64_t)n_seqs * hkv * cdiv(rows, r); };
+  // Rows of a workgroup, us in 64 / 128 / 256 of them.  Where one block holds a sequence's
+  // rows the keys are what it costs: 16 x 5 queries over 1.5k keys at 16/8 heads 22.8 / 30.6
+  // / 32.2, 64 x 4 over 4k at 32/8 190 / 185 / 186.  Short contexts of few items are a chain
+  // of latencies, shortest in small blocks that do not outnumber the CUs: 1 x 97 over 98
+  // 8.4 / 9.3 / 10.3, 11 x 64 over 171 at 32/8 18.2 / 11.3 / 13.6, 6 x 306 at 32/8 34.7 / 24.2
+  // / 19.4.  Else every key a workgroup brings in serves more rows in large ones: 2 x 265
+  // over 8.9k at 64/8 247 / 206 / 184, 26 x 1301 over 1.8k 624 / 450 / 388.
+  if (rows <= 64) p.rows = items_of(64) < n_cu ? 64 : 128;
+  else if (max_k <= 1024 && items_of(64) <= n_cu) p.rows = 64;
+  else if (rows <= 128 || (max_k <= 1024 && items_of(128) <= n_cu)) p.rows = 128;
+  else p.rows = 256;
+  const int64_t items = items_of(p.rows);
+  const int64_t keys = p.rows == 64 ? 128 : 64, its = cdiv(max_k, keys), start = p.rows == 256 ? 2 : 3;
+  // In iterations of a workgroup, if all sequences were as long as the longest: an item a
+  // workgroup takes whole rounds of the longest; shared work its even part, and some 8
+  // for finding it and joining.  (Uneven sequences only make the first worse.)
+  const int64_t alone = cdiv(items, n_cu) * (its + start), shared = items * (its + 2 * start) / n_cu + 8;
+  // units of a line below 2^30
+  const bool fits = n_seqs <= kMaxSharedSeqs && hkv <= n_cu &&
+                    cdiv(rows, p.rows) * n_seqs * (cdiv(cap, keys) + start) < (int64_t(1) << 30);
+  if (fits && items < 8 * (int64_t)n_cu && 20 * shared < 21 * alone) {
+    p.shares = n_cu / hkv;
+    p.bytes = (size_t)p.shares * hkv * (2 * p.rows * (D * 4 + 8) + sizeof(Cut));
+  }
   return p;
 }
 
 template <class S, bool CAUSAL, bool F16>
-static int launch_s(Args a, bool page16, int32_t max_q, int32_t, hipStream_t st) {
-  const int64_t rows = (int64_t)max_q * a.group;
-  a.n_rb = (int)cdiv(rows, 32 * S::R);
-  const int64_t grid = (int64_t)a.n_seqs * a.n_rb * a.n_split * a.hkv;
+static int launch_s(Args a, const Plan& p, bool page16, int32_t max_q, hipStream_t st) {
+  a.n_rb = (int)cdiv((int64_t)max_q * a.group, S::kRows);
+  const dim3 block(S::kThreads);
+  if (p.shares) {
+    const unsigned grid = (unsigned)p.shares * a.hkv;
+    a.ws_ml = (float2*)(a.ws_o + (size_t)grid * 2 * S::kRows * D);
+    a.ws_cut = (Cut*)(a.ws_ml + (size_t)grid * 2 * S::kRows);
+    if (page16) hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true, true>), dim3(grid), block, 0, st, a);
+    else hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false, true>), dim3(grid), block, 0, st, a);
+    if (p.shares > 1)
+      hipLaunchKernelGGL((prefill_paged_join_kernel<S, F16>),
+                         dim3((unsigned)(p.shares - 1) * a.hkv, S::R), dim3(256), 0, st, a);
+    return AAC_OK;
+  }
+  const int64_t grid = (int64_t)a.n_seqs * a.n_rb * a.hkv;
   if (grid >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
-  if (page16)
-    hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true>), dim3((unsigned)grid), dim3(S::kThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false>), dim3((unsigned)grid), dim3(S::kThreads), 0, st, a);
-  if (a.n_split > 1)
-    hipLaunchKernelGGL((prefill_paged_join_kernel<CAUSAL, F16, 32 * S::R>),
-                       dim3((unsigned)cdiv(rows, 4), (unsigned)a.hkv, (unsigned)std::min(a.n_seqs, 65535)), dim3(256), 0,
-                       st, a);
+  if (page16) hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true, false>), dim3((unsigned)grid), block, 0, st, a);
+  else hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false, false>), dim3((unsigned)grid), block, 0, st, a);
   return AAC_OK;
 }
 
 template <bool CAUSAL, bool F16>
-static int launch_r(const Args& a, const Plan& p, bool page16, int32_t max_q, int32_t max_k, hipStream_t st) {
+static int launch_r(const Args& a, const Plan& p, bool page16, int32_t max_q, hipStream_t st) {
   switch (p.rows) {
-    case 32: return launch_s<Rows32, CAUSAL, F16>(a, page16, max_q, max_k, st);
-    case 64: return launch_s<Rows64, CAUSAL, F16>(a, page16, max_q, max_k, st);
-    case 128: return launch_s<Rows128, CAUSAL, F16>(a, page16, max_q, max_k, st);
-    default: return launch_s<Rows256, CAUSAL, F16>(a, page16, max_q, max_k, st);
+    case 64: return launch_s<Rows64, CAUSAL, F16>(a, p, page16, max_q, st);
+    case 128: return launch_s<Rows128, CAUSAL, F16>(a, p, page16, max_q, st);
+    default: return launch_s<Rows256, CAUSAL, F16>(a, p, page16, max_q, st);
   }
 }
 
@@ -618,8 +786,8 @@ extern "C" size_t aac_prefill_paged_workspace_bytes(int64_t n_tokens, int32_t n_
   if (n_tokens <= 0 || n_seqs <= 0 || max_seqlen_q <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
       n_q_heads % n_kv_heads || block_size <= 0 || max_blocks_per_seq <= 0 || device_cu_count(&n_cu) != AAC_OK)
     return 0;
-  const int32_t max_k = longest_of(max_context_len, capacity_of(block_size, max_blocks_per_seq));
-  return pp::plan(n_tokens, n_seqs, max_seqlen_q, max_k, n_q_heads, n_kv_heads, n_cu).bytes;
+  const int64_t cap = capacity_of(block_size, max_blocks_per_seq);
+  return pp::plan(n_seqs, max_seqlen_q, longest_of(max_context_len, cap), cap, n_q_heads, n_kv_heads, n_cu).bytes;
 }
 
 extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, const void* k_cache,
@@ -690,22 +858,18 @@ extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_
   int n_cu = 0;
   int rc = device_cu_count(&n_cu);
   if (rc != AAC_OK) return rc;
-  const int32_t max_k = longest_of(max_context_len, cap);
-  const pp::Plan p = pp::plan(n_tokens, n_seqs, max_seqlen_q, max_k, n_q_heads, n_kv_heads, n_cu);
-  a.n_split = p.n_split;
-  a.min_sub = p.min_sub;
+  const pp::Plan p = pp::plan(n_seqs, max_seqlen_q, longest_of(max_context_len, cap), cap, n_q_heads, n_kv_heads, n_cu);
   if (p.bytes) {
     if (!workspace || workspace_bytes < p.bytes) return AAC_ERR_WORKSPACE;
     if ((uintptr_t)workspace % 16) return AAC_ERR_MISALIGNED;
     a.ws_o = (float*)workspace;
-    a.ws_ml = (float2*)(a.ws_o + (size_t)n_tokens * n_q_heads * p.n_split * pp::D);
   }
   hipStream_t st = (hipStream_t)stream;
   const bool f16 = dtype == AAC_DTYPE_FP16;
-  if (causal) rc = f16 ? pp::launch_r<true, true>(a, p, page16, max_seqlen_q, max_k, st)
-                       : pp::launch_r<true, false>(a, p, page16, max_seqlen_q, max_k, st);
-  else rc = f16 ? pp::launch_r<false, true>(a, p, page16, max_seqlen_q, max_k, st)
-                : pp::launch_r<false, false>(a, p, page16, max_seqlen_q, max_k, st);
+  if (causal) rc = f16 ? pp::launch_r<true, true>(a, p, page16, max_seqlen_q, st)
+                       : pp::launch_r<true, false>(a, p, page16, max_seqlen_q, st);
+  else rc = f16 ? pp::launch_r<false, true>(a, p, page16, max_seqlen_q, st)
+                : pp::launch_r<false, false>(a, p, page16, max_seqlen_q, st);
   if (rc != AAC_OK) return rc;
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? AAC_OK : (int)e;

@@ -117,6 +117,16 @@ CASES = [
     ("split keys", [40], [9000], 8, 1, 64),
     ("split keys, few rows", [2, 3], [20000, 700], 4, 1, 256),
     ("split keys, many rows", [513], [6000], 2, 1, 128),
+    # the work of a head shared out over its workgroups, whatever the sequences are
+    ("shared, uneven", [300, 1, 0, 77, 130, 2, 260, 0, 19], [4000, 3000, 700, 77, 2500, 0, 3333, 5, 40], 16, 8, 64),
+    ("shared, few rows", [1, 3, 0, 7, 2] * 9, [i * 37 % 2600 for i in range(45)], 4, 2, 16),
+    ("shared, middle rows", [20, 31, 5, 32], [900, 2000, 1300, 32], 8, 4, 48),
+    ("shared, half the rows", [60, 13, 64], [3000, 2000, 1700], 4, 2, 256),
+    ("shared, group of three", [100, 40, 7], [1500, 2100, 900], 6, 2, 16),
+    ("shared, odd pages", [150, 2, 33], [1000, 1200, 900], 2, 1, 20),
+    ("shared, prompts alone", [700, 1, 1300, 90], [700, 1, 1300, 90], 4, 2, 64),
+    ("shared, hundreds of sequences", [i % 4 for i in range(300)], [i * 53 % 1500 for i in range(300)], 2, 1, 16),
+    ("more sequences than shares take", [i % 2 for i in range(1100)], [i * 7 % 1200 for i in range(1100)], 1, 1, 16),
 ]
 
 
