@@ -351,14 +351,14 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
   const int key_base = 32 * j0;
   int ent[S::kGroups];  // block numbers of the next stage's groups
   auto first_key = [&](int n, int gi) { return key_base + n * S::kKeys + 16 * ((wave * S::kGroups + gi) % kKGroups); };
-  auto look_up = [&](int n) {
+  auto look_up = [&](int n, int* ent) {
     if constexpr (PAGE16) {
 #pragma unroll
       for (int gi = 0; gi < S::kGroups; ++gi)
         ent[gi] = tab[min(divide(a, first_key(n, gi) >> 4), a.max_blocks - 1)];
     }
   };
-  auto issue = [&](int n) {
+  auto issue = [&](int n, const int* ent) {
     const u32 st = lds0 + (u32)(n % STAGES * S::kStage);
 #pragma unroll
     for (int gi = 0; gi < S::kGroups; ++gi) {
@@ -394,13 +394,6 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
       }
     }
   };
-#pragma unroll
-  for (int n = 0; n < STAGES - 1; ++n)
-    if (n < n_it) {
-      look_up(n);
-      issue(n);
-    }
-
   // Q fragments (B operand of S^T = K Q^T: lane = row)
   u32x4 qf[8];
   {
@@ -408,6 +401,16 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
 #pragma unroll
     for (int t = 0; t < 8; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
   }
+  // the first stages: all their block numbers, then all their rows
+  {
+    int first[STAGES - 1][S::kGroups];
+#pragma unroll
+    for (int n = 0; n < STAGES - 1; ++n) look_up(n, first[n]);
+#pragma unroll
+    for (int n = 0; n < STAGES - 1; ++n)
+      if (n < n_it) issue(n, first[n]);
+  }
+
   // fragment addresses within a sub-tile (see prefill_wide.hip)
   int koff[8], vo[4];
 #pragma unroll
@@ -529,13 +532,13 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
   // all loads (vmcnt 0, the others unconstrained)
   __builtin_amdgcn_s_waitcnt(0x0F70);
 
-  look_up(STAGES - 1);
+  look_up(STAGES - 1, ent);
   for (int n = 0; n < n_it; ++n) {
     if (STAGES > 2 && n + STAGES - 2 < n_it) landed_barrier<(STAGES - 2) * S::kLoads>();
     else landed_barrier<0>();
     if (n + STAGES - 1 < n_it) {
-      issue(n + STAGES - 1);
-      look_up(n + STAGES);
+      issue(n + STAGES - 1, ent);
+      look_up(n + STAGES, ent);
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
