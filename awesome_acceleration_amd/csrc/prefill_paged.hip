@@ -69,6 +69,10 @@ __device__ __forceinline__ int divide(const Args& a, int x) { return (int)(((uin
 
 struct Seq {
   int q_beg, Lq, Lk;
+  // rows of a KV head (of more queries than the call says, as many as an int holds)
+  __device__ __forceinline__ int rows(const Args& a) const {
+    return Lq > 0 ? (int)min((int64_t)Lq * a.group, (int64_t)1 << 30) : 0;
+  }
 };
 __device__ __forceinline__ Seq seq_of(const Args& a, int s) {
   typedef const int32_t __attribute__((address_space(4))) cint;  // scalar loads
@@ -187,7 +191,7 @@ struct Item {
 };
 
 template <class S, bool CAUSAL> __device__ __forceinline__ int units_of(const Args& a, const Seq& sq, int& per) {
-  const int rows = sq.Lq > 0 ? sq.Lq * a.group : 0;
+  const int rows = sq.rows(a);
   // (the row block with the most keys stands for all of its sequence)
   per = (rows > 0 ? (end_of<CAUSAL>(a, sq, rows - 1) + S::kKeys - 1) / S::kKeys : 0) + S::kStart;
   return min((rows + S::kRows - 1) / S::kRows, a.n_rb) * per;
@@ -236,7 +240,7 @@ template <class S, bool CAUSAL> __device__ __forceinline__ Item item_at(const Ar
   it.sg = __builtin_amdgcn_readfirstlane(lo);
   const int begin = __builtin_amdgcn_readfirstlane(pre[lo]);
   it.sq = seq_of(a, it.sg);
-  it.rows = it.sq.Lq * a.group;
+  it.rows = it.sq.rows(a);
   const int nrb = min((it.rows + S::kRows - 1) / S::kRows, a.n_rb);
   units_of<S, CAUSAL>(a, it.sq, it.units);
   const int z = (u - begin) / it.units;
@@ -299,7 +303,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     const int i = blockIdx.x / a.hkv, z = i % a.n_rb;
     item.sg = i / a.n_rb;
     item.sq = seq_of(a, item.sg);
-    item.rows = item.sq.Lq > 0 ? item.sq.Lq * a.group : 0;
+    item.rows = item.sq.rows(a);
     const int nrb = min((item.rows + kRows - 1) / kRows, a.n_rb);
     if (z >= nrb) return;  // workgroup-uniform
     item.row0 = (nrb - 1 - z) * kRows;
@@ -805,7 +809,7 @@ extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_
   if (head_dim != pp::D) return AAC_ERR_UNSUPPORTED;
   if (n_tokens < 0 || n_seqs < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || max_seqlen_q < 0 || num_blocks < 0 ||
       block_size <= 0 || max_blocks_per_seq <= 0 || q_tok_stride < 0 || out_tok_stride < 0 || !(scale > 0.f) ||
-      scale > 3e38f)
+      scale > 1e38f)
     return AAC_ERR_INVALID_ARGUMENT;
   if (n_q_heads % n_kv_heads || n_tokens >= (int64_t(1) << 31) ||
       (!cu_seqlens_q && n_tokens != (int64_t)n_seqs * max_seqlen_q))

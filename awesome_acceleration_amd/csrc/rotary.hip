@@ -176,7 +176,7 @@ __device__ __forceinline__ bool target_of(const Args& a, int64_t t, int lane, Pl
     p.q_at = p.seq * a.q.out_seq + p.s * a.q.out_tok;
   }
   const int64_t first = a.offsets ? a.offsets[p.seq] : a.offset0;
-  if (a.context_lens && p.s == 0 && lane == 0) a.context_lens[p.seq] = (int)first + a.k.len;
+  if (a.context_lens && p.s == 0 && lane == 0) a.context_lens[p.seq] = (int)min(first + a.k.len, (int64_t)INT32_MAX);
   const int64_t last = max(a.table_rows - 1, 0);
   p.k_pos = (int)min(max(first + p.s, (int64_t)0), last);
   p.q_pos = (int)min(max(first + p.s * a.q_step, (int64_t)0), last);

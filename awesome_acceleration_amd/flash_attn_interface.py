@@ -389,7 +389,7 @@ def _prefill_paged(q, k_cache, v_cache, cu_q, tables, ctx, cu_k, max_q, max_k, s
             or not tables.is_contiguous()):
         raise RuntimeError("block_tables must be contiguous int32 [B, max_blocks]")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = q.shape[1] * q.shape[2]
     else:
         os = _token_rows(out, "out")
@@ -682,7 +682,7 @@ def _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqle
             q = rotary.apply_rotary_emb(
                 q if causal else q.reshape(B, 1, S * Hq, D), rotary_cos, rotary_sin,
                 interleaved=interleaved, seqlen_offsets=seqlens).view(B, S, Hq, D)
-    out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.numel() == 0:
         return out
     mb = tables.shape[1]

@@ -23,6 +23,7 @@ __all__ = ["apply_rotary_emb", "rotary_append_paged", "RotaryEmbedding", "scaled
 
 
 _CODES = _lib.AAC_DTYPE
+_DENSE = torch.contiguous_format
 
 
 def _bad_dtype(dtype):
@@ -113,7 +114,7 @@ def apply_rotary_emb(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, inte
             if s == 0 and n > 1:
                 raise RuntimeError("x is broadcast: it cannot be turned in place")
     else:
-        out = torch.empty(shape, dtype=dt, device=x.device)
+        out = torch.empty_like(x, memory_format=_DENSE)
         o2 = D
         o1 = shape[-2] * D
         o0 = S * o1
@@ -142,7 +143,7 @@ def _append(q, k, v, k_cache, v_cache, tables, seqlens, cos, sin, interleaved, c
     out = qp = qo = None
     q0 = q1 = q2 = sq = hq = 0
     if q is not None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=_DENSE)
         q0, q1, q2 = _strides(q)
         qp, qo, hq = q.data_ptr(), out.data_ptr(), q.shape[-2]
         if cu is None:
@@ -227,7 +228,7 @@ def scaled_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
     * ``llama3``: frequencies of more than ``high_freq_factor`` turns kept, of fewer than
       ``low_freq_factor`` divided by ``factor``, between them in proportion."""
     _require(rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_dim must be positive and even")
-    _require(theta > 0, "theta must be positive")
+    _require(theta > 1, "theta must be above 1")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     inv = float(theta) ** (-i / rotary_dim)
     if not scaling:
@@ -315,7 +316,7 @@ class RotaryEmbedding:
             raise RuntimeError("n must be given, 0 or more")
         half = self.rotary_dim // 2
         cos = torch.empty((n, half), dtype=dtype, device=self.device)
-        sin = torch.empty((n, half), dtype=dtype, device=self.device)
+        sin = torch.empty_like(cos)
         if n:
             _lib.launch("aac_rotary_tables", dev, self._turns.data_ptr(), half, at, int(start), n, self.factor,
                         cos.data_ptr(), sin.data_ptr(), code)

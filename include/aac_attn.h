@@ -610,8 +610,8 @@ int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, con
  *
  * aac_rotary_tables: cos_out, sin_out [n_positions, n_freqs] = factor * cos, sin of
  * 2 pi p turns[i] at positions p = positions[r] or, where that is null, start + r.  turns:
- * double [n_freqs] on the device, turns a position; the angle is reduced in 64 bits.
- * |start| up to 2^40; cos_out and sin_out 16-byte aligned where n_freqs is a multiple of 8 (FP32: of 4).
+ * double [n_freqs] on the device, turns a position, 1 at most; the angle is reduced in 64
+ * bits.  |start| up to 2^40; cos_out and sin_out 16-byte aligned where n_freqs is a multiple of 8 (FP32: of 4).
  */
 int aac_rotary(const void* x, int64_t x_seq_stride, int64_t x_tok_stride, int64_t x_head_stride,
                void* out, int64_t out_seq_stride, int64_t out_tok_stride, int64_t out_head_stride,

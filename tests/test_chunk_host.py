@@ -20,7 +20,7 @@ def test_chunk_refusals():
     for a in (dict(dt=2), dict(dt=7), dict(d=64), dict(bs=7, mb=1 << 25)):
         assert _chunk(**a) == -2, a
     for a in (dict(n=-1), dict(B=-1), dict(hq=0), dict(mq=-1), dict(bs=0), dict(mb=0), dict(scale=0.0),
-              dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(q=None), dict(out=None),
+              dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=2e38), dict(q=None), dict(out=None),
               dict(tab=None), dict(ctx=None), dict(kc=None), dict(vc=None), dict(nb=0), dict(nb=-1)):
         assert _chunk(**a) == -1, a
     for a in (dict(hq=12), dict(qs=2047 // 2), dict(os=1024), dict(cu=None, n=5), dict(n=1 << 31)):
@@ -125,7 +125,7 @@ def test_scaling_refusals():
                                     low_freq_factor=4, high_freq_factor=4))):
         with pytest.raises(RuntimeError, match=match):
             f(8, 100.0, a)
-    for dim, theta in ((7, 1.0), (0, 1.0), (8, 0.0)):
+    for dim, theta in ((7, 9.0), (0, 9.0), (8, 0.0), (8, 1.0), (8, -2.0)):
         with pytest.raises(RuntimeError):
             f(dim, theta)
     with pytest.raises(RuntimeError, match="GPU"):

@@ -214,6 +214,16 @@ def test_a_context_past_the_table_is_cut_to_it(gpu):
     x["tables"] = x["tables"][:, :4].contiguous()
     x["ctx"] += 1000
     _check(_run(x, False), x, False)
+    x["ctx"].fill_((1 << 31) - 1)
+    _check(_run(x, True), x, True)
+    # and one whose tokens are appended past its table: none is stored
+    lens = torch.tensor([(1 << 31) - 3], dtype=torch.int32, device=gpu)
+    k = torch.ones(1, 9, 4, 128, dtype=torch.bfloat16, device=gpu)
+    before = x["kc"].clone()
+    got = fai.flash_attn_with_kvcache(x["q"].view(1, 9, 8, 128), x["kc"], x["vc"], k=k, v=k, cache_seqlens=lens,
+                                      block_table=x["tables"], causal=False)
+    assert torch.equal(x["kc"], before)
+    _check(got[0], x, False)
 
 
 def test_more_queries_than_said(gpu):
