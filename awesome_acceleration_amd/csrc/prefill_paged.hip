@@ -45,6 +45,7 @@ struct Args {
   int64_t n_tokens;
   u32 num_blocks;       // those an int32 table can name
   int32_t n_seqs, hq, hkv, group;
+  u32 group31;          // ceil(2^31 / group)
   int32_t max_q;        // queries of every sequence where cu_q is null
   int32_t block_size, max_blocks;
   int32_t capacity;     // keys a table can name
@@ -96,9 +97,22 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int s) {
   return r;
 }
 
-// The keys [0, end) that rows up to `row` see.
+// The keys [0, end) that query q, and rows up to `row`, see.
+template <bool CAUSAL> __device__ __forceinline__ int sees(const Seq& s, int q) {
+  return CAUSAL ? max(q + 1 + (s.Lk - s.Lq), 0) : s.Lk;
+}
 template <bool CAUSAL> __device__ __forceinline__ int end_of(const Args& a, const Seq& s, int row) {
-  return CAUSAL ? max(row / a.group + 1 + (s.Lk - s.Lq), 0) : s.Lk;
+  return CAUSAL ? sees<CAUSAL>(s, row / a.group) : s.Lk;
+}
+
+// Query and head of the group of a row x past row (q, g); x below 2^14.
+struct RowAt {
+  int q, g;
+};
+__device__ __forceinline__ RowAt row_past(const Args& a, RowAt r, int x) {
+  // y / group as (2 y) * ceil(2^31 / group) >> 32, exact for y, group < 2^15
+  const u32 y = (u32)(r.g + x), d = __umulhi(2 * y, a.group31);
+  return {r.q + (int)d, (int)(y - d * (u32)a.group)};
 }
 
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
@@ -164,9 +178,11 @@ template <int R_, int SL_, int KT_, int STAGES_> struct Shape {
   static constexpr int kOut = kWaves * 32 * kOutPitch;
   static constexpr int kMl = kWaves * 32 * 8;
   static constexpr int kRing = STAGES * kStage;
+  // Q comes in through the last stages; those before them are filled at the start
+  static constexpr int kQ = kWaves * 8192, kEarly = (kRing - kQ) / kStage;
   static constexpr int kBody = kRing > kPart + kMl ? kRing : kPart + kMl;
   static constexpr int kLds = kBody > kOut ? kBody : kOut;
-  static_assert(2 * kKeys % (16 * kWaves) == 0, "whole groups a wave");
+  static_assert(2 * kKeys % (16 * kWaves) == 0 && kRing >= kQ + kStage && kEarly < STAGES && STAGES - kEarly <= 2, "the form");
   static constexpr int kRows = 32 * R;
   // shared work, in iterations: what an item's start, merge and output cost, and the
   // least a workgroup takes
@@ -264,10 +280,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
   __shared__ int pre[SHARED ? kMaxSharedSeqs + 1 + S::kWaves : 1];
   const u32 lds0 = (u32)(uintptr_t)(lds_u8*)lds;
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rb_w = wave % S::R, sl = wave / S::R;  // row block of the workgroup, key slice
-  const int hl = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x;
 
   // KV head fastest: one XCD per head when there are eight
   const int h = blockIdx.x % a.hkv;
@@ -277,26 +290,26 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     const Line l = line_of<S, CAUSAL, S::kThreads>(a, pre, pre + kMaxSharedSeqs + 1, gridDim.x / a.hkv);
     unit = (int)(blockIdx.x / a.hkv) * l.share;
     unit_end = min(unit + l.share, l.total);
-    // Whether the share starts inside an item, for the joining kernel
+    // for the joining kernel: whether the share starts inside an item
     Cut cut = {0, -1};
-    if (unit < unit_end) {
+    if (unit >= unit_end) {  // workgroup-uniform
+      if (tid == 0) a.ws_cut[blockIdx.x] = cut;
+      return;
+    }
+    item = item_at<S, CAUSAL>(a, pre, unit);
+    const int x = unit - item.begin;
+    if (x > 0 && x <= l.share) {  // the item's first cut
       const int w = (int)(blockIdx.x / a.hkv);
-      const Item it = item_at<S, CAUSAL>(a, pre, unit);
-      if (unit > it.begin && unit - l.share <= it.begin) {
-        // shares whose iterations of it are not none: all but perhaps its ends
-        const int head = min(l.share * w, it.begin + it.units) - it.begin, last = (it.begin + it.units - 1) / l.share;
-        cut.first = iteration_of<S>(it, head) > 0 ? w - 1 : w;
-        cut.last = w - 1;
-        for (int x = w; x <= last && iteration_of<S>(it, x * l.share - it.begin) < it.n_it; ++x)
-          if (iteration_of<S>(it, (x + 1) * l.share - it.begin) > 0) cut.last = x;
-        cut.opens = w - 1;
-        cut.row0 = it.row0;
-        cut.rows = it.rows;
-        cut.q_beg = it.sq.q_beg;
-      }
+      // the shares that hold iterations of it: all but perhaps those at its ends
+      cut.first = iteration_of<S>(item, x) > 0 ? w - 1 : w;
+      cut.last = w - 1;
+      for (int k = w; iteration_of<S>(item, k * l.share - item.begin) < item.n_it; ++k) cut.last = k;
+      cut.opens = w - 1;
+      cut.row0 = item.row0;
+      cut.rows = item.rows;
+      cut.q_beg = item.sq.q_beg;
     }
     if (tid == 0) a.ws_cut[blockIdx.x] = cut;
-    if (unit >= unit_end) return;  // workgroup-uniform
   } else {
     // an item a workgroup: the row blocks of a sequence together, the causal ones with
     // the most keys first
@@ -310,11 +323,22 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     item.end = __builtin_amdgcn_readfirstlane(end_of<CAUSAL>(a, item.sq, min(item.row0 + kRows, item.rows) - 1));
     item.n_it = (item.end + S::kKeys - 1) / S::kKeys;
   }
-  for (;;) {
+  auto next_item = [&]() {
+    if (unit >= unit_end) return false;
+    item = item_at<S, CAUSAL>(a, pre, unit);
+    return true;
+  };
+  for (bool more = true; more; more = SHARED && next_item()) {
+  // (opaque: else what hangs on them alone is kept from item to item, and registers spill)
+  int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if constexpr (SHARED) {
+    asm volatile("" : "+v"(lane));
+    asm volatile("" : "+s"(wave));
+  }
+  const int col = lane & 31, hl = lane >> 5;
+  const int rb_w = wave % S::R, sl = wave / S::R;  // row block of the workgroup, key slice
   int i0 = 0, i1, slot = -1;  // iterations, place of a partial result
   if constexpr (SHARED) {
-    if (unit >= unit_end) break;
-    item = item_at<S, CAUSAL>(a, pre, unit);
     const int x0 = unit - item.begin, x1 = min(item.units, unit_end - item.begin);
     unit = item.begin + x1;
     i0 = __builtin_amdgcn_readfirstlane(iteration_of<S>(item, x0));
@@ -334,11 +358,14 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
 
   // this wave's and lane's rows
   const int wrow = row0 + 32 * rb_w;
-  const int my_row = min(wrow + col, rows - 1);
-  const int my_q = my_row / a.group, my_head = h * a.group + (my_row - my_q * a.group);
+  const int w_row = min(wrow, rows - 1), w_last = rows - 1 - w_row;  // (a wave past the rows: the last one)
+  RowAt w_at;
+  w_at.q = __builtin_amdgcn_readfirstlane(w_row / a.group);
+  w_at.g = w_row - w_at.q * a.group;
+  const int my_q = row_past(a, w_at, min(col, w_last)).q;
   const int w_end = wrow < rows ? end_of<CAUSAL>(a, sq, min(wrow + 31, rows - 1)) : 0;
-  const int full = CAUSAL ? end_of<CAUSAL>(a, sq, wrow) : sq.Lk;  // keys below need no mask
-  const int my_lim = end_of<CAUSAL>(a, sq, my_row);
+  const int full = sees<CAUSAL>(sq, w_at.q);  // keys below need no mask
+  const int my_lim = sees<CAUSAL>(sq, my_q);
   const int w_sub = min(j1, (w_end + 31) / 32);
 
   // ---- staging: 16-row group g of a stage is rows 16 g of K, then of V; this wave's
@@ -398,22 +425,27 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
       }
     }
   };
-  // Q fragments (B operand of S^T = K Q^T: lane = row)
-  u32x4 qf[8];
-  {
-    const u16* qp = a.q + (int64_t)(sq.q_beg + my_q) * a.q_stride + my_head * D + hl * 8;
+  // ---- on their way: this wave's rows of Q, into its place in the last stages (chunks
+  // swizzled as K's), then the first stages: all their block numbers, then all their rows
+  const u32 q_lds = lds0 + (u32)(S::kRing - S::kQ + wave * 8192);
 #pragma unroll
-    for (int t = 0; t < 8; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + r4;
+    const RowAt at = row_past(a, w_at, min(r, w_last));
+    load_lds16(a.q + (int64_t)(sq.q_beg + at.q) * a.q_stride + (h * a.group + at.g) * D + 8 * ((lane & 15) ^ (r & 15)),
+               q_lds + i * 1024);
   }
-  // the first stages: all their block numbers, then all their rows
   {
-    int first[STAGES - 1][S::kGroups];
+    int first[S::kEarly][S::kGroups];
 #pragma unroll
-    for (int n = 0; n < STAGES - 1; ++n) look_up(n, first[n]);
+    for (int n = 0; n < S::kEarly; ++n) look_up(n, first[n]);
 #pragma unroll
-    for (int n = 0; n < STAGES - 1; ++n)
+    for (int n = 0; n < S::kEarly; ++n)
       if (n < n_it) issue(n, first[n]);
   }
+  int late[STAGES - S::kEarly][S::kGroups];  // of those that go out once Q has been read
+#pragma unroll
+  for (int n = S::kEarly; n < STAGES; ++n) look_up(n, late[n - S::kEarly]);
 
   // fragment addresses within a sub-tile (see prefill_wide.hip)
   int koff[8], vo[4];
@@ -436,7 +468,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
 
   f32x16 s;      // scores of a sub-tile, then:
   u32x4 pb[2];   // its probabilities, two steps of 16 keys
-  u32x4 kf[8], vf[8];
+  u32x4 qf[8], kf[8], vf[8];
   typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
   auto tile = [&](int n, int sub) { return (const lds_u8*)lds + n % STAGES * S::kStage + sub * kSubBytes; };
   auto read_k = [&](const lds_u8* kb) {
@@ -532,17 +564,30 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     }
   };
 
-  // Q has arrived: left pending into the loop it would make every iteration wait for
-  // all loads (vmcnt 0, the others unconstrained)
-  __builtin_amdgcn_s_waitcnt(0x0F70);
+  // Q fragments (B operand of S^T = K Q^T: lane = row), once the wave's own loads of them,
+  // the oldest, have landed
+  if (n_it >= S::kEarly) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kEarly * S::kLoads) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < 8; ++t) qf[t] = *reinterpret_cast<lds_u32x4*>((const lds_u8*)lds + (q_lds - lds0) + koff[t]);
 
-  look_up(STAGES - 1, ent);
+  // stage 0 has landed and every wave is done with Q
+  if (S::kEarly > 1 && n_it >= S::kEarly) landed_barrier<(S::kEarly - 1) * S::kLoads>();
+  else landed_barrier<0>();
+#pragma unroll
+  for (int k = S::kEarly; k < STAGES; ++k)
+    if (k < n_it) issue(k, late[k - S::kEarly]);
+  look_up(STAGES, ent);
+
   for (int n = 0; n < n_it; ++n) {
-    if (STAGES > 2 && n + STAGES - 2 < n_it) landed_barrier<(STAGES - 2) * S::kLoads>();
-    else landed_barrier<0>();
-    if (n + STAGES - 1 < n_it) {
-      issue(n + STAGES - 1, ent);
-      look_up(n + STAGES, ent);
+    if (n > 0) {
+      // stage n has landed and every wave is done with stage n - 1
+      if (STAGES > 2 && n + STAGES - 2 < n_it) landed_barrier<(STAGES - 2) * S::kLoads>();
+      else landed_barrier<0>();
+      if (n + STAGES - 1 < n_it) {
+        issue(n + STAGES - 1, ent);
+        look_up(n + STAGES, ent);
+      }
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -644,12 +689,12 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void prefill_p
     }
   __syncthreads();
   // whole rows: 16 lanes a row
-  for (int r = tid >> 4; r < kRows; r += S::kThreads / 16) {
-    const int row = row0 + r;
-    if (row >= rows) break;
-    const int qi = row / a.group;
-    *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.q_beg + qi) * a.o_stride +
-                              (h * a.group + row - qi * a.group) * D + (lane & 15) * 8) =
+  RowAt at0;
+  at0.q = __builtin_amdgcn_readfirstlane(row0 / a.group);
+  at0.g = row0 - at0.q * a.group;
+  for (int r = tid >> 4; r < min(kRows, rows - row0); r += S::kThreads / 16) {
+    const RowAt at = row_past(a, at0, r);
+    *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.q_beg + at.q) * a.o_stride + (h * a.group + at.g) * D + (lane & 15) * 8) =
         *reinterpret_cast<const u32x4*>(lds + (r >> 5) * (32 * kOutPitch) + (r & 31) * kOutPitch + (lane & 15) * 16);
   }
   if constexpr (!SHARED) break;
@@ -827,7 +872,7 @@ extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_
   // sequence numbered in int32; positions in 27 bits of groups or rows
   const int64_t cap = capacity_of(block_size, max_blocks_per_seq);
   if ((int64_t)n_kv_heads * head_dim * 2 * 16 >= (int64_t(1) << 31) ||
-      (int64_t)max_seqlen_q * (n_q_heads / n_kv_heads) >= (int64_t(1) << 30))
+      (int64_t)max_seqlen_q * (n_q_heads / n_kv_heads) >= (int64_t(1) << 30) || n_q_heads / n_kv_heads >= 1 << 14)
     return AAC_ERR_UNSUPPORTED;
   const bool one = max_blocks_per_seq == 1, page16 = one || block_size % 16 == 0;
   if (!page16 && cap > (int64_t(1) << 27)) return AAC_ERR_UNSUPPORTED;
@@ -848,6 +893,7 @@ extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_
   a.hq = n_q_heads;
   a.hkv = n_kv_heads;
   a.group = n_q_heads / n_kv_heads;
+  a.group31 = (u32)cdiv(int64_t(1) << 31, a.group);
   a.max_q = max_seqlen_q;
   a.block_size = block_size;
   a.max_blocks = max_blocks_per_seq;

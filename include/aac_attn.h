@@ -564,7 +564,7 @@ int aac_token_logprobs(const void* logits, int64_t row_stride, int64_t n_rows, i
  * sequences' queries (of a longer one, rows past it may be left unwritten);
  * max_context_len (<= 0: the table's capacity): an estimate of the longest context, which
  * only chooses how the work is split.
- * BF16 or FP16, head_dim 128, n_q_heads any multiple of n_kv_heads, scale > 0.  A
+ * BF16 or FP16, head_dim 128, n_q_heads any multiple (below 2^14) of n_kv_heads, scale > 0.  A
  * table of more than one block whose size is not a multiple of 16 names 2^27 tokens at most.
  * workspace: aac_prefill_paged_workspace_bytes(...) bytes (the same arguments) where
  * that is not 0, 16-byte aligned, any contents, not shared with a call that may overlap.

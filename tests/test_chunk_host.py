@@ -78,6 +78,17 @@ def test_page_of_a_key_by_multiplication():
                     assert x * m < 1 << 64 and (x * m) >> (27 + s) == x // d
 
 
+def test_row_of_a_group_by_multiplication():
+    """y / g as 2 y * ceil(2^31 / g) >> 32, exact for y, g < 2^15; a larger group is refused."""
+    for g in [*range(1, 70), 255, 256, 257, 4095, 4096, (1 << 14) - 1, 1 << 14, (1 << 15) - 1]:
+        m = -(-(1 << 31) // g)
+        assert m < 1 << 32
+        for y in {y for k in range((1 << 15) // g + 1) for y in (k * g - 1, k * g, k * g + g - 1)}:
+            if 0 <= y < 1 << 15:
+                assert (2 * y * m) >> 32 == y // g
+    assert _chunk(hq=1 << 14, hkv=1, mq=1, qs=1 << 21, os=1 << 21) == -2
+
+
 RULES = [
     dict(rope_type="linear", factor=4.0),
     dict(rope_type="dynamic", factor=4.0, original_max_position_embeddings=2048),
