@@ -759,13 +759,16 @@ static Plan plan(int32_t n_seqs, int32_t max_q, int32_t max_k, int64_t cap, int3
   const int64_t rows = (int64_t)max_q * (hq / hkv);
   auto items_of = [&](int r) { return (int64_t)n_seqs * hkv * cdiv(rows, r); };
   // Rows of a workgroup, us in 64 / 128 / 256 of them.  Where one block holds a sequence's
-  // rows the keys are what it costs: 16 x 5 queries over 1.5k keys at 16/8 heads 22.8 / 30.6
-  // / 32.2, 64 x 4 over 4k at 32/8 190 / 185 / 186.  Short contexts of few items are a chain
+  // rows the keys are what it costs: 16 x 5 queries over 1.5k keys at 16/8 heads 22.9 / 29.5
+  // / 31.1, 64 x 4 over 4k at 32/8 190 / 183 / 187.  Short contexts of few items are a chain
   // of latencies, shortest in small blocks that do not outnumber the CUs: 1 x 97 over 98
-  // 8.4 / 9.3 / 10.3, 11 x 64 over 171 at 32/8 18.2 / 11.3 / 13.6, 6 x 306 at 32/8 34.7 / 24.2
-  // / 19.4.  Else every key a workgroup brings in serves more rows in large ones: 2 x 265
-  // over 8.9k at 64/8 247 / 206 / 184, 26 x 1301 over 1.8k 624 / 450 / 388.
-  if (rows <= 64) p.rows = items_of(64) < n_cu ? 64 : 128;
+  // 7.6 / 8.3 / 9.2, 11 x 64 over 171 at 32/8 16.3 / 10.2 / 12.0, 6 x 306 at 32/8 32 / 22.5
+  // / 17.5; at one iteration of 64 keys in the large ones, which have no key slices to
+  // merge: 13 x 8 7.1 / 6.8 / 6.2, 28 x 42 13.1 / 7.9 / 7.3.  Else every key a workgroup
+  // brings in serves more rows in large ones: 2 x 265 over 8.9k at 64/8 250 / 205 / 180,
+  // 26 x 1301 over 1.8k 584 / 430 / 380.
+  if (max_k <= 64) p.rows = 256;
+  else if (rows <= 64) p.rows = items_of(64) < n_cu ? 64 : 128;
   else if (max_k <= 1024 && items_of(64) <= n_cu) p.rows = 64;
   else if (rows <= 128 || (max_k <= 1024 && items_of(128) <= n_cu)) p.rows = 128;
   else p.rows = 256;
