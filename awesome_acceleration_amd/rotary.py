@@ -148,7 +148,7 @@ def _append(q, k, v, k_cache, v_cache, tables, seqlens, cos, sin, interleaved, c
         qp, qo, hq = q.data_ptr(), out.data_ptr(), q.shape[-2]
         if cu is None:
             sq = q.shape[1]
-    if B and nblk and (k.numel() or (q is not None and q.numel())):
+    if B and (k.numel() or (q is not None and q.numel())):
         kc = k_cache.data_ptr()
         _lib.launch("aac_rotary_append_paged", k.get_device(), qp, q0, q1, q2, k.data_ptr() or kc, k0, k1, k2,
                     v.data_ptr() or kc, v0, v1, v2, qo, B, sq, sk, n, cu, seqlens.data_ptr(),
@@ -191,8 +191,8 @@ def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     if v.dtype is not dt or k_cache.dtype is not dt or v_cache.dtype is not dt:
         raise RuntimeError("dtype mismatch")
     D = cshape[3]
-    if D % 2 or cshape[1] == 0 or cshape[2] == 0:
-        raise RuntimeError("head_dim must be even, blocks and heads not empty")
+    if D % 2 or 0 in cshape:
+        raise RuntimeError("head_dim must be even, the caches not empty")
     if q is not None and (q.dim() != nd or q.dtype is not dt or q.shape[-1] != D
                           or q.shape[:nd - 2] != kshape[:nd - 2]):
         raise RuntimeError("q must be [B, S, Hq, D], or [N, Hq, D], of k's tokens and dtype")

@@ -144,6 +144,22 @@ def test_against_float64(gpu, case, dtype, causal):
     assert torch.equal(_run(x, causal), got)  # and the same on every run
 
 
+@pytest.mark.parametrize("new, ctx, hq, hkv, bs", [
+    ([9, 1, 4], [500, 40, 2100], 71, 1, 16),    # groups past a wave's rows
+    ([3, 2], [700, 300], 600, 2, 64),           # and past a workgroup's
+    ([1, 13, 2], [64, 63, 2], 16, 8, 16),       # one iteration of keys at most
+    ([64] * 9, [64] * 9, 8, 4, 32),
+    ([5, 64], [65, 64], 16, 8, 48),             # and one key more
+])
+def test_wide_groups_and_short_contexts(gpu, new, ctx, hq, hkv, bs):
+    _say("groups", hq, hkv, ctx)
+    x = _make(gpu, hq, new, ctx, hq, hkv, bs, torch.bfloat16)
+    for causal in (True, False):
+        got = _run(x, causal)
+        _check(got, x, causal)
+        _check(_run(x, causal, max_context_len=max(ctx)), x, causal, what="with the longest context")
+
+
 def test_slot_layout_of_any_length(gpu):
     """One block a sequence, its length no multiple of anything."""
     _say("slots")

@@ -331,3 +331,12 @@ def test_refusals(gpu):
     no("positions must", e.cos_sin, positions=i(5).long())
     no("unsupported dtype", e.cos_sin, 5, dtype=torch.float64)
     no("inconsistent", e.cos_sin, 5, start=1 << 50)
+
+
+def test_a_cache_without_blocks_is_refused(gpu):
+    q = torch.zeros(2, 3, 4, 128, device=gpu, dtype=torch.bfloat16)
+    cache = torch.zeros(0, 16, 4, 128, device=gpu, dtype=torch.bfloat16)
+    cos, sin = _tab(gpu, 9, 64, torch.float32)
+    with pytest.raises(RuntimeError, match="not empty"):
+        rotary.rotary_append_paged(q, q, q, cache, cache, torch.zeros(2, 1, dtype=torch.int32, device=gpu),
+                                   torch.zeros(2, dtype=torch.int32, device=gpu), cos, sin)
