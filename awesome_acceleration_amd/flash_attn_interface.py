@@ -20,8 +20,7 @@ paged cache: ``prefill_paged``, ``flash_attn_varlen_func(block_table=...)`` and
 (``rotary``) applied in the call where tables are given.
 
 Dropout, sliding windows, ALiBi, softcap and return_softmax_lse, which the reference
-does not use, are not accepted; they
-raise ``NotImplementedError`` instead of silently computing something else.
+does not use, raise ``NotImplementedError`` instead of silently computing something else.
 Every op runs on ``torch.cuda.current_stream()`` and never synchronises.
 Outputs are allocated here (FA2 returns a new tensor); caches are updated in
 place; ``cache_seqlens`` is never modified (the reference increments it
@@ -530,8 +529,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
                             *, max_context_len=None):
     """Decode with KV cache (model/model.py:233-240).
 
-    q ``[B, S, Hq, D]``, one token a sequence (S = 1) or a chunk of them (bf16 and fp16).  Without ``block_table`` the caches are the
-    reference's slot caches ``[num_slots, max_seq_len, Hkv, D]`` and batch
+    q ``[B, S, Hq, D]``, one token a sequence (S = 1) or a chunk of them (bf16 and fp16).
+    Without ``block_table`` the caches are the reference's slot caches ``[num_slots, max_seq_len, Hkv, D]`` and batch
     row ``b`` uses slot ``cache_batch_idx[b]`` (default ``b``); with
     ``block_table`` (int32 ``[B, max_blocks]``) they are paged caches
     ``[num_blocks, block_size, Hkv, D]``.  When ``k``/``v`` (``[B, 1, Hkv,

@@ -553,9 +553,9 @@ int aac_token_logprobs(const void* logits, int64_t row_stride, int64_t n_rows, i
 /*
  * Attention of a chunk of new tokens over the paged cache.  Sequence b's queries are rows
  * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q [n_tokens, n_q_heads, head_dim] (token stride
- * q_tok_stride), or, where cu_seqlens_q is null, max_seqlen_q rows each; its keys are the first L_b tokens of its blocks, L_b = context_lens[b]
- * or, where that is null, cu_seqlens_k[b+1] - cu_seqlens_k[b] (the new tokens' rows among
- * them: they are stored first).  With causal != 0 the mask is bottom-right aligned: query i
+ * q_tok_stride), or, where cu_seqlens_q is null, max_seqlen_q rows each; its keys are the
+ * first L_b tokens of its blocks, L_b = context_lens[b] or, where that is null,
+ * cu_seqlens_k[b+1] - cu_seqlens_k[b] (the new tokens' rows among them: they are stored first).  With causal != 0 the mask is bottom-right aligned: query i
  * of n sees keys j <= i + L_b - n.  A query that sees no key gets zeros; what a masked key's
  * value or a row behind the context holds, infinities and NaN too, reaches no query that
  * does not see it.  Rows of q behind the last sequence are left as they are in out.
