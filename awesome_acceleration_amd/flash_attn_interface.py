@@ -567,7 +567,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     nblk, bs, hkv, _ = k_cache.shape
     if block_table is None:
         if cache_batch_idx is None:
-            tables = torch.arange(B, dtype=torch.int32, device=q.device)
+            tables = torch.arange(B, dtype=torch.int32, device=q.device).view(B, 1)
         else:
             tables = cache_batch_idx.to(torch.int32).reshape(B, 1).contiguous()
         mb = 1

@@ -481,3 +481,36 @@ def test_nothing_to_do(gpu):
     none = fai.flash_attn_with_kvcache(x["q"][:0].view(0, 4, 16, 128), x["kc"], x["vc"], cache_seqlens=i(0),
                                        block_table=i(0, 3))
     assert none.shape == (0, 4, 16, 128)
+
+
+@pytest.mark.parametrize("rot", [0, 128])
+@pytest.mark.parametrize("sq, sk", [(1, 1), (5, 5), (1, 4), (6, 2), (3, 0)])
+def test_kvcache_call_on_slots_by_default(gpu, sq, sk, rot):
+    """Neither block_table nor cache_batch_idx: row b uses slot b."""
+    _say("slots by default", sq, sk, rot)
+    cached = [0, 31, 100]
+    x = _make(gpu, 18, [sq] * 3, [c + sk for c in cached], 16, 8, 120, torch.bfloat16)
+    x["tables"] = torch.arange(3, dtype=torch.int32, device=gpu).view(3, 1)
+    g = _gen(gpu, 4)
+    q, k, v = (torch.randn((3, s, h, 128), generator=g, device=gpu).to(torch.bfloat16)
+               for s, h in ((sq, 16), (sk, 8), (sk, 8)))
+    lens = torch.tensor(cached, dtype=torch.int32, device=gpu)
+    a = dict(cache_seqlens=lens, causal=True)
+    qt, kt = q, k
+    if rot:
+        a["rotary_cos"], a["rotary_sin"] = rotary.RotaryEmbedding(rot, device=gpu).cos_sin(200)
+        qt, kt = (rotary.apply_rotary_emb(t, a["rotary_cos"], a["rotary_sin"], True, seqlen_offsets=lens)
+                  for t in (q, k))
+    want = [c.clone() for c in (x["kc"], x["vc"])]
+    for b, c in enumerate(cached):
+        want[0][b, c:c + sk], want[1][b, c:c + sk] = kt[b], v[b]
+    kc, vc = x["kc"].clone(), x["vc"].clone()
+    got = fai.flash_attn_with_kvcache(q, x["kc"], x["vc"], k=k, v=v, **a)
+    assert torch.equal(x["kc"], want[0]) and torch.equal(x["vc"], want[1])
+    x["q"] = qt.reshape(-1, 16, 128)
+    _check(got.reshape(-1, 16, 128), x, True)
+    # and as with the slots named
+    named = fai.flash_attn_with_kvcache(q, kc, vc, k=k, v=v, cache_batch_idx=torch.arange(3, device=gpu), **a)
+    assert torch.equal(named, got) and torch.equal(kc, x["kc"]) and torch.equal(vc, x["vc"])
+    if sk == 0 and not rot:
+        assert torch.equal(fai.flash_attn_with_kvcache(q, kc, vc, **a), got)
