@@ -49,7 +49,8 @@ import torch
 from . import fused as fz
 from .paged import (MAX_MAP_SEQS, BlockAllocator, blocks_needed, build_prefill_metadata,
                     build_step_maps, pad_block_tables)
-from .qwen3 import PagedKV4Cache, PagedKVCache, Qwen3Config, Qwen3ForCausalLM, StepMeta
+from .qwen3 import (PagedKV4Cache, PagedKVCache, Qwen3Config, Qwen3ForCausalLM, StepMeta,
+                    scaling_rule)
 
 __all__ = ["LLM", "GenerationOutput"]
 
@@ -121,6 +122,13 @@ class LLM:
         self.device = torch.device(device)
         self.dtype = dtype
         self.config = config or Qwen3Config()
+        rule = scaling_rule(self.config.rope_scaling, self.config.max_position_embeddings)
+        if rule is not None and rule["rope_type"] == "dynamic":
+            # (past it theta follows each sequence's own length; the model has one table)
+            original = rule["original_max_position_embeddings"]
+            if max_seq_len > original:
+                raise ValueError(f"dynamic rope scaling serves contexts of the original {original} tokens "
+                                 f"at most (max_seq_len {max_seq_len})")
         self.max_seq_len = max_seq_len
         self.max_num_seqs = max_num_seqs
         self.block_size = block_size

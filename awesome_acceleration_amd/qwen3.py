@@ -59,7 +59,8 @@ class Qwen3Config:
     """Same fields and defaults as the reference's Qwen3Config (model/model.py:13-37), and
     ``rope_scaling``: the rule for long contexts as a configuration file holds it
     (``rotary.scaled_frequencies``; ``original_max_position_embeddings`` defaults to
-    ``max_position_embeddings``)."""
+    ``max_position_embeddings``).  ``dynamic`` serves contexts within the original one, which
+    it leaves unscaled."""
     vocab_size: int = 151936
     hidden_size: int = 1024
     intermediate_size: int = 3072
@@ -92,21 +93,38 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     return weight * xf.to(dt)
 
 
+def scaling_rule(scaling: dict | None, max_pos: int) -> dict | None:
+    """A ``rope_scaling`` rule with its ``rope_type`` and original context, or None: unscaled."""
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "default":
+        return None
+    rule = dict(scaling, rope_type=kind)
+    if rule.get("original_max_position_embeddings") is None:
+        rule["original_max_position_embeddings"] = max_pos
+    return rule
+
+
 class Rope:
     """cos/sin tables in the activation dtype (model/model.py:64-78), indexed
     by position on the device.  With ``scaling`` (a ``rope_scaling`` rule) they are
-    ``rotary.RotaryEmbedding``'s, of ``factor`` times the original context's positions."""
+    ``rotary.RotaryEmbedding``'s, of ``factor`` times the original context's positions.
+
+    ``dynamic`` leaves a context within the original one as it is and grows theta with the
+    length of a longer one, sequence by sequence, which one table for all of them cannot
+    follow: its tables are the unscaled ones, of the original context's positions."""
 
     def __init__(self, head_dim: int, max_pos: int, theta: float, device, dtype, scaling=None):
         self.half = head_dim // 2
-        if scaling and scaling.get("rope_type", scaling.get("type", "default")) != "default":
-            rule = dict(scaling)
-            if rule.get("original_max_position_embeddings") is None:
-                rule["original_max_position_embeddings"] = max_pos
-            n = max(max_pos, int(float(rule.get("factor") or 1) * rule["original_max_position_embeddings"]))
-            scaled = rotary.RotaryEmbedding(head_dim, theta, rule, seq_len=n, device=device)
-            self.cos, self.sin = (torch.cat((t, t), -1) for t in scaled.cos_sin(n, dtype=dtype))
-            return
+        rule = scaling_rule(scaling, max_pos)
+        if rule is not None:
+            old = rule["original_max_position_embeddings"]
+            if rule["rope_type"] != "dynamic":
+                n = max(max_pos, int(float(rule.get("factor") or 1) * old))
+                scaled = rotary.RotaryEmbedding(head_dim, theta, rule, seq_len=n, device=device)
+                self.cos, self.sin = (torch.cat((t, t), -1) for t in scaled.cos_sin(n, dtype=dtype))
+                return
+            rotary.scaled_frequencies(head_dim, theta, rule)  # (refuses what the rule lacks)
+            max_pos = int(old)
         inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))
         t = torch.arange(max_pos, dtype=torch.float32)
         freqs = torch.outer(t, inv)

@@ -151,3 +151,42 @@ def test_engine_refuses_a_chunk_of_no_tokens_and_chunks_with_the_4_bit_cache():
               dict(prefill_chunk=64, kv_cache_dtype="mxfp4")):
         with pytest.raises(ValueError, match="prefill_chunk"):
             LLM(**a)
+
+
+DYNAMIC = dict(rope_type="dynamic", factor=4.0, original_max_position_embeddings=300)
+
+
+@pytest.mark.parametrize("rule", [DYNAMIC, dict(type="dynamic", factor=4.0)], ids=["original", "model"])
+def test_dynamic_scaling_leaves_the_original_context_as_it_is(rule):
+    """transformers grows theta for a context past the original one alone; the model's tables
+    are the unscaled ones, as far as the original context."""
+    from awesome_acceleration_amd.qwen3 import Rope
+    plain = Rope(64, 300, 1e4, "cpu", torch.float32)
+    got = Rope(64, 300, 1e4, "cpu", torch.float32, rule)
+    assert torch.equal(got.cos, plain.cos) and torch.equal(got.sin, plain.sin)
+    longer = Rope(64, 4096, 1e4, "cpu", torch.float32, DYNAMIC)
+    assert torch.equal(longer.cos, plain.cos) and torch.equal(longer.sin, plain.sin)
+    with pytest.raises(RuntimeError, match="factor"):
+        Rope(64, 300, 1e4, "cpu", torch.float32, dict(rope_type="dynamic"))
+    transformers = pytest.importorskip("transformers.models.qwen3.modeling_qwen3")
+    from transformers import Qwen3Config as Theirs
+    try:
+        theirs = transformers.Qwen3RotaryEmbedding(Theirs(
+            hidden_size=64, num_attention_heads=1, head_dim=64, max_position_embeddings=300,
+            rope_parameters=dict(DYNAMIC, rope_theta=1e4)))
+        cos, sin = theirs(torch.zeros(1, 1, 64), torch.arange(300)[None])
+    except (KeyError, AttributeError, TypeError) as e:
+        pytest.skip(f"this transformers reads its configuration otherwise: {e!r}")
+    # an angle of up to 299 in float32, its frequency's power rounded here and there: 4 units
+    # of 2^-24 of it
+    assert (got.cos - cos[0]).abs().max() <= 300 * 2.0 ** -22
+    assert (got.sin - sin[0]).abs().max() <= 300 * 2.0 ** -22
+
+
+def test_engine_refuses_dynamic_scaling_past_the_original_context():
+    from awesome_acceleration_amd.llm import LLM
+    from awesome_acceleration_amd.qwen3 import Qwen3Config
+    for rule, limit in ((DYNAMIC, 300), (dict(type="dynamic", factor=2.0), 500)):
+        cfg = Qwen3Config(num_hidden_layers=1, max_position_embeddings=500, rope_scaling=rule)
+        with pytest.raises(ValueError, match=f"original {limit} tokens"):
+            LLM(cfg, max_seq_len=limit + 1)

@@ -178,3 +178,27 @@ def test_the_operators_together(gpu, dtype):
         _check(got.view(-1, hq, 128), dict(q=q.reshape(-1, hq, 128), kc=kc, vc=vc, tables=tables, new=[3] * 3,
                                            lens=[d + 3 for d in done], bs=bs), True, what=f"draft {n}")
         done = [d + n for d in done]  # some of them are kept
+
+
+@pytest.mark.parametrize("rule", [dict(rope_type="dynamic", factor=4.0, original_max_position_embeddings=512),
+                                  dict(type="dynamic", factor=2.0),
+                                  dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                       original_max_position_embeddings=64)],
+                         ids=["dynamic", "dynamic-model", "llama3"])
+def test_model_with_more_scaled_positions(gpu, rule, monkeypatch):
+    """(Contexts within the original one: dynamic scaling leaves them as they are.)"""
+    print("case: rope scaling", rule, flush=True)
+    cfg = Qwen3Config(**{**BASE, "max_position_embeddings": 512}, rope_scaling=rule)
+
+    def tables(positions, head_dim, theta):
+        f = theta ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
+        if rule.get("rope_type") == "llama3":
+            f, _ = rotary.scaled_frequencies(head_dim, theta, rule)
+        a = positions.double()[:, None].cpu() * f
+        a = torch.cat((a, a), -1)
+        return tuple(t.float().to(positions.device) for t in (a.cos(), a.sin()))
+
+    monkeypatch.setattr(qwen3_ref, "rope_tables", tables)
+    prompts = _prompts(4, 3, 200)
+    llm, outs = _run(prompts, [8] * 4, cfg=cfg, prefill_chunk=50)
+    _against_reference(llm, prompts, outs)
