@@ -81,6 +81,17 @@ class Qwen3Config:
     def from_json(cls, path: str):
         with open(path) as f:
             data = json.load(f)
+        # the scaling's rule, and in newer files theta, stand in rope_parameters; where both are
+        # there rope_scaling counts, and the rule's own theta before the file's
+        rule = dict(data.get("rope_scaling") or data.get("rope_parameters") or {})
+        if any(isinstance(v, dict) for v in rule.values()):
+            raise ValueError("rope parameters by layer type are not supported")
+        if rule.pop("partial_rotary_factor", 1.0) not in (None, 1.0):
+            raise ValueError("heads turned in part are not supported")
+        theta = rule.pop("rope_theta", None)
+        if theta is not None:
+            data["rope_theta"] = theta
+        data["rope_scaling"] = scaling_rule(rule, None) and rule
         return cls(**{k: v for k, v in data.items() if k in cls.__annotations__})
 
 
@@ -93,7 +104,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     return weight * xf.to(dt)
 
 
-def scaling_rule(scaling: dict | None, max_pos: int) -> dict | None:
+def scaling_rule(scaling: dict | None, max_pos: int | None) -> dict | None:
     """A ``rope_scaling`` rule with its ``rope_type`` and original context, or None: unscaled."""
     kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
     if kind == "default":

@@ -190,3 +190,48 @@ def test_engine_refuses_dynamic_scaling_past_the_original_context():
         cfg = Qwen3Config(num_hidden_layers=1, max_position_embeddings=500, rope_scaling=rule)
         with pytest.raises(ValueError, match=f"original {limit} tokens"):
             LLM(cfg, max_seq_len=limit + 1)
+
+
+def test_config_files_name_their_scaling_either_way(tmp_path):
+    """rope_scaling beside rope_theta, or rope_parameters with both in it, read as transformers
+    reads them."""
+    import json
+    from awesome_acceleration_amd.qwen3 import Qwen3Config
+    yarn = dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=16384)
+    linear = dict(type="linear", factor=4.0)
+
+    def read(**data):
+        path = tmp_path / "config.json"
+        path.write_text(json.dumps(dict(hidden_size=512, max_position_embeddings=32768, **data)))
+        c = Qwen3Config.from_json(path)
+        assert c.hidden_size == 512 and c.max_position_embeddings == 32768
+        return c.rope_theta, c.rope_scaling
+
+    assert read() == (1e6, None)
+    assert read(rope_theta=5e5) == (5e5, None)
+    assert read(rope_theta=5e5, rope_scaling=None) == (5e5, None)
+    assert read(rope_theta=5e5, rope_scaling=linear) == (5e5, linear)
+    assert read(rope_scaling=dict(linear, rope_theta=3e5), rope_theta=5e5) == (3e5, linear)
+    assert read(rope_parameters=dict(rope_type="default", rope_theta=2e4)) == (2e4, None)
+    assert read(rope_parameters=dict(yarn, rope_theta=2e4)) == (2e4, yarn)
+    assert read(rope_parameters=dict(yarn, rope_theta=2e4), rope_theta=5e5, rope_scaling=None) == (2e4, yarn)
+    assert read(rope_parameters=yarn, rope_theta=5e5) == (5e5, yarn)
+    assert read(rope_parameters=dict(yarn, rope_theta=2e4), rope_scaling=linear) == (1e6, linear)
+    with pytest.raises(ValueError, match="layer type"):
+        read(rope_parameters=dict(full_attention=yarn))
+    with pytest.raises(ValueError, match="in part"):
+        read(rope_parameters=dict(yarn, partial_rotary_factor=0.5))
+
+
+def test_config_file_of_the_installed_transformers(tmp_path):
+    transformers = pytest.importorskip("transformers")
+    from awesome_acceleration_amd.qwen3 import Qwen3Config
+    rule = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                original_max_position_embeddings=8192)
+    try:
+        theirs = transformers.Qwen3Config(rope_parameters=dict(rule, rope_theta=5e5))
+    except (KeyError, AttributeError, TypeError) as e:
+        pytest.skip(f"this transformers reads its configuration otherwise: {e!r}")
+    theirs.save_pretrained(tmp_path)
+    c = Qwen3Config.from_json(tmp_path / "config.json")
+    assert c.rope_theta == 5e5 and c.rope_scaling == rule
