@@ -477,6 +477,7 @@ class LLM:
         active: dict[int, _Seq] = {}
         pending: list[_Request] = []
         filling: list[_Seq] = []  # admitted, their prompts not all in the cache
+        admitted: list[_Seq] = []  # all whose results may not have been given yet
         try:
             while self._loop_running or pending or active or filling:
                 # Phase 1: drain the queue
@@ -491,6 +492,7 @@ class LLM:
                     time.sleep(0.001)
                     continue
                 # Phase 2: admit while a batch row and the blocks are free
+                admitted = [s for s in admitted if not s.done]
                 new: list[_Seq] = []
                 for req in list(pending):
                     while req.pending_indices and free_rows:
@@ -502,6 +504,7 @@ class LLM:
                         req.pending_indices.pop(0)
                         new.append(_Seq(req, pi, free_rows.pop(0), self.allocator.allocate(need),
                                         [], L))
+                        admitted.append(new[-1])
                     if not req.pending_indices:
                         pending.remove(req)
                     elif not free_rows or self.allocator.num_free == 0:
@@ -559,7 +562,8 @@ class LLM:
                         self._retire(seqs, self._tokens(h, seqs), active, free_rows)
                         break
         except BaseException as e:  # surface failures to every waiting caller
-            for s in (*active.values(), *filling):
+            # (those between two lists, whose step or end failed, are among the admitted)
+            for s in admitted:
                 if not s.req.future.done():
                     s.req.future.set_exception(e)
             for req in pending:

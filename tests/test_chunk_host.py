@@ -235,3 +235,59 @@ def test_config_file_of_the_installed_transformers(tmp_path):
     theirs.save_pretrained(tmp_path)
     c = Qwen3Config.from_json(tmp_path / "config.json")
     assert c.rope_theta == 5e5 and c.rope_scaling == rule
+
+
+def _engine(chunk=None, decode_fn=None):
+    """The engine's loop alone: prompts of any length, every token a 7, no model or device."""
+    import queue
+    from types import SimpleNamespace
+    from awesome_acceleration_amd import paged
+    from awesome_acceleration_amd.llm import LLM
+    llm = LLM.__new__(LLM)
+    llm.config = SimpleNamespace(vocab_size=9, eos_token_id=0)
+    llm.max_seq_len, llm.max_num_seqs, llm.block_size = 64, 3, 16
+    llm.allocator = paged.BlockAllocator(12 + 1)
+    llm.allocator.allocate(1)
+    llm.use_graphs, llm.prefill_chunk, llm.decode_fn = False, chunk, decode_fn
+    llm._request_queue, llm._loop_running, llm._loop_thread = queue.Queue(), False, None
+    llm.stats = dict(decode_tokens=0)
+
+    def chunk_step(filling):
+        for s in filling:
+            s.filled += chunk
+        ended = [s for s in filling if s.filled >= len(s.req.token_ids[s.prompt_idx])]
+        return torch.zeros(len(ended), 9), ended
+
+    llm._prefill = llm._decode_step = lambda seqs: torch.zeros(len(seqs), 9)
+    llm._prefill_chunk = chunk_step
+    llm._sample_step = lambda seqs, logits, temperature: [7] * len(seqs)
+    return llm
+
+
+@pytest.mark.filterwarnings("ignore::pytest.PytestUnhandledThreadExceptionWarning")
+@pytest.mark.parametrize("chunk", [None, 4])
+@pytest.mark.parametrize("where", ["sample", "end of a prompt", "end"])
+def test_a_step_that_fails_ends_every_request(chunk, where):
+    """Whichever list its sequences are in, a caller gets the exception and does not wait on."""
+    def fail(*a):
+        raise MemoryError("no memory")
+
+    llm = _engine(chunk, fail if where != "sample" else None)
+    if where == "sample":
+        llm._sample_step = fail
+    n = 1 if where == "end of a prompt" else 3
+    futs = [llm.generate([[2] * 3], max_tokens=n), llm.generate([[1] * 5, [3] * 30], max_tokens=9),
+            llm.generate([[4] * 9] * 4, max_tokens=9)]
+    for f in futs:
+        with pytest.raises(MemoryError):
+            f.result(timeout=20)
+
+
+@pytest.mark.parametrize("chunk", [None, 4])
+def test_the_engines_loop_alone(chunk):
+    llm = _engine(chunk, lambda tokens: "x" * len(tokens))
+    futs = [llm.generate([[1] * 5, [2] * 3], max_tokens=2), llm.generate([[3] * 30] * 5, max_tokens=9)]
+    got = [f.result(timeout=20) for f in futs]
+    llm.stop()
+    assert [[o.text for o in g] for g in got] == [["xx"] * 2, ["x" * 9] * 5]
+    assert llm.allocator.num_free == 12
