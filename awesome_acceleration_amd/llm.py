@@ -563,18 +563,18 @@ class LLM:
                         break
         except BaseException as e:  # surface failures to every waiting caller
             # (those between two lists, whose step or end failed, are among the admitted)
-            for s in admitted:
-                if not s.req.future.done():
-                    s.req.future.set_exception(e)
-            for req in pending:
-                if not req.future.done():
-                    req.future.set_exception(e)
+            failed = [s.req for s in admitted] + pending
             while True:
                 try:
-                    req = self._request_queue.get_nowait()
+                    failed.append(self._request_queue.get_nowait())
                 except queue.Empty:
                     break
+            # before any caller hears of it, so that one who tries again finds the pool whole
+            # and no loop that has ended
+            for s in admitted:
+                self.allocator.free(s.blocks)
+            self._loop_running = False
+            for req in failed:
                 if not req.future.done():
                     req.future.set_exception(e)
-            self._loop_running = False
             raise

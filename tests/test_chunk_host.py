@@ -291,3 +291,24 @@ def test_the_engines_loop_alone(chunk):
     llm.stop()
     assert [[o.text for o in g] for g in got] == [["xx"] * 2, ["x" * 9] * 5]
     assert llm.allocator.num_free == 12
+
+
+@pytest.mark.filterwarnings("ignore::pytest.PytestUnhandledThreadExceptionWarning")
+@pytest.mark.parametrize("chunk", [None, 4])
+def test_after_a_failed_step_the_engine_serves_again(chunk):
+    """Blocks of the sequences that a failure ends go back to the pool."""
+    llm = _engine(chunk)
+    works = llm._decode_step
+
+    def fail(seqs):
+        raise MemoryError("no memory")
+
+    for _ in range(3):
+        llm._decode_step = fail
+        with pytest.raises(MemoryError):
+            llm.generate([[1] * 40] * 5, max_tokens=20).result(timeout=20)
+        assert llm.allocator.num_free == 12
+        llm._decode_step = works
+        assert [o.token_ids for o in llm.generate([[1] * 40] * 5, max_tokens=20).result(timeout=20)] == [[7] * 20] * 5
+        assert llm.allocator.num_free == 12
+    llm.stop()
