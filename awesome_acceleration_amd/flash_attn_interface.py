@@ -645,6 +645,25 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     return out
 
 
+def _attend_checks(q, k_cache, v_cache, tables, scale, one):
+    """What the attention launch of ``_chunk_with_kvcache`` would refuse of checked shapes."""
+    B, S, Hq, D = q.shape
+    _, bs, hkv, _ = k_cache.shape
+    if D != 128:
+        raise RuntimeError("head_dim must be 128")
+    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise RuntimeError("caches must be 16-byte aligned")
+    if one:
+        return
+    mb, group = tables.shape[1], Hq // hkv
+    if scale > 1e38:
+        raise RuntimeError("softmax_scale is too large")
+    if group >= 1 << 14 or S * group >= 1 << 30 or B * S >= 1 << 31 or hkv * D * 32 >= 1 << 31:
+        raise RuntimeError("too many heads or tokens")
+    if mb > 1 and bs % 16 and mb * bs > 1 << 27:
+        raise RuntimeError("a table of blocks whose size is not a multiple of 16 names 2^27 tokens at most")
+
+
 def _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqlens, tables, softmax_scale,
                         causal, interleaved, max_context_len):
     """``flash_attn_with_kvcache`` of several tokens a sequence, or with rotary tables: the
@@ -669,6 +688,8 @@ def _chunk_with_kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, seqle
         if k.dtype is not q.dtype or v.dtype is not q.dtype:
             raise RuntimeError("k/v dtype mismatch")
         _on_gpu(q, rotary_cos, rotary_sin)
+        if q.numel():  # (nothing is refused once rows are stored)
+            _attend_checks(q, k_cache, v_cache, tables, scale, one)
         k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (k, v))
         if k.shape[1] and B and nblk:
             ctx = torch.empty_like(seqlens)

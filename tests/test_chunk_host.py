@@ -312,3 +312,48 @@ def test_after_a_failed_step_the_engine_serves_again(chunk):
         assert [o.token_ids for o in llm.generate([[1] * 40] * 5, max_tokens=20).result(timeout=20)] == [[7] * 20] * 5
         assert llm.allocator.num_free == 12
     llm.stop()
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The names of a call's launches, none of which is made."""
+    from awesome_acceleration_amd import flash_attn_interface as fai
+    names = []
+    for module in (fai, rotary):
+        monkeypatch.setattr(module, "_on_gpu", lambda *ts: None)
+    monkeypatch.setattr(fai, "_chunk_ws_bytes", lambda *a: 0)
+    monkeypatch.setattr(_lib, "launch", lambda name, *a: names.append(name))
+    return names
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_what_the_attention_refuses_is_refused_before_the_append(launches, turned):
+    from awesome_acceleration_amd import flash_attn_interface as fai
+
+    def call(S=3, hq=4, hkv=2, d=128, bs=16, mb=2, nb=4, odd=0, **o):
+        empty = torch.zeros(nb * bs * hkv * d + 8, dtype=torch.bfloat16)
+        kc = empty[odd:odd + nb * bs * hkv * d].view(nb, bs, hkv, d)
+        q = torch.zeros(1, dtype=torch.bfloat16).expand(2, S, hq, d)
+        k = torch.zeros(2, S, hkv, d, dtype=torch.bfloat16)
+        if turned:
+            o["rotary_cos"] = o["rotary_sin"] = torch.zeros(9, d // 2)
+        return fai.flash_attn_with_kvcache(q.contiguous(), kc, kc, k=k, v=k, cache_seqlens=1, causal=True,
+                                           block_table=torch.zeros(2, mb, dtype=torch.int32), **o)
+
+    call()
+    assert launches == ["aac_rotary_append_paged", "aac_prefill_paged"]
+    if turned:
+        call(S=1)
+        assert launches[2:] == ["aac_rotary_append_paged", "aac_decode_paged"]
+    del launches[:]
+    for S in (1, 3) if turned else (3,):
+        for match, a in (("head_dim", dict(d=64)), ("head_dim", dict(d=256)), ("aligned", dict(odd=4))):
+            with pytest.raises(RuntimeError, match=match):
+                call(S, **a)
+    for match, a in (("scale", dict(softmax_scale=2e38)), ("too many", dict(hq=1 << 14, hkv=1)),
+                     ("names 2.27 tokens", dict(bs=7, mb=20_000_000))):
+        with pytest.raises(RuntimeError, match=match):
+            call(**a)
+    assert launches == []
+    call(mb=1, bs=7)
+    assert len(launches) == 2

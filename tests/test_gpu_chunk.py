@@ -514,3 +514,16 @@ def test_kvcache_call_on_slots_by_default(gpu, sq, sk, rot):
     assert torch.equal(named, got) and torch.equal(kc, x["kc"]) and torch.equal(vc, x["vc"])
     if sk == 0 and not rot:
         assert torch.equal(fai.flash_attn_with_kvcache(q, kc, vc, **a), got)
+
+
+@pytest.mark.parametrize("S", [1, 3])
+def test_a_refused_call_leaves_the_cache(gpu, S):
+    """Heads of 64 dims, which the append takes and the attention does not."""
+    _say("refused", S)
+    kc, vc = (torch.ones(4, 16, 2, 64, dtype=torch.bfloat16, device=gpu) for _ in "kv")
+    q, k = (torch.randn(2, S, h, 64, device=gpu).to(torch.bfloat16) for h in (4, 2))
+    cos, sin = rotary.RotaryEmbedding(64, device=gpu).cos_sin(40)
+    t = torch.arange(4, dtype=torch.int32, device=gpu).view(2, 2)
+    with pytest.raises(RuntimeError, match="head_dim"):
+        fai.flash_attn_with_kvcache(q, kc, vc, k=k, v=k, rotary_cos=cos, rotary_sin=sin, cache_seqlens=5, block_table=t)
+    assert (kc == 1).all() and (vc == 1).all()
