@@ -817,10 +817,26 @@ static int launch_s(Args a, const Plan& p, bool page16, int32_t max_q, hipStream
                          dim3((unsigned)(p.shares - 1) * a.hkv, S::R), dim3(256), 0, st, a);
     return AAC_OK;
   }
-  const int64_t grid = (int64_t)a.n_seqs * a.n_rb * a.hkv;
-  if (grid >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
-  if (page16) hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true, false>), dim3((unsigned)grid), block, 0, st, a);
-  else hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false, false>), dim3((unsigned)grid), block, 0, st, a);
+  // A launch numbers its threads in 32 bits.  One holds whole sequences, each taken to be as
+  // long as the longest: where they are too many the next launch takes the others.
+  const int64_t of_seq = (int64_t)a.n_rb * a.hkv, most = ((int64_t(1) << 32) - 1) / S::kThreads;
+  if (of_seq > most) return AAC_ERR_UNSUPPORTED;  // (one sequence: its queries alone hold 512 GiB)
+  for (int64_t left = a.n_seqs; left > 0;) {
+    a.n_seqs = (int32_t)std::min(left, most / of_seq);
+    const dim3 grid((unsigned)(a.n_seqs * of_seq));
+    if (page16) hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, true, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((prefill_paged_kernel<S, CAUSAL, F16, false, false>), grid, block, 0, st, a);
+    left -= a.n_seqs;
+    if (a.cu_q) {
+      a.cu_q += a.n_seqs;
+    } else {
+      a.q += a.n_seqs * a.max_q * a.q_stride;
+      a.out += a.n_seqs * a.max_q * a.o_stride;
+    }
+    if (a.ctx) a.ctx += a.n_seqs;
+    else a.cu_k += a.n_seqs;
+    a.tables += (int64_t)a.n_seqs * a.max_blocks;
+  }
   return AAC_OK;
 }
 
@@ -856,7 +872,8 @@ extern "C" size_t aac_prefill_paged_workspace_bytes(int64_t n_tokens, int32_t n_
       n_q_heads % n_kv_heads || block_size <= 0 || max_blocks_per_seq <= 0 || device_cu_count(&n_cu) != AAC_OK)
     return 0;
   const int64_t cap = capacity_of(block_size, max_blocks_per_seq);
-  return pp::plan(n_seqs, max_seqlen_q, longest_of(max_context_len, cap), cap, n_q_heads, n_kv_heads, n_cu).bytes;
+  return pp::plan(n_seqs, (int32_t)std::min<int64_t>(max_seqlen_q, n_tokens), longest_of(max_context_len, cap), cap,
+                  n_q_heads, n_kv_heads, n_cu).bytes;
 }
 
 extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, const void* k_cache,
@@ -877,6 +894,7 @@ extern "C" int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_
       (!cu_seqlens_q && n_tokens != (int64_t)n_seqs * max_seqlen_q))
     return AAC_ERR_SHAPE;
   if (n_tokens == 0 || n_seqs == 0 || max_seqlen_q == 0) return AAC_OK;
+  max_seqlen_q = (int32_t)std::min<int64_t>(max_seqlen_q, n_tokens);  // (any bound will do)
   if (!q || !out || !block_tables || (!context_lens && !cu_seqlens_k))
     return AAC_ERR_INVALID_ARGUMENT;
   if (num_blocks == 0 || !k_cache || !v_cache) return AAC_ERR_INVALID_ARGUMENT;

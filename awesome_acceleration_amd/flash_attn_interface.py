@@ -401,8 +401,8 @@ def _prefill_paged(q, k_cache, v_cache, cu_q, tables, ctx, cu_k, max_q, max_k, s
         return out
     if k_cache.numel() == 0 or tables.shape[1] == 0:  # no key anywhere: every row sees none
         return out.zero_()
-    _launch_chunk(q, qs, q.shape[0], k_cache, v_cache, tables, cu_q, ctx, cu_k, B, int(max_q),
-                  int(max_k or 0), scale, causal, out, os)
+    _launch_chunk(q, qs, q.shape[0], k_cache, v_cache, tables, cu_q, ctx, cu_k, B,
+                  min(int(max_q), q.shape[0]), int(max_k or 0), scale, causal, out, os)
     return out
 
 

@@ -527,3 +527,46 @@ def test_a_refused_call_leaves_the_cache(gpu, S):
     with pytest.raises(RuntimeError, match="head_dim"):
         fai.flash_attn_with_kvcache(q, kc, vc, k=k, v=k, rotary_cos=cos, rotary_sin=sin, cache_seqlens=5, block_table=t)
     assert (kc == 1).all() and (vc == 1).all()
+
+
+def _part(x, got, seqs):
+    """The given sequences of a packed problem whose sequences have one length: a problem and its rows."""
+    n, at = x["new"][0], torch.tensor(seqs, device=got.device)
+    rows = (at[:, None] * n + torch.arange(n, device=got.device)).flatten()
+    return dict(x, q=x["q"][rows], tables=x["tables"][at], new=[n] * len(seqs),
+                lens=[x["lens"][b] for b in seqs]), got[rows]
+
+
+def test_any_bound_of_the_queries_will_do(gpu):
+    _say("bounds")
+    x = _make(gpu, 32, [3, 40, 1], [300, 41, 9], 16, 8, 16, torch.bfloat16)
+    for most in (44, 45, 1 << 20, (1 << 31) - 1, 1 << 31, (1 << 32) + 3, 1 << 40):
+        _check(fai.prefill_paged(x["q"], x["kc"], x["vc"], x["cu"], x["tables"], x["ctx"], most), x, True, what=str(most))
+
+
+def test_more_workgroups_than_a_launch_numbers(gpu):
+    """1030 sequences said to be of up to 32,768 queries: 8.4 million workgroups of 512 threads."""
+    _say("2^23 workgroups")
+    n, L, B = 32, 40, 1030
+    x = _make(gpu, 33, [n] * B, [L] * B, 64, 1, 16, torch.bfloat16)
+    got = fai.prefill_paged(x["q"], x["kc"], x["vc"], x["cu"], x["tables"], x["ctx"], 1 << 15)
+    y, rows = _part(x, got, [0, 1, 500, *range(1018, 1030)])
+    _check(rows, y, True)
+    # both within 3 half steps of 2^-8 (and float's) of the largest |v| from the same values
+    assert (got.float() - _run(x, True).float()).abs().max() <= 2 * 3.1 * 2.0 ** -8 * x["vc"].float().abs().max()
+
+
+def test_more_sequences_than_a_launch_holds(gpu):
+    """65,537 sequences of two tokens, 128 KV heads: the same without cu_seqlens."""
+    _say("2^23 sequences' heads")
+    B, h = 65537, 128
+    x = _make(gpu, 34, [2] * 8, [16] * 8, h, h, 16, torch.bfloat16)
+    g = _gen(gpu, 5)
+    q = torch.randn((B, 2, h, 128), generator=g, device=gpu, dtype=torch.bfloat16)
+    lens = torch.randint(1, 17, (B,), generator=g, device=gpu, dtype=torch.int32)
+    tables = torch.randint(0, x["kc"].shape[0], (B, 1), generator=g, device=gpu, dtype=torch.int32)
+    got = fai.flash_attn_with_kvcache(q, x["kc"], x["vc"], cache_seqlens=lens, block_table=tables, causal=True)
+    x.update(q=q.view(-1, h, 128), tables=tables, new=[2] * B, lens=lens.tolist())
+    y, rows = _part(x, got.view(-1, h, 128), [0, 40000, 65533, 65534, 65535, 65536])
+    _check(rows, y, True)
+    assert torch.isfinite(got).all()
