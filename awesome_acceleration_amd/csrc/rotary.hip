@@ -26,6 +26,7 @@ namespace aac {
 namespace rot {
 
 constexpr int kWaves = 4;
+constexpr int64_t kMaxGroups = 1 << 24;  // of 256 threads: a launch numbers its threads in 32 bits
 
 struct Rows {  // heads of one kind: element strides of a sequence, a token, a head
   const char* in;
@@ -363,9 +364,8 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_any_kernel(Args a) {
 template <Dt DT, bool T32, bool INTER>
 static int launch_i(Args a, bool fast, int n_cu, hipStream_t st) {
   if (!fast) {
-    const int64_t blocks = cdiv(a.n_tokens, kWaves);
-    if (blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((rotary_any_kernel<DT, T32, INTER>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, st, a);
+    hipLaunchKernelGGL((rotary_any_kernel<DT, T32, INTER>), dim3((unsigned)cdiv(a.n_tokens, kWaves)),
+                       dim3(64 * kWaves), 0, st, a);
     return AAC_OK;
   }
   const int per = 64 / (a.dim / (2 * Vec<DT>::kN)), total = a.q.heads + a.k.heads + a.v.heads;
@@ -378,9 +378,7 @@ static int launch_i(Args a, bool fast, int n_cu, hipStream_t st) {
   // against 823, 16 x 4096 x 32 heads rotated 180 against 198.
   const bool many = total > per && a.n_tokens * cdiv(total, 2 * (int64_t)per) >= 8 * (int64_t)n_cu;
   const bool large = many && a.n_tokens * total * a.dim * Elem<DT>::kBytes >= (int64_t(64) << 20);
-  const int64_t blocks = blocks_at(many ? 2 : 1);
-  if (blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)blocks), block(64 * kWaves);
+  const dim3 grid((unsigned)blocks_at(many ? 2 : 1)), block(64 * kWaves);
   if (large) hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 2, true>), grid, block, 0, st, a);
   else if (many) hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 2, false>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((rotary_kernel<DT, T32, INTER, 1, false>), grid, block, 0, st, a);
@@ -408,6 +406,10 @@ static int launch(const Args& a, int32_t table_dtype, bool inter, int32_t dtype,
       fast = fast && (((uintptr_t)r->in | (uintptr_t)r->out) % 16) == 0;
       for (int64_t s : {r->seq, r->tok, r->head, r->out_seq, r->out_tok, r->out_head}) fast = fast && s * es % 16 == 0;
     }
+  // Waves of so many tokens: the fast kernel's take two passes where one does not do.
+  if (a.n_tokens > kWaves * (kMaxGroups - 1)) return AAC_ERR_UNSUPPORTED;
+  const int64_t heads = (int64_t)a.q.heads + a.k.heads + a.v.heads, per = fast ? 64 / cpr : heads;
+  if (cdiv(a.n_tokens * (heads > per ? cdiv(heads, 2 * per) : 1), kWaves) >= kMaxGroups) return AAC_ERR_UNSUPPORTED;
   int n_cu = 0;
   int rc = device_cu_count(&n_cu);
   if (rc != AAC_OK) return rc;
@@ -582,7 +584,7 @@ extern "C" int aac_rotary_tables(const void* turns, int32_t n_freqs, const int32
   // (positions are whole numbers in fp64, and their product with 4 turns has a quadrant)
   if (start < -(int64_t(1) << 40) || start > (int64_t(1) << 40)) return AAC_ERR_SHAPE;
   const int64_t blocks = cdiv(n_positions * cdiv(n_freqs, vec), 256);
-  if (n_positions >= (int64_t(1) << 40) / n_freqs || blocks >= (int64_t(1) << 31)) return AAC_ERR_UNSUPPORTED;
+  if (n_positions >= (int64_t(1) << 40) / n_freqs || blocks >= rot::kMaxGroups) return AAC_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks), block(256);
   const double* f = (const double*)turns;
   hipStream_t st = (hipStream_t)stream;

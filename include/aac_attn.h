@@ -590,6 +590,8 @@ int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, con
  * at (p, d): in fp32, rounded once.  The other dims pass unchanged.  Positions outside the
  * tables take their first or last row.  dtype BF16, FP16 or FP32; table_dtype dtype or
  * FP32; head_dim even, rotary_dim even and at most head_dim.  Head strides are free.
+ * A call takes a wave for every 4 KiB of a token's rows that it turns or stores, begun or whole;
+ * 2^26 waves and more are refused.
  *
  * aac_rotary: x -> out (out may be x).  Without cu_seqlens: [n_seqs, seqlen, n_heads,
  * head_dim] by its strides, token i of sequence b at position offsets[b] + i (offsets null:
@@ -611,7 +613,7 @@ int aac_prefill_paged(const void* q, int64_t q_tok_stride, int64_t n_tokens, con
  * aac_rotary_tables: cos_out, sin_out [n_positions, n_freqs] = factor * cos, sin of
  * 2 pi p turns[i] at positions p = positions[r] or, where that is null, start + r.  turns:
  * double [n_freqs] on the device, turns a position, 1 at most; the angle is reduced in 64
- * bits.  |start| up to 2^40; cos_out and sin_out 16-byte aligned where n_freqs is a multiple of 8 (FP32: of 4).
+ * bits.  |start| up to 2^40, fewer than 2^32 vectors of 16 bytes in an output; cos_out and sin_out 16-byte aligned where n_freqs is a multiple of 8 (FP32: of 4).
  */
 int aac_rotary(const void* x, int64_t x_seq_stride, int64_t x_tok_stride, int64_t x_head_stride,
                void* out, int64_t out_seq_stride, int64_t out_tok_stride, int64_t out_head_stride,

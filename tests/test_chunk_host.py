@@ -357,3 +357,31 @@ def test_what_the_attention_refuses_is_refused_before_the_append(launches, turne
     assert launches == []
     call(mb=1, bs=7)
     assert len(launches) == 2
+
+
+def test_rotary_refuses_2_32_threads():
+    """Four waves a workgroup of 256 threads, 2^24 workgroups; the tables' threads a vector each."""
+    def turn(n, h=1, d=128, dt=0, cu=64):
+        return _lib.lib().aac_rotary(64, 0, h * d, d, 64, 0, h * d, d, 1, 0, n, cu, None, 0, h, d, 64, 64, 9, 2, 0,
+                                     0, 2, dt, None)
+
+    # a token a wave (rotary_dim 2: the element-wise kernel); n_seqs x seqlen as well
+    for n in ((1 << 26) - 3, 1 << 26, 1 << 62):
+        assert turn(n) == -2, n
+    assert _lib.lib().aac_rotary(64, 0, 128, 128, 64, 0, 128, 128, 1 << 30, 1 << 30, 0, None, None, 0, 1, 128, 64, 64,
+                                 9, 2, 0, 0, 2, 0, None) == -2
+
+    def append(n, hq, rot=128):
+        return _lib.lib().aac_rotary_append_paged(64, 0, hq * 128, 128, 64, 0, 512, 128, 64, 0, 512, 128, 64, 1, 0, 0,
+                                                  n, 64, 64, None, hq, 4, 128, 64, 64, 9, rot, 0, 0, 64, 64, 1, 16, 64,
+                                                  1, 2, 0, None)
+
+    # 16-bit rows of 128 dims, sixteen a wave: 8 + 2 x 4 heads take one, 9 + 8 two, 65,528 + 8 4096
+    for n, hq in (((1 << 26) - 3, 8), ((1 << 25) - 1, 9), (1 << 25, 9), (1 << 14, 65528)):
+        assert append(n, hq) == -2, (n, hq)
+
+    def tables(n, freqs, dt):
+        return _lib.lib().aac_rotary_tables(64, freqs, None, 0, n, 1.0, 64, 64, dt, None)
+
+    for n, freqs, dt in (((1 << 32) - 255, 4, 2), (1 << 32, 8, 0), ((1 << 28) - 15, 64, 2), (1 << 29, 64, 1)):
+        assert tables(n, freqs, dt) == -2, (n, freqs)

@@ -340,3 +340,17 @@ def test_a_cache_without_blocks_is_refused(gpu):
     with pytest.raises(RuntimeError, match="not empty"):
         rotary.rotary_append_paged(q, q, q, cache, cache, torch.zeros(2, 1, dtype=torch.int32, device=gpu),
                                    torch.zeros(2, dtype=torch.int32, device=gpu), cos, sin)
+
+
+def test_as_many_tokens_as_a_launch_takes(gpu):
+    """2^26 - 4 heads of two dims; one token more is refused."""
+    _say("2^26 tokens")
+    n = (1 << 26) - 4
+    x = torch.randn((1, n + 1, 1, 2), device=gpu, dtype=torch.bfloat16)
+    cos, sin = _tab(gpu, 1000, 2, torch.float32)
+    got = rotary.apply_rotary_emb(x[:, :n], cos, sin)
+    for a in (0, n // 2, n - 1500):
+        at = torch.arange(a, a + 1500, device=gpu).clamp(max=999)
+        _check(got[0, a:a + 1500], x[0, a:a + 1500], cos[at], sin[at], False)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        rotary.apply_rotary_emb(x, cos, sin)
