@@ -314,6 +314,8 @@ class RotaryEmbedding:
             at = _ints(positions, n, "positions")
         if n is None or n < 0:
             raise RuntimeError("n must be given, 0 or more")
+        if abs(start) > 1 << 40:  # (here, before it is cut to 64 bits)
+            raise RuntimeError("inconsistent arguments: start is past 2^40")
         half = self.rotary_dim // 2
         cos = torch.empty((n, half), dtype=dtype, device=self.device)
         sin = torch.empty_like(cos)

@@ -354,3 +354,12 @@ def test_as_many_tokens_as_a_launch_takes(gpu):
         _check(got[0, a:a + 1500], x[0, a:a + 1500], cos[at], sin[at], False)
     with pytest.raises(RuntimeError, match="unsupported"):
         rotary.apply_rotary_emb(x, cos, sin)
+
+
+def test_no_start_is_cut_to_64_bits(gpu):
+    e = rotary.RotaryEmbedding(64, device=gpu)
+    for start in ((1 << 64) + 5, -(1 << 64), 1 << 63, (1 << 40) + 1, -(1 << 40) - 1):
+        with pytest.raises(RuntimeError, match="inconsistent"):
+            e.cos_sin(5, start=start)
+    for start in (1 << 40, -(1 << 40)):
+        assert e.cos_sin(5, start=start)[0].shape == (5, 32)
