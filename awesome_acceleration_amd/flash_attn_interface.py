@@ -399,8 +399,9 @@ def _prefill_paged(q, k_cache, v_cache, cu_q, tables, ctx, cu_k, max_q, max_k, s
         raise RuntimeError("softmax_scale must be positive")
     if q.shape[0] == 0 or B == 0:
         return out
-    if k_cache.numel() == 0 or tables.shape[1] == 0:  # no key anywhere: every row sees none
-        return out.zero_()
+    if k_cache.numel() == 0 or tables.shape[1] == 0:  # no key anywhere: every sequence's rows see none
+        row = torch.arange(q.shape[0], dtype=torch.int32, device=q.device)
+        return out.masked_fill_(((row >= cu_q[0]) & (row < cu_q[-1]))[:, None, None], 0)
     _launch_chunk(q, qs, q.shape[0], k_cache, v_cache, tables, cu_q, ctx, cu_k, B,
                   min(int(max_q), q.shape[0]), int(max_k or 0), scale, causal, out, os)
     return out

@@ -570,3 +570,20 @@ def test_more_sequences_than_a_launch_holds(gpu):
     y, rows = _part(x, got.view(-1, h, 128), [0, 40000, 65533, 65534, 65535, 65536])
     _check(rows, y, True)
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("none", ["blocks", "columns", "keys"])
+def test_rows_of_no_sequence_without_any_key(gpu, none):
+    """Zeros for the sequences' rows; those before and behind them stay."""
+    _say("no key", none)
+    x = _make(gpu, 35, [3, 2], [20, 5], 16, 8, 16, torch.bfloat16, extra_rows=4)
+    x["cu"] += 1
+    if none == "blocks":
+        x["kc"], x["vc"] = x["kc"][:0], x["vc"][:0]
+    elif none == "columns":
+        x["tables"] = x["tables"][:, :0].contiguous()
+    else:
+        x["ctx"].zero_()
+    out = torch.full((9, 16, 128), 3.0, dtype=torch.bfloat16, device=gpu)
+    assert _run(x, True, out=out) is out
+    assert (out[1:6] == 0).all() and (out[0] == 3).all() and (out[6:] == 3).all()
