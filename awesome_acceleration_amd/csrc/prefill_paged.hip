@@ -15,12 +15,25 @@
 // block holds the sequence), so a wave finds their address with scalar loads and
 // arithmetic, one iteration ahead, and brings them with direct loads into LDS through a
 // buffer resource that ends at the context: rows behind it, whatever the page holds,
-// arrive as zeros.  Other block sizes look every row up in its lane (PAGE16 false).
+// arrive as zeros.  Other block sizes look every row up in its lane, right before its load
+// (PAGE16 false); the wait for the entry is one for all loads in flight, so nothing overlaps
+// there: pages of 20 / 40 tokens against 16, us, 777 queries over 7778 keys at 16/8 heads 86 /
+// 86 against 69, 16 x 5 over 1.0-2.0k 39 / 39 against 27, 4 x 1024 over 8192 at 32/8 570 / 566
+// against 463.
+//
+// Roundings.  Scores, softmax statistics and sums are fp32; the probabilities are rounded to
+// 16 bits once, the second product's operands (a second term for what that loses would cost
+// another of these products), and the row sum is of the rounded ones, so that the weights add
+// up to 1.  The reciprocal is the hardware's, a unit of 2^-23 off.  Against 64 bits outputs
+// are 2.0e-3 off in bf16 (root mean square, relative; fp32 throughout and rounded once at the
+// end 1.7e-3), 2.6e-4 in fp16 (2.1e-4).
 //
 // Queries.  A wave's rows come in the same way, into the place of the ring's last stages,
 // beside the first stages' keys (loaded to registers, with every load waited for at the
 // start, calls of 97 to 306 tokens took 8.2-19 us where they take 7.6-17.5).  What depends on the lane alone is
-// worked out again for each item of shared work: kept, 18 registers spilled.
+// worked out again for each item of shared work: kept, 18 vector registers of the 256-row
+// form spilled.  None does now but two with pages that are no multiple of 16; the shared forms
+// hold 4 to 35 scalar registers in vector lanes.
 //
 // Bounds.  8 sequences of 2048 over 14-30k keys at 32/8 heads (6.12 TFLOP) take 5.43-5.48
 // ms, 1.12 PFLOP/s at the 1.9 GHz that the card holds there: 1.88 us for the 64 keys of
@@ -76,7 +89,7 @@ struct Args {
 // first to last, where they are two or more and this is the item's first cut; share
 // `opens` holds its beginning.
 struct Cut {
-  int first, last, opens, row0, rows, q_beg, unused[2];
+  int first, last, opens, row0, rows, q_beg, pad[2];  // (32 bytes)
 };
 
 // x / d for x < 2^27: x * ceil(2^(27 + s) / d) >> (27 + s), s = ceil(log2 d).
@@ -770,6 +783,8 @@ struct Plan {
 
 static Plan plan(int32_t n_seqs, int32_t max_q, int32_t max_k, int64_t cap, int32_t hq, int32_t hkv, int n_cu) {
   Plan p = {};
+  // (every sequence is counted as long as the longest: of single tokens beside a long chunk the
+  // items are far fewer than this says)
   const int64_t rows = (int64_t)max_q * (hq / hkv);
   auto items_of = [&](int r) { return (int64_t)n_seqs * hkv * cdiv(rows, r); };
   // Rows of a workgroup, us in 64 / 128 / 256 of them.  Where one block holds a sequence's

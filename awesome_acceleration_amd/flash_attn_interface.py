@@ -416,11 +416,12 @@ def prefill_paged(q, k_cache, v_cache, cu_seqlens_q, block_tables, context_lens,
 
     block_tables int32 ``[B, max_blocks]``, caches ``[num_blocks, block_size, Hkv, D]``.
     ``causal``: query ``i`` of ``n`` sees keys ``j <= i + context_lens[b] - n``.  A query that
-    sees no key gets zeros; the value of a key it does not see, infinite or NaN though it
-    may be, does not reach it.  Rows of q of no sequence are left as they are in ``out`` (undefined
-    in a new one).  ``max_seqlen_q`` bounds the new tokens of a sequence, ``max_context_len``
-    (default: the tables' capacity) is an estimate that sizes the split of the keys.  bf16
-    and fp16, head_dim 128, any number of query heads a KV head."""
+    sees no key gets zeros; a context longer than the table counts as the table's capacity, in
+    the mask too; the value of a key it does not see, infinite or NaN though it may be, does
+    not reach it.  Rows of q of no sequence are left as they are in ``out`` (undefined in a new
+    one).  ``max_seqlen_q`` bounds the new tokens of a sequence, ``max_context_len`` (default:
+    the tables' capacity) is an estimate that sizes the split of the keys.  bf16 and fp16,
+    head_dim 128, any number of query heads a KV head."""
     return _prefill_paged(q, k_cache, v_cache, cu_seqlens_q, block_tables, context_lens, None,
                           max_seqlen_q, max_context_len, softmax_scale, causal, out)
 
@@ -544,10 +545,10 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
 
     With S > 1, k and v ``[B, S_new, Hkv, D]`` (S_new need not be S) go to positions
     ``cache_seqlens[b]`` and up, and ``causal`` masks as in ``prefill_paged``; ``num_splits`` is
-    then the library's choice.  ``rotary_cos`` and ``rotary_sin`` (``[positions, R / 2]``, q's
-    type or float32; with k and v) turn the first R dims of the new keys by their positions
-    and of the queries by ``cache_seqlens[b] + i`` if ``causal``, else all by
-    ``cache_seqlens[b]``, as ``rotary.apply_rotary_emb`` does (interleaved pairs unless
+    then, and with rotary tables, the library's choice.  ``rotary_cos`` and ``rotary_sin``
+    (``[positions, R / 2]``, q's type or float32; with k and v) turn the first R dims of the new
+    keys by their positions and of the queries by ``cache_seqlens[b] + i`` if ``causal``, else
+    all by ``cache_seqlens[b]``, as ``rotary.apply_rotary_emb`` does (interleaved pairs unless
     ``rotary_interleaved`` is false): rounded to their type, then stored and attended.
     """
     if softcap or alibi_slopes is not None or window_size != (-1, -1):
