@@ -447,6 +447,7 @@ class LLM:
             out.logprobs, out.entropies, out.top_logprobs = map(list, zip(*s.scores))
         req.results[s.prompt_idx] = out
         self.allocator.free(s.blocks)
+        s.blocks = []  # (no longer its own, should this step fail)
         bisect.insort(free_rows, s.row)
         if all(r is not None for r in req.results):
             req.future.set_result(req.results)

@@ -385,3 +385,21 @@ def test_rotary_refuses_2_32_threads():
 
     for n, freqs, dt in (((1 << 32) - 255, 4, 2), (1 << 32, 8, 0), ((1 << 28) - 15, 64, 2), (1 << 29, 64, 1)):
         assert tables(n, freqs, dt) == -2, (n, freqs)
+
+
+@pytest.mark.filterwarnings("ignore::pytest.PytestUnhandledThreadExceptionWarning")
+def test_a_failed_step_frees_no_block_of_another():
+    """A block that a sequence gave back before the failure may be someone else's by then."""
+    held, ended = [], []
+
+    def text(tokens):
+        ended.append(tokens)
+        if len(ended) == 2:
+            held.extend(llm.allocator.allocate(llm.allocator.num_free))
+            raise MemoryError("no memory")
+        return ""
+
+    llm = _engine(decode_fn=text)
+    with pytest.raises(MemoryError):
+        llm.generate([[1] * 5, [2] * 5], max_tokens=2).result(timeout=20)
+    assert len(held) == 11 and llm.allocator.num_free == 1
