@@ -281,6 +281,7 @@ def test_a_step_that_fails_ends_every_request(chunk, where):
     for f in futs:
         with pytest.raises(MemoryError):
             f.result(timeout=20)
+    llm._loop_thread.join(20)
 
 
 @pytest.mark.parametrize("chunk", [None, 4])
@@ -307,6 +308,7 @@ def test_after_a_failed_step_the_engine_serves_again(chunk):
         llm._decode_step = fail
         with pytest.raises(MemoryError):
             llm.generate([[1] * 40] * 5, max_tokens=20).result(timeout=20)
+        llm._loop_thread.join(20)
         assert llm.allocator.num_free == 12
         llm._decode_step = works
         assert [o.token_ids for o in llm.generate([[1] * 40] * 5, max_tokens=20).result(timeout=20)] == [[7] * 20] * 5
@@ -402,4 +404,5 @@ def test_a_failed_step_frees_no_block_of_another():
     llm = _engine(decode_fn=text)
     with pytest.raises(MemoryError):
         llm.generate([[1] * 5, [2] * 5], max_tokens=2).result(timeout=20)
+    llm._loop_thread.join(20)
     assert len(held) == 11 and llm.allocator.num_free == 1
