@@ -32,8 +32,8 @@
 // beside the first stages' keys (loaded to registers, with every load waited for at the
 // start, calls of 97 to 306 tokens took 8.2-19 us where they take 7.6-17.5).  What depends on the lane alone is
 // worked out again for each item of shared work: kept, 18 vector registers of the 256-row
-// form spilled.  None does now but two with pages that are no multiple of 16; the shared forms
-// hold 4 to 35 scalar registers in vector lanes.
+// form spilled.  Two still do with pages that are no multiple of 16; the shared forms keep up
+// to 35 scalar registers in vector lanes.
 //
 // Bounds.  8 sequences of 2048 over 14-30k keys at 32/8 heads (6.12 TFLOP) take 5.43-5.48
 // ms, 1.12 PFLOP/s at the 1.9 GHz that the card holds there: 1.88 us for the 64 keys of
